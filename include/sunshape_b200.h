@@ -47,6 +47,7 @@ extern "C" {
 #define SUNSHAPE_U8 3
 #define SUNSHAPE_I16 4
 #define SUNSHAPE_I32 5
+#define SUNSHAPE_I64 6     /* positions only */
 
 /* One layer's codec (the buffers of SunShapeBlockCodec, codec.py:230-245, E = I).
  * centroids holds n_cb codebooks; KV head h (h = flat_head % kv_heads) uses
@@ -211,6 +212,98 @@ int sunshape_exchange_merge(const float* partials, int64_t rows, int32_t value_d
                             const sunshape_peer_group_t* group, void* out, int32_t out_dtype, void* stream);
 int sunshape_exchange_error(const void* own_buffer, int32_t world, int64_t rows, int32_t value_dim,
                             int32_t* code);
+
+/* ---- Paged serving: head norms with rotation, append to a paged compressed cache, attention over it
+ * (no reference counterpart: the reference's caches are contiguous and its models rotate in torch).
+ *
+ * Rows [batch, heads, length, dim] of a tensor whose last axis has unit stride: row (b, h, l) starts at
+ * data + b * stride_b + h * stride_h + l * stride_l (elements). */
+typedef struct sunshape_rows {
+  void* data;
+  int64_t stride_b, stride_h, stride_l;
+  int32_t heads;
+} sunshape_rows_t;
+
+/* Rotary position embedding of the first rot_dim elements of a row at position p = positions[b, l]:
+ * pairs (i, i + rot_dim/2), or (2i, 2i + 1) when interleaved, turn by the angle whose cosine and sine
+ * are cos[p, i] and sin[p, i].  A position outside [0, table_len) makes the row NaN (or leaves the
+ * token out of an append) and records 131. */
+typedef struct sunshape_rotation {
+  const float* cos;            /* [table_len, rot_dim / 2] fp32 */
+  const float* sin;
+  const void* positions;       /* [batch, length] SUNSHAPE_I32 or SUNSHAPE_I64 */
+  int64_t position_stride_b, position_stride_l;
+  int64_t table_len;
+  int32_t position_dtype;
+  int32_t rot_dim;             /* even, <= dim; 0 = no rotation */
+  int32_t interleaved;
+} sunshape_rotation_t;
+
+/* y = rotate(x * weight / sqrt(mean(x^2) + eps)) for the rows of q and, in the same launch, of k (k and
+ * k_out NULL: only q).  A NULL weight leaves that tensor's norm out; rotation NULL leaves it unrotated.
+ * All arithmetic is fp32, rounded once to dtype.  out may be the input itself (same strides), not another
+ * overlapping range.  F32/BF16/F16 rows; weights [dim] F32/BF16/F16 of weight_dtype. */
+int sunshape_norm_rotate(const sunshape_rows_t* q, const sunshape_rows_t* q_out, const void* q_weight,
+                         const sunshape_rows_t* k, const sunshape_rows_t* k_out, const void* k_weight,
+                         int32_t dtype, int32_t weight_dtype, int32_t batch, int32_t length, int32_t dim,
+                         float eps, const sunshape_rotation_t* rotation, void* stream);
+
+/* One layer's pages.  Token slot s lies in page s / page_size at row s % page_size; page p, KV head h holds
+ * its rows contiguously: indices [num_pages, kv_heads, page_size, n_blocks] uint8, value [num_pages,
+ * kv_heads, page_size, value_dim] and, for a SunShape-Mixed codec, heavy [num_pages, kv_heads, page_size,
+ * n_heavy, block_dim], both of dtype (BF16 or F16).  page_size is a multiple of 16. */
+typedef struct sunshape_pages {
+  uint8_t* indices;
+  void* heavy;
+  void* value;
+  int64_t num_pages;
+  int32_t kv_heads;
+  int32_t page_size;
+  int32_t value_dim;
+  int32_t dtype;
+} sunshape_pages_t;
+
+/* Append key and value rows [batch, kv_heads, length, head_dim | value_dim] (dtype of the pages) to slots
+ * [batch, length] (int64; -1 = leave the row out): the key is rotated (rotation NULL: taken as it is),
+ * permuted and encoded to the nearest codeword of every block -- exactly: the first minimum of the distances
+ * in real arithmetic as 64-bit floats give it, of the rotated key without an intermediate rounding -- or
+ * kept, rounded to dtype, where the block is dense (index 0); the value is copied.  Slots must be distinct:
+ * of two rows for one slot either may stay.  A slot outside [-1, num_pages * page_size) is left out and
+ * records 132.  At most 256 codewords, block_dim 2, 4 or 8. */
+int sunshape_paged_append(const sunshape_codec_t* codec, const sunshape_pages_t* pages,
+                          const sunshape_rows_t* key, const sunshape_rows_t* value, int32_t batch, int32_t length,
+                          const int64_t* slots, int64_t slot_stride_b, int64_t slot_stride_l,
+                          const sunshape_rotation_t* rotation, void* stream);
+
+/* Attention over pages.  Sequence b's own tokens are rows 0 .. seq_lens[b]-1 of the pages
+ * page_table[b * table_stride + i] (int32, table_cols of them); before them, for every sequence alike, come
+ * the prefix_len tokens of the pages prefix_table (prefix_len 0: no prefix), whose attention is computed
+ * once for the whole batch.
+ * query [batch, q_heads, query_len, head_dim] (unit last stride; BF16 or F16, the pages' dtype), out
+ * [batch, q_heads, query_len, value_dim] contiguous, of the same dtype.
+ * The last query_len tokens of a sequence are the queries' own: query l sees all but the last
+ * query_len - 1 - l of the sequence's own tokens (and all of the prefix); causal = 0: all of them.  A row
+ * that sees no token is zero.  Softmax of scale * <q, k_hat>, statistics and sums in fp32.
+ * codebook: [n_cb, head_dim / 64, 256, 64] fp16, the codewords times codebook_scale[n_cb] (a power of two):
+ *   row (i, c) holds codeword c of the 64 / block_dim blocks from i * 64 / block_dim on, codewords above
+ *   n_centroids zero.
+ * head_dim and value_dim 64 or 128; block_dim 2, 4 or 8.  A page outside the pool records 133 and a length
+ * outside [0, table_cols * page_size] 134; both make the sequence's rows NaN.
+ * workspace: sunshape_paged_attention_workspace_bytes, 256-byte aligned, needs no initial value and keeps
+ * none; calls that overlap need separate ones. */
+int64_t sunshape_paged_attention_workspace_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t query_len,
+                                                 int32_t value_dim, int32_t table_cols, int32_t page_size,
+                                                 int32_t prefix_len);
+int sunshape_paged_attention(const sunshape_codec_t* codec, const sunshape_pages_t* pages, const void* codebook,
+                             const float* codebook_scale, const sunshape_rows_t* query, int32_t batch,
+                             int32_t query_len, const int32_t* page_table, int64_t table_stride, int32_t table_cols,
+                             const int32_t* seq_lens, const int32_t* prefix_table, int32_t prefix_len, float scale,
+                             int32_t causal, void* out, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* First code recorded on the current device by the kernels above since the last clear: 0 none, 131 position
+ * out of the table, 132 slot out of the pool, 133 page out of the pool, 134 sequence longer than its page
+ * table, 135 a bounded pipeline wait gave up.  Waits for the device's queued work. */
+int sunshape_paged_error(int32_t* code, int32_t clear);
 
 /* Size of the scratch array built into the library for sunshape_decode_attention_noalloc. */
 #define SUNSHAPE_NOALLOC_SCRATCH_BYTES (8 * 1024 * 1024)

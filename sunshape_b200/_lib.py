@@ -18,7 +18,7 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libsunshape_b200.so")
 
-F32, BF16, F16, U8, I16, I32 = 0, 1, 2, 3, 4, 5
+F32, BF16, F16, U8, I16, I32, I64 = 0, 1, 2, 3, 4, 5, 6
 _DTYPE_CODE = {
     torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16,
     torch.uint8: U8, torch.int16: I16, torch.int32: I32,
@@ -32,7 +32,8 @@ EXPORTED_SYMBOLS = (
     "sunshape_decode_attention_peers", "sunshape_decode_workspace_min_bytes", "sunshape_encode_error",
     "sunshape_decode_attention_noalloc_error", "sunshape_exchange_buffer_bytes", "sunshape_exchange_merge",
     "sunshape_exchange_error", "sunshape_index_row_bytes", "sunshape_pack_indices",
-    "sunshape_attention_scores_packed",
+    "sunshape_attention_scores_packed", "sunshape_norm_rotate", "sunshape_paged_append",
+    "sunshape_paged_attention_workspace_bytes", "sunshape_paged_attention", "sunshape_paged_error",
 )
 
 
@@ -66,6 +67,24 @@ class KVDesc(ctypes.Structure):
 
 class PeerGroupDesc(ctypes.Structure):
     _fields_ = [("rank", ctypes.c_int32), ("world", ctypes.c_int32), ("buffers", ctypes.c_void_p * 8)]
+
+
+class RowsDesc(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("stride_b", ctypes.c_int64), ("stride_h", ctypes.c_int64),
+                ("stride_l", ctypes.c_int64), ("heads", ctypes.c_int32)]
+
+
+class RotationDesc(ctypes.Structure):
+    _fields_ = [("cos", ctypes.c_void_p), ("sin", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+                ("position_stride_b", ctypes.c_int64), ("position_stride_l", ctypes.c_int64),
+                ("table_len", ctypes.c_int64), ("position_dtype", ctypes.c_int32), ("rot_dim", ctypes.c_int32),
+                ("interleaved", ctypes.c_int32)]
+
+
+class PagesDesc(ctypes.Structure):
+    _fields_ = [("indices", ctypes.c_void_p), ("heavy", ctypes.c_void_p), ("value", ctypes.c_void_p),
+                ("num_pages", ctypes.c_int64), ("kv_heads", ctypes.c_int32), ("page_size", ctypes.c_int32),
+                ("value_dim", ctypes.c_int32), ("dtype", ctypes.c_int32)]
 
 
 _lib = None
@@ -127,6 +146,17 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
             getattr(lib, name).restype = ctypes.c_int
         lib.sunshape_decode_attention_peers.argtypes = [pc, pk, vp, i32, i32, i32, i32, i32, vp, i32, i64, i64, i64,
                                                         f32, vp, i32, ctypes.POINTER(PeerGroupDesc), vp, i64, vp]
+        pr, pt, pp = ctypes.POINTER(RowsDesc), ctypes.POINTER(RotationDesc), ctypes.POINTER(PagesDesc)
+        lib.sunshape_norm_rotate.argtypes = [pr, pr, vp, pr, pr, vp, i32, i32, i32, i32, i32, f32, pt, vp]
+        lib.sunshape_paged_append.argtypes = [pc, pp, pr, pr, i32, i32, vp, i64, i64, pt, vp]
+        lib.sunshape_paged_attention_workspace_bytes.argtypes = [i32] * 8
+        lib.sunshape_paged_attention_workspace_bytes.restype = ctypes.c_int64
+        lib.sunshape_paged_attention.argtypes = [pc, pp, vp, vp, pr, i32, i32, vp, i64, i32, vp, vp, i32, f32, i32, vp, vp,
+                                                 i64, vp]
+        lib.sunshape_paged_error.argtypes = [ctypes.POINTER(ctypes.c_int32), i32]
+        for name in ("sunshape_norm_rotate", "sunshape_paged_append", "sunshape_paged_attention",
+                     "sunshape_paged_error"):
+            getattr(lib, name).restype = ctypes.c_int
         for name in ("sunshape_encode", "sunshape_dequantize", "sunshape_attention_scores",
                      "sunshape_decode_attention", "sunshape_merge_partials"):
             getattr(lib, name).restype = ctypes.c_int
@@ -333,3 +363,34 @@ def attention_scores_packed(cd: CodecDesc, indices: torch.Tensor, index_bits: in
         _check(load_library().sunshape_attention_scores_packed(
             ctypes.byref(cd), ptr(indices), index_bits, seq_len, head_stride, ptr(query), dtype_code(query), n_heads,
             kv_heads, rows, ptr(out), stream_ptr(dev)))
+
+
+def norm_rotate(dev, q: RowsDesc, q_out: RowsDesc, q_weight, k, k_out, k_weight, dtype: int, weight_dtype: int, batch: int,
+                length: int, dim: int, eps: float, rotation) -> None:
+    with torch.cuda.device(dev):
+        _check(load_library().sunshape_norm_rotate(q, q_out, ptr(q_weight), k, k_out, ptr(k_weight), dtype, weight_dtype,
+                                                   batch, length, dim, eps, rotation, stream_ptr(dev)))
+
+
+def paged_append(dev, cd: CodecDesc, pages: PagesDesc, key: RowsDesc, value: RowsDesc, batch: int, length: int,
+                 slots: torch.Tensor, rotation) -> None:
+    with torch.cuda.device(dev):
+        _check(load_library().sunshape_paged_append(cd, pages, key, value, batch, length, ptr(slots), slots.stride(0),
+                                                    slots.stride(1), rotation, stream_ptr(dev)))
+
+
+def paged_attention(dev, cd: CodecDesc, pages: PagesDesc, codebook: torch.Tensor, codebook_scale: torch.Tensor,
+                    query: RowsDesc, batch: int, query_len: int, page_table: torch.Tensor, seq_lens: torch.Tensor,
+                    prefix_table, prefix_len: int, scale: float, causal: bool, out: torch.Tensor) -> None:
+    lib = load_library()
+    cols = page_table.shape[1]
+    with torch.cuda.device(dev):
+        need = lib.sunshape_paged_attention_workspace_bytes(batch, query.heads, pages.kv_heads, query_len,
+                                                            pages.value_dim, cols, pages.page_size, prefix_len)
+        # a block of the allocator of the current stream (of the graph's own pool under capture): two streams or
+        # two captured graphs never share one
+        ws = torch.empty(max(need, 256), dtype=torch.uint8, device=dev)
+        _check(lib.sunshape_paged_attention(cd, pages, ptr(codebook), ptr(codebook_scale), query, batch, query_len,
+                                            ptr(page_table), page_table.stride(0), cols, ptr(seq_lens),
+                                            ptr(prefix_table), prefix_len, scale, 1 if causal else 0, ptr(out), ptr(ws),
+                                            ws.numel(), stream_ptr(dev)))

@@ -492,6 +492,9 @@ int check_kv(const sunshape_kv_t* kv, const sunshape_codec_t* c, bool need_value
 namespace sunshape {
 // lets other translation units of the library report errors through sunshape_last_error()
 int set_last_error(int code, const char* msg) { return fail(code, msg); }
+int launch_status(const char* what) { return cuda_status(what); }
+int check_codec_args(const sunshape_codec_t* c) { return check_codec(c); }
+int sm_count() { return num_sms(); }
 }  // namespace sunshape
 
 extern "C" {

@@ -1,0 +1,329 @@
+// Head norms of queries and keys with the position rotation in the same pass.
+//
+//   y = x * w / sqrt(mean(x^2) + eps),   z_i = y_i c_i - y_j s_i,   z_j = y_j c_i + y_i s_i
+//
+// Bound by memory: every row is read and written once, and the pass does about ten fp32 operations an
+// element.  A row is 256 bytes at dim 128, so one thread takes 16 elements of a row as two 16-byte loads that
+// hold whole pairs (elements 8s .. 8s+7 of each half, or 16s .. 16s+15 when neighbours pair up): the rotation
+// then needs no exchange between threads, only the norm's sum does (three shuffles at dim 128).  Cosines and
+// sines belong to the token, not to the head, so a thread keeps them in registers over the heads that it takes.
+#include "paged.cuh"
+
+namespace sunshape {
+namespace {
+
+struct NormRotateParams {
+  const void* x[2];
+  void* y[2];
+  int64_t xs[2][3], ys[2][3];   // strides of (b, h, l), elements
+  int heads[2];
+  const void* w[2];
+  int w_dtype;
+  float eps;
+  int L, dim, width;            // width: threads of a row (vector kernel)
+  int chunks[2];                // head chunks of q and k per token
+  int64_t tokens, items;
+  Rotation rot;
+  int* err;
+};
+
+template <typename T>
+struct Vec8 {
+  uint4 v[sizeof(T) / 2];
+};
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, Vec8<T>& r) {
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.v[i] = reinterpret_cast<const uint4*>(p)[i];
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack8(const Vec8<T>& r, float* f) {
+  const T* e = reinterpret_cast<const T*>(&r);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = Elem<T>::to_float(e[i]);
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float* f) {
+  Vec8<T> r;
+  T* e = reinterpret_cast<T*>(&r);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) e[i] = Elem<T>::from_float(f[i]);
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = r.v[i];
+}
+
+// HC heads of one token and one tensor per group of `width` threads; heads of a group are `chunks` apart, so
+// neighbouring groups touch neighbouring rows.
+template <typename T, int HC, bool INTER>
+__global__ void __launch_bounds__(128) norm_rotate_vec(const __grid_constant__ NormRotateParams p) {
+  const int W = p.width;
+  const int s = threadIdx.x & (W - 1);
+  const int64_t item = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / W;
+  if (item >= p.items) return;            // whole groups leave: the shuffles below stay within a group
+  const unsigned mask = W == 32 ? 0xffffffffu : ((1u << W) - 1) << ((threadIdx.x & 31) & ~(W - 1));
+  const int per = p.chunks[0] + p.chunks[1];
+  const int64_t token = item / per;
+  int chunk = (int)(item - token * per);
+  const int which = chunk >= p.chunks[0];
+  if (which) chunk -= p.chunks[0];
+  const int64_t b = token / p.L, l = token - b * p.L;
+  const int heads = p.heads[which], step = p.chunks[which];
+  const bool have = s * 16 < p.dim;       // the last threads of a group are idle when dim / 16 is no power of two
+  const int R = p.rot.rot;
+  const bool turned = s * 16 < R;
+  // first elements of this thread's two runs of eight
+  const int e0 = !INTER && turned ? 8 * s : 16 * s;
+  const int e1 = !INTER && turned ? 8 * s + R / 2 : 16 * s + 8;
+
+  const T* x = reinterpret_cast<const T*>(p.x[which]) + b * p.xs[which][0] + l * p.xs[which][2];
+  T* y = reinterpret_cast<T*>(p.y[which]) + b * p.ys[which][0] + l * p.ys[which][2];
+  Vec8<T> in[HC][2];
+#pragma unroll
+  for (int i = 0; i < HC; ++i) {
+    const int h = chunk + i * step;
+    if (have && h < heads) {
+      load8(x + h * p.xs[which][1] + e0, in[i][0]);
+      load8(x + h * p.xs[which][1] + e1, in[i][1]);
+    }
+  }
+  float c[8], sn[8];
+  bool bad = false;
+  if (R) {
+    const int64_t pos = position_of(p.rot, b, l);
+    bad = pos < 0 || pos >= p.rot.table_len;
+    if (bad && s == 0) record_error(p.err, kErrPosition);
+    if (turned) {
+      const int64_t at = (bad ? 0 : pos) * (R / 2) + 8 * s;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        reinterpret_cast<float4*>(c)[i] = reinterpret_cast<const float4*>(p.rot.cos + at)[i];
+        reinterpret_cast<float4*>(sn)[i] = reinterpret_cast<const float4*>(p.rot.sin + at)[i];
+      }
+    }
+  }
+  float w0[8], w1[8];
+  const void* w = p.w[which];
+  if (w && have) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      w0[i] = load_as_float(w, e0 + i, p.w_dtype);
+      w1[i] = load_as_float(w, e1 + i, p.w_dtype);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < HC; ++i) {
+    const int h = chunk + i * step;
+    if (h >= heads) break;                // the same for the whole group
+    float a0[8], a1[8];
+    unpack8(in[i][0], a0);
+    unpack8(in[i][1], a1);
+    if (w) {
+      float q = 0.f;
+      if (have) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q = fmaf(a0[e], a0[e], fmaf(a1[e], a1[e], q));
+      }
+      for (int o = W >> 1; o; o >>= 1) q += __shfl_xor_sync(mask, q, o);
+      const float r = rsqrtf(q / (float)p.dim + p.eps);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        a0[e] = a0[e] * r * w0[e];
+        a1[e] = a1[e] * r * w1[e];
+      }
+    }
+    if (turned) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float& u = INTER ? (e < 4 ? a0[2 * e] : a1[2 * e - 8]) : a0[e];
+        float& v = INTER ? (e < 4 ? a0[2 * e + 1] : a1[2 * e - 7]) : a1[e];
+        const float zu = u * c[e] - v * sn[e], zv = v * c[e] + u * sn[e];
+        u = zu;
+        v = zv;
+      }
+    }
+    if (bad) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) a0[e] = a1[e] = __int_as_float(0x7fffffff);
+    }
+    if (have) {
+      store8(y + h * p.ys[which][1] + e0, a0);
+      store8(y + h * p.ys[which][1] + e1, a1);
+    }
+  }
+}
+
+// Any dim, rot_dim, stride and alignment: one warp a row, the row staged in shared memory so that it may be
+// overwritten in place.
+template <typename T>
+__global__ void __launch_bounds__(128) norm_rotate_any(const __grid_constant__ NormRotateParams p) {
+  extern __shared__ float rows[];
+  const int lane = threadIdx.x & 31;
+  float* f = rows + (threadIdx.x >> 5) * p.dim;
+  const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (row >= p.items) return;
+  const int per = p.heads[0] + p.heads[1];
+  const int64_t token = row / per;
+  int h = (int)(row - token * per);
+  const int which = h >= p.heads[0];
+  if (which) h -= p.heads[0];
+  const int64_t b = token / p.L, l = token - b * p.L;
+  const T* x = reinterpret_cast<const T*>(p.x[which]) + b * p.xs[which][0] + h * p.xs[which][1] + l * p.xs[which][2];
+  T* y = reinterpret_cast<T*>(p.y[which]) + b * p.ys[which][0] + h * p.ys[which][1] + l * p.ys[which][2];
+  float q = 0.f;
+  for (int d = lane; d < p.dim; d += 32) {
+    const float v = Elem<T>::to_float(x[d]);
+    f[d] = v;
+    q = fmaf(v, v, q);
+  }
+  __syncwarp();
+  if (p.w[which]) {
+    for (int o = 16; o; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
+    const float r = rsqrtf(q / (float)p.dim + p.eps);
+    for (int d = lane; d < p.dim; d += 32) f[d] = f[d] * r * load_as_float(p.w[which], d, p.w_dtype);
+    __syncwarp();
+  }
+  int64_t pos = 0;
+  bool bad = false;
+  if (p.rot.rot) {
+    pos = position_of(p.rot, b, l);
+    bad = pos < 0 || pos >= p.rot.table_len;
+    if (bad && lane == 0) record_error(p.err, kErrPosition);
+    if (bad) pos = 0;
+  }
+  for (int d = lane; d < p.dim; d += 32) {
+    float v = f[d];
+    if (d < p.rot.rot) {
+      int other, i;
+      bool second;
+      pair_of(p.rot, d, other, i, second);
+      const float c = p.rot.cos[pos * (p.rot.rot / 2) + i], sn = p.rot.sin[pos * (p.rot.rot / 2) + i];
+      v = second ? v * c + f[other] * sn : v * c - f[other] * sn;
+    }
+    y[d] = Elem<T>::from_float(bad ? __int_as_float(0x7fffffff) : v);
+  }
+}
+
+template <typename T>
+void launch(NormRotateParams& p, bool vec, cudaStream_t st) {
+  if (!vec) {
+    p.items = p.tokens * (p.heads[0] + p.heads[1]);
+    norm_rotate_any<T><<<(unsigned)((p.items + 3) / 4), 128, 4 * p.dim * sizeof(float), st>>>(p);
+    return;
+  }
+  int w = 1;
+  while (w * 16 < p.dim) w *= 2;
+  p.width = w;
+  // four heads a thread group once that still leaves every SM two full blocks of threads several times over;
+  // below it one head, so that a decode step's few rows spread over the SMs
+  const bool four = p.tokens * (p.heads[0] + p.heads[1]) * w >= (int64_t)148 * 2048 * 4;
+  const int hc = four ? 4 : 1;
+  for (int i = 0; i < 2; ++i) p.chunks[i] = (p.heads[i] + hc - 1) / hc;
+  p.items = p.tokens * (p.chunks[0] + p.chunks[1]);
+  const unsigned grid = (unsigned)((p.items * w + 127) / 128);
+  if (p.rot.interleaved) {
+    if (four) norm_rotate_vec<T, 4, true><<<grid, 128, 0, st>>>(p);
+    else norm_rotate_vec<T, 1, true><<<grid, 128, 0, st>>>(p);
+  } else {
+    if (four) norm_rotate_vec<T, 4, false><<<grid, 128, 0, st>>>(p);
+    else norm_rotate_vec<T, 1, false><<<grid, 128, 0, st>>>(p);
+  }
+}
+
+bool float_type(int d) { return d == SUNSHAPE_F32 || d == SUNSHAPE_BF16 || d == SUNSHAPE_F16; }
+
+}  // namespace
+
+__device__ int g_paged_error;
+
+int* paged_error_word() {
+  void* a = nullptr;
+  return cudaGetSymbolAddress(&a, g_paged_error) == cudaSuccess ? static_cast<int*>(a) : nullptr;
+}
+
+int make_rotation(const sunshape_rotation_t* r, int dim, bool empty, Rotation* out) {
+  *out = Rotation{};
+  if (!r || r->rot_dim == 0) return SUNSHAPE_OK;
+  if (r->rot_dim < 0 || r->rot_dim > dim || r->rot_dim % 2)
+    return set_last_error(SUNSHAPE_E_INVALID, "rot_dim must be even and between 0 and the head dimension.");
+  if (!empty && (!r->cos || !r->sin || !r->positions)) return set_last_error(SUNSHAPE_E_INVALID, "rotation pointer is NULL.");
+  if (r->table_len < 0) return set_last_error(SUNSHAPE_E_INVALID, "rotation table length must be >= 0.");
+  if (r->position_dtype != SUNSHAPE_I32 && r->position_dtype != SUNSHAPE_I64)
+    return set_last_error(SUNSHAPE_E_INVALID, "positions must be I32 or I64.");
+  *out = Rotation{r->cos, r->sin, r->positions, r->position_stride_b, r->position_stride_l, r->table_len,
+                  r->position_dtype == SUNSHAPE_I64, r->rot_dim, r->interleaved != 0};
+  return SUNSHAPE_OK;
+}
+
+}  // namespace sunshape
+
+using namespace sunshape;
+
+extern "C" {
+
+int sunshape_paged_error(int32_t* code, int32_t clear) {
+  if (!code) return set_last_error(SUNSHAPE_E_INVALID, "code pointer is NULL.");
+  int* w = paged_error_word();
+  if (!w || cudaMemcpy(code, w, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess)
+    return set_last_error(SUNSHAPE_E_CUDA, "reading the paged error word failed.");
+  if (clear && cudaMemset(w, 0, sizeof(int)) != cudaSuccess)
+    return set_last_error(SUNSHAPE_E_CUDA, "clearing the paged error word failed.");
+  return SUNSHAPE_OK;
+}
+
+int sunshape_norm_rotate(const sunshape_rows_t* q, const sunshape_rows_t* q_out, const void* q_weight,
+                         const sunshape_rows_t* k, const sunshape_rows_t* k_out, const void* k_weight, int32_t dtype,
+                         int32_t weight_dtype, int32_t batch, int32_t length, int32_t dim, float eps,
+                         const sunshape_rotation_t* rotation, void* stream) {
+  if (!q || !q_out) return set_last_error(SUNSHAPE_E_INVALID, "query rows descriptor is NULL.");
+  if (!k != !k_out) return set_last_error(SUNSHAPE_E_INVALID, "key rows need both an input and an output.");
+  if (!float_type(dtype)) return set_last_error(SUNSHAPE_E_INVALID, "row dtype must be F32, BF16 or F16.");
+  if ((q_weight || k_weight) && !float_type(weight_dtype))
+    return set_last_error(SUNSHAPE_E_INVALID, "norm weight dtype must be F32, BF16 or F16.");
+  if (batch < 0 || length < 0 || dim < 1 || dim > 2048)
+    return set_last_error(SUNSHAPE_E_INVALID, "batch and length must be >= 0 and the head dimension 1 to 2048.");
+  NormRotateParams p{};
+  if (int rc = make_rotation(rotation, dim, batch == 0 || length == 0, &p.rot)) return rc;
+  const sunshape_rows_t* in[2] = {q, k};
+  const sunshape_rows_t* out[2] = {q_out, k_out};
+  const int size = dtype == SUNSHAPE_F32 ? 4 : 2, unit = 16 / size;
+  bool vec = dim % 16 == 0 && dim <= 512 && p.rot.rot % 16 == 0 && ((uintptr_t)p.rot.cos | (uintptr_t)p.rot.sin) % 16 == 0;
+  p.w[0] = q_weight;
+  p.w[1] = k_weight;
+  for (int i = 0; i < 2 && in[i]; ++i) {
+    if (in[i]->heads < 0 || in[i]->heads != out[i]->heads)
+      return set_last_error(SUNSHAPE_E_INVALID, "input and output rows must have the same number of heads.");
+    if (in[i]->heads && (!in[i]->data || !out[i]->data) && batch && length)
+      return set_last_error(SUNSHAPE_E_INVALID, "rows pointer is NULL.");
+    p.x[i] = in[i]->data;
+    p.y[i] = out[i]->data;
+    p.heads[i] = in[i]->heads;
+    const int64_t a[3] = {in[i]->stride_b, in[i]->stride_h, in[i]->stride_l};
+    const int64_t b[3] = {out[i]->stride_b, out[i]->stride_h, out[i]->stride_l};
+    for (int j = 0; j < 3; ++j) {
+      p.xs[i][j] = a[j];
+      p.ys[i][j] = b[j];
+      vec = vec && a[j] % unit == 0 && b[j] % unit == 0;
+    }
+    vec = vec && ((uintptr_t)p.x[i] | (uintptr_t)p.y[i]) % 16 == 0;
+  }
+  p.tokens = (int64_t)batch * length;
+  if (p.tokens * (p.heads[0] + p.heads[1]) == 0) return SUNSHAPE_OK;
+  if (p.tokens * (p.heads[0] + p.heads[1]) > (int64_t)1 << 31)
+    return set_last_error(SUNSHAPE_E_UNSUPPORTED, "at most 2^31 rows a call.");
+  p.w_dtype = weight_dtype;
+  p.eps = eps;
+  p.L = length;
+  p.dim = dim;
+  p.err = paged_error_word();
+  if (!p.err) return set_last_error(SUNSHAPE_E_CUDA, "the paged error word is unavailable on this device.");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == SUNSHAPE_F32) launch<float>(p, vec, st);
+  else if (dtype == SUNSHAPE_BF16) launch<__nv_bfloat16>(p, vec, st);
+  else launch<__half>(p, vec, st);
+  return launch_status("norm_rotate launch");
+}
+
+}  // extern "C"

@@ -1,0 +1,70 @@
+// Arguments and helpers shared by the paged-serving kernels (norm_rotate.cu, paged_append.cu,
+// paged_attention.cu).
+#pragma once
+
+#include "common.cuh"
+
+namespace sunshape {
+
+enum PagedError { kErrPosition = 131, kErrSlot = 132, kErrPage = 133, kErrLength = 134, kErrWait = 135 };
+
+// device address of the paged kernels' error word on the current device (null with a CUDA error set)
+int* paged_error_word();
+// reports through sunshape_last_error(), capi.cu
+int set_last_error(int code, const char* msg);
+// the status of the launches just made, capi.cu
+int launch_status(const char* what);
+// argument checks shared with the contiguous entry points, capi.cu
+int check_codec_args(const sunshape_codec_t* c);
+// SMs of the current device, capi.cu
+int sm_count();
+// checks a page pool against its codec, paged_append.cu
+int check_pages(const sunshape_codec_t* c, const sunshape_pages_t* pg);
+
+// Rotation arguments as the kernels take them; rot = 0 without a rotation.
+struct Rotation {
+  const float* cos;
+  const float* sin;
+  const void* pos;
+  int64_t pos_sb, pos_sl, table_len;
+  int pos64, rot, interleaved;
+};
+
+// checks a rotation; `empty`: the call has no rows and its pointers may be null
+int make_rotation(const sunshape_rotation_t* r, int dim, bool empty, Rotation* out);
+
+// position of token (b, l); the caller checks the table's range
+__device__ __forceinline__ int64_t position_of(const Rotation& r, int64_t b, int64_t l) {
+  const int64_t i = b * r.pos_sb + l * r.pos_sl;
+  return r.pos64 ? reinterpret_cast<const int64_t*>(r.pos)[i] : (int64_t) reinterpret_cast<const int32_t*>(r.pos)[i];
+}
+
+// the other element of element d's pair, the pair's index, and whether d is the second of the two (d < rot)
+__device__ __forceinline__ void pair_of(const Rotation& r, int d, int& other, int& i, bool& second) {
+  if (r.interleaved) {
+    other = d ^ 1;
+    i = d >> 1;
+    second = d & 1;
+  } else {
+    const int half = r.rot >> 1;
+    second = d >= half;
+    other = second ? d - half : d + half;
+    i = second ? d - half : d;
+  }
+}
+
+template <typename T> struct Elem;
+template <> struct Elem<float> {
+  static __device__ __forceinline__ float to_float(float v) { return v; }
+  static __device__ __forceinline__ float from_float(float v) { return v; }
+};
+template <> struct Elem<__nv_bfloat16> {
+  static __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+  static __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
+};
+template <> struct Elem<__half> {
+  static __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+  static __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
+};
+
+}  // namespace sunshape

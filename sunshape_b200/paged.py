@@ -1,0 +1,313 @@
+"""Paged compressed cache: what a serving engine calls around the quantized-key decode path.
+
+* ``norm_rotate``: per-head RMS norms of queries and keys with the rotary position embedding, one launch;
+* ``SunShapePagedCache``: one layer's pool of pages -- codeword indices ``[num_pages, kv_heads, page_size,
+  n_blocks]`` uint8, values ``[num_pages, kv_heads, page_size, value_dim]`` and, for SunShape-Mixed codecs,
+  dense key blocks ``[num_pages, kv_heads, page_size, n_heavy, block_dim]``.  The engine owns the page
+  allocator: it hands out page numbers and names them in page tables and slots;
+* ``append_paged``: rotates, permutes and encodes new keys and copies new values into token slots, one launch
+  for a decode step's single tokens as for whole prompts;
+* ``paged_attention``: decode attention over the pages of a ragged batch, optionally behind a prefix of pages
+  that all sequences share and whose attention is computed once for all of them.
+
+Counterpart for contiguous caches: ``codec.quantize_packed`` and ``vllm_attn_backend``.  16-bit keys and values
+only (bf16, f16); ``norm_rotate`` also takes fp32.  Every call runs on the current stream of its tensors' device,
+takes no workspace that outlives it and can be captured into a CUDA graph; tensors used on another stream than
+the one they were made on need the usual ``record_stream``.  What only the device can see is checked there: a
+position, slot, page or length out of range is skipped (or makes the row NaN) and recorded, see ``paged_error``.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from .codec import SunShapeBlockCodec
+
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+_ERRORS = {131: "a position is outside the cosine/sine table", 132: "a slot is outside the page pool",
+           133: "a page number is outside the page pool", 134: "a sequence is longer than its page table",
+           135: "a pipeline wait gave up"}
+
+
+def paged_error(device: torch.device | str | None = None, clear: bool = True) -> str | None:
+    """What the paged kernels recorded on ``device`` since the last clear (None: nothing).  Waits for the device."""
+    code = ctypes.c_int32(0)
+    dev = torch.device("cuda" if device is None else device)
+    with torch.cuda.device(dev):
+        _lib._check(_lib.load_library().sunshape_paged_error(ctypes.byref(code), 1 if clear else 0))
+    return _ERRORS.get(code.value, f"error {code.value}") if code.value else None
+
+
+def rotary_table(n_positions: int, rot_dim: int, *, base: float = 10000.0,
+                 device: torch.device | str | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """cos and sin ``[n_positions, rot_dim / 2]`` fp32 of the angles ``p * base^(-2i / rot_dim)``, computed in 64 bits
+    (at position 10^5 an fp32 angle is already off by 4e-3)."""
+    inv = base ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64, device=device) / max(rot_dim, 1))
+    angle = torch.arange(n_positions, dtype=torch.float64, device=device)[:, None] * inv
+    return angle.cos().float(), angle.sin().float()
+
+
+# ------------------------------------------------------------------------------------------- argument checks
+def _rows(t: torch.Tensor, what: str) -> _lib.RowsDesc:
+    """Descriptor of [B, heads, L, dim] rows; any strides but a unit last one."""
+    if t.stride(3) != 1 and t.shape[3] != 1:
+        raise RuntimeError(f"{what}: the last axis must have unit stride.")
+    return _lib.RowsDesc(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2), t.shape[1])
+
+
+def _rotation(cos, sin, positions, interleaved, B: int, L: int, dim: int, dev) -> _lib.RotationDesc | None:
+    if cos is None and sin is None and positions is None:
+        return None
+    if cos is None or sin is None or positions is None:
+        raise RuntimeError("a rotation needs cos, sin and positions.")
+    if cos.ndim != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        raise RuntimeError("cos and sin must be fp32 tables of one shape [n_positions, rot_dim / 2].")
+    rot = 2 * cos.shape[1]
+    if rot > dim:
+        raise RuntimeError(f"cos and sin rotate {rot} elements of a head of {dim}.")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError("positions must be int32 or int64.")
+    if cos.device != dev or sin.device != dev or positions.device != dev:
+        raise RuntimeError("all sunshape_b200 inputs must live on the same CUDA device.")
+    if not (cos.is_contiguous() and sin.is_contiguous()):
+        raise RuntimeError("cos and sin must be contiguous.")
+    sb, sl = _token_strides(positions, B, L, "positions")
+    return _lib.RotationDesc(cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), sb, sl, cos.shape[0],
+                             _lib.I32 if positions.dtype == torch.int32 else _lib.I64, rot, 1 if interleaved else 0)
+
+
+def _token_strides(t: torch.Tensor, B: int, L: int, what: str) -> tuple[int, int]:
+    """Strides of a [B, L] tensor, or of one that broadcasts to it: [L], [1, L], [B, 1]."""
+    if t.ndim == 1 and t.shape[0] == L:
+        return 0, t.stride(0)
+    if t.ndim == 2 and t.shape[0] in (1, B) and t.shape[1] in (1, L):
+        return (t.stride(0) if t.shape[0] == B else 0), (t.stride(1) if t.shape[1] == L else 0)
+    raise RuntimeError(f"{what} must have shape [batch, length] (or broadcast to it), got {list(t.shape)}.")
+
+
+# ----------------------------------------------------------------------------------------- norms and rotation
+def norm_rotate(query: torch.Tensor, key: torch.Tensor | None = None, *, q_weight: torch.Tensor | None = None,
+                k_weight: torch.Tensor | None = None, eps: float = 1e-6, cos: torch.Tensor | None = None,
+                sin: torch.Tensor | None = None, positions: torch.Tensor | None = None, interleaved: bool = False,
+                out: tuple[torch.Tensor, torch.Tensor | None] | None = None):
+    """RMS norm of each query and key head, then the rotary embedding, in one launch: ``(query', key')``.
+
+    ``query`` [B, q_heads, L, D] and ``key`` [B, kv_heads, L, D] (or None) of one dtype, any strides with a unit
+    last one (views of a fused projection's output are read in place).  A weight [D] turns that tensor's norm on:
+    ``x * w / sqrt(mean(x^2) + eps)``.  ``cos``/``sin`` [n_positions, R / 2] fp32 and ``positions`` [B, L] (int32 or
+    int64; [L] broadcasts) rotate the first R <= D elements: pairs (i, i + R/2), or (2i, 2i + 1) if
+    ``interleaved``.  fp32 arithmetic, one rounding to the inputs' dtype.  ``out`` may be the inputs themselves."""
+    dev = _lib.require_cuda(query, key, q_weight, k_weight)
+    for t, what in ((query, "query"), (key, "key")):
+        if t is not None and t.ndim != 4:
+            raise RuntimeError(f"norm_rotate expects {what} with shape [batch, heads, seq, dim].")
+    if query.dtype not in _FLOATS:
+        raise RuntimeError(f"norm_rotate takes fp32, bf16 or f16 rows, got {query.dtype}.")
+    B, _, L, D = query.shape
+    if key is not None and (key.dtype != query.dtype or (key.shape[0], key.shape[2], key.shape[3]) != (B, L, D)):
+        raise RuntimeError("query and key must agree in dtype, batch, length and head dimension.")
+    if k_weight is not None and key is None:
+        raise RuntimeError("k_weight without a key.")
+    for w in (q_weight, k_weight):
+        if w is not None and (w.shape != (D,) or w.dtype not in _FLOATS or not w.is_contiguous()):
+            raise RuntimeError(f"norm weights must be contiguous fp32, bf16 or f16 tensors of shape [{D}].")
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise RuntimeError("both norm weights must have one dtype.")
+    rot = _rotation(cos, sin, positions, interleaved, B, L, D, dev)
+    if out is None:
+        q_out, k_out = torch.empty_like(query), (None if key is None else torch.empty_like(key))
+    else:
+        q_out, k_out = out
+        for t, o in ((query, q_out), (key, k_out)):
+            if (t is None) != (o is None) or (t is not None and (
+                    o.shape != t.shape or o.dtype != t.dtype or o.device != dev)):
+                raise RuntimeError("out must hold tensors of the inputs' shapes, dtype and device.")
+            if t is not None and o.data_ptr() == t.data_ptr() and o.stride() != t.stride():
+                raise RuntimeError("out over its own input needs the input's strides.")
+    w = q_weight if q_weight is not None else k_weight
+    _lib.norm_rotate(dev, _rows(query, "query"), _rows(q_out, "out"), q_weight,
+                     None if key is None else _rows(key, "key"), None if key is None else _rows(k_out, "out"), k_weight,
+                     _lib.dtype_code(query), _lib.F32 if w is None else _lib.dtype_code(w), B, L, D, eps, rot)
+    return q_out, k_out
+
+
+# ---------------------------------------------------------------------------------------------------- the cache
+class SunShapePagedCache:
+    """One layer's page pool and the codec of its keys.  ``allocate`` makes the pool, ``from_pools`` takes one."""
+
+    def __init__(self, codec: SunShapeBlockCodec, indices: torch.Tensor, values: torch.Tensor,
+                 heavy: torch.Tensor | None = None):
+        dev = _lib.require_cuda(indices, values, heavy)
+        desc, keep, n_heavy = codec.kernel_desc()
+        if keep[0].device != dev:
+            raise RuntimeError("the codec and its page pools must live on the same CUDA device.")
+        if codec.block_dim not in (2, 4, 8) or codec.n_centroids > 256:
+            raise RuntimeError("the paged cache takes block_dim 2, 4 or 8 and at most 256 codewords a block.")
+        if indices.ndim != 4 or indices.dtype != torch.uint8 or indices.shape[3] != codec.n_blocks:
+            raise RuntimeError("indices must be uint8 [num_pages, kv_heads, page_size, n_blocks].")
+        if values.ndim != 4 or values.shape[:3] != indices.shape[:3] or values.dtype not in _FLOATS[1:]:
+            raise RuntimeError("values must be bf16 or f16 [num_pages, kv_heads, page_size, value_dim].")
+        if n_heavy:
+            if heavy is None or heavy.dtype != values.dtype or heavy.shape != (
+                    *indices.shape[:3], n_heavy, codec.block_dim):
+                raise RuntimeError("a codec with dense blocks needs heavy [num_pages, kv_heads, page_size, n_heavy, "
+                                   "block_dim] of the values' dtype.")
+        elif heavy is not None:
+            raise RuntimeError("heavy pool given, but the codec has no dense blocks.")
+        if indices.shape[2] < 16 or indices.shape[2] % 16:
+            raise RuntimeError("page_size must be a multiple of 16.")
+        if values.shape[3] % 8:
+            raise RuntimeError("value_dim must be a multiple of 8.")
+        if codec.n_codebooks not in (1, indices.shape[1]):
+            raise RuntimeError(f"codec holds {codec.n_codebooks} codebooks for {indices.shape[1]} KV heads.")
+        for t in (indices, values, heavy):
+            if t is not None and (not t.is_contiguous() or t.data_ptr() % 16):
+                raise RuntimeError("page pools must be contiguous and 16-byte aligned.")
+        self.codec, self.indices, self.values, self.heavy = codec, indices, values, heavy
+        self.device = dev
+        self._pages = _lib.PagesDesc(_lib.ptr(indices), _lib.ptr(heavy), _lib.ptr(values), indices.shape[0],
+                                     indices.shape[1], indices.shape[2], values.shape[3], _lib.dtype_code(values))
+        self._image()
+
+    @classmethod
+    def from_pools(cls, codec, indices, values, heavy=None) -> "SunShapePagedCache":
+        return cls(codec, indices, values, heavy)
+
+    @classmethod
+    def allocate(cls, codec: SunShapeBlockCodec, num_pages: int, kv_heads: int, *, page_size: int = 64,
+                 value_dim: int | None = None, dtype: torch.dtype = torch.bfloat16) -> "SunShapePagedCache":
+        """Zeroed pools of ``num_pages`` pages on the codec's device."""
+        dev, shape = codec.centroids.device, (num_pages, kv_heads, page_size)
+        n_heavy = codec.kernel_desc()[2]
+        return cls(codec, torch.zeros(*shape, codec.n_blocks, dtype=torch.uint8, device=dev),
+                   torch.zeros(*shape, value_dim or codec.head_dim, dtype=dtype, device=dev),
+                   torch.zeros(*shape, n_heavy, codec.block_dim, dtype=dtype, device=dev) if n_heavy else None)
+
+    num_pages = property(lambda self: int(self.indices.shape[0]))
+    kv_heads = property(lambda self: int(self.indices.shape[1]))
+    page_size = property(lambda self: int(self.indices.shape[2]))
+    value_dim = property(lambda self: int(self.values.shape[3]))
+    dtype = property(lambda self: self.values.dtype)
+
+    def _image(self):
+        """The codec's codewords as the attention kernel reads them (kept by the codec until ``invalidate``): fp16
+        times a power of two that puts a codebook's largest codeword norm into [0.5, 1), laid out [n_cb, D / 64,
+        256, 64] so that a block's codewords all lie in one 16-byte column of the shared-memory banks."""
+        c = self.codec
+        desc, keep, _ = c.kernel_desc()
+        kept = getattr(c, "_paged_image", None)
+        if kept is None or kept[2] is not keep[0]:
+            cents, norm = keep[0], keep[3]
+            n_cb, nb, C, bd = cents.shape
+            exponent = torch.where(norm > 0, torch.frexp(norm)[1], 0).clamp(-100, 100)
+            factor = torch.ldexp(torch.ones_like(norm), -exponent)
+            full = cents.new_zeros(n_cb, nb, 256, bd)
+            full[:, :, :C] = cents * factor[:, None, None, None]
+            if c.head_dim % 64 == 0:
+                full = full.view(n_cb, c.head_dim // 64, 64 // bd, 256, bd).transpose(2, 3)
+            kept = c._paged_image = (full.to(torch.float16).contiguous(), factor.contiguous(), cents)
+        return kept
+
+    def slots(self, page_table: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
+        """Slots [B, L] of the token positions [B, L] (within their sequences) under ``page_table`` [B, cols]; -1
+        where a position is negative."""
+        p = positions.long().clamp(min=0)
+        s = page_table.long().gather(1, p // self.page_size) * self.page_size + p % self.page_size
+        return torch.where(positions >= 0, s, s.new_full((), -1))
+
+    def append(self, key, value, slots, **rotation) -> None:
+        append_paged(self, key, value, slots, **rotation)
+
+    def attention(self, query, page_table, seq_lens, **kw) -> torch.Tensor:
+        return paged_attention(self, query, page_table, seq_lens, **kw)
+
+
+def append_paged(cache: SunShapePagedCache, key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor, *,
+                 cos: torch.Tensor | None = None, sin: torch.Tensor | None = None,
+                 positions: torch.Tensor | None = None, interleaved: bool = False) -> None:
+    """Write new tokens into their slots: keys rotated (with ``cos``, ``sin`` and ``positions`` as in
+    ``norm_rotate``), permuted and encoded, values copied.
+
+    ``key`` [B, kv_heads, L, D] and ``value`` [B, kv_heads, L, value_dim] of the cache's dtype, any strides with a unit
+    last one; ``slots`` [B, L] int64, ``page * page_size + row``, -1 for rows to leave out (padding).  A flat
+    ragged batch [N, kv_heads, D] is ``key.transpose(0, 1).unsqueeze(0)`` with slots [1, N].  Slots of one call
+    must be distinct.  The codeword is the nearest to the rotated key in real arithmetic (decided in 64 bits
+    where fp32 cannot tell; lowest index on ties), without rounding the rotated key in between."""
+    codec = cache.codec
+    dev = _lib.require_cuda(key, value, slots)
+    if dev != cache.device:
+        raise RuntimeError("all sunshape_b200 inputs must live on the same CUDA device.")
+    if codec.is_metric:
+        raise RuntimeError("append_paged does not encode under a SunShape-Pro metric; encode with "
+                           "codec.quantize_packed and copy the indices into the pages.")
+    if key.ndim != 4 or value.ndim != 4:
+        raise RuntimeError("append_paged expects key and value with shape [batch, kv_heads, seq, dim].")
+    B, H, L, D = key.shape
+    if D != codec.head_dim:
+        raise RuntimeError("Key head_dim does not match codec head_dim.")
+    if H != cache.kv_heads or value.shape != (B, H, L, cache.value_dim):
+        raise RuntimeError("key and value must agree with each other and with the cache's kv_heads and value_dim.")
+    if key.dtype != cache.dtype or value.dtype != cache.dtype:
+        raise RuntimeError(f"key and value must have the cache's dtype {cache.dtype}.")
+    if slots.dtype != torch.int64 or slots.shape != (B, L):
+        raise RuntimeError("slots must be int64 [batch, length].")
+    rot = _rotation(cos, sin, positions, interleaved, B, L, D, dev)
+    _lib.paged_append(dev, codec.kernel_desc()[0], cache._pages, _rows(key, "key"), _rows(value, "value"), B, L, slots,
+                      rot)
+
+
+def paged_attention(cache: SunShapePagedCache, query: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor, *,
+                    prefix_table: torch.Tensor | None = None, prefix_len: int = 0, scale: float | None = None,
+                    causal: bool = True, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of ``query`` [B, q_heads, L, D] over a paged cache: [B, q_heads, L, value_dim].
+
+    Sequence b's own tokens are the first ``seq_lens[b]`` rows of the pages ``page_table[b]`` ([B, cols] and [B], int32,
+    on the device: lengths never visit the host).  With ``prefix_table`` [n] int32 and ``prefix_len``, the first
+    ``prefix_len`` tokens of those pages come before every sequence's own, and are read and attended to once for
+    the whole batch.  The last L tokens of a sequence are the queries' own: query l sees all but the last L - 1 -
+    l of them, unless ``causal`` is false.  A row that sees nothing is zero.  ``scale`` defaults to 1 / sqrt(D).
+
+    Softmax statistics and sums are fp32.  Codewords are read as fp16 and softmax weights rounded to the cache's
+    dtype before they multiply values; queries are scaled by powers of two into fp16's range.  Dense key blocks
+    must stay below 65504 times the largest codeword's norm."""
+    codec = cache.codec
+    dev = _lib.require_cuda(query, page_table, seq_lens, prefix_table)
+    if dev != cache.device:
+        raise RuntimeError("all sunshape_b200 inputs must live on the same CUDA device.")
+    if query.ndim != 4:
+        raise RuntimeError("paged_attention expects query with shape [batch, heads, seq, dim].")
+    B, Hq, L, D = query.shape
+    if D != codec.head_dim:
+        raise RuntimeError("Query head_dim does not match codec head_dim.")
+    if Hq % cache.kv_heads:
+        raise RuntimeError("Query head count must be divisible by kv-head count.")
+    if query.dtype != cache.dtype:
+        raise RuntimeError(f"query must have the cache's dtype {cache.dtype}.")
+    if page_table.ndim != 2 or page_table.shape[0] != B or page_table.dtype != torch.int32:
+        raise RuntimeError("page_table must be int32 [batch, pages].")
+    if page_table.shape[1] > 1 and page_table.stride(1) != 1:
+        raise RuntimeError("page_table: the last axis must have unit stride.")
+    if seq_lens.shape != (B,) or seq_lens.dtype != torch.int32 or not seq_lens.is_contiguous():
+        raise RuntimeError("seq_lens must be contiguous int32 [batch].")
+    prefix_len = int(prefix_len)
+    if prefix_len < 0 or (prefix_len and prefix_table is None):
+        raise RuntimeError("prefix_len needs a prefix_table and must not be negative.")
+    if prefix_len and (prefix_table.ndim != 1 or prefix_table.dtype != torch.int32 or not prefix_table.is_contiguous()
+                       or prefix_table.shape[0] * cache.page_size < prefix_len):
+        raise RuntimeError("prefix_table must be contiguous int32 [pages] and hold prefix_len tokens.")
+    shape = (B, Hq, L, cache.value_dim)
+    if out is None:
+        out = torch.empty(shape, dtype=query.dtype, device=dev)
+    elif out.shape != shape or out.dtype != query.dtype or out.device != dev or not out.is_contiguous():
+        raise RuntimeError("out must be contiguous [batch, q_heads, query_len, value_dim] of the query's dtype.")
+    image, factor, _ = cache._image()
+    _lib.paged_attention(dev, codec.kernel_desc()[0], cache._pages, image, factor, _rows(query, "query"), B, L, page_table,
+                         seq_lens, prefix_table if prefix_len else None, prefix_len,
+                         1.0 / math.sqrt(D) if scale is None else float(scale), causal, out)
+    return out
+
+
+__all__ = ["SunShapePagedCache", "norm_rotate", "append_paged", "paged_attention", "paged_error", "rotary_table"]
