@@ -495,6 +495,22 @@ int set_last_error(int code, const char* msg) { return fail(code, msg); }
 int launch_status(const char* what) { return cuda_status(what); }
 int check_codec_args(const sunshape_codec_t* c) { return check_codec(c); }
 int sm_count() { return num_sms(); }
+
+// Map of 16-bit rows [rows, cols], boxes of box_rows rows x 64 columns, 128-byte swizzle.
+int make_rows_map(CUtensorMap* map, const void* base, bool bf16, int cols, int64_t rows, int box_rows) {
+  auto enc = tensor_map_encoder();
+  if (!enc) return fail(SUNSHAPE_E_CUDA, "cuTensorMapEncodeTiled is unavailable from the CUDA driver.");
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)cols * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r = enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                         const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(SUNSHAPE_E_CUDA, "cuTensorMapEncodeTiled failed for the page pool.");
+  return SUNSHAPE_OK;
+}
 }  // namespace sunshape
 
 extern "C" {

@@ -1,196 +1,55 @@
-// Attention of decode steps over a paged compressed cache, with an optional prefix that the batch shares.
-//
-//   o = sum_t e^(s_t - m) v_t / sum_t e^(s_t - m),   s_t = scale <q, k_hat_t>,   m = max_t s_t
-//
-// The tokens of a sequence are cut into runs; a CTA computes (m, l, acc) of 16 query rows over one run and a
-// second kernel joins the runs of a row.
-#include "paged.cuh"
+// C entry of paged attention: checks, workspace layout, launches.
+#include "paged_attention.cuh"
 
 namespace sunshape {
 namespace {
 
-constexpr int kRows = 16;       // query rows of a CTA
-constexpr int kTile = 32;       // tokens of a step
-constexpr int kRun = 512;       // tokens of a run
-constexpr int kThreads = 128;
+constexpr int kSmemMax = 232448;    // 227 KB
 
-struct AttnParams {
-  const void* q;
-  int64_t qs[3];
-  int B, Hq, H, L, G, D, Dv, nb, bd, C, n_cb, ps, n_heavy, cols, prefix, causal, runs, mtiles;
-  int64_t num_pages, table_stride;
-  float scale;
-  const int32_t* table;
-  const int32_t* lens;
-  const int32_t* prefix_table;
-  const float* cb;
-  const int64_t* perm;
-  const uint8_t* heavy_mask;
-  const uint8_t* idx;
-  const void* heavy;
-  const void* val;
-  void* out;
-  float* part;                  // [runs][B * Hq * L][2 + Dv]
-  int* err;
+int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
+
+struct Layout {
+  int64_t slots, desc, prefix, total;
 };
 
-// length of sequence b's own tokens; -1 where the call is invalid
-__device__ __forceinline__ int own_length(const AttnParams& p, int b) {
-  const int n = p.lens[b];
-  return n < 0 || n > (int64_t)p.cols * p.ps ? -1 : n;
+Layout layout(int grid, int64_t rows, int dv, bool prefix) {
+  Layout l;
+  l.slots = 0;
+  l.desc = round256((int64_t)2 * grid * kItemRows * (dv + 2) * 4);
+  l.prefix = l.desc + round256((int64_t)grid * 16);
+  l.total = l.prefix + (prefix ? round256(rows * (dv + 2) * 4) : 0);
+  return l;
+}
+
+// Shared memory beside the ring of the memory-bound kernel.
+int fixed_smem(int d, int dv, int nb) {
+  return 1024 + d * 512 + kConsumers * kItemRows * (dv + 2) * 4 + kItemRows * (d + 8) * 2 + kItemRows * 4 + d * 4 +
+         (kPlanChunks + 1) * 8 + 8 + nb;
+}
+
+bool plan(AttnParams& p, int d, int dv, int bd) {
+  p.off_idx = kTile * dv * 2;
+  p.off_heavy = p.off_idx + kTile * p.nb;
+  p.stage_bytes = (p.off_heavy + kTile * p.n_heavy * bd * 2 + 1023) / 1024 * 1024;
+  const int fixed = fixed_smem(d, dv, p.nb);
+  p.stages = (kSmemMax - fixed) / (p.stage_bytes + 20);
+  p.smem = fixed + p.stages * (p.stage_bytes + 20);
+  return p.stages >= 2;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) attention_simple(const __grid_constant__ AttnParams p) {
-  extern __shared__ float sm[];
-  float* q_s = sm;                                  // [16][D]
-  float* k_s = q_s + kRows * p.D;                   // [32][D + 1]
-  float* v_s = k_s + kTile * (p.D + 1);             // [32][Dv]
-  float* p_s = v_s + kTile * p.Dv;                  // [16][33]
-  float* m_s = p_s + kRows * (kTile + 1);           // [16] max, sum, factor
-  float* l_s = m_s + kRows;
-  float* f_s = l_s + kRows;
-  __shared__ int64_t row_s[kTile];
-  __shared__ int bad_s;
-  const float INF = __int_as_float(0x7f800000);
-  const int tid = threadIdx.x, run = blockIdx.x, h = blockIdx.y / p.mtiles, mt = blockIdx.y % p.mtiles, b = blockIdx.z;
-  const int rows = p.G * p.L, r0 = mt * kRows, nr = min(kRows, rows - r0);
-  const int own = own_length(p, b);
-  if (own < 0 && run == 0 && tid == 0) record_error(p.err, kErrLength);
-  const int total = own < 0 ? 0 : p.prefix + own;
-  const int t0 = run * kRun, t1 = min(total, t0 + kRun);
-  if (tid == 0) bad_s = own < 0;
-  for (int i = tid; i < nr * p.D; i += kThreads) {
-    const int r = r0 + i / p.D, d = i % p.D;
-    const int hq = h * p.G + r / p.L, l = r % p.L;
-    q_s[i] = Elem<T>::to_float(reinterpret_cast<const T*>(p.q)[b * p.qs[0] + hq * p.qs[1] + l * p.qs[2] + p.perm[d]]);
+bool launch(const AttnParams& p, const CUtensorMap& vmap, int d, int dv, int bd, int grid, cudaStream_t st) {
+#define SUNSHAPE_PAGED_CASE(D, DV, BD)                       \
+  if (d == D && dv == DV && bd == BD) {                      \
+    launch_paged_attention<D, DV, BD, T>(p, vmap, grid, st); \
+    return true;                                             \
   }
-  if (tid < kRows) {
-    m_s[tid] = -INF;
-    l_s[tid] = 0.f;
-  }
-  const int per = kThreads / p.Dv == 0 ? 1 : kThreads / p.Dv;   // threads of one output column (Dv 64 or 128)
-  const int col = tid % p.Dv, rg = tid / p.Dv;
-  float acc[kRows];
-#pragma unroll
-  for (int i = 0; i < kRows; ++i) acc[i] = 0.f;
-  __syncthreads();
-  for (int t = t0; t < t1; t += kTile) {
-    const int nt = min(kTile, t1 - t);
-    if (tid < nt) {
-      const int tok = t + tid;
-      const int at = tok < p.prefix ? tok : tok - p.prefix;
-      const int page = tok < p.prefix ? p.prefix_table[at / p.ps] : p.table[b * p.table_stride + at / p.ps];
-      if (page < 0 || page >= p.num_pages) {
-        record_error(p.err, kErrPage);
-        bad_s = 1;
-        row_s[tid] = -1;
-      } else {
-        row_s[tid] = ((int64_t)page * p.H + h) * p.ps + at % p.ps;
-      }
-    }
-    __syncthreads();
-    for (int i = tid; i < nt * p.nb; i += kThreads) {
-      const int n = i / p.nb, bl = i % p.nb;
-      const int64_t row = row_s[n];
-      if (row < 0) continue;
-      float* dst = k_s + n * (p.D + 1) + bl * p.bd;
-      if (p.heavy_mask && p.heavy_mask[bl]) {
-        int at = 0;
-        for (int j = 0; j < bl; ++j) at += p.heavy_mask[j] != 0;
-        for (int w = 0; w < p.bd; ++w)
-          dst[w] = Elem<T>::to_float(reinterpret_cast<const T*>(p.heavy)[(row * p.n_heavy + at) * p.bd + w]);
-      } else {
-        const int c = min((int)p.idx[row * p.nb + bl], p.C - 1);
-        const float* src = p.cb + (((int64_t)(p.n_cb == 1 ? 0 : h % p.n_cb) * p.nb + bl) * p.C + c) * p.bd;
-        for (int w = 0; w < p.bd; ++w) dst[w] = src[w];
-      }
-    }
-    for (int i = tid; i < nt * p.Dv; i += kThreads) {
-      const int64_t row = row_s[i / p.Dv];
-      v_s[i] = row < 0 ? 0.f : Elem<T>::to_float(reinterpret_cast<const T*>(p.val)[row * p.Dv + i % p.Dv]);
-    }
-    __syncthreads();
-    for (int i = tid; i < kRows * kTile; i += kThreads) {
-      const int r = i / kTile, n = i % kTile;
-      float s = -INF;
-      // query l sees all but the last L - 1 - l of the sequence's own tokens
-      const int seen = p.prefix + (p.causal ? max(0, own - (p.L - 1 - (r0 + r) % p.L)) : own);
-      if (r < nr && n < nt && t + n < seen) {
-        s = 0.f;
-        for (int d = 0; d < p.D; ++d) s = fmaf(q_s[r * p.D + d], k_s[n * (p.D + 1) + d], s);
-        s *= p.scale * kLog2e;
-      }
-      p_s[r * (kTile + 1) + n] = s;
-    }
-    __syncthreads();
-    if (tid < kRows) {
-      float m = m_s[tid];
-      for (int n = 0; n < kTile; ++n) m = fmaxf(m, p_s[tid * (kTile + 1) + n]);
-      const float base = m == -INF ? 0.f : m;
-      float l = 0.f;
-      for (int n = 0; n < kTile; ++n) {
-        const float e = exp2f(p_s[tid * (kTile + 1) + n] - base);
-        p_s[tid * (kTile + 1) + n] = e;
-        l += e;
-      }
-      f_s[tid] = exp2f(m_s[tid] - base);
-      l_s[tid] = l_s[tid] * f_s[tid] + l;
-      m_s[tid] = m;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      if (i % per != rg) continue;
-      float a = acc[i] * f_s[i];
-      for (int n = 0; n < nt; ++n) a = fmaf(p_s[i * (kTile + 1) + n], v_s[n * p.Dv + col], a);
-      acc[i] = a;
-    }
-    __syncthreads();
-  }
-  const bool bad = bad_s != 0;
-  for (int i = 0; i < kRows; ++i) {
-    if (i >= nr || i % per != rg) continue;
-    const int r = r0 + i, hq = h * p.G + r / p.L, l = r % p.L;
-    float* dst = p.part + ((int64_t)run * p.B * p.Hq * p.L + ((int64_t)b * p.Hq + hq) * p.L + l) * (2 + p.Dv);
-    dst[2 + col] = bad ? __int_as_float(0x7fffffff) : acc[i];
-    if (col == 0) {
-      dst[0] = bad ? 0.f : m_s[i];
-      dst[1] = bad ? 1.f : l_s[i];
-    }
-  }
-}
-
-template <typename T>
-__global__ void join_simple(const __grid_constant__ AttnParams p) {
-  const float INF = __int_as_float(0x7f800000);
-  const int64_t row = blockIdx.x, rows = (int64_t)p.B * p.Hq * p.L;
-  const int own = own_length(p, (int)(row / ((int64_t)p.Hq * p.L)));
-  const int used = own < 0 ? 1 : max(1, (p.prefix + own + kRun - 1) / kRun);
-  float m = -INF;
-  for (int k = 0; k < used; ++k) m = fmaxf(m, p.part[(k * rows + row) * (2 + p.Dv)]);
-  const float base = m == -INF ? 0.f : m;
-  float l = 0.f, a = 0.f;
-  for (int k = 0; k < used; ++k) {
-    const float* src = p.part + (k * rows + row) * (2 + p.Dv);
-    const float f = exp2f(src[0] - base);
-    l = fmaf(src[1], f, l);
-    a = fmaf(src[2 + threadIdx.x], f, a);
-  }
-  reinterpret_cast<T*>(p.out)[row * p.Dv + threadIdx.x] = Elem<T>::from_float(l > 0.f ? a / l : (l == 0.f ? 0.f : l));
-}
-
-template <typename T>
-void launch(const AttnParams& p, cudaStream_t st) {
-  const int smem = (kRows * p.D + kTile * (p.D + 1) + kTile * p.Dv + kRows * (kTile + 1) + 3 * kRows) * 4;
-  cudaFuncSetAttribute(attention_simple<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  attention_simple<T><<<dim3(p.runs, p.H * p.mtiles, p.B), kThreads, smem, st>>>(p);
-  join_simple<T><<<(unsigned)((int64_t)p.B * p.Hq * p.L), p.Dv, 0, st>>>(p);
-}
-
-int64_t max_runs(int64_t cols, int64_t ps, int64_t prefix) {
-  const int64_t n = (cols * ps + prefix + kRun - 1) / kRun;
-  return n < 1 ? 1 : n;
+  SUNSHAPE_PAGED_CASE(64, 64, 2) SUNSHAPE_PAGED_CASE(64, 64, 4) SUNSHAPE_PAGED_CASE(64, 64, 8)
+  SUNSHAPE_PAGED_CASE(64, 128, 2) SUNSHAPE_PAGED_CASE(64, 128, 4) SUNSHAPE_PAGED_CASE(64, 128, 8)
+  SUNSHAPE_PAGED_CASE(128, 64, 2) SUNSHAPE_PAGED_CASE(128, 64, 4) SUNSHAPE_PAGED_CASE(128, 64, 8)
+  SUNSHAPE_PAGED_CASE(128, 128, 2) SUNSHAPE_PAGED_CASE(128, 128, 4) SUNSHAPE_PAGED_CASE(128, 128, 8)
+#undef SUNSHAPE_PAGED_CASE
+  return false;
 }
 
 }  // namespace
@@ -204,7 +63,9 @@ int64_t sunshape_paged_attention_workspace_bytes(int32_t batch, int32_t q_heads,
                                                  int32_t value_dim, int32_t table_cols, int32_t page_size,
                                                  int32_t prefix_len) {
   (void)kv_heads;
-  return max_runs(table_cols, page_size, prefix_len) * batch * q_heads * query_len * (2 + value_dim) * 4;
+  (void)table_cols;
+  (void)page_size;
+  return layout(sm_count(), (int64_t)batch * q_heads * query_len, value_dim, prefix_len > 0).total;
 }
 
 int sunshape_paged_attention(const sunshape_codec_t* codec, const sunshape_pages_t* pages, const void* codebook,
@@ -246,38 +107,54 @@ int sunshape_paged_attention(const sunshape_codec_t* codec, const sunshape_pages
   p.H = pages->kv_heads;
   p.L = query_len;
   p.G = p.Hq / p.H;
-  p.D = codec->head_dim;
-  p.Dv = pages->value_dim;
-  p.bd = codec->block_dim;
-  p.nb = p.D / p.bd;
-  p.C = codec->n_centroids;
+  const int d = codec->head_dim, dv = pages->value_dim, bd = codec->block_dim;
+  p.nb = d / bd;
   p.n_cb = codec->n_cb;
   p.ps = pages->page_size;
   p.n_heavy = codec->heavy_mask ? codec->n_heavy : 0;
   p.cols = table_cols;
-  p.prefix = prefix_len;
   p.causal = causal;
-  p.runs = (int)max_runs(table_cols, p.ps, prefix_len);
-  p.mtiles = (p.G * p.L + kRows - 1) / kRows;
+  p.chunk = p.ps % kTile ? 16 : kTile;
   p.num_pages = pages->num_pages;
   p.table_stride = table_stride;
-  p.scale = scale;
+  p.scale_log2 = scale * kLog2e;
   p.table = page_table;
   p.lens = seq_lens;
-  p.prefix_table = prefix_table;
-  p.cb = codec->centroids;
   p.perm = codec->permutation;
   p.heavy_mask = p.n_heavy ? codec->heavy_mask : nullptr;
   p.idx = pages->indices;
   p.heavy = pages->heavy;
-  p.val = pages->value;
+  p.image = codebook;
+  p.image_scale = codebook_scale;
   p.out = out;
-  p.part = static_cast<float*>(workspace);
+  const int grid = sm_count();
+  const Layout at = layout(grid, rows, dv, prefix_len > 0);
+  uint8_t* const ws = static_cast<uint8_t*>(workspace);
+  p.slots = reinterpret_cast<float*>(ws + at.slots);
+  p.desc = reinterpret_cast<int4*>(ws + at.desc);
+  p.prefix_part = reinterpret_cast<float*>(ws + at.prefix);
+  if (!plan(p, d, dv, bd)) return set_last_error(SUNSHAPE_E_UNSUPPORTED, "paged attention: too little shared memory.");
+  const int64_t pool_rows = p.num_pages * p.H * p.ps;
+  if (pool_rows > 0x7fffffff) return set_last_error(SUNSHAPE_E_UNSUPPORTED, "at most 2^31 - 1 page rows in a pool.");
+  CUtensorMap vmap{};
+  if (pool_rows)
+    if (int rc = make_rows_map(&vmap, pages->value, pages->dtype == SUNSHAPE_BF16, dv, pool_rows, p.chunk)) return rc;
   p.err = paged_error_word();
   if (!p.err) return set_last_error(SUNSHAPE_E_CUDA, "the paged error word is unavailable on this device.");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (pages->dtype == SUNSHAPE_BF16) launch<__nv_bfloat16>(p, st);
-  else launch<__half>(p, st);
+  const bool bf16 = pages->dtype == SUNSHAPE_BF16;
+  if (prefix_len) {
+    AttnParams f = p;
+    f.prefix_mode = 1;
+    f.prefix_len = prefix_len;
+    f.table = prefix_table;
+    f.table_stride = 0;
+    if (bf16) launch<__nv_bfloat16>(f, vmap, d, dv, bd, grid, st);
+    else launch<__half>(f, vmap, d, dv, bd, grid, st);
+    p.prefix_parts = 1;
+  }
+  if (bf16) launch<__nv_bfloat16>(p, vmap, d, dv, bd, grid, st);
+  else launch<__half>(p, vmap, d, dv, bd, grid, st);
   return launch_status("paged attention launch");
 }
 

@@ -1,0 +1,6 @@
+// Paged attention, head_dim 64, f16 values.
+#include "paged_attention_kernel.cuh"
+
+namespace sunshape {
+SUNSHAPE_PAGED_INSTANCES(64, __half)
+}  // namespace sunshape

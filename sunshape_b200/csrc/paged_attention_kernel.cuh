@@ -1,0 +1,588 @@
+// The memory-bound kernel of paged attention (few query rows per KV head).
+//
+// Bound by HBM: a token and KV head cost n_blocks + 2 DV bytes (+ dense blocks).  One producer warp keeps a ring
+// of tiles in flight (values by TMA with the 128-byte swizzle, index and dense-block rows by bulk copies, page
+// by page); eight consumer warps take tiles in turn, each with its own running softmax, and meet only at the
+// end of an item.
+//
+// Scores are a matrix product over rebuilt keys that never leave registers: the contraction's order is free, so
+// lane t of a quad takes whole codewords of the blocks 4u + t -- one shared-memory load of 2 BD bytes from the
+// head's codebook gives BD / 4 MMA steps of its B operand, and Q is laid out to match once per item.  Each
+// block's codewords lie in one column of the shared-memory banks, and the tokens that share a load phase walk
+// the columns in rotated order, so the random gathers are free of bank conflicts; a barrel of selects puts the
+// registers back in order.  P goes from the score accumulators to the A operand of P V without a shuffle.
+#pragma once
+
+#include <type_traits>
+
+#include "paged_attention.cuh"
+
+namespace sunshape {
+
+__device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <typename T>
+__device__ __forceinline__ void mma_pv(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value) {
+    mma_f16(c, a0, a1, a2, a3, b0, b1);
+  } else {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __half>::value) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t* r, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+
+template <int BYTES>
+__device__ __forceinline__ void lds_words(uint32_t* w, uint32_t addr) {
+  if constexpr (BYTES == 16)
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
+  else if constexpr (BYTES == 8)
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
+  else
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
+}
+
+// dense block words (two 16-bit elements each) into the codebook's fp16 scale
+template <typename T>
+__device__ __forceinline__ uint32_t dense_word(uint32_t w, float s) {
+  float lo, hi;
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 v = *reinterpret_cast<const __half2*>(&w);
+    lo = __low2float(v);
+    hi = __high2float(v);
+  } else {
+    lo = __uint_as_float(w << 16);
+    hi = __uint_as_float(w & 0xffff0000u);
+  }
+  return pack2<__half>(lo * s, hi * s);
+}
+
+// Where a CTA stands in the list of tiles; the producer and every consumer thread walk it alike.
+struct Walk {
+  int64_t at, end;       // tiles of the list
+  int h, b, mt, t;       // the item and the tile within it
+  int len, tiles;        // the sequence's length (-1: invalid) and tiles
+};
+
+template <int D, int DV, int BD, typename T>
+__global__ void __launch_bounds__(kAttnThreads, 1)
+    paged_attention_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap vmap) {
+  constexpr int NB = D / BD, UNITS = NB / 4, WORDS = BD / 2;   // units: gathers of a lane per token
+  constexpr int ROT = 16 / BD;                                 // tokens that share a load phase and a column set
+  constexpr int KS = D / 16;
+  constexpr int IMAGE = D * 512;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* const base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* const ring = base;
+  uint8_t* const image = ring + (size_t)p.stages * p.stage_bytes;
+  float* const acc_s = reinterpret_cast<float*>(image + IMAGE);              // [consumers][16][DV + 2]
+  __half* const q_s = reinterpret_cast<__half*>(acc_s + kConsumers * kItemRows * (DV + 2));   // [16][D + 8]
+  float* const qf_s = reinterpret_cast<float*>(q_s + kItemRows * (D + 8));   // [16] factor of a row's scores
+  int* const perm_s = reinterpret_cast<int*>(qf_s + kItemRows);              // [D]
+  int64_t* const cum_s = reinterpret_cast<int64_t*>(perm_s + D);             // [kPlanChunks + 1]
+  uint64_t* const full = reinterpret_cast<uint64_t*>(cum_s + kPlanChunks + 1);
+  uint64_t* const empty = full + p.stages;
+  uint64_t* const cb_bar = empty + p.stages;
+  int* const stage_bad = reinterpret_cast<int*>(cb_bar + 1);                 // [stages]
+  int8_t* const hslot_s = reinterpret_cast<int8_t*>(stage_bad + p.stages);   // [NB] dense slot, -1: codeword
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const float INF = __int_as_float(0x7f800000);
+
+  // ---- set-up and plan: prefix sums of tiles over chunks of sequences
+  if (tid == 0) {
+    for (int i = 0; i < p.stages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(cb_bar, 1);
+    fence_mbar_init();
+    int n = 0;
+    for (int b = 0; b < NB; ++b) hslot_s[b] = p.heavy_mask && p.heavy_mask[b] ? (int8_t)n++ : (int8_t)-1;
+  }
+  for (int d = tid; d < D; d += kAttnThreads) perm_s[d] = (int)p.perm[d];
+  const int seqs = p.prefix_mode ? 1 : p.B;
+  const int mtiles = (item_rows_total(p) + kItemRows - 1) / kItemRows;
+  const int per = (seqs + kPlanChunks - 1) / kPlanChunks;
+  if (tid < kPlanChunks) {
+    int64_t n = 0;
+    for (int i = tid * per; i < min(seqs, (tid + 1) * per); ++i) n += tiles_of(own_length(p, i));
+    int64_t v = n;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    cum_s[tid + 1] = v;          // within the warp's 32 chunks
+  }
+  if (tid == 0) cum_s[0] = 0;
+  __syncthreads();
+  int64_t before = 0;
+  if (tid < kPlanChunks)
+    for (int i = 0; i < warp; ++i) before += cum_s[i * 32 + 32];
+  __syncthreads();
+  if (tid < kPlanChunks) cum_s[tid + 1] += before;
+  __syncthreads();
+  const int64_t per_head = cum_s[kPlanChunks] * mtiles, total = per_head * p.H;
+  const int grid = (int)min((int64_t)gridDim.x, total), cta = blockIdx.x;
+  if (cta >= grid) {
+    if (tid == 0) p.desc[cta] = make_int4(0, -1, 0, 0);
+    return;
+  }
+  Walk w;
+  w.at = total * cta / grid;
+  w.end = total * (cta + 1) / grid;
+  {
+    w.h = (int)(w.at / per_head);
+    int64_t o = w.at - w.h * per_head;
+    int lo = 0, hi = kPlanChunks - 1;        // last chunk that begins at or before o
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (cum_s[mid] * mtiles <= o) lo = mid;
+      else hi = mid - 1;
+    }
+    o -= cum_s[lo] * mtiles;
+    w.b = lo * per;
+    w.len = own_length(p, w.b);
+    w.tiles = tiles_of(w.len);
+    while (o >= (int64_t)w.tiles * mtiles) {
+      o -= (int64_t)w.tiles * mtiles;
+      ++w.b;
+      w.len = own_length(p, w.b);
+      w.tiles = tiles_of(w.len);
+    }
+    w.mt = (int)(o / w.tiles);
+    w.t = (int)(o - (int64_t)w.mt * w.tiles);
+  }
+  auto next_item = [&](int n) {              // n: tiles of the item just walked
+    w.at += n;
+    w.t = 0;
+    if (++w.mt < mtiles) return;
+    w.mt = 0;
+    if (++w.b == seqs) {
+      w.b = 0;
+      ++w.h;
+    }
+    if (w.at < w.end) {
+      w.len = own_length(p, w.b);
+      w.tiles = tiles_of(w.len);
+    }
+  };
+
+  if (warp == kConsumers) {
+    // ------------------------------------------------------------------ producer
+    int stage = 0, phase = 0;
+    const int cpt = kTile / p.chunk;           // copies of a tile
+    const int vbytes = p.chunk * DV * 2, ibytes = p.chunk * NB, hbytes = p.chunk * p.n_heavy * BD * 2;
+    while (w.at < w.end) {
+      const int n = (int)min(w.end - w.at, (int64_t)(w.tiles - w.t));
+      const int32_t* row = p.table + (int64_t)w.b * p.table_stride;
+      int page = 0, loaded = -1;               // this lane's page of chunk group `loaded`
+      for (int i = 0; i < n; ++i) {
+        const int first = (w.t + i) * cpt;     // chunk number within the sequence
+        if (first / 32 != loaded) {
+          loaded = first / 32;
+          const int64_t tok = (int64_t)(loaded * 32 + lane) * p.chunk;
+          page = tok < w.len ? row[tok / p.ps] : -1;
+        }
+        const int pg0 = __shfl_sync(0xffffffffu, page, first & 31);
+        const int pg1 = __shfl_sync(0xffffffffu, page, (first + cpt - 1) & 31);
+        if (lane == 0) {
+          mbar_wait(&empty[stage], phase ^ 1, p.err, kErrWait);
+          uint8_t* const st = ring + (size_t)stage * p.stage_bytes;
+          int bad = w.len < 0, copies = 0;
+          int64_t rows[2] = {-1, -1};
+          for (int j = 0; j < cpt; ++j) {
+            const int64_t tok = (int64_t)(first + j) * p.chunk;
+            if (tok >= w.len) break;
+            const int pg = j ? pg1 : pg0;
+            if (pg < 0 || pg >= p.num_pages) {
+              bad = 1;
+              record_error(p.err, kErrPage);
+              continue;
+            }
+            rows[j] = ((int64_t)pg * p.H + w.h) * p.ps + tok % p.ps;
+            ++copies;
+          }
+          if (w.len < 0) record_error(p.err, kErrLength);
+          stage_bad[stage] = bad;
+          mbar_arrive_expect_tx(&full[stage], copies * (vbytes + ibytes + hbytes));
+          for (int j = 0; j < cpt; ++j) {
+            if (rows[j] < 0) continue;
+#pragma unroll
+            for (int c = 0; c < DV / 64; ++c)
+              tma_load_2d(st + c * kTile * 128 + j * p.chunk * 128, &vmap, c * 64, (int)rows[j], &full[stage]);
+            bulk_g2s(st + p.off_idx + j * ibytes, p.idx + rows[j] * NB, ibytes, &full[stage]);
+            if (hbytes)
+              bulk_g2s(st + p.off_heavy + j * hbytes,
+                       reinterpret_cast<const uint8_t*>(p.heavy) + rows[j] * p.n_heavy * BD * 2, hbytes, &full[stage]);
+          }
+        }
+        if (++stage == p.stages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+      next_item(n);
+    }
+    __syncwarp();
+    return;
+  }
+
+  // -------------------------------------------------------------------- consumers
+  const int g = lane >> 2, t = lane & 3;
+  const uint32_t image_a = smem_u32(image);
+  int head = -1, cb_phase = 0;
+  float k_scale = 1.f;
+  uint32_t hmask = 0;                          // bit u: unit u of this lane is a dense block
+  for (int u = 0; u < UNITS; ++u) hmask |= (uint32_t)(hslot_s[4 * u + t] >= 0) << u;
+  int64_t seq_tile = 0;                        // tiles of this CTA so far
+  int head_piece = 0;
+  int4 tail = make_int4(0, -1, 0, 0);
+  const int rows_total = item_rows_total(p);
+
+  while (w.at < w.end) {
+    const int n = (int)min(w.end - w.at, (int64_t)(w.tiles - w.t));
+    const int r0 = w.mt * kItemRows, nr = min(kItemRows, rows_total - r0);
+    // the head's codebook
+    if (w.h != head) {
+      const int cb = p.n_cb == 1 ? 0 : w.h % p.n_cb;
+      if (head < 0 || p.n_cb > 1) {
+        if (tid == 0) {                        // no warp reads the old codebook: the last item's barriers
+          fence_proxy_async_smem();
+          mbar_arrive_expect_tx(cb_bar, IMAGE);
+          bulk_g2s(image, reinterpret_cast<const uint8_t*>(p.image) + (int64_t)cb * IMAGE, IMAGE, cb_bar);
+        }
+        k_scale = p.image_scale[cb];
+      }
+    }
+    // queries of the item: permuted, scaled by a power of two into fp16
+    for (int r = warp; r < kItemRows; r += kConsumers) {
+      float x[D / 32], mx = 0.f;
+      if (r < nr) {
+        const RowMap at = row_of(p, w.h, w.b, r0 + r);
+        const T* src = reinterpret_cast<const T*>(p.q) + at.b * p.qs[0] + at.hq * p.qs[1] + at.l * p.qs[2];
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          x[i] = Elem<T>::to_float(src[perm_s[i * 32 + lane]]);
+          mx = fmaxf(mx, fabsf(x[i]));
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) x[i] = 0.f;
+      }
+      for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      // 2^-e with mx in [2^e, 2^(e+1)), within the exponents that have a normal reciprocal; 1 for 0, infinity
+      const int e = (__float_as_int(mx) >> 23) - 127;
+      const int ec = mx == 0.f || mx == INF ? 0 : max(-126, min(126, e));
+      const float s = __int_as_float((127 - ec) << 23);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) q_s[r * (D + 8) + i * 32 + lane] = __float2half_rn(x[i] * s);
+      if (lane == 0) qf_s[r] = p.scale_log2 * __int_as_float((127 + ec) << 23) / k_scale;
+    }
+    named_barrier(1, kConsumers * 32);
+    if (w.h != head) {
+      if (head < 0 || p.n_cb > 1) {
+        mbar_wait(cb_bar, cb_phase, p.err, kErrWait);
+        cb_phase ^= 1;
+      }
+      head = w.h;
+    }
+    uint32_t qa[KS][4];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int word = 2 * ks + i, u = word / WORDS;
+        const int d = (4 * u + t) * BD + 2 * (word % WORDS);
+        qa[ks][2 * i] = *reinterpret_cast<const uint32_t*>(q_s + g * (D + 8) + d);
+        qa[ks][2 * i + 1] = *reinterpret_cast<const uint32_t*>(q_s + (g + 8) * (D + 8) + d);
+      }
+    const float f0 = qf_s[g], f1 = qf_s[g + 8];
+    // tokens that rows g and g + 8 see
+    int seen0 = w.len, seen1 = w.len;
+    if (p.causal && p.L > 1 && !p.prefix_mode) {
+      seen0 = max(0, w.len - (p.L - 1 - (r0 + g) % p.L));
+      seen1 = max(0, w.len - (p.L - 1 - (r0 + g + 8) % p.L));
+    }
+    const int seen_all = p.causal && p.L > 1 && !p.prefix_mode ? max(0, w.len - (p.L - 1)) : w.len;
+
+    float o[DV / 8][4];
+#pragma unroll
+    for (int i = 0; i < DV / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m0 = -INF, m1 = -INF, l0 = 0.f, l1 = 0.f;
+    bool bad = false;
+    const int w0 = (int)(seq_tile % kConsumers);                   // warp of the piece's first tile
+    for (int i = (warp - w0 + kConsumers) % kConsumers; i < n; i += kConsumers) {
+      const int64_t k = seq_tile + i;
+      const int stage = (int)(k % p.stages);
+      const int first = (w.t + i) * kTile;
+      mbar_wait(&full[stage], (int)(k / p.stages) & 1, p.err, kErrWait);
+      const uint8_t* st = ring + (size_t)stage * p.stage_bytes;
+      const uint32_t st_a = smem_u32(st);
+      bad |= stage_bad[stage] != 0;
+      float s[kTile / 8][4];
+#pragma unroll
+      for (int nt = 0; nt < kTile / 8; ++nt) {
+        const int tok = nt * 8 + g;
+        uint32_t ib[UNITS];
+#pragma unroll
+        for (int u = 0; u < UNITS; u += 4) {
+          if constexpr (UNITS >= 4) lds_words<16>(ib + u, st_a + p.off_idx + tok * NB + u * 4);
+          else lds_words<8>(ib + u, st_a + p.off_idx + tok * NB + u * 4);
+        }
+        uint32_t kw[D / 8];
+        // unit u of a token with rotation r is loaded in turn (u - r) mod ROT of its group of ROT units
+        const int r = g & (ROT - 1);
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) {
+          const int u0 = u & ~(ROT - 1);
+          int uu = u0 | ((u + r) & (ROT - 1));
+          uint32_t word = 0;
+#pragma unroll
+          for (int x = 0; x < ROT; ++x)
+            if ((uu & (ROT - 1)) == x) word = ib[u0 + x];
+          const uint32_t c = (word >> (8 * t)) & 0xffu;
+          const int b = 4 * uu + t;
+          uint32_t a = image_a + ((uint32_t)(b / (64 / BD)) * 256 + c) * 128 + (b % (64 / BD)) * (2 * BD);
+          const bool dense = (hmask >> uu) & 1;
+          if (dense) a = st_a + p.off_heavy + (tok * p.n_heavy + hslot_s[b]) * (2 * BD);
+          uint32_t* dst = kw + u * WORDS;
+          lds_words<2 * BD>(dst, a);
+          if (dense) {
+#pragma unroll
+            for (int x = 0; x < WORDS; ++x) dst[x] = dense_word<T>(dst[x], k_scale);
+          }
+        }
+        // put the units back in order: rotate each group by r
+#pragma unroll
+        for (int u0 = 0; u0 < UNITS; u0 += ROT)
+#pragma unroll
+          for (int bit = 1; bit < ROT; bit <<= 1) {
+            uint32_t tmp[ROT * WORDS];
+#pragma unroll
+            for (int x = 0; x < ROT; ++x)
+#pragma unroll
+              for (int y = 0; y < WORDS; ++y)
+                tmp[x * WORDS + y] = (r & bit) ? kw[(u0 + ((x - bit) & (ROT - 1))) * WORDS + y] : kw[(u0 + x) * WORDS + y];
+#pragma unroll
+            for (int x = 0; x < ROT * WORDS; ++x) kw[u0 * WORDS + x] = tmp[x];
+          }
+        s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+          mma_f16(s[nt], qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], kw[2 * ks], kw[2 * ks + 1]);
+      }
+      // online softmax, in powers of two
+      float x0 = -INF, x1 = -INF;
+      const bool edge = first + kTile > seen_all;
+#pragma unroll
+      for (int nt = 0; nt < kTile / 8; ++nt) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          s[nt][j] *= f0;
+          s[nt][j + 2] *= f1;
+          if (edge) {
+            const int tok = first + nt * 8 + 2 * t + j;
+            if (tok >= seen0) s[nt][j] = -INF;
+            if (tok >= seen1) s[nt][j + 2] = -INF;
+          }
+          x0 = fmaxf(x0, s[nt][j]);
+          x1 = fmaxf(x1, s[nt][j + 2]);
+        }
+      }
+#pragma unroll
+      for (int of = 1; of < 4; of <<= 1) {
+        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, of));
+        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, of));
+      }
+      if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
+        const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+        const float e0 = m0 == -INF ? 0.f : fast_exp2(m0 - n0), e1 = m1 == -INF ? 0.f : fast_exp2(m1 - n1);
+        m0 = n0;
+        m1 = n1;
+        l0 *= e0;
+        l1 *= e1;
+#pragma unroll
+        for (int d = 0; d < DV / 8; ++d) {
+          o[d][0] *= e0;
+          o[d][1] *= e0;
+          o[d][2] *= e1;
+          o[d][3] *= e1;
+        }
+      }
+      const float b0 = m0 == -INF ? 0.f : m0, b1 = m1 == -INF ? 0.f : m1;
+      uint32_t pa[kTile / 8][2];
+#pragma unroll
+      for (int nt = 0; nt < kTile / 8; ++nt) {
+        const float a0 = fast_exp2(s[nt][0] - b0), a1 = fast_exp2(s[nt][1] - b0);
+        const float c0 = fast_exp2(s[nt][2] - b1), c1 = fast_exp2(s[nt][3] - b1);
+        l0 += a0 + a1;
+        l1 += c0 + c1;
+        pa[nt][0] = pack2<T>(a0, a1);
+        pa[nt][1] = pack2<T>(c0, c1);
+      }
+      const bool tail_tile = first + kTile > w.len;                 // rows behind the end hold anything
+#pragma unroll
+      for (int kk = 0; kk < kTile / 16; ++kk) {
+        const int mtok = kk * 16 + (lane & 15);                     // ldmatrix row of this lane
+        uint32_t k0 = 0xffffffffu, k1 = 0xffffffffu;
+        if (tail_tile) {
+          const int tok = first + kk * 16 + 2 * t;
+          k0 = (tok < w.len ? 0xffffu : 0u) | (tok + 1 < w.len ? 0xffff0000u : 0u);
+          k1 = (tok + 8 < w.len ? 0xffffu : 0u) | (tok + 9 < w.len ? 0xffff0000u : 0u);
+        }
+#pragma unroll
+        for (int d = 0; d < DV / 8; d += 2) {
+          const int col = d + (lane >> 4);
+          uint32_t v[4];
+          ldmatrix_x4_trans(v, st_a + (col >> 3) * (kTile * 128) + mtok * 128 + (((col & 7) ^ (mtok & 7)) << 4));
+          if (tail_tile) {
+            v[0] &= k0;
+            v[1] &= k1;
+            v[2] &= k0;
+            v[3] &= k1;
+          }
+          mma_pv<T>(o[d], pa[2 * kk][0], pa[2 * kk][1], pa[2 * kk + 1][0], pa[2 * kk + 1][1], v[0], v[1]);
+          mma_pv<T>(o[d + 1], pa[2 * kk][0], pa[2 * kk][1], pa[2 * kk + 1][0], pa[2 * kk + 1][1], v[2], v[3]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[stage]);
+    }
+    seq_tile += n;
+
+    // join the warps that took tiles of this piece
+    const int warps = min(kConsumers, n);
+    const int mine = (warp - w0 + kConsumers) % kConsumers;         // rank among them
+    if (mine < warps) {
+#pragma unroll
+      for (int of = 1; of < 4; of <<= 1) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, of);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, of);
+      }
+      if (__any_sync(0xffffffffu, bad)) l0 = l1 = m0 = m1 = __int_as_float(0x7fffffff);
+      float* dst = acc_s + (size_t)mine * kItemRows * (DV + 2);
+      if (t == 0) {
+        dst[g * (DV + 2) + DV] = m0;
+        dst[g * (DV + 2) + DV + 1] = l0;
+        dst[(g + 8) * (DV + 2) + DV] = m1;
+        dst[(g + 8) * (DV + 2) + DV + 1] = l1;
+      }
+#pragma unroll
+      for (int d = 0; d < DV / 8; ++d) {
+        *reinterpret_cast<float2*>(dst + g * (DV + 2) + d * 8 + 2 * t) = make_float2(o[d][0], o[d][1]);
+        *reinterpret_cast<float2*>(dst + (g + 8) * (DV + 2) + d * 8 + 2 * t) = make_float2(o[d][2], o[d][3]);
+      }
+    }
+    named_barrier(1, kConsumers * 32);
+    const bool begins = w.t == 0, ends = w.t + n == w.tiles;
+    float* slot = begins && ends ? nullptr : p.slots + (int64_t)(2 * cta + (begins ? 1 : 0)) * kItemRows * (DV + 2);
+    for (int e = tid; e < nr * DV; e += kConsumers * 32) {
+      const int r = e / DV, d = e % DV;
+      float M = -INF;
+      bool nan = false;
+      for (int k = 0; k < warps; ++k) {
+        const float m = acc_s[((size_t)k * kItemRows + r) * (DV + 2) + DV];
+        M = fmaxf(M, m);
+        nan |= m != m;
+      }
+      const float bs = M == -INF ? 0.f : M;
+      float l = 0.f, a = 0.f;
+      for (int k = 0; k < warps; ++k) {
+        const float* src = acc_s + ((size_t)k * kItemRows + r) * (DV + 2);
+        const float f = fast_exp2(src[DV] - bs);
+        l = fmaf(src[DV + 1], f, l);
+        a = fmaf(src[d], f, a);
+      }
+      if (nan) M = 0.f, l = a = __int_as_float(0x7fffffff);
+      if (slot) {
+        slot[r * (DV + 2) + 2 + d] = a;
+        if (d == 0) {
+          slot[r * (DV + 2)] = M;
+          slot[r * (DV + 2) + 1] = l;
+        }
+      } else {
+        finish_element<T, DV>(p, row_of(p, w.h, w.b, r0 + r), d, M, l, a);
+      }
+    }
+    if (!begins) head_piece = ends ? 2 : 1;
+    else if (!ends) tail = make_int4(0, w.h, w.b, w.mt);
+    next_item(n);
+  }
+  if (tid == 0) {
+    tail.x = head_piece;
+    p.desc[cta] = tail;
+  }
+}
+
+// Joins the pieces of items that were cut: block (c, r) takes row r of the item that begins in CTA c's range
+// and does not end there, in the order of the ranges.
+template <int DV, typename T>
+__global__ void __launch_bounds__(DV) paged_attention_join(const __grid_constant__ AttnParams p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int c = blockIdx.x, r = blockIdx.y, d = threadIdx.x;
+  const int4 tail = p.desc[c];
+  if (tail.y < 0) return;
+  const int row = tail.w * kItemRows + r;
+  if (row >= item_rows_total(p)) return;
+  int last = c + 1;
+  while (last < gridDim.x && p.desc[last].x == 1) ++last;
+  const float INF = __int_as_float(0x7f800000);
+  const float* own = p.slots + ((int64_t)(2 * c + 1) * kItemRows + r) * (DV + 2);
+  float m = own[0], l = own[1], a = own[2 + d];
+  for (int k = c + 1; k <= last && k < gridDim.x; ++k) {
+    const float* src = p.slots + ((int64_t)(2 * k) * kItemRows + r) * (DV + 2);
+    const float mk = src[0], M = fmaxf(m, mk), bs = M == -INF ? 0.f : M;
+    const float f = fast_exp2(m - bs), fk = fast_exp2(mk - bs);
+    l = l * f + src[1] * fk;
+    a = a * f + src[2 + d] * fk;
+    m = M;
+  }
+  finish_element<T, DV>(p, row_of(p, tail.y, tail.z, row), d, m, l, a);
+}
+
+template <int D, int DV, int BD, typename T>
+void launch_paged_attention(const AttnParams& p, const CUtensorMap& vmap, int grid, cudaStream_t st) {
+  auto* k = paged_attention_kernel<D, DV, BD, T>;
+  cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem);
+  k<<<grid, kAttnThreads, p.smem, st>>>(p, vmap);
+  // the join may be scheduled while the main grid drains; it waits for its end before it reads
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid, kItemRows);
+  cfg.blockDim = dim3(DV);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, paged_attention_join<DV, T>, p);
+}
+
+#define SUNSHAPE_PAGED_INSTANCE(D, DV, BD, T) \
+  template void launch_paged_attention<D, DV, BD, T>(const AttnParams&, const CUtensorMap&, int, cudaStream_t);
+#define SUNSHAPE_PAGED_INSTANCES(D, T)                                                                          \
+  SUNSHAPE_PAGED_INSTANCE(D, 64, 2, T) SUNSHAPE_PAGED_INSTANCE(D, 64, 4, T) SUNSHAPE_PAGED_INSTANCE(D, 64, 8, T) \
+  SUNSHAPE_PAGED_INSTANCE(D, 128, 2, T) SUNSHAPE_PAGED_INSTANCE(D, 128, 4, T) SUNSHAPE_PAGED_INSTANCE(D, 128, 8, T)
+
+}  // namespace sunshape
