@@ -85,7 +85,8 @@ struct Walk {
   int len, tiles;        // the sequence's length (-1: invalid) and tiles
 };
 
-template <int D, int DV, int BD, typename T>
+// R8: items have at most eight rows, the other half of the MMA's M stays zero and is left out elsewhere
+template <int D, int DV, int BD, typename T, bool R8>
 __global__ void __launch_bounds__(kAttnThreads, 1)
     paged_attention_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap vmap) {
   constexpr int NB = D / BD, UNITS = NB / 4, WORDS = BD / 2;   // units: gathers of a lane per token
@@ -190,56 +191,56 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 
   if (warp == kConsumers) {
     // ------------------------------------------------------------------ producer
+    // Each lane finds the pool row of one copy of a group of 32 (and reads the group's next page number ahead);
+    // lane 0 then only waits for a stage and issues.
     int stage = 0, phase = 0;
-    const int cpt = kTile / p.chunk;           // copies of a tile
+    const int cpt = kTile / p.chunk;           // copies of a tile, 1 or 2
     const int vbytes = p.chunk * DV * 2, ibytes = p.chunk * NB, hbytes = p.chunk * p.n_heavy * BD * 2;
+    const uint8_t* const heavy = reinterpret_cast<const uint8_t*>(p.heavy);
+    const unsigned ps = (unsigned)p.ps;
     while (w.at < w.end) {
       const int n = (int)min(w.end - w.at, (int64_t)(w.tiles - w.t));
-      const int32_t* row = p.table + (int64_t)w.b * p.table_stride;
-      int page = 0, loaded = -1;               // this lane's page of chunk group `loaded`
-      for (int i = 0; i < n; ++i) {
-        const int first = (w.t + i) * cpt;     // chunk number within the sequence
-        if (first / 32 != loaded) {
-          loaded = first / 32;
-          const int64_t tok = (int64_t)(loaded * 32 + lane) * p.chunk;
-          page = tok < w.len ? row[tok / p.ps] : -1;
-        }
-        const int pg0 = __shfl_sync(0xffffffffu, page, first & 31);
-        const int pg1 = __shfl_sync(0xffffffffu, page, (first + cpt - 1) & 31);
-        if (lane == 0) {
-          mbar_wait(&empty[stage], phase ^ 1, p.err, kErrWait);
-          uint8_t* const st = ring + (size_t)stage * p.stage_bytes;
-          int bad = w.len < 0, copies = 0;
-          int64_t rows[2] = {-1, -1};
-          for (int j = 0; j < cpt; ++j) {
-            const int64_t tok = (int64_t)(first + j) * p.chunk;
-            if (tok >= w.len) break;
-            const int pg = j ? pg1 : pg0;
-            if (pg < 0 || pg >= p.num_pages) {
-              bad = 1;
-              record_error(p.err, kErrPage);
-              continue;
-            }
-            rows[j] = ((int64_t)pg * p.H + w.h) * p.ps + tok % p.ps;
-            ++copies;
-          }
-          if (w.len < 0) record_error(p.err, kErrLength);
-          stage_bad[stage] = bad;
-          mbar_arrive_expect_tx(&full[stage], copies * (vbytes + ibytes + hbytes));
-          for (int j = 0; j < cpt; ++j) {
-            if (rows[j] < 0) continue;
+      const int32_t* table = p.table + (int64_t)w.b * p.table_stride;
+      const int c0 = w.t * cpt, c1 = (w.t + n) * cpt;      // copies of this piece
+      auto page_of_copy = [&](int c) {
+        const unsigned tok = (unsigned)c * (unsigned)p.chunk;
+        return c < c1 && (int)tok < w.len ? table[tok / ps] : -1;
+      };
+      int ahead = page_of_copy(c0 + lane);
+      if (w.len < 0 && lane == 0) record_error(p.err, kErrLength);
+      for (int cg = c0; cg < c1; cg += 32) {
+        const int page = ahead;
+        ahead = page_of_copy(cg + 32 + lane);
+        const unsigned tok = (unsigned)(cg + lane) * (unsigned)p.chunk;
+        const bool wanted = cg + lane < c1 && (int)tok < w.len;
+        const bool found = wanted && page >= 0 && page < p.num_pages;
+        if (wanted && !found) record_error(p.err, kErrPage);
+        const int row = found ? (int)(((unsigned)page * (unsigned)p.H + (unsigned)w.h) * ps + tok % ps) : (wanted ? -2 : -1);
+        const int tiles = min(32, c1 - cg) / cpt;
+        for (int i = 0; i < tiles; ++i) {
+          const int ra = __shfl_sync(0xffffffffu, row, i * cpt);
+          const int rb = cpt == 2 ? __shfl_sync(0xffffffffu, row, i * 2 + 1) : -1;
+          if (lane == 0) {
+            mbar_wait(&empty[stage], phase ^ 1, p.err, kErrWait);
+            uint8_t* const st = ring + (size_t)stage * p.stage_bytes;
+            stage_bad[stage] = w.len < 0 || ra == -2 || rb == -2;
+            mbar_arrive_expect_tx(&full[stage], ((ra >= 0) + (rb >= 0)) * (vbytes + ibytes + hbytes));
 #pragma unroll
-            for (int c = 0; c < DV / 64; ++c)
-              tma_load_2d(st + c * kTile * 128 + j * p.chunk * 128, &vmap, c * 64, (int)rows[j], &full[stage]);
-            bulk_g2s(st + p.off_idx + j * ibytes, p.idx + rows[j] * NB, ibytes, &full[stage]);
-            if (hbytes)
-              bulk_g2s(st + p.off_heavy + j * hbytes,
-                       reinterpret_cast<const uint8_t*>(p.heavy) + rows[j] * p.n_heavy * BD * 2, hbytes, &full[stage]);
+            for (int j = 0; j < 2; ++j) {
+              const int r = j ? rb : ra;
+              if (r < 0) continue;
+#pragma unroll
+              for (int c = 0; c < DV / 64; ++c)
+                tma_load_2d(st + c * kTile * 128 + j * p.chunk * 128, &vmap, c * 64, r, &full[stage]);
+              bulk_g2s(st + p.off_idx + j * ibytes, p.idx + (int64_t)r * NB, ibytes, &full[stage]);
+              if (hbytes)
+                bulk_g2s(st + p.off_heavy + j * hbytes, heavy + (int64_t)r * p.n_heavy * BD * 2, hbytes, &full[stage]);
+            }
           }
-        }
-        if (++stage == p.stages) {
-          stage = 0;
-          phase ^= 1;
+          if (++stage == p.stages) {
+            stage = 0;
+            phase ^= 1;
+          }
         }
       }
       next_item(n);
@@ -255,7 +256,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   float k_scale = 1.f;
   uint32_t hmask = 0;                          // bit u: unit u of this lane is a dense block
   for (int u = 0; u < UNITS; ++u) hmask |= (uint32_t)(hslot_s[4 * u + t] >= 0) << u;
-  int64_t seq_tile = 0;                        // tiles of this CTA so far
+  int turn = 0;                                // warp that takes the next tile of the CTA's list
+  int stage = warp % p.stages, phase = (warp / p.stages) & 1;   // stage of this warp's next tile
   int head_piece = 0;
   int4 tail = make_int4(0, -1, 0, 0);
   const int rows_total = item_rows_total(p);
@@ -276,7 +278,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       }
     }
     // queries of the item: permuted, scaled by a power of two into fp16
-    for (int r = warp; r < kItemRows; r += kConsumers) {
+    for (int r = warp; r < (R8 ? 8 : kItemRows); r += kConsumers) {
       float x[D / 32], mx = 0.f;
       if (r < nr) {
         const RowMap at = row_of(p, w.h, w.b, r0 + r);
@@ -315,9 +317,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         const int word = 2 * ks + i, u = word / WORDS;
         const int d = (4 * u + t) * BD + 2 * (word % WORDS);
         qa[ks][2 * i] = *reinterpret_cast<const uint32_t*>(q_s + g * (D + 8) + d);
-        qa[ks][2 * i + 1] = *reinterpret_cast<const uint32_t*>(q_s + (g + 8) * (D + 8) + d);
+        qa[ks][2 * i + 1] = R8 ? 0u : *reinterpret_cast<const uint32_t*>(q_s + (g + 8) * (D + 8) + d);
       }
-    const float f0 = qf_s[g], f1 = qf_s[g + 8];
+    const float f0 = qf_s[g], f1 = R8 ? 0.f : qf_s[g + 8];
     // tokens that rows g and g + 8 see
     int seen0 = w.len, seen1 = w.len;
     if (p.causal && p.L > 1 && !p.prefix_mode) {
@@ -331,12 +333,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     for (int i = 0; i < DV / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     float m0 = -INF, m1 = -INF, l0 = 0.f, l1 = 0.f;
     bool bad = false;
-    const int w0 = (int)(seq_tile % kConsumers);                   // warp of the piece's first tile
+    const int w0 = turn;                                           // warp of the piece's first tile
     for (int i = (warp - w0 + kConsumers) % kConsumers; i < n; i += kConsumers) {
-      const int64_t k = seq_tile + i;
-      const int stage = (int)(k % p.stages);
       const int first = (w.t + i) * kTile;
-      mbar_wait(&full[stage], (int)(k / p.stages) & 1, p.err, kErrWait);
+      mbar_wait(&full[stage], phase, p.err, kErrWait);
       const uint8_t* st = ring + (size_t)stage * p.stage_bytes;
       const uint32_t st_a = smem_u32(st);
       bad |= stage_bad[stage] != 0;
@@ -400,22 +400,22 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           s[nt][j] *= f0;
-          s[nt][j + 2] *= f1;
+          if constexpr (!R8) s[nt][j + 2] *= f1;
           if (edge) {
             const int tok = first + nt * 8 + 2 * t + j;
             if (tok >= seen0) s[nt][j] = -INF;
-            if (tok >= seen1) s[nt][j + 2] = -INF;
+            if (!R8 && tok >= seen1) s[nt][j + 2] = -INF;
           }
           x0 = fmaxf(x0, s[nt][j]);
-          x1 = fmaxf(x1, s[nt][j + 2]);
+          if constexpr (!R8) x1 = fmaxf(x1, s[nt][j + 2]);
         }
       }
 #pragma unroll
       for (int of = 1; of < 4; of <<= 1) {
         x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, of));
-        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, of));
+        if constexpr (!R8) x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, of));
       }
-      if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
+      if (__any_sync(0xffffffffu, x0 > m0 || (!R8 && x1 > m1))) {
         const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
         const float e0 = m0 == -INF ? 0.f : fast_exp2(m0 - n0), e1 = m1 == -INF ? 0.f : fast_exp2(m1 - n1);
         m0 = n0;
@@ -426,8 +426,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         for (int d = 0; d < DV / 8; ++d) {
           o[d][0] *= e0;
           o[d][1] *= e0;
-          o[d][2] *= e1;
-          o[d][3] *= e1;
+          if constexpr (!R8) {
+            o[d][2] *= e1;
+            o[d][3] *= e1;
+          }
         }
       }
       const float b0 = m0 == -INF ? 0.f : m0, b1 = m1 == -INF ? 0.f : m1;
@@ -435,11 +437,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 #pragma unroll
       for (int nt = 0; nt < kTile / 8; ++nt) {
         const float a0 = fast_exp2(s[nt][0] - b0), a1 = fast_exp2(s[nt][1] - b0);
-        const float c0 = fast_exp2(s[nt][2] - b1), c1 = fast_exp2(s[nt][3] - b1);
         l0 += a0 + a1;
-        l1 += c0 + c1;
         pa[nt][0] = pack2<T>(a0, a1);
-        pa[nt][1] = pack2<T>(c0, c1);
+        pa[nt][1] = 0u;
+        if constexpr (!R8) {
+          const float c0 = fast_exp2(s[nt][2] - b1), c1 = fast_exp2(s[nt][3] - b1);
+          l1 += c0 + c1;
+          pa[nt][1] = pack2<T>(c0, c1);
+        }
       }
       const bool tail_tile = first + kTile > w.len;                 // rows behind the end hold anything
 #pragma unroll
@@ -468,8 +473,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[stage]);
+      stage += kConsumers;                                          // this warp's next tile
+      while (stage >= p.stages) {
+        stage -= p.stages;
+        phase ^= 1;
+      }
     }
-    seq_tile += n;
+    turn = (turn + n) % kConsumers;
 
     // join the warps that took tiles of this piece
     const int warps = min(kConsumers, n);
@@ -485,13 +495,16 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       if (t == 0) {
         dst[g * (DV + 2) + DV] = m0;
         dst[g * (DV + 2) + DV + 1] = l0;
-        dst[(g + 8) * (DV + 2) + DV] = m1;
-        dst[(g + 8) * (DV + 2) + DV + 1] = l1;
+        if constexpr (!R8) {
+          dst[(g + 8) * (DV + 2) + DV] = m1;
+          dst[(g + 8) * (DV + 2) + DV + 1] = l1;
+        }
       }
 #pragma unroll
       for (int d = 0; d < DV / 8; ++d) {
         *reinterpret_cast<float2*>(dst + g * (DV + 2) + d * 8 + 2 * t) = make_float2(o[d][0], o[d][1]);
-        *reinterpret_cast<float2*>(dst + (g + 8) * (DV + 2) + d * 8 + 2 * t) = make_float2(o[d][2], o[d][3]);
+        if constexpr (!R8)
+          *reinterpret_cast<float2*>(dst + (g + 8) * (DV + 2) + d * 8 + 2 * t) = make_float2(o[d][2], o[d][3]);
       }
     }
     named_barrier(1, kConsumers * 32);
@@ -563,7 +576,8 @@ __global__ void __launch_bounds__(DV) paged_attention_join(const __grid_constant
 
 template <int D, int DV, int BD, typename T>
 void launch_paged_attention(const AttnParams& p, const CUtensorMap& vmap, int grid, cudaStream_t st) {
-  auto* k = paged_attention_kernel<D, DV, BD, T>;
+  const int64_t rows = p.prefix_mode ? (int64_t)p.B * p.G * p.L : (int64_t)p.G * p.L;
+  auto* k = rows <= 8 ? paged_attention_kernel<D, DV, BD, T, true> : paged_attention_kernel<D, DV, BD, T, false>;
   cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem);
   k<<<grid, kAttnThreads, p.smem, st>>>(p, vmap);
   // the join may be scheduled while the main grid drains; it waits for its end before it reads
