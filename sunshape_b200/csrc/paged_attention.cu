@@ -21,17 +21,15 @@ Layout layout(int grid, int64_t rows, int dv, bool prefix) {
   return l;
 }
 
-// Shared memory beside the ring of the memory-bound kernel.
-int fixed_smem(int d, int dv, int nb) {
-  return 1024 + d * 512 + kConsumers * kItemRows * (dv + 2) * 4 + kItemRows * (d + 8) * 2 + kItemRows * 4 + d * 4 +
-         (kPlanChunks + 1) * 8 + 8 + nb;
-}
-
+// Stages of the ring: what is left beside the codebook, the warps' results and the plan.
 bool plan(AttnParams& p, int d, int dv, int bd) {
+  const int64_t rows = (p.prefix_mode ? (int64_t)p.B : 1) * p.G * p.L;
+  p.item_rows = rows <= 8 ? 8 : 16;
   p.off_idx = kTile * dv * 2;
   p.off_heavy = p.off_idx + kTile * p.nb;
   p.stage_bytes = (p.off_heavy + kTile * p.n_heavy * bd * 2 + 1023) / 1024 * 1024;
-  const int fixed = fixed_smem(d, dv, p.nb);
+  const int fixed = 1024 + d * 512 + kConsumers * p.item_rows * (dv + 2) * 4 + p.item_rows * ((d + 8) * 2 + 4) + d * 4 +
+                    (kPlanChunks + 1) * 8 + 8 + p.nb;
   p.stages = (kSmemMax - fixed) / (p.stage_bytes + 20);
   p.smem = fixed + p.stages * (p.stage_bytes + 20);
   return p.stages >= 2;
@@ -133,7 +131,6 @@ int sunshape_paged_attention(const sunshape_codec_t* codec, const sunshape_pages
   p.slots = reinterpret_cast<float*>(ws + at.slots);
   p.desc = reinterpret_cast<int4*>(ws + at.desc);
   p.prefix_part = reinterpret_cast<float*>(ws + at.prefix);
-  if (!plan(p, d, dv, bd)) return set_last_error(SUNSHAPE_E_UNSUPPORTED, "paged attention: too little shared memory.");
   const int64_t pool_rows = p.num_pages * p.H * p.ps;
   if (pool_rows > 0x7fffffff) return set_last_error(SUNSHAPE_E_UNSUPPORTED, "at most 2^31 - 1 page rows in a pool.");
   CUtensorMap vmap{};
@@ -143,10 +140,12 @@ int sunshape_paged_attention(const sunshape_codec_t* codec, const sunshape_pages
   if (!p.err) return set_last_error(SUNSHAPE_E_CUDA, "the paged error word is unavailable on this device.");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool bf16 = pages->dtype == SUNSHAPE_BF16;
+  AttnParams f = p;
+  f.prefix_mode = 1;
+  f.prefix_len = prefix_len;
+  if (!plan(p, d, dv, bd) || !plan(f, d, dv, bd))
+    return set_last_error(SUNSHAPE_E_UNSUPPORTED, "paged attention: too little shared memory.");
   if (prefix_len) {
-    AttnParams f = p;
-    f.prefix_mode = 1;
-    f.prefix_len = prefix_len;
     f.table = prefix_table;
     f.table_stride = 0;
     if (bf16) launch<__nv_bfloat16>(f, vmap, d, dv, bd, grid, st);

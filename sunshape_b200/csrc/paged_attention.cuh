@@ -44,6 +44,7 @@ struct AttnParams {
   int4* desc;                      // [grid] (head piece: 0 none, 1 cut again, 2 last; tail item h, b, row tile) -- h -1: none
   float* prefix_part;              // [prefix_parts][B * Hq * L][2 + DV]
   int* err;
+  int item_rows;                   // 8 or 16: which kernel
   int smem;
 };
 

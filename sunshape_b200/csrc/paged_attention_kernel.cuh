@@ -5,12 +5,14 @@
 // by page); eight consumer warps take tiles in turn, each with its own running softmax, and meet only at the
 // end of an item.
 //
-// Scores are a matrix product over rebuilt keys that never leave registers: the contraction's order is free, so
-// lane t of a quad takes whole codewords of the blocks 4u + t -- one shared-memory load of 2 BD bytes from the
-// head's codebook gives BD / 4 MMA steps of its B operand, and Q is laid out to match once per item.  Each
-// block's codewords lie in one column of the shared-memory banks, and the tokens that share a load phase walk
-// the columns in rotated order, so the random gathers are free of bank conflicts; a barrel of selects puts the
-// registers back in order.  P goes from the score accumulators to the A operand of P V without a shuffle.
+// Both products are taken transposed, S^T = K Q^T and O^T = V^T P^T, so that the few query rows are the N of the
+// MMA (8 or 16 of them) and the 32 tokens fill its M.
+// S^T multiplies rebuilt keys that never leave registers: the contraction's order is free, so lane t of a quad takes
+// whole codewords of the blocks 4u + t -- one shared-memory load of 2 BD bytes from the head's codebook gives the
+// A operand of BD / 4 MMA steps, and Q is laid out to match once per item.  Each block's codewords lie in one
+// column of the shared-memory banks, and the tokens that share a load phase walk the columns in rotated order, so
+// the random gathers are free of bank conflicts; a barrel of selects puts the registers back in order.
+// P^T comes from the accumulators of S^T by a register transpose (movmatrix).
 #pragma once
 
 #include <type_traits>
@@ -47,6 +49,13 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return r;
 }
 
+// transposes an 8x8 matrix of 16-bit elements held as one MMA fragment register
+__device__ __forceinline__ uint32_t movmatrix(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
 __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t* r, uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -78,6 +87,10 @@ __device__ __forceinline__ uint32_t dense_word(uint32_t w, float s) {
   return pack2<__half>(lo * s, hi * s);
 }
 
+// A running maximum may fall behind by a factor of 2^kSlack before sums and accumulators are rescaled to a new one;
+// weights stay below 2^kSlack, in reach of every type.
+constexpr float kSlack = 8.f;
+
 // Where a CTA stands in the list of tiles; the producer and every consumer thread walk it alike.
 struct Walk {
   int64_t at, end;       // tiles of the list
@@ -85,22 +98,22 @@ struct Walk {
   int len, tiles;        // the sequence's length (-1: invalid) and tiles
 };
 
-// R8: items have at most eight rows, the other half of the MMA's M stays zero and is left out elsewhere
-template <int D, int DV, int BD, typename T, bool R8>
+// NT: groups of eight query rows of an item (1: items have at most eight rows)
+template <int D, int DV, int BD, typename T, int NT>
 __global__ void __launch_bounds__(kAttnThreads, 1)
     paged_attention_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap vmap) {
   constexpr int NB = D / BD, UNITS = NB / 4, WORDS = BD / 2;   // units: gathers of a lane per token
   constexpr int ROT = 16 / BD;                                 // tokens that share a load phase and a column set
-  constexpr int KS = D / 16;
+  constexpr int KS = D / 16, ROWS = 8 * NT;
   constexpr int IMAGE = D * 512;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* const ring = base;
   uint8_t* const image = ring + (size_t)p.stages * p.stage_bytes;
-  float* const acc_s = reinterpret_cast<float*>(image + IMAGE);              // [consumers][16][DV + 2]
-  __half* const q_s = reinterpret_cast<__half*>(acc_s + kConsumers * kItemRows * (DV + 2));   // [16][D + 8]
-  float* const qf_s = reinterpret_cast<float*>(q_s + kItemRows * (D + 8));   // [16] factor of a row's scores
-  int* const perm_s = reinterpret_cast<int*>(qf_s + kItemRows);              // [D]
+  float* const acc_s = reinterpret_cast<float*>(image + IMAGE);              // [consumers][ROWS][DV + 2]
+  __half* const q_s = reinterpret_cast<__half*>(acc_s + kConsumers * ROWS * (DV + 2));        // [ROWS][D + 8]
+  float* const qf_s = reinterpret_cast<float*>(q_s + ROWS * (D + 8));        // [ROWS] factor of a row's scores
+  int* const perm_s = reinterpret_cast<int*>(qf_s + ROWS);                   // [D]
   int64_t* const cum_s = reinterpret_cast<int64_t*>(perm_s + D);             // [kPlanChunks + 1]
   uint64_t* const full = reinterpret_cast<uint64_t*>(cum_s + kPlanChunks + 1);
   uint64_t* const empty = full + p.stages;
@@ -256,6 +269,20 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   float k_scale = 1.f;
   uint32_t hmask = 0;                          // bit u: unit u of this lane is a dense block
   for (int u = 0; u < UNITS; ++u) hmask |= (uint32_t)(hslot_s[4 * u + t] >= 0) << u;
+  const int rot = g & (ROT - 1);
+  const uint32_t byte_sel = 0x4440u | t;       // byte t of an index word
+  uint32_t col_a[UNITS];                       // codebook column of the unit that slot u loads
+#pragma unroll
+  for (int u = 0; u < UNITS; ++u) {
+    const int b = 4 * ((u & ~(ROT - 1)) | ((u + rot) & (ROT - 1))) + t;
+    col_a[u] = image_a + (b / (64 / BD)) * 32768 + (b % (64 / BD)) * (2 * BD);
+  }
+  uint32_t v_off[4];                           // this lane's ldmatrix row of 16 tokens x 16 columns, by column group
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    const int tok = ((lane >> 4) & 1) * 8 + (lane & 7);
+    v_off[d] = tok * 128 + (((2 * d + ((lane >> 3) & 1)) ^ (lane & 7)) << 4);
+  }
   int turn = 0;                                // warp that takes the next tile of the CTA's list
   int stage = warp % p.stages, phase = (warp / p.stages) & 1;   // stage of this warp's next tile
   int head_piece = 0;
@@ -277,8 +304,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         k_scale = p.image_scale[cb];
       }
     }
-    // queries of the item: permuted, scaled by a power of two into fp16
-    for (int r = warp; r < (R8 ? 8 : kItemRows); r += kConsumers) {
+    // queries of the item: permuted, scaled by a power of two into fp16; a negative scale goes into their sign, so
+    // that the factor of a row's scores is not negative and maxima can be taken before it
+    for (int r = warp; r < ROWS; r += kConsumers) {
       float x[D / 32], mx = 0.f;
       if (r < nr) {
         const RowMap at = row_of(p, w.h, w.b, r0 + r);
@@ -296,10 +324,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       // 2^-e with mx in [2^e, 2^(e+1)), within the exponents that have a normal reciprocal; 1 for 0, infinity
       const int e = (__float_as_int(mx) >> 23) - 127;
       const int ec = mx == 0.f || mx == INF ? 0 : max(-126, min(126, e));
-      const float s = __int_as_float((127 - ec) << 23);
+      const float s = copysignf(__int_as_float((127 - ec) << 23), p.scale_log2);
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) q_s[r * (D + 8) + i * 32 + lane] = __float2half_rn(x[i] * s);
-      if (lane == 0) qf_s[r] = p.scale_log2 * __int_as_float((127 + ec) << 23) / k_scale;
+      if (lane == 0) qf_s[r] = fabsf(p.scale_log2) * __int_as_float((127 + ec) << 23) / k_scale;
     }
     named_barrier(1, kConsumers * 32);
     if (w.h != head) {
@@ -309,168 +337,175 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       }
       head = w.h;
     }
-    uint32_t qa[KS][4];
+    uint32_t qb[NT][KS][2];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
+    for (int c = 0; c < NT; ++c)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int word = 2 * ks + i, u = word / WORDS;
-        const int d = (4 * u + t) * BD + 2 * (word % WORDS);
-        qa[ks][2 * i] = *reinterpret_cast<const uint32_t*>(q_s + g * (D + 8) + d);
-        qa[ks][2 * i + 1] = R8 ? 0u : *reinterpret_cast<const uint32_t*>(q_s + (g + 8) * (D + 8) + d);
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int word = 2 * ks + i, u = word / WORDS;
+          const int d = (4 * u + t) * BD + 2 * (word % WORDS);
+          qb[c][ks][i] = *reinterpret_cast<const uint32_t*>(q_s + (8 * c + g) * (D + 8) + d);
+        }
+    // this lane's rows are 8c + 2t + j: their score factors, and the tokens that each sees
+    const bool limited = p.causal && p.L > 1 && !p.prefix_mode;
+    float f[NT][2];
+    int seen[NT][2];
+#pragma unroll
+    for (int c = 0; c < NT; ++c)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        f[c][j] = qf_s[8 * c + 2 * t + j];
+        seen[c][j] = limited ? max(0, w.len - (p.L - 1 - (r0 + 8 * c + 2 * t + j) % p.L)) : w.len;
       }
-    const float f0 = qf_s[g], f1 = R8 ? 0.f : qf_s[g + 8];
-    // tokens that rows g and g + 8 see
-    int seen0 = w.len, seen1 = w.len;
-    if (p.causal && p.L > 1 && !p.prefix_mode) {
-      seen0 = max(0, w.len - (p.L - 1 - (r0 + g) % p.L));
-      seen1 = max(0, w.len - (p.L - 1 - (r0 + g + 8) % p.L));
-    }
-    const int seen_all = p.causal && p.L > 1 && !p.prefix_mode ? max(0, w.len - (p.L - 1)) : w.len;
+    const int seen_all = limited ? max(0, w.len - (p.L - 1)) : w.len;
 
-    float o[DV / 8][4];
+    float o[NT][DV / 16][4];
 #pragma unroll
-    for (int i = 0; i < DV / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m0 = -INF, m1 = -INF, l0 = 0.f, l1 = 0.f;
+    for (int c = 0; c < NT; ++c)
+#pragma unroll
+      for (int i = 0; i < DV / 16; ++i) o[c][i][0] = o[c][i][1] = o[c][i][2] = o[c][i][3] = 0.f;
+    // m: the largest score before its factor, or one that it exceeds by at most kSlack after it; mb: m, 0 for none yet
+    float m[NT][2], mb[NT][2], l[NT][2];
+#pragma unroll
+    for (int c = 0; c < NT; ++c) m[c][0] = m[c][1] = -INF, mb[c][0] = mb[c][1] = l[c][0] = l[c][1] = 0.f;
     bool bad = false;
     const int w0 = turn;                                           // warp of the piece's first tile
     for (int i = (warp - w0 + kConsumers) % kConsumers; i < n; i += kConsumers) {
       const int first = (w.t + i) * kTile;
       mbar_wait(&full[stage], phase, p.err, kErrWait);
-      const uint8_t* st = ring + (size_t)stage * p.stage_bytes;
+      uint8_t* const st = ring + (size_t)stage * p.stage_bytes;
       const uint32_t st_a = smem_u32(st);
       bad |= stage_bad[stage] != 0;
-      float s[kTile / 8][4];
+      float s[2][NT][4];
 #pragma unroll
-      for (int nt = 0; nt < kTile / 8; ++nt) {
-        const int tok = nt * 8 + g;
-        uint32_t ib[UNITS];
+      for (int mt = 0; mt < 2; ++mt) {
+        uint32_t kw[2][D / 8];
 #pragma unroll
-        for (int u = 0; u < UNITS; u += 4) {
-          if constexpr (UNITS >= 4) lds_words<16>(ib + u, st_a + p.off_idx + tok * NB + u * 4);
-          else lds_words<8>(ib + u, st_a + p.off_idx + tok * NB + u * 4);
-        }
-        uint32_t kw[D / 8];
-        // unit u of a token with rotation r is loaded in turn (u - r) mod ROT of its group of ROT units
-        const int r = g & (ROT - 1);
+        for (int y = 0; y < 2; ++y) {
+          const int tok = mt * 16 + y * 8 + g;
+          uint32_t ib[UNITS];
 #pragma unroll
-        for (int u = 0; u < UNITS; ++u) {
-          const int u0 = u & ~(ROT - 1);
-          int uu = u0 | ((u + r) & (ROT - 1));
-          uint32_t word = 0;
+          for (int u = 0; u < UNITS; u += 4) {
+            if constexpr (UNITS >= 4) lds_words<16>(ib + u, st_a + p.off_idx + tok * NB + u * 4);
+            else lds_words<8>(ib + u, st_a + p.off_idx + tok * NB + u * 4);
+          }
+          // slot u loads unit (u + r) mod ROT of its group of ROT units
 #pragma unroll
-          for (int x = 0; x < ROT; ++x)
-            if ((uu & (ROT - 1)) == x) word = ib[u0 + x];
-          const uint32_t c = (word >> (8 * t)) & 0xffu;
-          const int b = 4 * uu + t;
-          uint32_t a = image_a + ((uint32_t)(b / (64 / BD)) * 256 + c) * 128 + (b % (64 / BD)) * (2 * BD);
-          const bool dense = (hmask >> uu) & 1;
-          if (dense) a = st_a + p.off_heavy + (tok * p.n_heavy + hslot_s[b]) * (2 * BD);
-          uint32_t* dst = kw + u * WORDS;
-          lds_words<2 * BD>(dst, a);
-          if (dense) {
+          for (int u = 0; u < UNITS; ++u) {
+            uint32_t word = ib[u];
 #pragma unroll
-            for (int x = 0; x < WORDS; ++x) dst[x] = dense_word<T>(dst[x], k_scale);
+            for (int x = 1; x < ROT; ++x)
+              if (rot == x) word = ib[(u & ~(ROT - 1)) | ((u + x) & (ROT - 1))];
+            lds_words<2 * BD>(kw[y] + u * WORDS, col_a[u] + (__byte_perm(word, 0, byte_sel) << 7));
+          }
+          // put the units back in order: rotate each group by r
+#pragma unroll
+          for (int u0 = 0; u0 < UNITS; u0 += ROT)
+#pragma unroll
+            for (int bit = 1; bit < ROT; bit <<= 1) {
+              uint32_t tmp[ROT * WORDS];
+#pragma unroll
+              for (int x = 0; x < ROT; ++x)
+#pragma unroll
+                for (int z = 0; z < WORDS; ++z)
+                  tmp[x * WORDS + z] =
+                      (rot & bit) ? kw[y][(u0 + ((x - bit) & (ROT - 1))) * WORDS + z] : kw[y][(u0 + x) * WORDS + z];
+#pragma unroll
+              for (int x = 0; x < ROT * WORDS; ++x) kw[y][u0 * WORDS + x] = tmp[x];
+            }
+          if (p.n_heavy) {                       // dense blocks take the place of their codeword 0
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u)
+              if ((hmask >> u) & 1) {
+                uint32_t* dst = kw[y] + u * WORDS;
+                lds_words<2 * BD>(dst, st_a + p.off_heavy + (tok * p.n_heavy + hslot_s[4 * u + t]) * (2 * BD));
+#pragma unroll
+                for (int x = 0; x < WORDS; ++x) dst[x] = dense_word<T>(dst[x], k_scale);
+              }
           }
         }
-        // put the units back in order: rotate each group by r
 #pragma unroll
-        for (int u0 = 0; u0 < UNITS; u0 += ROT)
+        for (int c = 0; c < NT; ++c) {
+          s[mt][c][0] = s[mt][c][1] = s[mt][c][2] = s[mt][c][3] = 0.f;
 #pragma unroll
-          for (int bit = 1; bit < ROT; bit <<= 1) {
-            uint32_t tmp[ROT * WORDS];
-#pragma unroll
-            for (int x = 0; x < ROT; ++x)
-#pragma unroll
-              for (int y = 0; y < WORDS; ++y)
-                tmp[x * WORDS + y] = (r & bit) ? kw[(u0 + ((x - bit) & (ROT - 1))) * WORDS + y] : kw[(u0 + x) * WORDS + y];
-#pragma unroll
-            for (int x = 0; x < ROT * WORDS; ++x) kw[u0 * WORDS + x] = tmp[x];
-          }
-        s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-          mma_f16(s[nt], qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], kw[2 * ks], kw[2 * ks + 1]);
+          for (int ks = 0; ks < KS; ++ks)
+            mma_f16(s[mt][c], kw[0][2 * ks], kw[1][2 * ks], kw[0][2 * ks + 1], kw[1][2 * ks + 1], qb[c][ks][0], qb[c][ks][1]);
+        }
       }
       // online softmax, in powers of two
-      float x0 = -INF, x1 = -INF;
       const bool edge = first + kTile > seen_all;
+      if (edge) {
 #pragma unroll
-      for (int nt = 0; nt < kTile / 8; ++nt) {
+        for (int c = 0; c < NT; ++c)
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (first + (e >> 2) * 16 + ((e >> 1) & 1) * 8 + g >= seen[c][e & 1]) s[e >> 2][c][e & 3] = -INF;
+      }
+      bool grows = false;
+      float top[NT][2];
+#pragma unroll
+      for (int c = 0; c < NT; ++c)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          s[nt][j] *= f0;
-          if constexpr (!R8) s[nt][j + 2] *= f1;
-          if (edge) {
-            const int tok = first + nt * 8 + 2 * t + j;
-            if (tok >= seen0) s[nt][j] = -INF;
-            if (!R8 && tok >= seen1) s[nt][j + 2] = -INF;
+          top[c][j] = fmaxf(fmaxf(s[0][c][j], s[0][c][j + 2]), fmaxf(s[1][c][j], s[1][c][j + 2]));
+          grows |= m[c][j] == -INF ? top[c][j] != -INF : (top[c][j] - m[c][j]) * f[c][j] > kSlack;
+        }
+      if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+        for (int c = 0; c < NT; ++c)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float x = top[c][j];
+#pragma unroll
+            for (int of = 4; of < 32; of <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, of));
+            const float nm = fmaxf(m[c][j], x);
+            const float e = m[c][j] == -INF ? 0.f : fast_exp2((m[c][j] - nm) * f[c][j]);
+            m[c][j] = nm;
+            mb[c][j] = nm == -INF ? 0.f : nm;
+            l[c][j] *= e;
+#pragma unroll
+            for (int d = 0; d < DV / 16; ++d) {
+              o[c][d][j] *= e;
+              o[c][d][j + 2] *= e;
+            }
           }
-          x0 = fmaxf(x0, s[nt][j]);
-          if constexpr (!R8) x1 = fmaxf(x1, s[nt][j + 2]);
-        }
       }
+      uint32_t pb[2][NT][2];
 #pragma unroll
-      for (int of = 1; of < 4; of <<= 1) {
-        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, of));
-        if constexpr (!R8) x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, of));
-      }
-      if (__any_sync(0xffffffffu, x0 > m0 || (!R8 && x1 > m1))) {
-        const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
-        const float e0 = m0 == -INF ? 0.f : fast_exp2(m0 - n0), e1 = m1 == -INF ? 0.f : fast_exp2(m1 - n1);
-        m0 = n0;
-        m1 = n1;
-        l0 *= e0;
-        l1 *= e1;
+      for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-        for (int d = 0; d < DV / 8; ++d) {
-          o[d][0] *= e0;
-          o[d][1] *= e0;
-          if constexpr (!R8) {
-            o[d][2] *= e1;
-            o[d][3] *= e1;
+        for (int c = 0; c < NT; ++c) {
+          float e[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) e[x] = fast_exp2((s[mt][c][x] - mb[c][x & 1]) * f[c][x & 1]);
+          if (edge) {                            // -inf times a factor of zero
+#pragma unroll
+            for (int x = 0; x < 4; ++x) e[x] = s[mt][c][x] == -INF ? 0.f : e[x];
           }
+          l[c][0] += e[0] + e[2];
+          l[c][1] += e[1] + e[3];
+          pb[mt][c][0] = movmatrix(pack2<T>(e[0], e[1]));
+          pb[mt][c][1] = movmatrix(pack2<T>(e[2], e[3]));
         }
+      if (first + kTile > w.len) {               // rows behind the end hold anything: zero times it is not zero
+        for (int k = max(0, w.len - first) * (DV / 8) + lane; k < kTile * (DV / 8); k += 32) {
+          const int tok = k / (DV / 8), c = k % (DV / 8);
+          *reinterpret_cast<uint4*>(st + (c >> 3) * (kTile * 128) + tok * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
       }
-      const float b0 = m0 == -INF ? 0.f : m0, b1 = m1 == -INF ? 0.f : m1;
-      uint32_t pa[kTile / 8][2];
 #pragma unroll
-      for (int nt = 0; nt < kTile / 8; ++nt) {
-        const float a0 = fast_exp2(s[nt][0] - b0), a1 = fast_exp2(s[nt][1] - b0);
-        l0 += a0 + a1;
-        pa[nt][0] = pack2<T>(a0, a1);
-        pa[nt][1] = 0u;
-        if constexpr (!R8) {
-          const float c0 = fast_exp2(s[nt][2] - b1), c1 = fast_exp2(s[nt][3] - b1);
-          l1 += c0 + c1;
-          pa[nt][1] = pack2<T>(c0, c1);
-        }
-      }
-      const bool tail_tile = first + kTile > w.len;                 // rows behind the end hold anything
+      for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-      for (int kk = 0; kk < kTile / 16; ++kk) {
-        const int mtok = kk * 16 + (lane & 15);                     // ldmatrix row of this lane
-        uint32_t k0 = 0xffffffffu, k1 = 0xffffffffu;
-        if (tail_tile) {
-          const int tok = first + kk * 16 + 2 * t;
-          k0 = (tok < w.len ? 0xffffu : 0u) | (tok + 1 < w.len ? 0xffff0000u : 0u);
-          k1 = (tok + 8 < w.len ? 0xffffu : 0u) | (tok + 9 < w.len ? 0xffff0000u : 0u);
-        }
-#pragma unroll
-        for (int d = 0; d < DV / 8; d += 2) {
-          const int col = d + (lane >> 4);
+        for (int d = 0; d < DV / 16; ++d) {
           uint32_t v[4];
-          ldmatrix_x4_trans(v, st_a + (col >> 3) * (kTile * 128) + mtok * 128 + (((col & 7) ^ (mtok & 7)) << 4));
-          if (tail_tile) {
-            v[0] &= k0;
-            v[1] &= k1;
-            v[2] &= k0;
-            v[3] &= k1;
-          }
-          mma_pv<T>(o[d], pa[2 * kk][0], pa[2 * kk][1], pa[2 * kk + 1][0], pa[2 * kk + 1][1], v[0], v[1]);
-          mma_pv<T>(o[d + 1], pa[2 * kk][0], pa[2 * kk][1], pa[2 * kk + 1][0], pa[2 * kk + 1][1], v[2], v[3]);
+          ldmatrix_x4_trans(v, st_a + v_off[d & 3] + (d >> 2) * (kTile * 128) + mt * 2048);
+#pragma unroll
+          for (int c = 0; c < NT; ++c) mma_pv<T>(o[c][d], v[0], v[1], v[2], v[3], pb[mt][c][0], pb[mt][c][1]);
         }
-      }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[stage]);
       stage += kConsumers;                                          // this warp's next tile
@@ -485,27 +520,25 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     const int warps = min(kConsumers, n);
     const int mine = (warp - w0 + kConsumers) % kConsumers;         // rank among them
     if (mine < warps) {
+      bad = __any_sync(0xffffffffu, bad);
+      float* dst = acc_s + (size_t)mine * ROWS * (DV + 2);
 #pragma unroll
-      for (int of = 1; of < 4; of <<= 1) {
-        l0 += __shfl_xor_sync(0xffffffffu, l0, of);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, of);
-      }
-      if (__any_sync(0xffffffffu, bad)) l0 = l1 = m0 = m1 = __int_as_float(0x7fffffff);
-      float* dst = acc_s + (size_t)mine * kItemRows * (DV + 2);
-      if (t == 0) {
-        dst[g * (DV + 2) + DV] = m0;
-        dst[g * (DV + 2) + DV + 1] = l0;
-        if constexpr (!R8) {
-          dst[(g + 8) * (DV + 2) + DV] = m1;
-          dst[(g + 8) * (DV + 2) + DV + 1] = l1;
+      for (int c = 0; c < NT; ++c)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+          for (int of = 4; of < 32; of <<= 1) l[c][j] += __shfl_xor_sync(0xffffffffu, l[c][j], of);
+          float* to = dst + (8 * c + 2 * t + j) * (DV + 2);
+          if (g == 0) {
+            to[DV] = m[c][j] == -INF ? -INF : m[c][j] * f[c][j];
+            to[DV + 1] = bad ? __int_as_float(0x7fffffff) : l[c][j];
+          }
+#pragma unroll
+          for (int d = 0; d < DV / 16; ++d) {
+            to[d * 16 + g] = o[c][d][j];
+            to[d * 16 + 8 + g] = o[c][d][j + 2];
+          }
         }
-      }
-#pragma unroll
-      for (int d = 0; d < DV / 8; ++d) {
-        *reinterpret_cast<float2*>(dst + g * (DV + 2) + d * 8 + 2 * t) = make_float2(o[d][0], o[d][1]);
-        if constexpr (!R8)
-          *reinterpret_cast<float2*>(dst + (g + 8) * (DV + 2) + d * 8 + 2 * t) = make_float2(o[d][2], o[d][3]);
-      }
     }
     named_barrier(1, kConsumers * 32);
     const bool begins = w.t == 0, ends = w.t + n == w.tiles;
@@ -513,21 +546,15 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     for (int e = tid; e < nr * DV; e += kConsumers * 32) {
       const int r = e / DV, d = e % DV;
       float M = -INF;
-      bool nan = false;
-      for (int k = 0; k < warps; ++k) {
-        const float m = acc_s[((size_t)k * kItemRows + r) * (DV + 2) + DV];
-        M = fmaxf(M, m);
-        nan |= m != m;
-      }
+      for (int k = 0; k < warps; ++k) M = fmaxf(M, acc_s[((size_t)k * ROWS + r) * (DV + 2) + DV]);
       const float bs = M == -INF ? 0.f : M;
       float l = 0.f, a = 0.f;
       for (int k = 0; k < warps; ++k) {
-        const float* src = acc_s + ((size_t)k * kItemRows + r) * (DV + 2);
-        const float f = fast_exp2(src[DV] - bs);
-        l = fmaf(src[DV + 1], f, l);
-        a = fmaf(src[d], f, a);
+        const float* src = acc_s + ((size_t)k * ROWS + r) * (DV + 2);
+        const float e = fast_exp2(src[DV] - bs);
+        l = fmaf(src[DV + 1], e, l);
+        a = fmaf(src[d], e, a);
       }
-      if (nan) M = 0.f, l = a = __int_as_float(0x7fffffff);
       if (slot) {
         slot[r * (DV + 2) + 2 + d] = a;
         if (d == 0) {
@@ -576,8 +603,7 @@ __global__ void __launch_bounds__(DV) paged_attention_join(const __grid_constant
 
 template <int D, int DV, int BD, typename T>
 void launch_paged_attention(const AttnParams& p, const CUtensorMap& vmap, int grid, cudaStream_t st) {
-  const int64_t rows = p.prefix_mode ? (int64_t)p.B * p.G * p.L : (int64_t)p.G * p.L;
-  auto* k = rows <= 8 ? paged_attention_kernel<D, DV, BD, T, true> : paged_attention_kernel<D, DV, BD, T, false>;
+  auto* k = p.item_rows == 8 ? paged_attention_kernel<D, DV, BD, T, 1> : paged_attention_kernel<D, DV, BD, T, 2>;
   cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem);
   k<<<grid, kAttnThreads, p.smem, st>>>(p, vmap);
   // the join may be scheduled while the main grid drains; it waits for its end before it reads
