@@ -30,24 +30,23 @@ bool plan(AttnParams& p, int d, int dv, int bd) {
   p.stage_bytes = (p.off_heavy + kTile * p.n_heavy * bd * 2 + 1023) / 1024 * 1024;
   const int fixed = 1024 + d * 512 + kConsumers * p.item_rows * (dv + 2) * 4 + p.item_rows * ((d + 8) * 2 + 4) + d * 4 +
                     (kPlanChunks + 1) * 8 + 8 + p.nb;
-  p.stages = (kSmemMax - fixed) / (p.stage_bytes + 20);
+  p.stages = (kSmemMax - fixed) / (p.stage_bytes + 20) / kProducers * kProducers;
   p.smem = fixed + p.stages * (p.stage_bytes + 20);
-  return p.stages >= 2;
+  return p.stages >= kProducers;
 }
 
 template <typename T>
-bool launch(const AttnParams& p, const CUtensorMap& vmap, int d, int dv, int bd, int grid, cudaStream_t st) {
+int launch(const AttnParams& p, const CUtensorMap& vmap, int d, int dv, int bd, int grid, cudaStream_t st) {
 #define SUNSHAPE_PAGED_CASE(D, DV, BD)                       \
   if (d == D && dv == DV && bd == BD) {                      \
-    launch_paged_attention<D, DV, BD, T>(p, vmap, grid, st); \
-    return true;                                             \
+    return launch_paged_attention<D, DV, BD, T>(p, vmap, grid, st); \
   }
   SUNSHAPE_PAGED_CASE(64, 64, 2) SUNSHAPE_PAGED_CASE(64, 64, 4) SUNSHAPE_PAGED_CASE(64, 64, 8)
   SUNSHAPE_PAGED_CASE(64, 128, 2) SUNSHAPE_PAGED_CASE(64, 128, 4) SUNSHAPE_PAGED_CASE(64, 128, 8)
   SUNSHAPE_PAGED_CASE(128, 64, 2) SUNSHAPE_PAGED_CASE(128, 64, 4) SUNSHAPE_PAGED_CASE(128, 64, 8)
   SUNSHAPE_PAGED_CASE(128, 128, 2) SUNSHAPE_PAGED_CASE(128, 128, 4) SUNSHAPE_PAGED_CASE(128, 128, 8)
 #undef SUNSHAPE_PAGED_CASE
-  return false;
+  return set_last_error(SUNSHAPE_E_UNSUPPORTED, "paged attention: no kernel for these dimensions.");
 }
 
 }  // namespace
@@ -148,12 +147,12 @@ int sunshape_paged_attention(const sunshape_codec_t* codec, const sunshape_pages
   if (prefix_len) {
     f.table = prefix_table;
     f.table_stride = 0;
-    if (bf16) launch<__nv_bfloat16>(f, vmap, d, dv, bd, grid, st);
-    else launch<__half>(f, vmap, d, dv, bd, grid, st);
+    if (int rc = bf16 ? launch<__nv_bfloat16>(f, vmap, d, dv, bd, grid, st) : launch<__half>(f, vmap, d, dv, bd, grid, st))
+      return rc;
     p.prefix_parts = 1;
   }
-  if (bf16) launch<__nv_bfloat16>(p, vmap, d, dv, bd, grid, st);
-  else launch<__half>(p, vmap, d, dv, bd, grid, st);
+  if (int rc = bf16 ? launch<__nv_bfloat16>(p, vmap, d, dv, bd, grid, st) : launch<__half>(p, vmap, d, dv, bd, grid, st))
+    return rc;
   return launch_status("paged attention launch");
 }
 

@@ -17,9 +17,13 @@ namespace sunshape {
 
 constexpr int kTile = 32;          // tokens of a tile, consumed by one warp
 constexpr int kItemRows = 16;      // query rows of an item: the M of one MMA
-constexpr int kConsumers = 7;      // consumer warps: with the producer 8, so that a thread may use 255 registers
-constexpr int kAttnThreads = (kConsumers + 1) * 32;
-constexpr int kPlanChunks = kAttnThreads;   // sequence chunks of the in-kernel plan
+constexpr int kConsumers = 8;      // consumer warps, two warpgroups
+constexpr int kProducers = 4;      // producer warps, one warpgroup
+constexpr int kAttnThreads = (kConsumers + kProducers) * 32;
+// Registers of a thread: what the block is launched with, and its split between the roles (setmaxnreg).
+constexpr int kLaunchRegs = 168, kConsumerRegs = 216, kProducerRegs = 72;
+static_assert(kConsumers * kConsumerRegs + kProducers * kProducerRegs <= (kConsumers + kProducers) * kLaunchRegs, "");
+constexpr int kPlanChunks = 256;   // sequence chunks of the in-kernel plan
 
 struct AttnParams {
   const void* q;
@@ -113,6 +117,6 @@ __device__ __forceinline__ void finish_element(const AttnParams& p, const RowMap
 }
 
 template <int D, int DV, int BD, typename T>
-void launch_paged_attention(const AttnParams& p, const CUtensorMap& vmap, int grid, cudaStream_t st);
+int launch_paged_attention(const AttnParams& p, const CUtensorMap& vmap, int grid, cudaStream_t st);
 
 }  // namespace sunshape

@@ -118,8 +118,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   uint64_t* const full = reinterpret_cast<uint64_t*>(cum_s + kPlanChunks + 1);
   uint64_t* const empty = full + p.stages;
   uint64_t* const cb_bar = empty + p.stages;
-  int* const stage_bad = reinterpret_cast<int*>(cb_bar + 1);                 // [stages]
-  int8_t* const hslot_s = reinterpret_cast<int8_t*>(stage_bad + p.stages);   // [NB] dense slot, -1: codeword
+  // number of the tile that a stage holds or waits for, times 2, plus 1 where its pages are invalid
+  volatile int* const tag_s = reinterpret_cast<volatile int*>(cb_bar + 1);   // [stages]
+  int8_t* const hslot_s = reinterpret_cast<int8_t*>(cb_bar + 1) + 4 * p.stages;   // [NB] dense slot, -1: codeword
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const float INF = __int_as_float(0x7f800000);
 
@@ -128,6 +129,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     for (int i = 0; i < p.stages; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
+      tag_s[i] = -1;
     }
     mbar_init(cb_bar, 1);
     fence_mbar_init();
@@ -202,60 +204,71 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     }
   };
 
-  if (warp == kConsumers) {
-    // ------------------------------------------------------------------ producer
-    // Each lane finds the pool row of one copy of a group of 32 (and reads the group's next page number ahead);
-    // lane 0 then only waits for a stage and issues.
-    int stage = 0, phase = 0;
-    const int cpt = kTile / p.chunk;           // copies of a tile, 1 or 2
+  if (warp >= kConsumers) {
+    // ----------------------------------------------------------------- producers
+    // Producer x takes the tiles x, x + kProducers, ... of the CTA's list.  Each lane finds the pool row of one of
+    // its next 32 copies (and reads the page numbers of the 32 after them ahead); lane 0 then only waits for a
+    // stage and issues.
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
+    const int x = warp - kConsumers;
+    int stage = x, phase = 0, turn = 0, tile = x;   // stages: a multiple of the producers, so each has one of its own
+    const int two = p.chunk != kTile;          // two copies make a tile
     const int vbytes = p.chunk * DV * 2, ibytes = p.chunk * NB, hbytes = p.chunk * p.n_heavy * BD * 2;
     const uint8_t* const heavy = reinterpret_cast<const uint8_t*>(p.heavy);
     const unsigned ps = (unsigned)p.ps;
     while (w.at < w.end) {
       const int n = (int)min(w.end - w.at, (int64_t)(w.tiles - w.t));
       const int32_t* table = p.table + (int64_t)w.b * p.table_stride;
-      const int c0 = w.t * cpt, c1 = (w.t + n) * cpt;      // copies of this piece
-      auto page_of_copy = [&](int c) {
-        const unsigned tok = (unsigned)c * (unsigned)p.chunk;
-        return c < c1 && (int)tok < w.len ? table[tok / ps] : -1;
+      const int i0 = (x - turn + kProducers) % kProducers;          // first of the piece's tiles that is this warp's
+      const int mine = n > i0 ? (n - i0 + kProducers - 1) / kProducers : 0;
+      // first token of this lane's copy in the group of tiles from number j on; -1: none
+      auto token_of = [&](int j) {
+        j += lane >> two;
+        const int tok = (w.t + i0 + j * kProducers) * kTile + (two ? (lane & 1) * 16 : 0);
+        return j < mine && tok < w.len ? tok : -1;
       };
-      int ahead = page_of_copy(c0 + lane);
+      int tok = token_of(0);
+      int ahead = tok >= 0 ? table[(unsigned)tok / ps] : -1;
       if (w.len < 0 && lane == 0) record_error(p.err, kErrLength);
-      for (int cg = c0; cg < c1; cg += 32) {
+      const int group = 32 >> two;
+      for (int j = 0; j < mine; j += group) {
         const int page = ahead;
-        ahead = page_of_copy(cg + 32 + lane);
-        const unsigned tok = (unsigned)(cg + lane) * (unsigned)p.chunk;
-        const bool wanted = cg + lane < c1 && (int)tok < w.len;
-        const bool found = wanted && page >= 0 && page < p.num_pages;
-        if (wanted && !found) record_error(p.err, kErrPage);
-        const int row = found ? (int)(((unsigned)page * (unsigned)p.H + (unsigned)w.h) * ps + tok % ps) : (wanted ? -2 : -1);
-        const int tiles = min(32, c1 - cg) / cpt;
+        const bool found = tok >= 0 && page >= 0 && page < p.num_pages;
+        if (tok >= 0 && !found) record_error(p.err, kErrPage);
+        const int row =
+            found ? (int)(((unsigned)page * (unsigned)p.H + (unsigned)w.h) * ps + (unsigned)tok % ps) : (tok >= 0 ? -2 : -1);
+        tok = token_of(j + group);
+        ahead = tok >= 0 ? table[(unsigned)tok / ps] : -1;
+        const int tiles = min(group, mine - j);
         for (int i = 0; i < tiles; ++i) {
-          const int ra = __shfl_sync(0xffffffffu, row, i * cpt);
-          const int rb = cpt == 2 ? __shfl_sync(0xffffffffu, row, i * 2 + 1) : -1;
+          const int ra = __shfl_sync(0xffffffffu, row, i << two);
+          const int rb = two ? __shfl_sync(0xffffffffu, row, 2 * i + 1) : -1;
           if (lane == 0) {
             mbar_wait(&empty[stage], phase ^ 1, p.err, kErrWait);
             uint8_t* const st = ring + (size_t)stage * p.stage_bytes;
-            stage_bad[stage] = w.len < 0 || ra == -2 || rb == -2;
+            tag_s[stage] = 2 * tile + (w.len < 0 || ra == -2 || rb == -2);
             mbar_arrive_expect_tx(&full[stage], ((ra >= 0) + (rb >= 0)) * (vbytes + ibytes + hbytes));
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const int r = j ? rb : ra;
+            for (int k = 0; k < 2; ++k) {
+              const int r = k ? rb : ra;
               if (r < 0) continue;
 #pragma unroll
               for (int c = 0; c < DV / 64; ++c)
-                tma_load_2d(st + c * kTile * 128 + j * p.chunk * 128, &vmap, c * 64, r, &full[stage]);
-              bulk_g2s(st + p.off_idx + j * ibytes, p.idx + (int64_t)r * NB, ibytes, &full[stage]);
+                tma_load_2d(st + c * kTile * 128 + k * 2048, &vmap, c * 64, r, &full[stage]);
+              bulk_g2s(st + p.off_idx + k * ibytes, p.idx + (int64_t)r * NB, ibytes, &full[stage]);
               if (hbytes)
-                bulk_g2s(st + p.off_heavy + j * hbytes, heavy + (int64_t)r * p.n_heavy * BD * 2, hbytes, &full[stage]);
+                bulk_g2s(st + p.off_heavy + k * hbytes, heavy + (int64_t)r * p.n_heavy * BD * 2, hbytes, &full[stage]);
             }
           }
-          if (++stage == p.stages) {
-            stage = 0;
+          tile += kProducers;
+          stage += kProducers;
+          if (stage == p.stages + x) {
+            stage = x;
             phase ^= 1;
           }
         }
       }
+      turn = (turn + n) % kProducers;
       next_item(n);
     }
     __syncwarp();
@@ -263,6 +276,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   }
 
   // -------------------------------------------------------------------- consumers
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kConsumerRegs));
   const int g = lane >> 2, t = lane & 3;
   const uint32_t image_a = smem_u32(image);
   int head = -1, cb_phase = 0;
@@ -284,7 +298,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     v_off[d] = tok * 128 + (((2 * d + ((lane >> 3) & 1)) ^ (lane & 7)) << 4);
   }
   int turn = 0;                                // warp that takes the next tile of the CTA's list
-  int stage = warp % p.stages, phase = (warp / p.stages) & 1;   // stage of this warp's next tile
+  int stage = warp % p.stages, phase = (warp / p.stages) & 1, tile = warp;   // this warp's next tile
   int head_piece = 0;
   int4 tail = make_int4(0, -1, 0, 0);
   const int rows_total = item_rows_total(p);
@@ -374,10 +388,22 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     const int w0 = turn;                                           // warp of the piece's first tile
     for (int i = (warp - w0 + kConsumers) % kConsumers; i < n; i += kConsumers) {
       const int first = (w.t + i) * kTile;
+      // Tiles of a stage go to different warps: only the tag tells that the stage has come to this one, and that its
+      // barrier cannot be a whole turn behind, where the wait for a parity would pass at once.
+      int tag = tag_s[stage];
+      if (tag >> 1 != tile) {
+        const uint64_t t0 = global_ns();
+        while ((tag = tag_s[stage]) >> 1 != tile)
+          if (global_ns() - t0 > kWaitLimitNs) {
+            record_error(p.err, kErrWait);
+            break;
+          }
+      }
       mbar_wait(&full[stage], phase, p.err, kErrWait);
+      tile += kConsumers;
       uint8_t* const st = ring + (size_t)stage * p.stage_bytes;
       const uint32_t st_a = smem_u32(st);
-      bad |= stage_bad[stage] != 0;
+      bad |= tag & 1;
       float s[2][NT][4];
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
@@ -602,8 +628,12 @@ __global__ void __launch_bounds__(DV) paged_attention_join(const __grid_constant
 }
 
 template <int D, int DV, int BD, typename T>
-void launch_paged_attention(const AttnParams& p, const CUtensorMap& vmap, int grid, cudaStream_t st) {
+int launch_paged_attention(const AttnParams& p, const CUtensorMap& vmap, int grid, cudaStream_t st) {
+  // the split of registers waits forever where the block has fewer than it was planned for
   auto* k = p.item_rows == 8 ? paged_attention_kernel<D, DV, BD, T, 1> : paged_attention_kernel<D, DV, BD, T, 2>;
+  cudaFuncAttributes fa;
+  if (cudaFuncGetAttributes(&fa, k) != cudaSuccess || fa.numRegs != kLaunchRegs)
+    return set_last_error(SUNSHAPE_E_CUDA, "paged attention kernel was built for another register count.");
   cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem);
   k<<<grid, kAttnThreads, p.smem, st>>>(p, vmap);
   // the join may be scheduled while the main grid drains; it waits for its end before it reads
@@ -617,10 +647,11 @@ void launch_paged_attention(const AttnParams& p, const CUtensorMap& vmap, int gr
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   cudaLaunchKernelEx(&cfg, paged_attention_join<DV, T>, p);
+  return SUNSHAPE_OK;
 }
 
 #define SUNSHAPE_PAGED_INSTANCE(D, DV, BD, T) \
-  template void launch_paged_attention<D, DV, BD, T>(const AttnParams&, const CUtensorMap&, int, cudaStream_t);
+  template int launch_paged_attention<D, DV, BD, T>(const AttnParams&, const CUtensorMap&, int, cudaStream_t);
 #define SUNSHAPE_PAGED_INSTANCES(D, T)                                                                          \
   SUNSHAPE_PAGED_INSTANCE(D, 64, 2, T) SUNSHAPE_PAGED_INSTANCE(D, 64, 4, T) SUNSHAPE_PAGED_INSTANCE(D, 64, 8, T) \
   SUNSHAPE_PAGED_INSTANCE(D, 128, 2, T) SUNSHAPE_PAGED_INSTANCE(D, 128, 4, T) SUNSHAPE_PAGED_INSTANCE(D, 128, 8, T)
