@@ -1,4 +1,6 @@
 // C entry of paged attention: checks, workspace layout, launches.
+#include <algorithm>
+
 #include "paged_attention.cuh"
 
 namespace sunshape {
@@ -9,30 +11,40 @@ constexpr int kSmemMax = 232448;    // 227 KB
 int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
 
 struct Layout {
-  int64_t slots, desc, prefix, total;
+  int64_t slots, desc, pieces, prefix, total;
 };
 
-Layout layout(int grid, int64_t rows, int dv, bool prefix) {
+Layout layout(int grid, int64_t rows, int64_t item_rows, int dv, bool prefix) {
+  const int64_t row = row_floats(dv) * 4;
   Layout l;
   l.slots = 0;
-  l.desc = round256((int64_t)2 * grid * kItemRows * (dv + 2) * 4);
-  l.prefix = l.desc + round256((int64_t)grid * 16);
-  l.total = l.prefix + (prefix ? round256(rows * (dv + 2) * 4) : 0);
+  l.desc = round256(2 * grid * kItemRows * row);
+  l.pieces = l.desc + round256((int64_t)grid * 16);
+  l.prefix = l.pieces + round256((int64_t)grid * kPairs * 2 * item_rows * row);
+  l.total = l.prefix + (prefix ? round256(rows * row) : 0);
   return l;
 }
 
-// Stages of the ring: what is left beside the codebook, the warps' results and the plan.
+// 8 or 16 query rows an item
+int item_rows(int64_t rows) { return rows <= 8 ? 8 : 16; }
+
+// Stages of the rings: what is left beside the codebook and the plan, at least two for each pair of warps that works.
 bool plan(AttnParams& p, int d, int dv, int bd) {
-  const int64_t rows = (p.prefix_mode ? (int64_t)p.B : 1) * p.G * p.L;
-  p.item_rows = rows <= 8 ? 8 : 16;
+  p.item_rows = item_rows((p.prefix_mode ? (int64_t)p.B : 1) * p.G * p.L);
   p.off_idx = kTile * dv * 2;
   p.off_heavy = p.off_idx + kTile * p.nb;
-  p.stage_bytes = (p.off_heavy + kTile * p.n_heavy * bd * 2 + 1023) / 1024 * 1024;
-  const int fixed = 1024 + d * 512 + kConsumers * p.item_rows * (dv + 2) * 4 + p.item_rows * ((d + 8) * 2 + 4) + d * 4 +
-                    (kPlanChunks + 1) * 8 + 8 + p.nb;
-  p.stages = (kSmemMax - fixed) / (p.stage_bytes + 20) / kProducers * kProducers;
-  p.smem = fixed + p.stages * (p.stage_bytes + 20);
-  return p.stages >= kProducers;
+  p.stage_bytes = (p.off_heavy + kTile * p.n_heavy * bd * 2 + 4 + 1023) / 1024 * 1024;
+  // alignment, codebook, permutation, plan, codebook barrier, pieces' descriptions, dense slots
+  const int fixed = 1024 + d * 512 + d * 4 + (kPlanChunks + 1) * 8 + 8 + 16 + kPairs * 32 + p.nb;
+  const int left = kSmemMax - fixed;
+  p.stages = std::min(6, left / (kPairs * (p.stage_bytes + 16)));
+  p.pairs = kPairs;
+  if (p.stages < 2) {
+    p.stages = 2;
+    p.pairs = (left - kPairs * 2 * 16) / (2 * p.stage_bytes);
+  }
+  p.smem = fixed + p.pairs * p.stages * p.stage_bytes + kPairs * p.stages * 16;
+  return p.pairs >= 1;
 }
 
 template <typename T>
@@ -59,10 +71,11 @@ extern "C" {
 int64_t sunshape_paged_attention_workspace_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t query_len,
                                                  int32_t value_dim, int32_t table_cols, int32_t page_size,
                                                  int32_t prefix_len) {
-  (void)kv_heads;
   (void)table_cols;
   (void)page_size;
-  return layout(sm_count(), (int64_t)batch * q_heads * query_len, value_dim, prefix_len > 0).total;
+  const int64_t rows = (int64_t)batch * q_heads * query_len;
+  const int64_t own = kv_heads > 0 ? (int64_t)q_heads / kv_heads * query_len : 0;
+  return layout(sm_count(), rows, item_rows(prefix_len > 0 ? own * batch : own), value_dim, prefix_len > 0).total;
 }
 
 int sunshape_paged_attention(const sunshape_codec_t* codec, const sunshape_pages_t* pages, const void* codebook,
@@ -125,10 +138,11 @@ int sunshape_paged_attention(const sunshape_codec_t* codec, const sunshape_pages
   p.image_scale = codebook_scale;
   p.out = out;
   const int grid = sm_count();
-  const Layout at = layout(grid, rows, dv, prefix_len > 0);
+  const Layout at = layout(grid, rows, item_rows((prefix_len ? (int64_t)p.B : 1) * p.G * p.L), dv, prefix_len > 0);
   uint8_t* const ws = static_cast<uint8_t*>(workspace);
   p.slots = reinterpret_cast<float*>(ws + at.slots);
   p.desc = reinterpret_cast<int4*>(ws + at.desc);
+  p.pieces = reinterpret_cast<float*>(ws + at.pieces);
   p.prefix_part = reinterpret_cast<float*>(ws + at.prefix);
   const int64_t pool_rows = p.num_pages * p.H * p.ps;
   if (pool_rows > 0x7fffffff) return set_last_error(SUNSHAPE_E_UNSUPPORTED, "at most 2^31 - 1 page rows in a pool.");

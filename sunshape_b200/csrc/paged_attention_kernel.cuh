@@ -1,9 +1,10 @@
 // The memory-bound kernel of paged attention (few query rows per KV head).
 //
-// Bound by HBM: a token and KV head cost n_blocks + 2 DV bytes (+ dense blocks).  One producer warp keeps a ring
-// of tiles in flight (values by TMA with the 128-byte swizzle, index and dense-block rows by bulk copies, page
-// by page); eight consumer warps take tiles in turn, each with its own running softmax, and meet only at the
-// end of an item.
+// Bound by HBM: a token and KV head cost n_blocks + 2 DV bytes (+ dense blocks).  Each producer warp keeps its
+// consumer's ring of tiles in flight (values by TMA with the 128-byte swizzle, index and dense-block rows by bulk
+// copies, page by page); one producer per consumer, since one warp takes about 670 cycles to look up, wait for and
+// issue a tile, and HBM delivers one to an SM in 380.  A pair's ring is its own, so a wait for a parity can not
+// pass a turn too early.
 //
 // Both products are taken transposed, S^T = K Q^T and O^T = V^T P^T, so that the few query rows are the N of the
 // MMA (8 or 16 of them) and the 32 tokens fill its M.
@@ -91,7 +92,7 @@ __device__ __forceinline__ uint32_t dense_word(uint32_t w, float s) {
 // weights stay below 2^kSlack, in reach of every type.
 constexpr float kSlack = 8.f;
 
-// Where a CTA stands in the list of tiles; the producer and every consumer thread walk it alike.
+// Where a pair stands in the list; its producer and its consumer walk it alike.
 struct Walk {
   int64_t at, end;       // tiles of the list
   int h, b, mt, t;       // the item and the tile within it
@@ -104,51 +105,46 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     paged_attention_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap vmap) {
   constexpr int NB = D / BD, UNITS = NB / 4, WORDS = BD / 2;   // units: gathers of a lane per token
   constexpr int ROT = 16 / BD;                                 // tokens that share a load phase and a column set
-  constexpr int KS = D / 16, ROWS = 8 * NT;
+  constexpr int KS = D / 16, ROWS = 8 * NT, RF = row_floats(DV);
   constexpr int IMAGE = D * 512;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* const base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* const ring = base;
-  uint8_t* const image = ring + (size_t)p.stages * p.stage_bytes;
-  float* const acc_s = reinterpret_cast<float*>(image + IMAGE);              // [consumers][ROWS][DV + 2]
-  __half* const q_s = reinterpret_cast<__half*>(acc_s + kConsumers * ROWS * (DV + 2));        // [ROWS][D + 8]
-  float* const qf_s = reinterpret_cast<float*>(q_s + ROWS * (D + 8));        // [ROWS] factor of a row's scores
-  int* const perm_s = reinterpret_cast<int*>(qf_s + ROWS);                   // [D]
+  uint8_t* const ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int ring_bytes = p.stages * p.stage_bytes;             // of a pair
+  uint8_t* const image = ring + (size_t)p.pairs * ring_bytes;
+  int* const perm_s = reinterpret_cast<int*>(image + IMAGE);                 // [D]
   int64_t* const cum_s = reinterpret_cast<int64_t*>(perm_s + D);             // [kPlanChunks + 1]
-  uint64_t* const full = reinterpret_cast<uint64_t*>(cum_s + kPlanChunks + 1);
-  uint64_t* const empty = full + p.stages;
-  uint64_t* const cb_bar = empty + p.stages;
-  // number of the tile that a stage holds or waits for, times 2, plus 1 where its pages are invalid
-  volatile int* const tag_s = reinterpret_cast<volatile int*>(cb_bar + 1);   // [stages]
-  int8_t* const hslot_s = reinterpret_cast<int8_t*>(cb_bar + 1) + 4 * p.stages;   // [NB] dense slot, -1: codeword
+  uint64_t* const full_s = reinterpret_cast<uint64_t*>(cum_s + kPlanChunks + 1);   // [kPairs][stages]
+  uint64_t* const empty_s = full_s + kPairs * p.stages;
+  uint64_t* const cb_bar = empty_s + kPairs * p.stages;
+  // of a pair: head piece (-1: no tiles, 0: none, 1: cut again, 2: last), its item; tail piece (0, 1), its item
+  int4* const head_s = reinterpret_cast<int4*>((reinterpret_cast<uintptr_t>(cb_bar + 1) + 15) & ~uintptr_t(15));
+  int4* const tail_s = head_s + kPairs;
+  int8_t* const hslot_s = reinterpret_cast<int8_t*>(tail_s + kPairs);        // [NB] dense slot, -1: codeword
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const float INF = __int_as_float(0x7f800000);
 
   // ---- set-up and plan: prefix sums of tiles over chunks of sequences
   if (tid == 0) {
-    for (int i = 0; i < p.stages; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
-      tag_s[i] = -1;
-    }
-    mbar_init(cb_bar, 1);
+    for (int i = 0; i < 2 * kPairs * p.stages + 1; ++i) mbar_init(&full_s[i], 1);
     fence_mbar_init();
+  } else if (tid == kAttnThreads - 1) {
     int n = 0;
     for (int b = 0; b < NB; ++b) hslot_s[b] = p.heavy_mask && p.heavy_mask[b] ? (int8_t)n++ : (int8_t)-1;
   }
-  for (int d = tid; d < D; d += kAttnThreads) perm_s[d] = (int)p.perm[d];
+  if (tid >= kPlanChunks)
+    for (int d = tid - kPlanChunks; d < D; d += kAttnThreads - kPlanChunks) perm_s[d] = (int)p.perm[d];
   const int seqs = p.prefix_mode ? 1 : p.B;
-  const int mtiles = (item_rows_total(p) + kItemRows - 1) / kItemRows;
+  const int rows_total = item_rows_total(p);
+  const int mtiles = (rows_total + ROWS - 1) / ROWS;
   const int per = (seqs + kPlanChunks - 1) / kPlanChunks;
   if (tid < kPlanChunks) {
     int64_t n = 0;
     for (int i = tid * per; i < min(seqs, (tid + 1) * per); ++i) n += tiles_of(own_length(p, i));
-    int64_t v = n;
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v += u;
+      const int64_t u = __shfl_up_sync(0xffffffffu, n, o);
+      if (lane >= o) n += u;
     }
-    cum_s[tid + 1] = v;          // within the warp's 32 chunks
+    cum_s[tid + 1] = n;          // within the warp's 32 chunks
   }
   if (tid == 0) cum_s[0] = 0;
   __syncthreads();
@@ -158,19 +154,40 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   __syncthreads();
   if (tid < kPlanChunks) cum_s[tid + 1] += before;
   __syncthreads();
-  const int64_t per_head = cum_s[kPlanChunks] * mtiles, total = per_head * p.H;
-  const int grid = (int)min((int64_t)gridDim.x, total), cta = blockIdx.x;
+
+  // ---- this CTA's range.  With a codebook per head, a head's tiles are followed by kHeadTiles that stand for the
+  // change and a range falls into one portion per head; with one codebook for all it is one portion.
+  const int64_t per_head = cum_s[kPlanChunks] * mtiles;
+  const int gap = p.n_cb > 1 ? kHeadTiles : 0;
+  const int64_t stride = per_head + gap, total = stride * p.H - gap;
+  const int cta = blockIdx.x;
+  const int grid = (int)min((int64_t)gridDim.x, (total + kMinTiles - 1) / kMinTiles);
   if (cta >= grid) {
     if (tid == 0) p.desc[cta] = make_int4(0, -1, 0, 0);
     return;
   }
+  const int64_t from = total * cta / grid, to = total * (cta + 1) / grid;
+  const int h0 = (int)(from / stride), h1 = (int)((to - 1) / stride);
+  const int portions = gap ? h1 - h0 + 1 : 1;
+
+  const int pair = warp & (kPairs - 1);
   Walk w;
-  w.at = total * cta / grid;
-  w.end = total * (cta + 1) / grid;
-  {
+  // the pair's part of portion k, in tiles without gaps
+  auto enter = [&](int k) {
+    int64_t a = from, b = to;
+    if (gap) {
+      const int h = h0 + k;
+      a = max(from - h * stride, (int64_t)0) + h * per_head;
+      b = min(to - h * stride, per_head) + h * per_head;
+      if (a > b) a = b;                        // the range begins in the gap behind head h
+    }
+    const int n = p.pairs;
+    w.at = pair < n ? a + (b - a) * pair / n : b;
+    w.end = pair < n ? a + (b - a) * (pair + 1) / n : b;
+    if (w.at >= w.end) return;
     w.h = (int)(w.at / per_head);
     int64_t o = w.at - w.h * per_head;
-    int lo = 0, hi = kPlanChunks - 1;        // last chunk that begins at or before o
+    int lo = 0, hi = kPlanChunks - 1;          // last chunk that begins at or before o
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
       if (cum_s[mid] * mtiles <= o) lo = mid;
@@ -188,8 +205,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     }
     w.mt = (int)(o / w.tiles);
     w.t = (int)(o - (int64_t)w.mt * w.tiles);
-  }
-  auto next_item = [&](int n) {              // n: tiles of the item just walked
+  };
+  auto next_item = [&](int n) {                // n: tiles of the item just walked
     w.at += n;
     w.t = 0;
     if (++w.mt < mtiles) return;
@@ -203,84 +220,83 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       w.tiles = tiles_of(w.len);
     }
   };
+  uint8_t* const my_ring = ring + (size_t)pair * ring_bytes;
+  uint64_t* const full = full_s + pair * p.stages;
+  uint64_t* const empty = empty_s + pair * p.stages;
+  int stage = 0, phase = 0;                    // of the pair's next tile
 
-  if (warp >= kConsumers) {
-    // ----------------------------------------------------------------- producers
-    // Producer x takes the tiles x, x + kProducers, ... of the CTA's list.  Each lane finds the pool row of one of
-    // its next 32 copies (and reads the page numbers of the 32 after them ahead); lane 0 then only waits for a
-    // stage and issues.
+  if (warp >= kPairs) {
+    // ------------------------------------------------------------------ producer
+    // Each lane finds the pool row of one of the next 32 copies (and reads the page numbers of the 32 after them
+    // ahead); lane 0 then only waits for a stage and issues.
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
-    const int x = warp - kConsumers;
-    int stage = x, phase = 0, turn = 0, tile = x;   // stages: a multiple of the producers, so each has one of its own
     const int two = p.chunk != kTile;          // two copies make a tile
     const int vbytes = p.chunk * DV * 2, ibytes = p.chunk * NB, hbytes = p.chunk * p.n_heavy * BD * 2;
     const uint8_t* const heavy = reinterpret_cast<const uint8_t*>(p.heavy);
     const unsigned ps = (unsigned)p.ps;
-    while (w.at < w.end) {
-      const int n = (int)min(w.end - w.at, (int64_t)(w.tiles - w.t));
-      const int32_t* table = p.table + (int64_t)w.b * p.table_stride;
-      const int i0 = (x - turn + kProducers) % kProducers;          // first of the piece's tiles that is this warp's
-      const int mine = n > i0 ? (n - i0 + kProducers - 1) / kProducers : 0;
-      // first token of this lane's copy in the group of tiles from number j on; -1: none
-      auto token_of = [&](int j) {
-        j += lane >> two;
-        const int tok = (w.t + i0 + j * kProducers) * kTile + (two ? (lane & 1) * 16 : 0);
-        return j < mine && tok < w.len ? tok : -1;
-      };
-      int tok = token_of(0);
-      int ahead = tok >= 0 ? table[(unsigned)tok / ps] : -1;
-      if (w.len < 0 && lane == 0) record_error(p.err, kErrLength);
-      const int group = 32 >> two;
-      for (int j = 0; j < mine; j += group) {
-        const int page = ahead;
-        const bool found = tok >= 0 && page >= 0 && page < p.num_pages;
-        if (tok >= 0 && !found) record_error(p.err, kErrPage);
-        const int row =
-            found ? (int)(((unsigned)page * (unsigned)p.H + (unsigned)w.h) * ps + (unsigned)tok % ps) : (tok >= 0 ? -2 : -1);
-        tok = token_of(j + group);
-        ahead = tok >= 0 ? table[(unsigned)tok / ps] : -1;
-        const int tiles = min(group, mine - j);
-        for (int i = 0; i < tiles; ++i) {
-          const int ra = __shfl_sync(0xffffffffu, row, i << two);
-          const int rb = two ? __shfl_sync(0xffffffffu, row, 2 * i + 1) : -1;
-          if (lane == 0) {
-            mbar_wait(&empty[stage], phase ^ 1, p.err, kErrWait);
-            uint8_t* const st = ring + (size_t)stage * p.stage_bytes;
-            tag_s[stage] = 2 * tile + (w.len < 0 || ra == -2 || rb == -2);
-            mbar_arrive_expect_tx(&full[stage], ((ra >= 0) + (rb >= 0)) * (vbytes + ibytes + hbytes));
+    for (int k = 0; k < portions; ++k) {
+      enter(k);
+      while (w.at < w.end) {
+        const int n = (int)min(w.end - w.at, (int64_t)(w.tiles - w.t));
+        const int32_t* table = p.table + (int64_t)w.b * p.table_stride;
+        // first token of this lane's copy in the group of tiles from number j on; -1: none
+        auto token_of = [&](int j) {
+          j += lane >> two;
+          const int tok = (w.t + j) * kTile + (two ? (lane & 1) * 16 : 0);
+          return j < n && tok < w.len ? tok : -1;
+        };
+        int tok = token_of(0);
+        int ahead = tok >= 0 ? table[(unsigned)tok / ps] : -1;
+        if (w.len < 0 && lane == 0) record_error(p.err, kErrLength);
+        const int group = 32 >> two;
+        for (int j = 0; j < n; j += group) {
+          const int page = ahead;
+          const bool found = tok >= 0 && page >= 0 && page < p.num_pages;
+          if (tok >= 0 && !found) record_error(p.err, kErrPage);
+          // -1: no copy, -2: an invalid page
+          const int row =
+              found ? (int)(((unsigned)page * (unsigned)p.H + (unsigned)w.h) * ps + (unsigned)tok % ps) : (tok >= 0 ? -2 : -1);
+          tok = token_of(j + group);
+          ahead = tok >= 0 ? table[(unsigned)tok / ps] : -1;
+          const int tiles = min(group, n - j);
+          for (int i = 0; i < tiles; ++i) {
+            const int ra = __shfl_sync(0xffffffffu, row, i << two);
+            const int rb = two ? __shfl_sync(0xffffffffu, row, 2 * i + 1) : -1;
+            if (lane == 0) {
+              mbar_wait(&empty[stage], phase ^ 1, p.err, kErrWait);
+              uint8_t* const st = my_ring + stage * p.stage_bytes;
+              // the stage's last word: whether the tile is invalid
+              *reinterpret_cast<volatile int*>(st + p.stage_bytes - 4) = w.len < 0 || ra == -2 || rb == -2;
+              mbar_arrive_expect_tx(&full[stage], ((ra >= 0) + (rb >= 0)) * (vbytes + ibytes + hbytes));
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const int r = k ? rb : ra;
-              if (r < 0) continue;
+              for (int c = 0; c < 2; ++c) {
+                const int r = c ? rb : ra;
+                if (r < 0) continue;
 #pragma unroll
-              for (int c = 0; c < DV / 64; ++c)
-                tma_load_2d(st + c * kTile * 128 + k * 2048, &vmap, c * 64, r, &full[stage]);
-              bulk_g2s(st + p.off_idx + k * ibytes, p.idx + (int64_t)r * NB, ibytes, &full[stage]);
-              if (hbytes)
-                bulk_g2s(st + p.off_heavy + k * hbytes, heavy + (int64_t)r * p.n_heavy * BD * 2, hbytes, &full[stage]);
+                for (int x = 0; x < DV / 64; ++x)
+                  tma_load_2d(st + x * kTile * 128 + c * 2048, &vmap, x * 64, r, &full[stage]);
+                bulk_g2s(st + p.off_idx + c * ibytes, p.idx + (int64_t)r * NB, ibytes, &full[stage]);
+                if (hbytes)
+                  bulk_g2s(st + p.off_heavy + c * hbytes, heavy + (int64_t)r * p.n_heavy * BD * 2, hbytes, &full[stage]);
+              }
+            }
+            if (++stage == p.stages) {
+              stage = 0;
+              phase ^= 1;
             }
           }
-          tile += kProducers;
-          stage += kProducers;
-          if (stage == p.stages + x) {
-            stage = x;
-            phase ^= 1;
-          }
         }
+        next_item(n);
       }
-      turn = (turn + n) % kProducers;
-      next_item(n);
     }
     __syncwarp();
     return;
   }
 
-  // -------------------------------------------------------------------- consumers
+  // -------------------------------------------------------------------- consumer
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kConsumerRegs));
   const int g = lane >> 2, t = lane & 3;
   const uint32_t image_a = smem_u32(image);
-  int head = -1, cb_phase = 0;
-  float k_scale = 1.f;
   uint32_t hmask = 0;                          // bit u: unit u of this lane is a dense block
   for (int u = 0; u < UNITS; ++u) hmask |= (uint32_t)(hslot_s[4 * u + t] >= 0) << u;
   const int rot = g & (ROT - 1);
@@ -297,334 +313,376 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     const int tok = ((lane >> 4) & 1) * 8 + (lane & 7);
     v_off[d] = tok * 128 + (((2 * d + ((lane >> 3) & 1)) ^ (lane & 7)) << 4);
   }
-  int turn = 0;                                // warp that takes the next tile of the CTA's list
-  int stage = warp % p.stages, phase = (warp / p.stages) & 1, tile = warp;   // this warp's next tile
-  int head_piece = 0;
-  int4 tail = make_int4(0, -1, 0, 0);
-  const int rows_total = item_rows_total(p);
+  int4 desc = make_int4(0, -1, 0, 0);
+  // pieces of this CTA's pairs, [kPairs][2][ROWS] rows: written and read by this CTA, from L2
+  float* const pieces = p.pieces + (int64_t)cta * kPairs * 2 * ROWS * RF;
 
-  while (w.at < w.end) {
-    const int n = (int)min(w.end - w.at, (int64_t)(w.tiles - w.t));
-    const int r0 = w.mt * kItemRows, nr = min(kItemRows, rows_total - r0);
-    // the head's codebook
-    if (w.h != head) {
-      const int cb = p.n_cb == 1 ? 0 : w.h % p.n_cb;
-      if (head < 0 || p.n_cb > 1) {
-        if (tid == 0) {                        // no warp reads the old codebook: the last item's barriers
-          fence_proxy_async_smem();
-          mbar_arrive_expect_tx(cb_bar, IMAGE);
-          bulk_g2s(image, reinterpret_cast<const uint8_t*>(p.image) + (int64_t)cb * IMAGE, IMAGE, cb_bar);
-        }
-        k_scale = p.image_scale[cb];
-      }
+  for (int k = 0; k < portions; ++k) {
+    if (tid == 0) {                            // the portion's codebook; no warp reads the last one any more
+      if (k) fence_proxy_async_smem();
+      const int cb = p.n_cb == 1 ? 0 : (h0 + k) % p.n_cb;
+      mbar_arrive_expect_tx(cb_bar, IMAGE);
+      bulk_g2s(image, reinterpret_cast<const uint8_t*>(p.image) + (int64_t)cb * IMAGE, IMAGE, cb_bar);
     }
-    // queries of the item: permuted, scaled by a power of two into fp16; a negative scale goes into their sign, so
-    // that the factor of a row's scores is not negative and maxima can be taken before it
-    for (int r = warp; r < ROWS; r += kConsumers) {
-      float x[D / 32], mx = 0.f;
-      if (r < nr) {
-        const RowMap at = row_of(p, w.h, w.b, r0 + r);
-        const T* src = reinterpret_cast<const T*>(p.q) + at.b * p.qs[0] + at.hq * p.qs[1] + at.l * p.qs[2];
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-          x[i] = Elem<T>::to_float(src[perm_s[i * 32 + lane]]);
-          mx = fmaxf(mx, fabsf(x[i]));
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) x[i] = 0.f;
-      }
-      for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      // 2^-e with mx in [2^e, 2^(e+1)), within the exponents that have a normal reciprocal; 1 for 0, infinity
-      const int e = (__float_as_int(mx) >> 23) - 127;
-      const int ec = mx == 0.f || mx == INF ? 0 : max(-126, min(126, e));
-      const float s = copysignf(__int_as_float((127 - ec) << 23), p.scale_log2);
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) q_s[r * (D + 8) + i * 32 + lane] = __float2half_rn(x[i] * s);
-      if (lane == 0) qf_s[r] = fabsf(p.scale_log2) * __int_as_float((127 + ec) << 23) / k_scale;
-    }
-    named_barrier(1, kConsumers * 32);
-    if (w.h != head) {
-      if (head < 0 || p.n_cb > 1) {
-        mbar_wait(cb_bar, cb_phase, p.err, kErrWait);
-        cb_phase ^= 1;
-      }
-      head = w.h;
-    }
-    uint32_t qb[NT][KS][2];
-#pragma unroll
-    for (int c = 0; c < NT; ++c)
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int word = 2 * ks + i, u = word / WORDS;
-          const int d = (4 * u + t) * BD + 2 * (word % WORDS);
-          qb[c][ks][i] = *reinterpret_cast<const uint32_t*>(q_s + (8 * c + g) * (D + 8) + d);
-        }
-    // this lane's rows are 8c + 2t + j: their score factors, and the tokens that each sees
-    const bool limited = p.causal && p.L > 1 && !p.prefix_mode;
-    float f[NT][2];
-    int seen[NT][2];
-#pragma unroll
-    for (int c = 0; c < NT; ++c)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        f[c][j] = qf_s[8 * c + 2 * t + j];
-        seen[c][j] = limited ? max(0, w.len - (p.L - 1 - (r0 + 8 * c + 2 * t + j) % p.L)) : w.len;
-      }
-    const int seen_all = limited ? max(0, w.len - (p.L - 1)) : w.len;
+    const float k_scale = p.image_scale[p.n_cb == 1 ? 0 : (h0 + k) % p.n_cb];
+    enter(k);
+    int4 head = make_int4(w.at < w.end ? 0 : -1, 0, 0, 0), tail = make_int4(0, 0, 0, 0);
+    bool waited = false;
 
-    float o[NT][DV / 16][4];
+    while (w.at < w.end) {
+      const int n = (int)min(w.end - w.at, (int64_t)(w.tiles - w.t));
+      const int r0 = w.mt * ROWS, nr = min(ROWS, rows_total - r0);
+      // Queries as the B operand: this lane's words of row 8c + g, scaled by a power of two into fp16.  A negative
+      // scale goes into their sign, so that the factor of a row's scores is not negative and maxima can be taken
+      // before it.
+      uint32_t qb[NT][KS][2];
+      float f[NT][2];
+      int seen[NT][2];
+      const bool limited = p.causal && p.L > 1 && !p.prefix_mode;
 #pragma unroll
-    for (int c = 0; c < NT; ++c)
+      for (int c = 0; c < NT; ++c) {
+        float mx = 0.f;
+        T raw[D / 8][2];
+        if (8 * c + g < nr) {
+          const RowMap at = row_of(p, w.h, w.b, r0 + 8 * c + g);
+          const T* src = reinterpret_cast<const T*>(p.q) + at.b * p.qs[0] + at.hq * p.qs[1] + at.l * p.qs[2];
 #pragma unroll
-      for (int i = 0; i < DV / 16; ++i) o[c][i][0] = o[c][i][1] = o[c][i][2] = o[c][i][3] = 0.f;
-    // m: the largest score before its factor, or one that it exceeds by at most kSlack after it; mb: m, 0 for none yet
-    float m[NT][2], mb[NT][2], l[NT][2];
-#pragma unroll
-    for (int c = 0; c < NT; ++c) m[c][0] = m[c][1] = -INF, mb[c][0] = mb[c][1] = l[c][0] = l[c][1] = 0.f;
-    bool bad = false;
-    const int w0 = turn;                                           // warp of the piece's first tile
-    for (int i = (warp - w0 + kConsumers) % kConsumers; i < n; i += kConsumers) {
-      const int first = (w.t + i) * kTile;
-      // Tiles of a stage go to different warps: only the tag tells that the stage has come to this one, and that its
-      // barrier cannot be a whole turn behind, where the wait for a parity would pass at once.
-      int tag = tag_s[stage];
-      if (tag >> 1 != tile) {
-        const uint64_t t0 = global_ns();
-        while ((tag = tag_s[stage]) >> 1 != tile)
-          if (global_ns() - t0 > kWaitLimitNs) {
-            record_error(p.err, kErrWait);
-            break;
+          for (int i = 0; i < D / 8; ++i) {
+            const int d = (4 * (i / WORDS) + t) * BD + 2 * (i % WORDS);
+            raw[i][0] = src[perm_s[d]];
+            raw[i][1] = src[perm_s[d + 1]];
           }
-      }
-      mbar_wait(&full[stage], phase, p.err, kErrWait);
-      tile += kConsumers;
-      uint8_t* const st = ring + (size_t)stage * p.stage_bytes;
-      const uint32_t st_a = smem_u32(st);
-      bad |= tag & 1;
-      float s[2][NT][4];
+        } else {
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        uint32_t kw[2][D / 8];
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const int tok = mt * 16 + y * 8 + g;
-          uint32_t ib[UNITS];
-#pragma unroll
-          for (int u = 0; u < UNITS; u += 4) {
-            if constexpr (UNITS >= 4) lds_words<16>(ib + u, st_a + p.off_idx + tok * NB + u * 4);
-            else lds_words<8>(ib + u, st_a + p.off_idx + tok * NB + u * 4);
-          }
-          // slot u loads unit (u + r) mod ROT of its group of ROT units
-#pragma unroll
-          for (int u = 0; u < UNITS; ++u) {
-            uint32_t word = ib[u];
-#pragma unroll
-            for (int x = 1; x < ROT; ++x)
-              if (rot == x) word = ib[(u & ~(ROT - 1)) | ((u + x) & (ROT - 1))];
-            lds_words<2 * BD>(kw[y] + u * WORDS, col_a[u] + (__byte_perm(word, 0, byte_sel) << 7));
-          }
-          // put the units back in order: rotate each group by r
-#pragma unroll
-          for (int u0 = 0; u0 < UNITS; u0 += ROT)
-#pragma unroll
-            for (int bit = 1; bit < ROT; bit <<= 1) {
-              uint32_t tmp[ROT * WORDS];
-#pragma unroll
-              for (int x = 0; x < ROT; ++x)
-#pragma unroll
-                for (int z = 0; z < WORDS; ++z)
-                  tmp[x * WORDS + z] =
-                      (rot & bit) ? kw[y][(u0 + ((x - bit) & (ROT - 1))) * WORDS + z] : kw[y][(u0 + x) * WORDS + z];
-#pragma unroll
-              for (int x = 0; x < ROT * WORDS; ++x) kw[y][u0 * WORDS + x] = tmp[x];
-            }
-          if (p.n_heavy) {                       // dense blocks take the place of their codeword 0
-#pragma unroll
-            for (int u = 0; u < UNITS; ++u)
-              if ((hmask >> u) & 1) {
-                uint32_t* dst = kw[y] + u * WORDS;
-                lds_words<2 * BD>(dst, st_a + p.off_heavy + (tok * p.n_heavy + hslot_s[4 * u + t]) * (2 * BD));
-#pragma unroll
-                for (int x = 0; x < WORDS; ++x) dst[x] = dense_word<T>(dst[x], k_scale);
-              }
-          }
+          for (int i = 0; i < D / 8; ++i) raw[i][0] = raw[i][1] = Elem<T>::from_float(0.f);
         }
 #pragma unroll
-        for (int c = 0; c < NT; ++c) {
-          s[mt][c][0] = s[mt][c][1] = s[mt][c][2] = s[mt][c][3] = 0.f;
+        for (int i = 0; i < D / 8; ++i)
+          mx = fmaxf(mx, fmaxf(fabsf(Elem<T>::to_float(raw[i][0])), fabsf(Elem<T>::to_float(raw[i][1]))));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        // 2^-e with mx in [2^e, 2^(e+1)), within the exponents that have a normal reciprocal; 1 for 0, infinity
+        const int e = (__float_as_int(mx) >> 23) - 127;
+        const int ec = mx == 0.f || mx == INF ? 0 : max(-126, min(126, e));
+        const float sc = copysignf(__int_as_float((127 - ec) << 23), p.scale_log2);
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks)
-            mma_f16(s[mt][c], kw[0][2 * ks], kw[1][2 * ks], kw[0][2 * ks + 1], kw[1][2 * ks + 1], qb[c][ks][0], qb[c][ks][1]);
+        for (int i = 0; i < D / 8; ++i)
+          qb[c][i / 2][i % 2] = pack2<__half>(Elem<T>::to_float(raw[i][0]) * sc, Elem<T>::to_float(raw[i][1]) * sc);
+        const float qf = fabsf(p.scale_log2) * __int_as_float((127 + ec) << 23) / k_scale;
+        // this lane's columns of S^T are the rows 8c + 2t + j: their factors, and the tokens that each sees
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          f[c][j] = __shfl_sync(0xffffffffu, qf, 4 * (2 * t + j));
+          seen[c][j] = limited ? max(0, w.len - (p.L - 1 - (r0 + 8 * c + 2 * t + j) % p.L)) : w.len;
         }
       }
-      // online softmax, in powers of two
-      const bool edge = first + kTile > seen_all;
-      if (edge) {
-#pragma unroll
-        for (int c = 0; c < NT; ++c)
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (first + (e >> 2) * 16 + ((e >> 1) & 1) * 8 + g >= seen[c][e & 1]) s[e >> 2][c][e & 3] = -INF;
+      const int seen_all = limited ? max(0, w.len - (p.L - 1)) : w.len;
+      if (!waited) {
+        mbar_wait(cb_bar, k & 1, p.err, kErrWait);
+        waited = true;
       }
-      bool grows = false;
-      float top[NT][2];
+
+      float o[NT][DV / 16][4];
 #pragma unroll
       for (int c = 0; c < NT; ++c)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          top[c][j] = fmaxf(fmaxf(s[0][c][j], s[0][c][j + 2]), fmaxf(s[1][c][j], s[1][c][j + 2]));
-          grows |= m[c][j] == -INF ? top[c][j] != -INF : (top[c][j] - m[c][j]) * f[c][j] > kSlack;
+        for (int i = 0; i < DV / 16; ++i) o[c][i][0] = o[c][i][1] = o[c][i][2] = o[c][i][3] = 0.f;
+      // m: the largest score before its factor, or one that it exceeds by at most kSlack after it; mb: m, 0 for none yet
+      float m[NT][2], mb[NT][2], l[NT][2];
+#pragma unroll
+      for (int c = 0; c < NT; ++c) m[c][0] = m[c][1] = -INF, mb[c][0] = mb[c][1] = l[c][0] = l[c][1] = 0.f;
+      bool bad = false;
+      for (int i = 0; i < n; ++i) {
+        const int first = (w.t + i) * kTile;
+        mbar_wait(&full[stage], phase, p.err, kErrWait);
+        uint8_t* const st = my_ring + stage * p.stage_bytes;
+        const uint32_t st_a = smem_u32(st);
+        bad |= *reinterpret_cast<volatile int*>(st + p.stage_bytes - 4) != 0;
+        float s[2][NT][4];
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+          uint32_t kw[2][D / 8];
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const int tok = mt * 16 + y * 8 + g;
+            uint32_t ib[UNITS];
+#pragma unroll
+            for (int u = 0; u < UNITS; u += 4) {
+              if constexpr (UNITS >= 4) lds_words<16>(ib + u, st_a + p.off_idx + tok * NB + u * 4);
+              else lds_words<8>(ib + u, st_a + p.off_idx + tok * NB + u * 4);
+            }
+            // slot u loads unit (u + rot) mod ROT of its group of ROT units
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u) {
+              uint32_t word = ib[u];
+#pragma unroll
+              for (int x = 1; x < ROT; ++x)
+                if (rot == x) word = ib[(u & ~(ROT - 1)) | ((u + x) & (ROT - 1))];
+              lds_words<2 * BD>(kw[y] + u * WORDS, col_a[u] + (__byte_perm(word, 0, byte_sel) << 7));
+            }
+            // put the units back in order: rotate each group by rot
+#pragma unroll
+            for (int u0 = 0; u0 < UNITS; u0 += ROT)
+#pragma unroll
+              for (int bit = 1; bit < ROT; bit <<= 1) {
+                uint32_t tmp[ROT * WORDS];
+#pragma unroll
+                for (int x = 0; x < ROT; ++x)
+#pragma unroll
+                  for (int z = 0; z < WORDS; ++z)
+                    tmp[x * WORDS + z] =
+                        (rot & bit) ? kw[y][(u0 + ((x - bit) & (ROT - 1))) * WORDS + z] : kw[y][(u0 + x) * WORDS + z];
+#pragma unroll
+                for (int x = 0; x < ROT * WORDS; ++x) kw[y][u0 * WORDS + x] = tmp[x];
+              }
+            if (p.n_heavy) {                       // dense blocks take the place of their codeword 0
+#pragma unroll
+              for (int u = 0; u < UNITS; ++u)
+                if ((hmask >> u) & 1) {
+                  uint32_t* dst = kw[y] + u * WORDS;
+                  lds_words<2 * BD>(dst, st_a + p.off_heavy + (tok * p.n_heavy + hslot_s[4 * u + t]) * (2 * BD));
+#pragma unroll
+                  for (int x = 0; x < WORDS; ++x) dst[x] = dense_word<T>(dst[x], k_scale);
+                }
+            }
+          }
+#pragma unroll
+          for (int c = 0; c < NT; ++c) {
+            s[mt][c][0] = s[mt][c][1] = s[mt][c][2] = s[mt][c][3] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+              mma_f16(s[mt][c], kw[0][2 * ks], kw[1][2 * ks], kw[0][2 * ks + 1], kw[1][2 * ks + 1], qb[c][ks][0],
+                      qb[c][ks][1]);
+          }
         }
-      if (__any_sync(0xffffffffu, grows)) {
+        // online softmax, in powers of two
+        const bool edge = first + kTile > seen_all;
+        if (edge) {
+#pragma unroll
+          for (int c = 0; c < NT; ++c)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (first + (e >> 2) * 16 + ((e >> 1) & 1) * 8 + g >= seen[c][e & 1]) s[e >> 2][c][e & 3] = -INF;
+        }
+        bool grows = false;
+        float top[NT][2];
 #pragma unroll
         for (int c = 0; c < NT; ++c)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float x = top[c][j];
+            top[c][j] = fmaxf(fmaxf(s[0][c][j], s[0][c][j + 2]), fmaxf(s[1][c][j], s[1][c][j + 2]));
+            grows |= m[c][j] == -INF ? top[c][j] != -INF : (top[c][j] - m[c][j]) * f[c][j] > kSlack;
+          }
+        if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
-            for (int of = 4; of < 32; of <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, of));
-            const float nm = fmaxf(m[c][j], x);
-            const float e = m[c][j] == -INF ? 0.f : fast_exp2((m[c][j] - nm) * f[c][j]);
-            m[c][j] = nm;
-            mb[c][j] = nm == -INF ? 0.f : nm;
-            l[c][j] *= e;
+          for (int c = 0; c < NT; ++c)
 #pragma unroll
-            for (int d = 0; d < DV / 16; ++d) {
-              o[c][d][j] *= e;
-              o[c][d][j + 2] *= e;
+            for (int j = 0; j < 2; ++j) {
+              float x = top[c][j];
+#pragma unroll
+              for (int of = 4; of < 32; of <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, of));
+              const float nm = fmaxf(m[c][j], x);
+              const float e = m[c][j] == -INF ? 0.f : fast_exp2((m[c][j] - nm) * f[c][j]);
+              m[c][j] = nm;
+              mb[c][j] = nm == -INF ? 0.f : nm;
+              l[c][j] *= e;
+#pragma unroll
+              for (int d = 0; d < DV / 16; ++d) {
+                o[c][d][j] *= e;
+                o[c][d][j + 2] *= e;
+              }
             }
-          }
-      }
-      uint32_t pb[2][NT][2];
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-        for (int c = 0; c < NT; ++c) {
-          float e[4];
-#pragma unroll
-          for (int x = 0; x < 4; ++x) e[x] = fast_exp2((s[mt][c][x] - mb[c][x & 1]) * f[c][x & 1]);
-          if (edge) {                            // -inf times a factor of zero
-#pragma unroll
-            for (int x = 0; x < 4; ++x) e[x] = s[mt][c][x] == -INF ? 0.f : e[x];
-          }
-          l[c][0] += e[0] + e[2];
-          l[c][1] += e[1] + e[3];
-          pb[mt][c][0] = movmatrix(pack2<T>(e[0], e[1]));
-          pb[mt][c][1] = movmatrix(pack2<T>(e[2], e[3]));
         }
-      if (first + kTile > w.len) {               // rows behind the end hold anything: zero times it is not zero
-        for (int k = max(0, w.len - first) * (DV / 8) + lane; k < kTile * (DV / 8); k += 32) {
-          const int tok = k / (DV / 8), c = k % (DV / 8);
-          *reinterpret_cast<uint4*>(st + (c >> 3) * (kTile * 128) + tok * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+        uint32_t pb[2][NT][2];
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int c = 0; c < NT; ++c) {
+            float e[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) e[x] = fast_exp2((s[mt][c][x] - mb[c][x & 1]) * f[c][x & 1]);
+            if (edge) {                            // -inf times a factor of zero
+#pragma unroll
+              for (int x = 0; x < 4; ++x) e[x] = s[mt][c][x] == -INF ? 0.f : e[x];
+            }
+            l[c][0] += e[0] + e[2];
+            l[c][1] += e[1] + e[3];
+            pb[mt][c][0] = movmatrix(pack2<T>(e[0], e[1]));
+            pb[mt][c][1] = movmatrix(pack2<T>(e[2], e[3]));
+          }
+        if (first + kTile > w.len) {               // rows behind the end hold anything: zero times it is not zero
+          for (int x = max(0, w.len - first) * (DV / 8) + lane; x < kTile * (DV / 8); x += 32) {
+            const int tok = x / (DV / 8), c = x % (DV / 8);
+            *reinterpret_cast<uint4*>(st + (c >> 3) * (kTile * 128) + tok * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
         }
-        fence_proxy_async_smem();
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int d = 0; d < DV / 16; ++d) {
+            uint32_t v[4];
+            ldmatrix_x4_trans(v, st_a + v_off[d & 3] + (d >> 2) * (kTile * 128) + mt * 2048);
+#pragma unroll
+            for (int c = 0; c < NT; ++c) mma_pv<T>(o[c][d], v[0], v[1], v[2], v[3], pb[mt][c][0], pb[mt][c][1]);
+          }
         __syncwarp();
-      }
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-        for (int d = 0; d < DV / 16; ++d) {
-          uint32_t v[4];
-          ldmatrix_x4_trans(v, st_a + v_off[d & 3] + (d >> 2) * (kTile * 128) + mt * 2048);
-#pragma unroll
-          for (int c = 0; c < NT; ++c) mma_pv<T>(o[c][d], v[0], v[1], v[2], v[3], pb[mt][c][0], pb[mt][c][1]);
+        if (lane == 0) mbar_arrive(&empty[stage]);
+        if (++stage == p.stages) {
+          stage = 0;
+          phase ^= 1;
         }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[stage]);
-      stage += kConsumers;                                          // this warp's next tile
-      while (stage >= p.stages) {
-        stage -= p.stages;
-        phase ^= 1;
       }
-    }
-    turn = (turn + n) % kConsumers;
-
-    // join the warps that took tiles of this piece
-    const int warps = min(kConsumers, n);
-    const int mine = (warp - w0 + kConsumers) % kConsumers;         // rank among them
-    if (mine < warps) {
+      // the item's or piece's result
       bad = __any_sync(0xffffffffu, bad);
-      float* dst = acc_s + (size_t)mine * ROWS * (DV + 2);
+      const bool begins = w.t == 0, ends = w.t + n == w.tiles;
 #pragma unroll
       for (int c = 0; c < NT; ++c)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
 #pragma unroll
           for (int of = 4; of < 32; of <<= 1) l[c][j] += __shfl_xor_sync(0xffffffffu, l[c][j], of);
-          float* to = dst + (8 * c + 2 * t + j) * (DV + 2);
-          if (g == 0) {
-            to[DV] = m[c][j] == -INF ? -INF : m[c][j] * f[c][j];
-            to[DV + 1] = bad ? __int_as_float(0x7fffffff) : l[c][j];
-          }
+          if (bad) l[c][j] = __int_as_float(0x7fffffff);
+          m[c][j] = m[c][j] == -INF ? -INF : m[c][j] * f[c][j];
+        }
 #pragma unroll
-          for (int d = 0; d < DV / 16; ++d) {
-            to[d * 16 + g] = o[c][d][j];
-            to[d * 16 + 8 + g] = o[c][d][j + 2];
+      for (int c = 0; c < NT; ++c)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int r = 8 * c + 2 * t + j;
+          float* dst = nullptr;
+          if (!(begins && ends)) dst = pieces + ((pair * 2 + begins) * ROWS + r) * RF;
+          else if (p.prefix_mode && r < nr) dst = p.prefix_part + flat_row(p, row_of(p, w.h, w.b, r0 + r)) * RF;
+          if (dst) {
+#pragma unroll
+            for (int d = 0; d < DV / 16; ++d) {
+              dst[d * 16 + g] = o[c][d][j];
+              dst[d * 16 + 8 + g] = o[c][d][j + 2];
+            }
+            if (g == 0) *reinterpret_cast<float2*>(dst + DV) = make_float2(m[c][j], l[c][j]);
+          } else if (begins && ends && r < nr) {
+            const int64_t row = flat_row(p, row_of(p, w.h, w.b, r0 + r));
+            const Finish e = finish_of<DV>(p, row, m[c][j], l[c][j]);
+            T* out = reinterpret_cast<T*>(p.out) + row * DV;
+            const int64_t rows = (int64_t)p.B * p.Hq * p.L;
+#pragma unroll
+            for (int d = 0; d < DV / 16; ++d) {
+              o[c][d][j] *= e.f;
+              o[c][d][j + 2] *= e.f;
+            }
+            for (int y = 0; y < p.prefix_parts; ++y) {
+              const float* src = p.prefix_part + (y * rows + row) * RF;
+              const float fk = fast_exp2(src[DV] - e.base);
+#pragma unroll
+              for (int d = 0; d < DV / 16; ++d) {
+                o[c][d][j] = fmaf(src[d * 16 + g], fk, o[c][d][j]);
+                o[c][d][j + 2] = fmaf(src[d * 16 + 8 + g], fk, o[c][d][j + 2]);
+              }
+            }
+#pragma unroll
+            for (int d = 0; d < DV / 16; ++d) {
+              out[d * 16 + g] = Elem<T>::from_float(o[c][d][j] * e.inv);
+              out[d * 16 + 8 + g] = Elem<T>::from_float(o[c][d][j + 2] * e.inv);
+            }
           }
         }
+      if (!begins) head = make_int4(ends ? 2 : 1, w.h, w.b, w.mt);
+      else if (!ends) tail = make_int4(1, w.h, w.b, w.mt);
+      next_item(n);
     }
-    named_barrier(1, kConsumers * 32);
-    const bool begins = w.t == 0, ends = w.t + n == w.tiles;
-    float* slot = begins && ends ? nullptr : p.slots + (int64_t)(2 * cta + (begins ? 1 : 0)) * kItemRows * (DV + 2);
-    for (int e = tid; e < nr * DV; e += kConsumers * 32) {
-      const int r = e / DV, d = e % DV;
-      float M = -INF;
-      for (int k = 0; k < warps; ++k) M = fmaxf(M, acc_s[((size_t)k * ROWS + r) * (DV + 2) + DV]);
-      const float bs = M == -INF ? 0.f : M;
-      float l = 0.f, a = 0.f;
-      for (int k = 0; k < warps; ++k) {
-        const float* src = acc_s + ((size_t)k * ROWS + r) * (DV + 2);
-        const float e = fast_exp2(src[DV] - bs);
-        l = fmaf(src[DV + 1], e, l);
-        a = fmaf(src[d], e, a);
-      }
-      if (slot) {
-        slot[r * (DV + 2) + 2 + d] = a;
-        if (d == 0) {
-          slot[r * (DV + 2)] = M;
-          slot[r * (DV + 2) + 1] = l;
-        }
+    if (!waited) mbar_wait(cb_bar, k & 1, p.err, kErrWait);      // a pair without tiles: the barrier keeps its phase
+    if (lane == 0) {
+      head_s[pair] = head;
+      tail_s[pair] = tail;
+    }
+    named_barrier(1, kPairs * 32);
+
+    // Items cut between pairs, in the list's order: each starts with a pair's tail piece (or, begun by an earlier
+    // CTA, with the first head piece) and goes on through head pieces.
+    for (int x = -1; x < kPairs; ++x) {
+      int y = x;
+      int4 item;
+      if (x < 0) {
+        y = 0;
+        while (y < kPairs && head_s[y].x < 0) ++y;
+        if (y == kPairs || head_s[y].x == 0) continue;
+        item = head_s[y];
       } else {
-        finish_element<T, DV>(p, row_of(p, w.h, w.b, r0 + r), d, M, l, a);
+        if (tail_s[x].x == 0) continue;
+        item = tail_s[x];
       }
+      const int nr = min(ROWS, rows_total - item.w * ROWS);
+      bool ended = x < 0 && item.x == 2;
+      int last = y;                                              // last pair of the item
+      for (int z = y + 1; z < kPairs && !ended; ++z) {
+        if (head_s[z].x <= 0) continue;
+        last = z;
+        ended = head_s[z].x == 2;
+      }
+      for (int e = tid; e < nr * (DV / 4); e += kPairs * 32) {
+        const int r = e / (DV / 4), d = e % (DV / 4) * 4;
+        const float* src = pieces + ((y * 2 + (x >= 0)) * ROWS + r) * RF;
+        float m = src[DV], l = src[DV + 1];
+        float4 a = *reinterpret_cast<const float4*>(src + d);
+        for (int z = y + 1; z <= last; ++z) {
+          if (head_s[z].x <= 0) continue;
+          src = pieces + (z * 2 * ROWS + r) * RF;
+          join4(m, l, a, src[DV], src[DV + 1], *reinterpret_cast<const float4*>(src + d));
+        }
+        if (x >= 0 && ended) {
+          finish4<T, DV>(p, row_of(p, item.y, item.z, item.w * ROWS + r), d, m, l, a);
+        } else {
+          float* dst = p.slots + ((int64_t)(2 * cta + (x < 0 ? 0 : 1)) * kItemRows + r) * RF;
+          *reinterpret_cast<float4*>(dst + d) = a;
+          if (d == 0) *reinterpret_cast<float2*>(dst + DV) = make_float2(m, l);
+        }
+      }
+      if (x < 0) desc.x = ended ? 2 : 1;
+      else if (!ended) desc = make_int4(desc.x, item.y, item.z, item.w);
     }
-    if (!begins) head_piece = ends ? 2 : 1;
-    else if (!ends) tail = make_int4(0, w.h, w.b, w.mt);
-    next_item(n);
+    if (k + 1 < portions) named_barrier(1, kPairs * 32);
   }
-  if (tid == 0) {
-    tail.x = head_piece;
-    p.desc[cta] = tail;
-  }
+  if (tid == 0) p.desc[cta] = desc;
 }
 
-// Joins the pieces of items that were cut: block (c, r) takes row r of the item that begins in CTA c's range
-// and does not end there, in the order of the ranges.
+// Joins the pieces of items that were cut between CTAs: block (c, r) takes row r of the item that begins in CTA c's
+// range and does not end there, in the order of the ranges.
+constexpr int kJoinParts = 4;      // parts of an item's pieces that are joined side by side
+
 template <int DV, typename T>
-__global__ void __launch_bounds__(DV) paged_attention_join(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(kJoinParts * DV / 4) paged_attention_join(const __grid_constant__ AttnParams p) {
+  constexpr int RF = row_floats(DV);
+  __shared__ int last_s;
+  __shared__ float4 acc_s[kJoinParts][DV / 4];
+  __shared__ float2 ml_s[kJoinParts];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int c = blockIdx.x, r = blockIdx.y, d = threadIdx.x;
+  const int c = blockIdx.x, r = blockIdx.y, part = threadIdx.x / (DV / 4), d = threadIdx.x % (DV / 4) * 4;
   const int4 tail = p.desc[c];
   if (tail.y < 0) return;
-  const int row = tail.w * kItemRows + r;
+  const int row = tail.w * p.item_rows + r;
   if (row >= item_rows_total(p)) return;
-  int last = c + 1;
-  while (last < gridDim.x && p.desc[last].x == 1) ++last;
-  const float INF = __int_as_float(0x7f800000);
-  const float* own = p.slots + ((int64_t)(2 * c + 1) * kItemRows + r) * (DV + 2);
-  float m = own[0], l = own[1], a = own[2 + d];
-  for (int k = c + 1; k <= last && k < gridDim.x; ++k) {
-    const float* src = p.slots + ((int64_t)(2 * k) * kItemRows + r) * (DV + 2);
-    const float mk = src[0], M = fmaxf(m, mk), bs = M == -INF ? 0.f : M;
-    const float f = fast_exp2(m - bs), fk = fast_exp2(mk - bs);
-    l = l * f + src[1] * fk;
-    a = a * f + src[2 + d] * fk;
-    m = M;
+  if (threadIdx.x == 0) last_s = gridDim.x;
+  __syncthreads();
+  for (int k = c + 1; k < gridDim.x && last_s == gridDim.x; k += blockDim.x) {
+    __syncthreads();
+    if (k + threadIdx.x < gridDim.x && p.desc[k + threadIdx.x].x != 1) atomicMin(&last_s, k + (int)threadIdx.x);
+    __syncthreads();
   }
-  finish_element<T, DV>(p, row_of(p, tail.y, tail.z, row), d, m, l, a);
+  const int n = min(last_s, (int)gridDim.x - 1) - c + 1;       // pieces: c's tail and the heads behind it
+  float m = -__int_as_float(0x7f800000), l = 0.f;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int k = n * part / kJoinParts; k < n * (part + 1) / kJoinParts; ++k) {
+    const float* src = p.slots + ((int64_t)(2 * (c + k) + (k == 0)) * kItemRows + r) * RF;
+    join4(m, l, a, src[DV], src[DV + 1], *reinterpret_cast<const float4*>(src + d));
+  }
+  acc_s[part][d / 4] = a;
+  if (d == 0) ml_s[part] = make_float2(m, l);
+  __syncthreads();
+  if (part) return;
+  for (int k = 1; k < kJoinParts; ++k) join4(m, l, a, ml_s[k].x, ml_s[k].y, acc_s[k][d / 4]);
+  finish4<T, DV>(p, row_of(p, tail.y, tail.z, row), d, m, l, a);
 }
 
 template <int D, int DV, int BD, typename T>
@@ -638,8 +696,8 @@ int launch_paged_attention(const AttnParams& p, const CUtensorMap& vmap, int gri
   k<<<grid, kAttnThreads, p.smem, st>>>(p, vmap);
   // the join may be scheduled while the main grid drains; it waits for its end before it reads
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid, kItemRows);
-  cfg.blockDim = dim3(DV);
+  cfg.gridDim = dim3(grid, p.item_rows);
+  cfg.blockDim = dim3(kJoinParts * DV / 4);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
