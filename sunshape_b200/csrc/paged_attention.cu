@@ -35,7 +35,7 @@ bool plan(AttnParams& p, int d, int dv, int bd) {
   p.off_heavy = p.off_idx + kTile * p.nb;
   p.stage_bytes = (p.off_heavy + kTile * p.n_heavy * bd * 2 + 4 + 1023) / 1024 * 1024;
   // alignment, codebook, permutation, plan, codebook barrier, pieces' descriptions, dense slots
-  const int fixed = 1024 + d * 512 + d * 4 + (kPlanChunks + 1) * 8 + 8 + 16 + kPairs * 32 + p.nb;
+  const int fixed = 1024 + d * 512 + d * 4 + (2 * kPlanChunks + 2) * 4 + 8 + 16 + kPairs * 32 + p.nb;
   const int left = kSmemMax - fixed;
   p.stages = std::min(6, left / (kPairs * (p.stage_bytes + 16)));
   p.pairs = kPairs;
@@ -146,6 +146,12 @@ int sunshape_paged_attention(const sunshape_codec_t* codec, const sunshape_pages
   p.prefix_part = reinterpret_cast<float*>(ws + at.prefix);
   const int64_t pool_rows = p.num_pages * p.H * p.ps;
   if (pool_rows > 0x7fffffff) return set_last_error(SUNSHAPE_E_UNSUPPORTED, "at most 2^31 - 1 page rows in a pool.");
+  // the kernels count tiles, and the gaps between heads, in 31 bits
+  const int64_t most = (int64_t)std::max(batch, 1) * (((int64_t)table_cols * p.ps + kTile - 1) / kTile + 1) *
+                       ((p.G * (int64_t)p.L + 7) / 8);
+  const int64_t most_prefix = (prefix_len / kTile + 1) * ((rows / p.H + 7) / 8);
+  if ((std::max(most, most_prefix) + kHeadTiles) * p.H > 0x7fffffff)
+    return set_last_error(SUNSHAPE_E_UNSUPPORTED, "paged attention: more than 2^31 tiles of 32 tokens in a call.");
   CUtensorMap vmap{};
   if (pool_rows)
     if (int rc = make_rows_map(&vmap, pages->value, pages->dtype == SUNSHAPE_BF16, dv, pool_rows, p.chunk)) return rc;

@@ -25,7 +25,7 @@ constexpr int kMinTiles = kPairs;  // tiles of a CTA's range, unless there are f
 constexpr int kHeadTiles = 16;     // tiles that the change to another head's codebook is charged in the split
 constexpr int kPlanChunks = 256;   // sequence chunks of the in-kernel plan
 // Registers of a thread: what the block is launched with, and its split between the roles (setmaxnreg).
-constexpr int kLaunchRegs = 128, kConsumerRegs = 208, kProducerRegs = 48;
+constexpr int kLaunchRegs = 128, kConsumerRegs = 216, kProducerRegs = 40;
 static_assert(kConsumerRegs + kProducerRegs <= 2 * kLaunchRegs, "the split waits forever where it exceeds the launch");
 
 // One row of a piece or partial set: acc[DV], m (in powers of two), l, two unused.

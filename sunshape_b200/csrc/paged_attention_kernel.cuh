@@ -17,6 +17,7 @@
 #pragma once
 
 #include <type_traits>
+#include <utility>
 
 #include "paged_attention.cuh"
 
@@ -57,20 +58,38 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t v) {
   return r;
 }
 
+// the address is addr + OFF, folded into the instruction
+template <int OFF>
 __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t* r, uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4+%5];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
+               : "r"(addr), "n"(OFF));
 }
 
-template <int BYTES>
+template <int BYTES, int OFF>
 __device__ __forceinline__ void lds_words(uint32_t* w, uint32_t addr) {
   if constexpr (BYTES == 16)
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4+%5];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "r"(addr), "n"(OFF));
   else if constexpr (BYTES == 8)
-    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2+%3];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr), "n"(OFF));
   else
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
+    asm volatile("ld.shared.u32 %0, [%1+%2];" : "=r"(w[0]) : "r"(addr), "n"(OFF));
+}
+
+// f(Index<0>()), ..., f(Index<N - 1>()): loops whose counter is a constant expression
+template <int I>
+struct Index {
+  static constexpr int v = I;
+};
+template <int... I, typename F>
+__device__ __forceinline__ void unrolled(std::integer_sequence<int, I...>, F&& f) {
+  (f(Index<I>()), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void unrolled(F&& f) {
+  unrolled(std::make_integer_sequence<int, N>(), f);
 }
 
 // dense block words (two 16-bit elements each) into the codebook's fp16 scale
@@ -94,7 +113,7 @@ constexpr float kSlack = 8.f;
 
 // Where a pair stands in the list; its producer and its consumer walk it alike.
 struct Walk {
-  int64_t at, end;       // tiles of the list
+  int at, end;           // tiles of the list
   int h, b, mt, t;       // the item and the tile within it
   int len, tiles;        // the sequence's length (-1: invalid) and tiles
 };
@@ -107,13 +126,15 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   constexpr int ROT = 16 / BD;                                 // tokens that share a load phase and a column set
   constexpr int KS = D / 16, ROWS = 8 * NT, RF = row_floats(DV);
   constexpr int IMAGE = D * 512;
+  constexpr int MT = 2;                                        // groups of 16 tokens of a step
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int ring_bytes = p.stages * p.stage_bytes;             // of a pair
   uint8_t* const image = ring + (size_t)p.pairs * ring_bytes;
   int* const perm_s = reinterpret_cast<int*>(image + IMAGE);                 // [D]
-  int64_t* const cum_s = reinterpret_cast<int64_t*>(perm_s + D);             // [kPlanChunks + 1]
-  uint64_t* const full_s = reinterpret_cast<uint64_t*>(cum_s + kPlanChunks + 1);   // [kPairs][stages]
+  int* const len_s = perm_s + D;                                             // [kPlanChunks] lengths, where chunks are single
+  int* const cum_s = len_s + kPlanChunks;                                    // [kPlanChunks + 2]
+  uint64_t* const full_s = reinterpret_cast<uint64_t*>(cum_s + kPlanChunks + 2);   // [kPairs][stages]
   uint64_t* const empty_s = full_s + kPairs * p.stages;
   uint64_t* const cb_bar = empty_s + kPairs * p.stages;
   // of a pair: head piece (-1: no tiles, 0: none, 1: cut again, 2: last), its item; tail piece (0, 1), its item
@@ -138,17 +159,21 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   const int mtiles = (rows_total + ROWS - 1) / ROWS;
   const int per = (seqs + kPlanChunks - 1) / kPlanChunks;
   if (tid < kPlanChunks) {
-    int64_t n = 0;
-    for (int i = tid * per; i < min(seqs, (tid + 1) * per); ++i) n += tiles_of(own_length(p, i));
+    int n = 0;
+    for (int i = tid * per; i < min(seqs, (tid + 1) * per); ++i) {
+      const int len = own_length(p, i);
+      n += tiles_of(len);
+      if (per == 1) len_s[i] = len;
+    }
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t u = __shfl_up_sync(0xffffffffu, n, o);
+      const int u = __shfl_up_sync(0xffffffffu, n, o);
       if (lane >= o) n += u;
     }
     cum_s[tid + 1] = n;          // within the warp's 32 chunks
   }
   if (tid == 0) cum_s[0] = 0;
   __syncthreads();
-  int64_t before = 0;
+  int before = 0;
   if (tid < kPlanChunks)
     for (int i = 0; i < warp; ++i) before += cum_s[i * 32 + 32];
   __syncthreads();
@@ -157,36 +182,40 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 
   // ---- this CTA's range.  With a codebook per head, a head's tiles are followed by kHeadTiles that stand for the
   // change and a range falls into one portion per head; with one codebook for all it is one portion.
-  const int64_t per_head = cum_s[kPlanChunks] * mtiles;
+  // the entry refuses calls whose tiles may not fit into 31 bits
+  const int per_head = cum_s[kPlanChunks] * mtiles;
   const int gap = p.n_cb > 1 ? kHeadTiles : 0;
-  const int64_t stride = per_head + gap, total = stride * p.H - gap;
+  const int stride = per_head + gap, total = stride * p.H - gap;
   const int cta = blockIdx.x;
-  const int grid = (int)min((int64_t)gridDim.x, (total + kMinTiles - 1) / kMinTiles);
+  const int grid = min((int)gridDim.x, (total + kMinTiles - 1) / kMinTiles);
+  asm volatile("griddepcontrol.launch_dependents;");           // the join waits for this grid's end by itself
   if (cta >= grid) {
     if (tid == 0) p.desc[cta] = make_int4(0, -1, 0, 0);
     return;
   }
-  const int64_t from = total * cta / grid, to = total * (cta + 1) / grid;
-  const int h0 = (int)(from / stride), h1 = (int)((to - 1) / stride);
+  // part i of n of a range of `size`: the first size % n parts are one longer
+  auto part = [](int size, int i, int n) { return size / n * i + min(i, size % n); };
+  const int from = part(total, cta, grid), to = part(total, cta + 1, grid);
+  const int h0 = from / stride, h1 = (to - 1) / stride;
   const int portions = gap ? h1 - h0 + 1 : 1;
+  auto length_of = [&](int b) { return per == 1 ? len_s[b] : own_length(p, b); };
 
   const int pair = warp & (kPairs - 1);
   Walk w;
   // the pair's part of portion k, in tiles without gaps
   auto enter = [&](int k) {
-    int64_t a = from, b = to;
+    int a = from, b = to;
     if (gap) {
       const int h = h0 + k;
-      a = max(from - h * stride, (int64_t)0) + h * per_head;
+      a = max(from - h * stride, 0) + h * per_head;
       b = min(to - h * stride, per_head) + h * per_head;
-      if (a > b) a = b;                        // the range begins in the gap behind head h
+      a = min(a, b);                           // the range begins in the gap behind head h
     }
-    const int n = p.pairs;
-    w.at = pair < n ? a + (b - a) * pair / n : b;
-    w.end = pair < n ? a + (b - a) * (pair + 1) / n : b;
+    w.at = pair < p.pairs ? a + part(b - a, pair, p.pairs) : b;
+    w.end = pair < p.pairs ? a + part(b - a, pair + 1, p.pairs) : b;
     if (w.at >= w.end) return;
-    w.h = (int)(w.at / per_head);
-    int64_t o = w.at - w.h * per_head;
+    w.h = w.at / per_head;
+    int o = w.at - w.h * per_head;
     int lo = 0, hi = kPlanChunks - 1;          // last chunk that begins at or before o
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -195,16 +224,16 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     }
     o -= cum_s[lo] * mtiles;
     w.b = lo * per;
-    w.len = own_length(p, w.b);
+    w.len = length_of(w.b);
     w.tiles = tiles_of(w.len);
-    while (o >= (int64_t)w.tiles * mtiles) {
-      o -= (int64_t)w.tiles * mtiles;
+    while (o >= w.tiles * mtiles) {
+      o -= w.tiles * mtiles;
       ++w.b;
-      w.len = own_length(p, w.b);
+      w.len = length_of(w.b);
       w.tiles = tiles_of(w.len);
     }
-    w.mt = (int)(o / w.tiles);
-    w.t = (int)(o - (int64_t)w.mt * w.tiles);
+    w.mt = o / w.tiles;
+    w.t = o - w.mt * w.tiles;
   };
   auto next_item = [&](int n) {                // n: tiles of the item just walked
     w.at += n;
@@ -216,7 +245,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       ++w.h;
     }
     if (w.at < w.end) {
-      w.len = own_length(p, w.b);
+      w.len = length_of(w.b);
       w.tiles = tiles_of(w.len);
     }
   };
@@ -237,7 +266,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     for (int k = 0; k < portions; ++k) {
       enter(k);
       while (w.at < w.end) {
-        const int n = (int)min(w.end - w.at, (int64_t)(w.tiles - w.t));
+        const int n = min(w.end - w.at, w.tiles - w.t);
         const int32_t* table = p.table + (int64_t)w.b * p.table_stride;
         // first token of this lane's copy in the group of tiles from number j on; -1: none
         auto token_of = [&](int j) {
@@ -301,12 +330,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   for (int u = 0; u < UNITS; ++u) hmask |= (uint32_t)(hslot_s[4 * u + t] >= 0) << u;
   const int rot = g & (ROT - 1);
   const uint32_t byte_sel = 0x4440u | t;       // byte t of an index word
-  uint32_t col_a[UNITS];                       // codebook column of the unit that slot u loads
+  // codebook column of the unit that slot x of a group loads; a group's blocks fill the columns, groups are 32 KB apart
+  uint32_t col_a[ROT];
 #pragma unroll
-  for (int u = 0; u < UNITS; ++u) {
-    const int b = 4 * ((u & ~(ROT - 1)) | ((u + rot) & (ROT - 1))) + t;
-    col_a[u] = image_a + (b / (64 / BD)) * 32768 + (b % (64 / BD)) * (2 * BD);
-  }
+  for (int x = 0; x < ROT; ++x) col_a[x] = image_a + (4 * ((x + rot) & (ROT - 1)) + t) * (2 * BD);
   uint32_t v_off[4];                           // this lane's ldmatrix row of 16 tokens x 16 columns, by column group
 #pragma unroll
   for (int d = 0; d < 4; ++d) {
@@ -330,14 +357,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     bool waited = false;
 
     while (w.at < w.end) {
-      const int n = (int)min(w.end - w.at, (int64_t)(w.tiles - w.t));
+      const int n = min(w.end - w.at, w.tiles - w.t);
       const int r0 = w.mt * ROWS, nr = min(ROWS, rows_total - r0);
       // Queries as the B operand: this lane's words of row 8c + g, scaled by a power of two into fp16.  A negative
       // scale goes into their sign, so that the factor of a row's scores is not negative and maxima can be taken
       // before it.
       uint32_t qb[NT][KS][2];
       float f[NT][2];
-      int seen[NT][2];
       const bool limited = p.causal && p.L > 1 && !p.prefix_mode;
 #pragma unroll
       for (int c = 0; c < NT; ++c) {
@@ -369,12 +395,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         for (int i = 0; i < D / 8; ++i)
           qb[c][i / 2][i % 2] = pack2<__half>(Elem<T>::to_float(raw[i][0]) * sc, Elem<T>::to_float(raw[i][1]) * sc);
         const float qf = fabsf(p.scale_log2) * __int_as_float((127 + ec) << 23) / k_scale;
-        // this lane's columns of S^T are the rows 8c + 2t + j: their factors, and the tokens that each sees
+        // this lane's columns of S^T are the rows 8c + 2t + j: their factors
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          f[c][j] = __shfl_sync(0xffffffffu, qf, 4 * (2 * t + j));
-          seen[c][j] = limited ? max(0, w.len - (p.L - 1 - (r0 + 8 * c + 2 * t + j) % p.L)) : w.len;
-        }
+        for (int j = 0; j < 2; ++j) f[c][j] = __shfl_sync(0xffffffffu, qf, 4 * (2 * t + j));
       }
       const int seen_all = limited ? max(0, w.len - (p.L - 1)) : w.len;
       if (!waited) {
@@ -387,10 +410,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       for (int c = 0; c < NT; ++c)
 #pragma unroll
         for (int i = 0; i < DV / 16; ++i) o[c][i][0] = o[c][i][1] = o[c][i][2] = o[c][i][3] = 0.f;
-      // m: the largest score before its factor, or one that it exceeds by at most kSlack after it; mb: m, 0 for none yet
-      float m[NT][2], mb[NT][2], l[NT][2];
+      // m: the largest score before its factor, or one that it exceeds by at most kSlack after it
+      float m[NT][2], l[NT][2];
 #pragma unroll
-      for (int c = 0; c < NT; ++c) m[c][0] = m[c][1] = -INF, mb[c][0] = mb[c][1] = l[c][0] = l[c][1] = 0.f;
+      for (int c = 0; c < NT; ++c) m[c][0] = m[c][1] = -INF, l[c][0] = l[c][1] = 0.f;
       bool bad = false;
       for (int i = 0; i < n; ++i) {
         const int first = (w.t + i) * kTile;
@@ -398,118 +421,6 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         uint8_t* const st = my_ring + stage * p.stage_bytes;
         const uint32_t st_a = smem_u32(st);
         bad |= *reinterpret_cast<volatile int*>(st + p.stage_bytes - 4) != 0;
-        float s[2][NT][4];
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-          uint32_t kw[2][D / 8];
-#pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const int tok = mt * 16 + y * 8 + g;
-            uint32_t ib[UNITS];
-#pragma unroll
-            for (int u = 0; u < UNITS; u += 4) {
-              if constexpr (UNITS >= 4) lds_words<16>(ib + u, st_a + p.off_idx + tok * NB + u * 4);
-              else lds_words<8>(ib + u, st_a + p.off_idx + tok * NB + u * 4);
-            }
-            // slot u loads unit (u + rot) mod ROT of its group of ROT units
-#pragma unroll
-            for (int u = 0; u < UNITS; ++u) {
-              uint32_t word = ib[u];
-#pragma unroll
-              for (int x = 1; x < ROT; ++x)
-                if (rot == x) word = ib[(u & ~(ROT - 1)) | ((u + x) & (ROT - 1))];
-              lds_words<2 * BD>(kw[y] + u * WORDS, col_a[u] + (__byte_perm(word, 0, byte_sel) << 7));
-            }
-            // put the units back in order: rotate each group by rot
-#pragma unroll
-            for (int u0 = 0; u0 < UNITS; u0 += ROT)
-#pragma unroll
-              for (int bit = 1; bit < ROT; bit <<= 1) {
-                uint32_t tmp[ROT * WORDS];
-#pragma unroll
-                for (int x = 0; x < ROT; ++x)
-#pragma unroll
-                  for (int z = 0; z < WORDS; ++z)
-                    tmp[x * WORDS + z] =
-                        (rot & bit) ? kw[y][(u0 + ((x - bit) & (ROT - 1))) * WORDS + z] : kw[y][(u0 + x) * WORDS + z];
-#pragma unroll
-                for (int x = 0; x < ROT * WORDS; ++x) kw[y][u0 * WORDS + x] = tmp[x];
-              }
-            if (p.n_heavy) {                       // dense blocks take the place of their codeword 0
-#pragma unroll
-              for (int u = 0; u < UNITS; ++u)
-                if ((hmask >> u) & 1) {
-                  uint32_t* dst = kw[y] + u * WORDS;
-                  lds_words<2 * BD>(dst, st_a + p.off_heavy + (tok * p.n_heavy + hslot_s[4 * u + t]) * (2 * BD));
-#pragma unroll
-                  for (int x = 0; x < WORDS; ++x) dst[x] = dense_word<T>(dst[x], k_scale);
-                }
-            }
-          }
-#pragma unroll
-          for (int c = 0; c < NT; ++c) {
-            s[mt][c][0] = s[mt][c][1] = s[mt][c][2] = s[mt][c][3] = 0.f;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
-              mma_f16(s[mt][c], kw[0][2 * ks], kw[1][2 * ks], kw[0][2 * ks + 1], kw[1][2 * ks + 1], qb[c][ks][0],
-                      qb[c][ks][1]);
-          }
-        }
-        // online softmax, in powers of two
-        const bool edge = first + kTile > seen_all;
-        if (edge) {
-#pragma unroll
-          for (int c = 0; c < NT; ++c)
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (first + (e >> 2) * 16 + ((e >> 1) & 1) * 8 + g >= seen[c][e & 1]) s[e >> 2][c][e & 3] = -INF;
-        }
-        bool grows = false;
-        float top[NT][2];
-#pragma unroll
-        for (int c = 0; c < NT; ++c)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            top[c][j] = fmaxf(fmaxf(s[0][c][j], s[0][c][j + 2]), fmaxf(s[1][c][j], s[1][c][j + 2]));
-            grows |= m[c][j] == -INF ? top[c][j] != -INF : (top[c][j] - m[c][j]) * f[c][j] > kSlack;
-          }
-        if (__any_sync(0xffffffffu, grows)) {
-#pragma unroll
-          for (int c = 0; c < NT; ++c)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              float x = top[c][j];
-#pragma unroll
-              for (int of = 4; of < 32; of <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, of));
-              const float nm = fmaxf(m[c][j], x);
-              const float e = m[c][j] == -INF ? 0.f : fast_exp2((m[c][j] - nm) * f[c][j]);
-              m[c][j] = nm;
-              mb[c][j] = nm == -INF ? 0.f : nm;
-              l[c][j] *= e;
-#pragma unroll
-              for (int d = 0; d < DV / 16; ++d) {
-                o[c][d][j] *= e;
-                o[c][d][j + 2] *= e;
-              }
-            }
-        }
-        uint32_t pb[2][NT][2];
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-          for (int c = 0; c < NT; ++c) {
-            float e[4];
-#pragma unroll
-            for (int x = 0; x < 4; ++x) e[x] = fast_exp2((s[mt][c][x] - mb[c][x & 1]) * f[c][x & 1]);
-            if (edge) {                            // -inf times a factor of zero
-#pragma unroll
-              for (int x = 0; x < 4; ++x) e[x] = s[mt][c][x] == -INF ? 0.f : e[x];
-            }
-            l[c][0] += e[0] + e[2];
-            l[c][1] += e[1] + e[3];
-            pb[mt][c][0] = movmatrix(pack2<T>(e[0], e[1]));
-            pb[mt][c][1] = movmatrix(pack2<T>(e[2], e[3]));
-          }
         if (first + kTile > w.len) {               // rows behind the end hold anything: zero times it is not zero
           for (int x = max(0, w.len - first) * (DV / 8) + lane; x < kTile * (DV / 8); x += 32) {
             const int tok = x / (DV / 8), c = x % (DV / 8);
@@ -518,15 +429,134 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           fence_proxy_async_smem();
           __syncwarp();
         }
+#pragma unroll 1
+        for (int half = 0; half < 2; half += MT) {
+          float s[MT][NT][4];
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
+          for (int mt = 0; mt < MT; ++mt) {
+            uint32_t kw[2][D / 8];
 #pragma unroll
-          for (int d = 0; d < DV / 16; ++d) {
+            for (int y = 0; y < 2; ++y) {
+              const int tok = (half + mt) * 16 + y * 8 + g;
+              uint32_t ib[UNITS];
+              const uint32_t idx_a = st_a + p.off_idx + tok * NB;
+              unrolled<(UNITS + 3) / 4>([&](auto i) {
+                lds_words<UNITS >= 4 ? 16 : 8, 16 * decltype(i)::v>(ib + 4 * decltype(i)::v, idx_a);
+              });
+              // slot u loads unit (u + rot) mod ROT of its group of ROT units
+              unrolled<UNITS>([&](auto i) {
+                constexpr int u = decltype(i)::v;
+                uint32_t word = ib[u];
+#pragma unroll
+                for (int x = 1; x < ROT; ++x)
+                  if (rot == x) word = ib[(u & ~(ROT - 1)) | ((u + x) & (ROT - 1))];
+                lds_words<2 * BD, (u / ROT) * 32768>(kw[y] + u * WORDS, col_a[u % ROT] + (__byte_perm(word, 0, byte_sel) << 7));
+              });
+              // put the units back in order: rotate each group by rot
+#pragma unroll
+              for (int u0 = 0; u0 < UNITS; u0 += ROT)
+#pragma unroll
+                for (int bit = 1; bit < ROT; bit <<= 1) {
+                  uint32_t tmp[ROT * WORDS];
+#pragma unroll
+                  for (int x = 0; x < ROT; ++x)
+#pragma unroll
+                    for (int z = 0; z < WORDS; ++z)
+                      tmp[x * WORDS + z] =
+                          (rot & bit) ? kw[y][(u0 + ((x - bit) & (ROT - 1))) * WORDS + z] : kw[y][(u0 + x) * WORDS + z];
+#pragma unroll
+                  for (int x = 0; x < ROT * WORDS; ++x) kw[y][u0 * WORDS + x] = tmp[x];
+                }
+              if (p.n_heavy) {                       // dense blocks take the place of their codeword 0
+#pragma unroll
+                for (int u = 0; u < UNITS; ++u)
+                  if ((hmask >> u) & 1) {
+                    uint32_t* dst = kw[y] + u * WORDS;
+                    lds_words<2 * BD, 0>(dst, st_a + p.off_heavy + (tok * p.n_heavy + hslot_s[4 * u + t]) * (2 * BD));
+#pragma unroll
+                    for (int x = 0; x < WORDS; ++x) dst[x] = dense_word<T>(dst[x], k_scale);
+                  }
+              }
+            }
+#pragma unroll
+            for (int c = 0; c < NT; ++c) {
+              s[mt][c][0] = s[mt][c][1] = s[mt][c][2] = s[mt][c][3] = 0.f;
+#pragma unroll
+              for (int ks = 0; ks < KS; ++ks)
+                mma_f16(s[mt][c], kw[0][2 * ks], kw[1][2 * ks], kw[0][2 * ks + 1], kw[1][2 * ks + 1], qb[c][ks][0],
+                        qb[c][ks][1]);
+            }
+          }
+          // online softmax, in powers of two
+          const int from_tok = first + half * 16;               // the step's first token
+          const bool edge = from_tok + MT * 16 > seen_all;
+          if (edge) {
+#pragma unroll
+            for (int c = 0; c < NT; ++c)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                // tokens that row 8c + 2t + j sees
+                const int seen = limited ? max(0, w.len - (p.L - 1 - (r0 + 8 * c + 2 * t + j) % p.L)) : w.len;
+#pragma unroll
+                for (int e = 0; e < 2 * MT; ++e)
+                  if (from_tok + e * 8 + g >= seen) s[e >> 1][c][(e & 1) * 2 + j] = -INF;
+              }
+          }
+          bool grows = false;
+          float top[NT][2];
+#pragma unroll
+          for (int c = 0; c < NT; ++c)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              top[c][j] = fmaxf(s[0][c][j], s[0][c][j + 2]);
+              if constexpr (MT == 2) top[c][j] = fmaxf(top[c][j], fmaxf(s[MT - 1][c][j], s[MT - 1][c][j + 2]));
+              grows |= m[c][j] == -INF ? top[c][j] != -INF : (top[c][j] - m[c][j]) * f[c][j] > kSlack;
+            }
+          if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+            for (int c = 0; c < NT; ++c)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                float x = top[c][j];
+#pragma unroll
+                for (int of = 4; of < 32; of <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, of));
+                const float nm = fmaxf(m[c][j], x);
+                const float e = m[c][j] == -INF ? 0.f : fast_exp2((m[c][j] - nm) * f[c][j]);
+                m[c][j] = nm;
+                l[c][j] *= e;
+#pragma unroll
+                for (int d = 0; d < DV / 16; ++d) {
+                  o[c][d][j] *= e;
+                  o[c][d][j + 2] *= e;
+                }
+              }
+          }
+          uint32_t pb[MT][NT][2];
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int c = 0; c < NT; ++c) {
+              float e[4];
+              const float mb[2] = {m[c][0] == -INF ? 0.f : m[c][0], m[c][1] == -INF ? 0.f : m[c][1]};
+#pragma unroll
+              for (int x = 0; x < 4; ++x) e[x] = fast_exp2((s[mt][c][x] - mb[x & 1]) * f[c][x & 1]);
+              if (edge) {                            // -inf times a factor of zero
+#pragma unroll
+                for (int x = 0; x < 4; ++x) e[x] = s[mt][c][x] == -INF ? 0.f : e[x];
+              }
+              l[c][0] += e[0] + e[2];
+              l[c][1] += e[1] + e[3];
+              pb[mt][c][0] = movmatrix(pack2<T>(e[0], e[1]));
+              pb[mt][c][1] = movmatrix(pack2<T>(e[2], e[3]));
+            }
+          unrolled<MT * DV / 16>([&](auto i) {
+            constexpr int mt = decltype(i)::v / (DV / 16), d = decltype(i)::v % (DV / 16);
             uint32_t v[4];
-            ldmatrix_x4_trans(v, st_a + v_off[d & 3] + (d >> 2) * (kTile * 128) + mt * 2048);
+            ldmatrix_x4_trans<(d >> 2) * (kTile * 128) + mt * 2048>(v, st_a + v_off[d & 3] + half * 2048);
 #pragma unroll
             for (int c = 0; c < NT; ++c) mma_pv<T>(o[c][d], v[0], v[1], v[2], v[3], pb[mt][c][0], pb[mt][c][1]);
-          }
+          });
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[stage]);
         if (++stage == p.stages) {
@@ -599,47 +629,68 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     named_barrier(1, kPairs * 32);
 
     // Items cut between pairs, in the list's order: each starts with a pair's tail piece (or, begun by an earlier
-    // CTA, with the first head piece) and goes on through head pieces.
-    for (int x = -1; x < kPairs; ++x) {
-      int y = x;
-      int4 item;
-      if (x < 0) {
-        y = 0;
-        while (y < kPairs && head_s[y].x < 0) ++y;
-        if (y == kPairs || head_s[y].x == 0) continue;
-        item = head_s[y];
-      } else {
-        if (tail_s[x].x == 0) continue;
-        item = tail_s[x];
-      }
+    // CTA, with the first head piece) and goes on through head pieces to the first that ends.  A warp takes one row
+    // of one item at a time, all of its pieces in flight at once.
+    const int4 hd = lane < kPairs ? head_s[lane] : make_int4(-1, 0, 0, 0);
+    const unsigned some = __ballot_sync(0xffffffffu, hd.x >= 0), heads = __ballot_sync(0xffffffffu, hd.x > 0);
+    const unsigned last = __ballot_sync(0xffffffffu, hd.x == 2);
+    const unsigned tails = __ballot_sync(0xffffffffu, lane < kPairs && tail_s[lane & (kPairs - 1)].x);
+    // chain 0: the first head piece; chain 1 + x: pair x's tail
+    unsigned chains = tails << 1 | ((some & (0u - some) & heads) != 0);
+    int task = warp;                                           // counts (chain, row) from the first chain on
+    for (; chains; chains &= chains - 1) {
+      const int x = __ffs(chains) - 2;
+      const int first = x < 0 ? __ffs(some) - 1 : x;
+      const int4 item = x < 0 ? head_s[first] : tail_s[x];
+      const unsigned behind = x < 0 ? ~0u << first : ~1u << x;
+      const unsigned ends = last & behind;
+      const unsigned upto = ends ? (ends & (0u - ends)) * 2 - 1 : ~0u;
+      const unsigned members = heads & behind & upto;          // whose head pieces belong to it
       const int nr = min(ROWS, rows_total - item.w * ROWS);
-      bool ended = x < 0 && item.x == 2;
-      int last = y;                                              // last pair of the item
-      for (int z = y + 1; z < kPairs && !ended; ++z) {
-        if (head_s[z].x <= 0) continue;
-        last = z;
-        ended = head_s[z].x == 2;
-      }
-      for (int e = tid; e < nr * (DV / 4); e += kPairs * 32) {
-        const int r = e / (DV / 4), d = e % (DV / 4) * 4;
-        const float* src = pieces + ((y * 2 + (x >= 0)) * ROWS + r) * RF;
-        float m = src[DV], l = src[DV + 1];
-        float4 a = *reinterpret_cast<const float4*>(src + d);
-        for (int z = y + 1; z <= last; ++z) {
-          if (head_s[z].x <= 0) continue;
-          src = pieces + (z * 2 * ROWS + r) * RF;
-          join4(m, l, a, src[DV], src[DV + 1], *reinterpret_cast<const float4*>(src + d));
+      if (x < 0) desc.x = ends ? 2 : 1;
+      else if (!ends) desc = make_int4(desc.x, item.y, item.z, item.w);
+      for (; task < nr; task += kPairs) {
+        const int d = lane * 4;
+        if (d < DV) {
+          float m[kPairs + 1], l[kPairs + 1], M = -INF;
+          float4 a[kPairs + 1];
+#pragma unroll
+          for (int z = 0; z <= kPairs; ++z) {
+            const bool in = z < kPairs ? (members >> z) & 1 : x >= 0;
+            m[z] = -INF;
+            if (in) {
+              const float* src = pieces + ((z < kPairs ? 2 * z : 2 * x + 1) * ROWS + task) * RF;
+              const float2 ml = *reinterpret_cast<const float2*>(src + DV);
+              m[z] = ml.x;
+              l[z] = ml.y;
+              a[z] = *reinterpret_cast<const float4*>(src + d);
+            }
+          }
+#pragma unroll
+          for (int z = 0; z <= kPairs; ++z) M = fmaxf(M, m[z]);
+          const float base = M == -INF ? 0.f : M;
+          float ls = 0.f;
+          float4 as = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int i = 0; i <= kPairs; ++i) {
+            const int z = (i + kPairs) % (kPairs + 1);         // the tail first
+            const bool in = z < kPairs ? (members >> z) & 1 : x >= 0;
+            if (in) {
+              const float e = fast_exp2(m[z] - base);
+              ls = fmaf(l[z], e, ls);
+              as = make_float4(fmaf(a[z].x, e, as.x), fmaf(a[z].y, e, as.y), fmaf(a[z].z, e, as.z), fmaf(a[z].w, e, as.w));
+            }
+          }
+          if (x >= 0 && ends) {
+            finish4<T, DV>(p, row_of(p, item.y, item.z, item.w * ROWS + task), d, M, ls, as);
+          } else {
+            float* dst = p.slots + ((int64_t)(2 * cta + (x < 0 ? 0 : 1)) * kItemRows + task) * RF;
+            *reinterpret_cast<float4*>(dst + d) = as;
+            if (d == 0) *reinterpret_cast<float2*>(dst + DV) = make_float2(M, ls);
+          }
         }
-        if (x >= 0 && ended) {
-          finish4<T, DV>(p, row_of(p, item.y, item.z, item.w * ROWS + r), d, m, l, a);
-        } else {
-          float* dst = p.slots + ((int64_t)(2 * cta + (x < 0 ? 0 : 1)) * kItemRows + r) * RF;
-          *reinterpret_cast<float4*>(dst + d) = a;
-          if (d == 0) *reinterpret_cast<float2*>(dst + DV) = make_float2(m, l);
-        }
       }
-      if (x < 0) desc.x = ended ? 2 : 1;
-      else if (!ended) desc = make_int4(desc.x, item.y, item.z, item.w);
+      task -= nr;
     }
     if (k + 1 < portions) named_barrier(1, kPairs * 32);
   }
