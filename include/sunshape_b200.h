@@ -263,14 +263,19 @@ typedef struct sunshape_pages {
   int32_t dtype;
 } sunshape_pages_t;
 
+/* What the paged kernels read of a codec (at most 256 codewords, block_dim 2, 4 or 8), derived from its codebooks
+ * once and kept as long as they stay: tables is a buffer of sunshape_paged_tables_bytes, 256-byte aligned. */
+int64_t sunshape_paged_tables_bytes(const sunshape_codec_t* codec);
+int sunshape_paged_tables(const sunshape_codec_t* codec, void* tables, int64_t tables_bytes, void* stream);
+
 /* Append key and value rows [batch, kv_heads, length, head_dim | value_dim] (dtype of the pages) to slots
  * [batch, length] (int64; -1 = leave the row out): the key is rotated (rotation NULL: taken as it is),
  * permuted and encoded to the nearest codeword of every block -- exactly: the first minimum of the distances
  * in real arithmetic as 64-bit floats give it, of the rotated key without an intermediate rounding -- or
  * kept, rounded to dtype, where the block is dense (index 0); the value is copied.  Slots must be distinct:
  * of two rows for one slot either may stay.  A slot outside [-1, num_pages * page_size) is left out and
- * records 132.  At most 256 codewords, block_dim 2, 4 or 8. */
-int sunshape_paged_append(const sunshape_codec_t* codec, const sunshape_pages_t* pages,
+ * records 132. */
+int sunshape_paged_append(const sunshape_codec_t* codec, const void* tables, const sunshape_pages_t* pages,
                           const sunshape_rows_t* key, const sunshape_rows_t* value, int32_t batch, int32_t length,
                           const int64_t* slots, int64_t slot_stride_b, int64_t slot_stride_l,
                           const sunshape_rotation_t* rotation, void* stream);
@@ -284,9 +289,6 @@ int sunshape_paged_append(const sunshape_codec_t* codec, const sunshape_pages_t*
  * The last query_len tokens of a sequence are the queries' own: query l sees all but the last
  * query_len - 1 - l of the sequence's own tokens (and all of the prefix); causal = 0: all of them.  A row
  * that sees no token is zero.  Softmax of scale * <q, k_hat>, statistics and sums in fp32.
- * codebook: [n_cb, head_dim / 64, 256, 64] fp16, the codewords times codebook_scale[n_cb] (a power of two):
- *   row (i, c) holds codeword c of the 64 / block_dim blocks from i * 64 / block_dim on, codewords above
- *   n_centroids zero.
  * head_dim and value_dim 64 or 128; block_dim 2, 4 or 8.  A page outside the pool records 133 and a length
  * outside [0, table_cols * page_size] 134; both make the sequence's rows NaN.
  * workspace: sunshape_paged_attention_workspace_bytes, 256-byte aligned, needs no initial value and keeps
@@ -294,9 +296,9 @@ int sunshape_paged_append(const sunshape_codec_t* codec, const sunshape_pages_t*
 int64_t sunshape_paged_attention_workspace_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t query_len,
                                                  int32_t value_dim, int32_t table_cols, int32_t page_size,
                                                  int32_t prefix_len);
-int sunshape_paged_attention(const sunshape_codec_t* codec, const sunshape_pages_t* pages, const void* codebook,
-                             const float* codebook_scale, const sunshape_rows_t* query, int32_t batch,
-                             int32_t query_len, const int32_t* page_table, int64_t table_stride, int32_t table_cols,
+int sunshape_paged_attention(const sunshape_codec_t* codec, const void* tables, const sunshape_pages_t* pages,
+                             const sunshape_rows_t* query, int32_t batch, int32_t query_len,
+                             const int32_t* page_table, int64_t table_stride, int32_t table_cols,
                              const int32_t* seq_lens, const int32_t* prefix_table, int32_t prefix_len, float scale,
                              int32_t causal, void* out, void* workspace, int64_t workspace_bytes, void* stream);
 

@@ -34,6 +34,7 @@ EXPORTED_SYMBOLS = (
     "sunshape_exchange_error", "sunshape_index_row_bytes", "sunshape_pack_indices",
     "sunshape_attention_scores_packed", "sunshape_norm_rotate", "sunshape_paged_append",
     "sunshape_paged_attention_workspace_bytes", "sunshape_paged_attention", "sunshape_paged_error",
+    "sunshape_paged_tables_bytes", "sunshape_paged_tables",
 )
 
 
@@ -148,14 +149,17 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
                                                         f32, vp, i32, ctypes.POINTER(PeerGroupDesc), vp, i64, vp]
         pr, pt, pp = ctypes.POINTER(RowsDesc), ctypes.POINTER(RotationDesc), ctypes.POINTER(PagesDesc)
         lib.sunshape_norm_rotate.argtypes = [pr, pr, vp, pr, pr, vp, i32, i32, i32, i32, i32, f32, pt, vp]
-        lib.sunshape_paged_append.argtypes = [pc, pp, pr, pr, i32, i32, vp, i64, i64, pt, vp]
+        lib.sunshape_paged_tables_bytes.argtypes = [pc]
+        lib.sunshape_paged_tables_bytes.restype = ctypes.c_int64
+        lib.sunshape_paged_tables.argtypes = [pc, vp, i64, vp]
+        lib.sunshape_paged_append.argtypes = [pc, vp, pp, pr, pr, i32, i32, vp, i64, i64, pt, vp]
         lib.sunshape_paged_attention_workspace_bytes.argtypes = [i32] * 8
         lib.sunshape_paged_attention_workspace_bytes.restype = ctypes.c_int64
-        lib.sunshape_paged_attention.argtypes = [pc, pp, vp, vp, pr, i32, i32, vp, i64, i32, vp, vp, i32, f32, i32, vp, vp,
-                                                 i64, vp]
+        lib.sunshape_paged_attention.argtypes = [pc, vp, pp, pr, i32, i32, vp, i64, i32, vp, vp, i32, f32, i32, vp, vp, i64,
+                                                 vp]
         lib.sunshape_paged_error.argtypes = [ctypes.POINTER(ctypes.c_int32), i32]
         for name in ("sunshape_norm_rotate", "sunshape_paged_append", "sunshape_paged_attention",
-                     "sunshape_paged_error"):
+                     "sunshape_paged_error", "sunshape_paged_tables"):
             getattr(lib, name).restype = ctypes.c_int
         for name in ("sunshape_encode", "sunshape_dequantize", "sunshape_attention_scores",
                      "sunshape_decode_attention", "sunshape_merge_partials"):
@@ -372,16 +376,28 @@ def norm_rotate(dev, q: RowsDesc, q_out: RowsDesc, q_weight, k, k_out, k_weight,
                                                    batch, length, dim, eps, rotation, stream_ptr(dev)))
 
 
-def paged_append(dev, cd: CodecDesc, pages: PagesDesc, key: RowsDesc, value: RowsDesc, batch: int, length: int,
-                 slots: torch.Tensor, rotation) -> None:
+def paged_tables(cd: CodecDesc, dev) -> torch.Tensor:
+    """What the paged kernels read of a codec, in one buffer."""
+    lib = load_library()
+    n = lib.sunshape_paged_tables_bytes(cd)
+    if n < 0:
+        _check(int(n))
+    tables = torch.empty(n, dtype=torch.uint8, device=dev)
     with torch.cuda.device(dev):
-        _check(load_library().sunshape_paged_append(cd, pages, key, value, batch, length, ptr(slots), slots.stride(0),
-                                                    slots.stride(1), rotation, stream_ptr(dev)))
+        _check(lib.sunshape_paged_tables(cd, ptr(tables), n, stream_ptr(dev)))
+    return tables
 
 
-def paged_attention(dev, cd: CodecDesc, pages: PagesDesc, codebook: torch.Tensor, codebook_scale: torch.Tensor,
-                    query: RowsDesc, batch: int, query_len: int, page_table: torch.Tensor, seq_lens: torch.Tensor,
-                    prefix_table, prefix_len: int, scale: float, causal: bool, out: torch.Tensor) -> None:
+def paged_append(dev, cd: CodecDesc, tables: torch.Tensor, pages: PagesDesc, key: RowsDesc, value: RowsDesc, batch: int,
+                 length: int, slots: torch.Tensor, rotation) -> None:
+    with torch.cuda.device(dev):
+        _check(load_library().sunshape_paged_append(cd, ptr(tables), pages, key, value, batch, length, ptr(slots),
+                                                    slots.stride(0), slots.stride(1), rotation, stream_ptr(dev)))
+
+
+def paged_attention(dev, cd: CodecDesc, tables: torch.Tensor, pages: PagesDesc, query: RowsDesc, batch: int, query_len: int,
+                    page_table: torch.Tensor, seq_lens: torch.Tensor, prefix_table, prefix_len: int, scale: float,
+                    causal: bool, out: torch.Tensor) -> None:
     lib = load_library()
     cols = page_table.shape[1]
     with torch.cuda.device(dev):
@@ -390,7 +406,6 @@ def paged_attention(dev, cd: CodecDesc, pages: PagesDesc, codebook: torch.Tensor
         # a block of the allocator of the current stream (of the graph's own pool under capture): two streams or
         # two captured graphs never share one
         ws = torch.empty(max(need, 256), dtype=torch.uint8, device=dev)
-        _check(lib.sunshape_paged_attention(cd, pages, ptr(codebook), ptr(codebook_scale), query, batch, query_len,
-                                            ptr(page_table), page_table.stride(0), cols, ptr(seq_lens),
-                                            ptr(prefix_table), prefix_len, scale, 1 if causal else 0, ptr(out), ptr(ws),
-                                            ws.numel(), stream_ptr(dev)))
+        _check(lib.sunshape_paged_attention(cd, ptr(tables), pages, query, batch, query_len, ptr(page_table),
+                                            page_table.stride(0), cols, ptr(seq_lens), ptr(prefix_table), prefix_len,
+                                            scale, 1 if causal else 0, ptr(out), ptr(ws), ws.numel(), stream_ptr(dev)))

@@ -18,7 +18,7 @@ struct NormRotateParams {
   int64_t xs[2][3], ys[2][3];   // strides of (b, h, l), elements
   int heads[2];
   const void* w[2];
-  int w_dtype;
+  int w_dtype, w_vec;           // w_vec: weights are 16-byte aligned
   float eps;
   int L, dim, width;            // width: threads of a row (vector kernel)
   int chunks[2];                // head chunks of q and k per token
@@ -55,21 +55,41 @@ __device__ __forceinline__ void store8(T* p, const float* f) {
   for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = r.v[i];
 }
 
+// eight weights from element e on (a multiple of eight)
+__device__ __forceinline__ void load_weights(const void* w, int e, int dtype, bool vec, float* f) {
+  if (!vec) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = load_as_float(w, e + i, dtype);
+  } else if (dtype == SUNSHAPE_F32) {
+    Vec8<float> r;
+    load8(reinterpret_cast<const float*>(w) + e, r);
+    unpack8(r, f);
+  } else if (dtype == SUNSHAPE_BF16) {
+    Vec8<__nv_bfloat16> r;
+    load8(reinterpret_cast<const __nv_bfloat16*>(w) + e, r);
+    unpack8(r, f);
+  } else {
+    Vec8<__half> r;
+    load8(reinterpret_cast<const __half*>(w) + e, r);
+    unpack8(r, f);
+  }
+}
+
 // HC heads of one token and one tensor per group of `width` threads; heads of a group are `chunks` apart, so
 // neighbouring groups touch neighbouring rows.
 template <typename T, int HC, bool INTER>
 __global__ void __launch_bounds__(128) norm_rotate_vec(const __grid_constant__ NormRotateParams p) {
   const int W = p.width;
   const int s = threadIdx.x & (W - 1);
-  const int64_t item = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / W;
-  if (item >= p.items) return;            // whole groups leave: the shuffles below stay within a group
+  const unsigned item = (blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32) * (32 / W) + (threadIdx.x & 31) / W;
+  if (item >= (unsigned)p.items) return;            // whole groups leave: the shuffles below stay within a group
   const unsigned mask = W == 32 ? 0xffffffffu : ((1u << W) - 1) << ((threadIdx.x & 31) & ~(W - 1));
-  const int per = p.chunks[0] + p.chunks[1];
-  const int64_t token = item / per;
+  const unsigned per = p.chunks[0] + p.chunks[1];
+  const unsigned token = item / per;
   int chunk = (int)(item - token * per);
   const int which = chunk >= p.chunks[0];
   if (which) chunk -= p.chunks[0];
-  const int64_t b = token / p.L, l = token - b * p.L;
+  const int64_t b = token / (unsigned)p.L, l = token - (unsigned)b * (unsigned)p.L;
   const int heads = p.heads[which], step = p.chunks[which];
   const bool have = s * 16 < p.dim;       // the last threads of a group are idle when dim / 16 is no power of two
   const int R = p.rot.rot;
@@ -107,11 +127,8 @@ __global__ void __launch_bounds__(128) norm_rotate_vec(const __grid_constant__ N
   float w0[8], w1[8];
   const void* w = p.w[which];
   if (w && have) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      w0[i] = load_as_float(w, e0 + i, p.w_dtype);
-      w1[i] = load_as_float(w, e1 + i, p.w_dtype);
-    }
+    load_weights(w, e0, p.w_dtype, p.w_vec, w0);
+    load_weights(w, e1, p.w_dtype, p.w_vec, w1);
   }
 #pragma unroll
   for (int i = 0; i < HC; ++i) {
@@ -314,6 +331,7 @@ int sunshape_norm_rotate(const sunshape_rows_t* q, const sunshape_rows_t* q_out,
   if (p.tokens * (p.heads[0] + p.heads[1]) > (int64_t)1 << 31)
     return set_last_error(SUNSHAPE_E_UNSUPPORTED, "at most 2^31 rows a call.");
   p.w_dtype = weight_dtype;
+  p.w_vec = ((uintptr_t)q_weight | (uintptr_t)k_weight) % 16 == 0;
   p.eps = eps;
   p.L = length;
   p.dim = dim;

@@ -1,9 +1,19 @@
 // Append to a paged compressed cache: rotate, permute and encode keys, copy values, into token slots.
 //
-// index = argmin_c |z_b - C_b[c]|^2 for block b of the rotated, permuted key z.  The choice is made exactly:
-// a scan in fp32 of  |c|^2 - 2 z.c  (|z|^2 is common to all codewords) keeps the smallest and the second
-// smallest value, whose errors against real arithmetic are below E (see kBound); where they lie within 2 E of
-// each other the block is decided by a scan in 64 bits.
+// index = argmin_c |z_b - C_b[c]|^2 = argmax_c z_b.C_b[c] - |C_b[c]|^2 / 2  for block b of the rotated, permuted
+// key z, decided exactly in three steps of growing precision:
+//   1. on the tensor cores, z and c as sums of two fp16 numbers and -|c|^2 / 2 as the accumulator's start, every
+//      thread keeps the maximum of each group of 16 codewords that it sees.  Where one group alone comes within
+//      twice the error bound (kFilter) of the overall maximum, the answer is in it;
+//   2. its 16 codewords are compared in fp32, keeping the smallest and the second smallest distance.  Where they
+//      differ by more than twice the bound kBound, the smallest is the answer;
+//   3. otherwise (borders between codewords, repeated codewords, infinities and NaN) a warp scans the block in 64 bits.
+//
+// Bound by instructions: 256 distances for every block against 2 (D + Dv) bytes a key and head.  Step 1 takes per 16
+// tokens x 8 codewords one or two MMAs and four maxima -- comparing all in fp32 (the kernel before this) takes 8
+// multiply-adds and 3 comparisons a distance.
+#include <algorithm>
+
 #include "paged.cuh"
 
 namespace sunshape {
@@ -13,11 +23,15 @@ struct AppendParams {
   const void* key;
   const void* val;
   int64_t ks[3], vs[3];       // strides of (b, h, l), elements
-  int L, H, D, Dv, nb, bd, C, n_cb, ps, n_heavy;
+  int L, H, D, Dv, nb, C, n_cb, ps, n_heavy;
+  int blocks, splits;         // blocks of a CTA, CTAs that share a head's blocks
   int64_t tokens, slots_total;
   const int64_t* slots;
   int64_t slot_sb, slot_sl;
   const float* cb;
+  const uint2* frags;
+  const float* norms;
+  const float* bscale;
   const int64_t* perm;
   const uint8_t* heavy_mask;
   uint8_t* idx;
@@ -27,182 +41,438 @@ struct AppendParams {
   int* err;
 };
 
-// The fp32 scan's error: z rounded to fp32 (relative u = 2^-24), bd products summed by fma, |c|^2 summed by
-// fma, one last fma: at most u (bd + 2) (|c|^2 + 2 |z| |c|) <= 10 u (...) for bd <= 8; 16 covers the terms of
-// second order and the rounding of the bound itself, kTiny what underflows.
+// Step 1's error relative to |c|max (|z| + |c|max), the block's scale bringing |c|max below 1: each factor is off by at
+// most 2^-22 of itself + 2^-25 (its remainder in fp16), the product of the remainders is left out, and 24 products and
+// the start are summed in fp32 with at most 2^-23 of the largest term each: below 2^-18 in all.
+constexpr float kFilter = 1.f / 131072.f;
+// Step 2's: z rounded to fp32 (relative u = 2^-24), bd products summed by fma, |c|^2 summed by fma, one last fma: at most
+// u (bd + 2) (|c|^2 + 2 |z| |c|) <= 10 u (...) for bd <= 8; 16 covers the terms of second order and the rounding of the
+// bound itself, kTiny what underflows.
 constexpr float kBound = 16.f / 16777216.f;
 constexpr float kTiny = 1e-37f;
 
-constexpr int kTokens = 64;   // tokens of a CTA
-constexpr int kLanes = 4;     // threads that share a token's codewords
+constexpr int kWarps = 4;
+constexpr int kTokens = 32 * kWarps;   // tokens of a CTA: two groups of 16 a warp
 
 // element d of the rotated key in 64 bits: the products of a 16-bit by a 24-bit significand are exact
 template <typename T>
-__device__ __forceinline__ double rotated(const AppendParams& p, const T* row, int d, int64_t pos) {
+__device__ __forceinline__ double rotated(const Rotation& r, const T* row, int d, int64_t pos) {
   const double y = (double)Elem<T>::to_float(row[d]);
-  if (d >= p.rot.rot) return y;
+  if (d >= r.rot) return y;
   int other, i;
   bool second;
-  pair_of(p.rot, d, other, i, second);
+  pair_of(r, d, other, i, second);
   const double o = (double)Elem<T>::to_float(row[other]);
-  const double c = (double)p.rot.cos[pos * (p.rot.rot / 2) + i], s = (double)p.rot.sin[pos * (p.rot.rot / 2) + i];
+  const double c = (double)r.cos[pos * (r.rot / 2) + i], s = (double)r.sin[pos * (r.rot / 2) + i];
   return second ? y * c + o * s : y * c - o * s;
 }
 
 // slot of a token, -1 where it is left out; records what is out of range
 __device__ __forceinline__ int64_t slot_of(const AppendParams& p, int64_t b, int64_t l, int64_t& pos) {
   int64_t slot = p.slots[b * p.slot_sb + l * p.slot_sl];
+  pos = p.rot.rot ? position_of(p.rot, b, l) : 0;
   if (slot < -1 || slot >= p.slots_total) {
     record_error(p.err, kErrSlot);
     slot = -1;
   }
-  pos = 0;
-  if (slot >= 0 && p.rot.rot) {
-    pos = position_of(p.rot, b, l);
-    if (pos < 0 || pos >= p.rot.table_len) {
-      record_error(p.err, kErrPosition);
-      slot = -1;
-    }
+  if (slot >= 0 && p.rot.rot && (pos < 0 || pos >= p.rot.table_len)) {
+    record_error(p.err, kErrPosition);
+    slot = -1;
   }
   return slot;
 }
 
-// grid (token tiles, heads, blocks + 1): the last z copies the values
-template <typename T, int BD>
-__global__ void __launch_bounds__(kTokens * kLanes) append_kernel(const __grid_constant__ AppendParams p) {
-  __shared__ __align__(16) float cb_s[256 * BD];
-  __shared__ float cn_s[256];
-  __shared__ int cmax_s;
-  const int tid = threadIdx.x, h = blockIdx.y, blk = blockIdx.z;
-  const int64_t t = (int64_t)blockIdx.x * kTokens + tid / kLanes;
-  const int s = tid % kLanes;
-  int64_t b = 0, l = 0, slot = -1, pos = 0;
-  if (t < p.tokens) {
-    b = t / p.L;
-    l = t - b * p.L;
-    slot = slot_of(p, b, l, pos);
-  }
-  const int64_t row = slot < 0 ? 0 : (slot / p.ps * p.H + h) * p.ps + slot % p.ps;   // page row of this head
-  if (blk == p.nb) {
-    if (slot < 0) return;
-    const T* src = reinterpret_cast<const T*>(p.val) + b * p.vs[0] + h * p.vs[1] + l * p.vs[2];
-    T* dst = reinterpret_cast<T*>(p.out_val) + row * p.Dv;
-    if ((uintptr_t)src % 16 == 0) {
-      for (int i = s; i < p.Dv / 8; i += kLanes)
-        reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(src)[i];
-    } else {
-      for (int i = s; i < p.Dv; i += kLanes) dst[i] = src[i];
-    }
-    return;
-  }
-  const T* krow = reinterpret_cast<const T*>(p.key) + b * p.ks[0] + h * p.ks[1] + l * p.ks[2];
-  if (p.heavy_mask && p.heavy_mask[blk]) {
-    if (slot < 0) return;
-    int at = 0;
-    for (int i = 0; i < blk; ++i) at += p.heavy_mask[i] != 0;
-    T* dst = reinterpret_cast<T*>(p.heavy) + (row * p.n_heavy + at) * BD;
-    for (int w = s; w < BD; w += kLanes)
-      dst[w] = Elem<T>::from_float((float)rotated(p, krow, (int)p.perm[blk * BD + w], pos));
-    if (s == 0) p.idx[row * p.nb + blk] = 0;
-    return;
-  }
-  const float* cb = p.cb + ((int64_t)(p.n_cb == 1 ? 0 : h % p.n_cb) * p.nb + blk) * p.C * BD;
-  if (tid == 0) cmax_s = 0;
-  for (int i = tid; i < p.C * BD; i += blockDim.x) cb_s[i] = cb[i];
-  __syncthreads();
-  for (int c = tid; c < p.C; c += blockDim.x) {
-    float n = 0.f;
-#pragma unroll
-    for (int w = 0; w < BD; ++w) n = fmaf(cb_s[c * BD + w], cb_s[c * BD + w], n);
-    cn_s[c] = n;
-    atomicMax(&cmax_s, __float_as_int(n));       // not negative: ordered as integers; NaN above all
-  }
-  __syncthreads();
-  const float INF = __int_as_float(0x7f800000);
-  double z[BD];
-  float x[BD], zn = 0.f;
+__device__ __forceinline__ void mma_k16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_k8(float* c, uint32_t a0, uint32_t a1, uint32_t b0) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(b0));
+}
+
+// two fp32 numbers as a pair of fp16 and the pair of their remainders
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const __half2 l = __floats2half2_rn(x - __low2float(h), y - __high2float(h));
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+// Which codewords of a lane's fragment row: the contraction of a block is over its BD elements, z_hi c_hi + z_lo c_hi +
+// z_hi c_lo, laid into the MMA's K:
+//   BD 8: one k16 step [z_hi | z_lo] [c_hi | c_hi] and one k8 step z_hi c_lo
+//   BD 4: one k16 step [z_hi | z_lo | z_hi | 0] [c_hi | c_hi | c_lo | 0]
+//   BD 2: one k8 step  [z_hi | z_lo | z_hi | 0] [c_hi | c_hi | c_lo | 0]
+
+// Codebooks into the attention image and the encoder's fragments: a CTA a block, a thread a codeword.
+template <int BD>
+__global__ void __launch_bounds__(256) tables_kernel(const float* cb, const float* norm_max, int C, int nb, int D,
+                                                     uint8_t* out, Tables at) {
+  __shared__ float red[256];
+  __shared__ float v_s[256][BD];
+  const int blk = blockIdx.x, k = blockIdx.y, c = threadIdx.x;
+  const float* block = cb + ((int64_t)k * nb + blk) * C * BD;
+  float n = 0.f;
 #pragma unroll
   for (int w = 0; w < BD; ++w) {
-    z[w] = slot < 0 ? 0.0 : rotated(p, krow, (int)p.perm[blk * BD + w], pos);
-    x[w] = (float)z[w];
-    zn = fmaf(x[w], x[w], zn);
+    v_s[c][w] = c < C ? block[c * BD + w] : 0.f;
+    n = fmaf(v_s[c][w], v_s[c][w], n);
   }
-  float best = INF, next = INF;
-  int at = p.C;
-  for (int c = s; c < p.C; c += kLanes) {
-    float dot = 0.f;
+  // largest norm of the block, and of the codebook where the caller did not give it
+  float all = n;
+  if (!norm_max)
+    for (int i = c; i < nb * C; i += 256) {
+      float m = 0.f;
+      for (int w = 0; w < BD; ++w) {
+        const float v = cb[((int64_t)k * nb * C + i) * BD + w];
+        m = fmaf(v, v, m);
+      }
+      all = fmaxf(all, m);
+    }
+  auto most = [&](float v) {
+    __syncthreads();
+    red[c] = v;
+    __syncthreads();
+    for (int o = 128; o; o >>= 1) {
+      if (c < o) red[c] = fmaxf(red[c], red[c + o]);
+      __syncthreads();
+    }
+    return red[0];
+  };
+  // the power of two that brings a norm into [0.5, 1); 1 for 0
+  auto factor = [](float norm) {
+    if (!(norm > 0.f)) return 1.f;
+    int e;
+    frexpf(norm, &e);
+    return ldexpf(1.f, -max(-100, min(100, e)));
+  };
+  const float bs = factor(sqrtf(most(n)));
+  const float is = factor(norm_max ? norm_max[k] : sqrtf(most(all)));
+  constexpr int PER = 64 / BD;      // blocks of an image row
+  __half* image = reinterpret_cast<__half*>(out + at.image) +
+                  (((int64_t)k * ((D + 63) / 64) + blk / PER) * 256 + c) * 64 + blk % PER * BD;
 #pragma unroll
-    for (int w = 0; w < BD; ++w) dot = fmaf(x[w], cb_s[c * BD + w], dot);
-    const float d = fmaf(-2.f, dot, cn_s[c]);
-    if (d < best) {
-      next = best;
-      best = d;
-      at = c;
+  for (int w = 0; w < BD; ++w) image[w] = __float2half_rn(v_s[c][w] * is);
+  reinterpret_cast<float*>(out + at.norms)[((int64_t)k * nb + blk) * 256 + c] = c < C ? -0.5f * (n * bs) * bs : -1e30f;
+  if (c == 0) {
+    reinterpret_cast<float*>(out + at.bscale)[(int64_t)k * nb + blk] = bs;
+    if (blk == 0) reinterpret_cast<float*>(out + at.iscale)[k] = is;
+  }
+  uint2* frags = reinterpret_cast<uint2*>(out + at.frags) + ((int64_t)k * nb + blk) * 1024;
+  for (int i = c; i < 1024; i += 256) {
+    const int word = i >> 5, g = (i & 31) >> 2, t = i & 3;
+    const float* v = v_s[word * 8 + g];
+    uint32_t hi, lo;
+    uint2 f = make_uint2(0u, 0u);
+    if constexpr (BD == 8) {
+      split2(v[2 * t] * bs, v[2 * t + 1] * bs, hi, lo);
+      f = make_uint2(hi, lo);
+    } else if constexpr (BD == 4) {
+      split2(v[2 * (t & 1)] * bs, v[2 * (t & 1) + 1] * bs, hi, lo);
+      f = make_uint2(hi, t < 2 ? lo : 0u);
     } else {
-      next = fminf(next, d);
+      split2(v[0] * bs, v[1] * bs, hi, lo);
+      f = make_uint2(t < 2 ? hi : (t == 2 ? lo : 0u), 0u);
     }
+    frags[i] = f;
   }
-#pragma unroll
-  for (int o = 1; o < kLanes; o <<= 1) {
-    const float ob = __shfl_xor_sync(0xffffffffu, best, o), on = __shfl_xor_sync(0xffffffffu, next, o);
-    const int oa = __shfl_xor_sync(0xffffffffu, at, o);
-    next = fminf(fminf(next, on), fmaxf(best, ob));
-    if (ob < best) {
-      best = ob;
-      at = oa;
+}
+
+// grid (token tiles, heads, splits + 1): the last z copies the values
+template <typename T, int BD>
+__global__ void __launch_bounds__(kWarps * 32) append_kernel(const __grid_constant__ AppendParams p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int width = p.blocks * BD, ld = width + 8;                 // permuted elements of this CTA, row stride
+  float* const z_s = reinterpret_cast<float*>(smem);               // [kTokens][ld]
+  float* const cb_s = z_s + kTokens * ld;                          // [256][BD]
+  uint2* const frag_s = reinterpret_cast<uint2*>(cb_s + 256 * BD); // [32][32]
+  float* const norm_s = reinterpret_cast<float*>(frag_s + 1024);   // [256]
+  int64_t* const slot_s = reinterpret_cast<int64_t*>(norm_s + 256);   // [kTokens] page row of this head, -1: left out
+  int64_t* const pos_s = slot_s + kTokens;
+  int64_t* const key_s = pos_s + kTokens;                          // offset of the key row
+  uint8_t* const idx_s = reinterpret_cast<uint8_t*>(key_s + kTokens);   // [kTokens][blocks]
+  __shared__ int most_s;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y;
+  const int64_t t0 = (int64_t)blockIdx.x * kTokens;
+  const int n_tok = (int)min((int64_t)kTokens, p.tokens - t0);
+  const bool values = blockIdx.z == p.splits;
+  if (tid < kTokens) {
+    int64_t slot = -1, pos = 0, at = 0;
+    if (tid < n_tok) {
+      const int64_t b = (t0 + tid) / p.L, l = t0 + tid - b * p.L;
+      slot = slot_of(p, b, l, pos);
+      if (slot >= 0) slot = (slot / p.ps * p.H + h) * p.ps + slot % p.ps;
+      at = values ? b * p.vs[0] + h * p.vs[1] + l * p.vs[2] : b * p.ks[0] + h * p.ks[1] + l * p.ks[2];
     }
+    slot_s[tid] = slot;
+    pos_s[tid] = pos;
+    key_s[tid] = at;
   }
-  const float cm2 = __int_as_float(cmax_s);
-  const float E = kBound * (cm2 + 2.f * sqrtf(zn) * sqrtf(cm2)) + kTiny;
-  const bool unsure = slot >= 0 && !(next - best > 2.f * E);    // NaN and infinities are unsure
-  if (__any_sync(0xffffffffu, unsure)) {
-    double bd64 = __longlong_as_double(0x7ff0000000000000ll);
-    int a64 = p.C;
-    if (unsure) {
-      for (int c = s; c < p.C; c += kLanes) {
-        double d = 0.0;
+  __syncthreads();
+  if (values) {
+    const T* const v = reinterpret_cast<const T*>(p.val);
+    T* const out = reinterpret_cast<T*>(p.out_val);
+    const int per = p.Dv / 8;
+    for (int i = tid; i < n_tok * per; i += kWarps * 32) {
+      const int tok = i / per, d = (i - tok * per) * 8;
+      if (slot_s[tok] < 0) continue;
+      const T* src = v + key_s[tok] + d;
+      T* dst = out + slot_s[tok] * p.Dv + d;
+      if ((uintptr_t)src % 16 == 0) {
+        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
+      } else {
+        for (int j = 0; j < 8; ++j) dst[j] = src[j];
+      }
+    }
+    return;
+  }
+  const int b0 = blockIdx.z * p.blocks, nblk = min(p.blocks, p.nb - b0);
+  const T* const keys = reinterpret_cast<const T*>(p.key);
+  // rotated keys, rounded once to fp32
+  for (int i = tid; i < n_tok * width; i += kWarps * 32) {
+    const int tok = i / width, e = i - tok * width;
+    if (e >= nblk * BD) continue;
+    z_s[tok * ld + e] = slot_s[tok] < 0 ? 0.f : (float)rotated(p.rot, keys + key_s[tok], (int)p.perm[b0 * BD + e], pos_s[tok]);
+  }
+  const int64_t kb = (int64_t)(p.n_cb == 1 ? 0 : h % p.n_cb) * p.nb;
+  const int g = lane >> 2, t = lane & 3;
+  const float INF = __int_as_float(0x7f800000);
+  const int w0 = warp * 32;                     // the warp's first token
+
+  for (int j = 0; j < nblk; ++j) {
+    const int blk = b0 + j;
+    __syncthreads();                            // keys are staged, the last block's codebook is read
+    if (p.heavy_mask && p.heavy_mask[blk]) {
+      int at = 0;
+      for (int i = 0; i < blk; ++i) at += p.heavy_mask[i] != 0;
+      for (int i = tid; i < n_tok * BD; i += kWarps * 32) {
+        const int tok = i / BD, w = i % BD;
+        if (slot_s[tok] >= 0)
+          reinterpret_cast<T*>(p.heavy)[(slot_s[tok] * p.n_heavy + at) * BD + w] = Elem<T>::from_float(z_s[tok * ld + j * BD + w]);
+      }
+      if (tid < n_tok) idx_s[tid * p.blocks + j] = 0;
+      continue;
+    }
+    const float* cb = p.cb + (kb + blk) * p.C * BD;
+    const float4* fr = reinterpret_cast<const float4*>(p.frags + (kb + blk) * 1024);
+    if (tid == 0) most_s = 0;
+    for (int i = tid; i < 512; i += kWarps * 32) reinterpret_cast<float4*>(frag_s)[i] = fr[i];
+    for (int i = tid; i < p.C * BD; i += kWarps * 32) cb_s[i] = cb[i];
+    for (int i = tid; i < 256; i += kWarps * 32) norm_s[i] = p.norms[(kb + blk) * 256 + i];
+    const float scale = p.bscale[kb + blk];
+    __syncthreads();
+    for (int c = tid; c < p.C; c += kWarps * 32) {                 // largest |c|^2, as step 2 sums it
+      float n = 0.f;
 #pragma unroll
-        for (int w = 0; w < BD; ++w) {
-          const double e = z[w] - (double)cb_s[c * BD + w];
-          d = fma(e, e, d);
-        }
-        if (d < bd64) {
-          bd64 = d;
-          a64 = c;
+      for (int w = 0; w < BD; ++w) n = fmaf(cb_s[c * BD + w], cb_s[c * BD + w], n);
+      atomicMax(&most_s, __float_as_int(n));                       // not negative: ordered as integers, NaN above all
+    }
+    // ---- step 1
+    uint32_t a[2][4], a8[2][2];
+    float bound[2][2];                                             // twice the error of rows g and g + 8
+    const bool some[2] = {w0 < n_tok, w0 + 16 < n_tok};
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const float* z = z_s + min(w0 + mt * 16 + y * 8 + g, n_tok - 1) * ld + j * BD;
+        float q = 0.f;
+#pragma unroll
+        for (int w = 0; w < BD; ++w) q = fmaf(z[w] * scale, z[w] * scale, q);
+        bound[mt][y] = 2.f * kFilter * (sqrtf(q) + 1.f);
+        uint32_t hi, lo;
+        const int e = BD == 8 ? 2 * t : (BD == 4 ? 2 * (t & 1) : 0);
+        split2(z[e] * scale, z[e + 1] * scale, hi, lo);
+        if constexpr (BD == 8) {
+          a[mt][y] = hi;
+          a[mt][2 + y] = lo;
+          a8[mt][y] = hi;
+        } else if constexpr (BD == 4) {
+          a[mt][y] = t < 2 ? hi : lo;
+          a[mt][2 + y] = t < 2 ? hi : 0u;
+        } else {
+          a8[mt][y] = t == 1 ? lo : (t == 3 ? 0u : hi);
         }
       }
     }
+    float top[2][2][4];                                            // maxima of groups of eight n-tiles
 #pragma unroll
-    for (int o = 1; o < kLanes; o <<= 1) {
-      const double od = __shfl_xor_sync(0xffffffffu, bd64, o);
-      const int oa = __shfl_xor_sync(0xffffffffu, a64, o);
-      if (od < bd64 || (od == bd64 && oa < a64)) {
-        bd64 = od;
-        a64 = oa;
+    for (int grp = 0; grp < 4; ++grp) {
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) top[mt][0][grp] = top[mt][1][grp] = -INF;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int nt = grp * 8 + i;
+        const uint2 f = frag_s[nt * 32 + lane];
+        const float2 nn = *reinterpret_cast<const float2*>(norm_s + nt * 8 + 2 * t);
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+          float s[4] = {nn.x, nn.y, nn.x, nn.y};
+          if constexpr (BD == 8) {
+            mma_k16(s, a[mt], f.x, f.x);
+            mma_k8(s, a8[mt][0], a8[mt][1], f.y);
+          } else if constexpr (BD == 4) {
+            mma_k16(s, a[mt], f.x, f.y);
+          } else {
+            mma_k8(s, a8[mt][0], a8[mt][1], f.x);
+          }
+          top[mt][0][grp] = fmaxf(top[mt][0][grp], fmaxf(s[0], s[1]));
+          top[mt][1][grp] = fmaxf(top[mt][1][grp], fmaxf(s[2], s[3]));
+        }
       }
     }
-    if (unsure) at = a64;
+    __syncthreads();                                               // most_s
+    const float cm2 = __int_as_float(most_s);
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+      if (!some[mt]) continue;
+      // the group of 16 codewords (lane of the quad, n-tile group) that alone is near the maximum; -1: not one
+      int where[2];
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        float m = fmaxf(fmaxf(top[mt][y][0], top[mt][y][1]), fmaxf(top[mt][y][2], top[mt][y][3]));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        int v = 0;                                                 // number of groups, and the sum of what names them
+#pragma unroll
+        for (int grp = 0; grp < 4; ++grp)
+          if (top[mt][y][grp] >= m - bound[mt][y]) v += 256 + (grp * 4 + t);
+        v += __shfl_xor_sync(0xffffffffu, v, 1);
+        v += __shfl_xor_sync(0xffffffffu, v, 2);
+        // a bound that is no number, or a key beyond fp16 in the block's scale, decides nothing
+        where[y] = (v >> 8) == 1 && bound[mt][y] < 2.f * kFilter * 30000.f ? v & 255 : -1;
+      }
+      // ---- step 2: two lanes a token
+      const int r = lane >> 1, half = lane & 1, tok = w0 + mt * 16 + r;
+      const int from_lo = __shfl_sync(0xffffffffu, where[0], (r & 7) * 4);
+      const int from_hi = __shfl_sync(0xffffffffu, where[1], (r & 7) * 4);
+      const int found = r < 8 ? from_lo : from_hi;
+      const bool live = tok < n_tok && slot_s[min(tok, n_tok - 1)] >= 0;
+      const float* z = z_s + min(tok, n_tok - 1) * ld + j * BD;
+      float x[BD], zn = 0.f, best = INF, next = INF;
+      int at = p.C;
+#pragma unroll
+      for (int w = 0; w < BD; ++w) {
+        x[w] = z[w];
+        zn = fmaf(x[w], x[w], zn);
+      }
+      if (found >= 0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int c = ((found >> 2) * 8 + half * 4 + (i >> 1)) * 8 + 2 * (found & 3) + (i & 1);
+          if (c >= p.C) continue;
+          const float* v = cb_s + c * BD;
+          float dot = 0.f, n = 0.f;
+#pragma unroll
+          for (int w = 0; w < BD; ++w) {
+            dot = fmaf(x[w], v[w], dot);
+            n = fmaf(v[w], v[w], n);
+          }
+          const float d = fmaf(-2.f, dot, n);
+          if (d < best) {
+            next = best;
+            best = d;
+            at = c;
+          } else {
+            next = fminf(next, d);
+          }
+        }
+      }
+      const float ob = __shfl_xor_sync(0xffffffffu, best, 1), on = __shfl_xor_sync(0xffffffffu, next, 1);
+      const int oa = __shfl_xor_sync(0xffffffffu, at, 1);
+      next = fminf(fminf(next, on), fmaxf(best, ob));
+      if (ob < best) {
+        best = ob;
+        at = oa;
+      }
+      const float E = kBound * (cm2 + 2.f * sqrtf(zn) * sqrtf(cm2)) + kTiny;
+      // ---- step 3
+      unsigned unsure = __ballot_sync(0xffffffffu, live && !(found >= 0 && next - best > 2.f * E));
+      for (; unsure; unsure &= unsure - 1, unsure &= unsure - 1) {   // both lanes of a token
+        const int who = __ffs(unsure) - 1, tk = w0 + mt * 16 + (who >> 1);
+        double zz[BD], bd64 = __longlong_as_double(0x7ff0000000000000ll);
+        int a64 = p.C;
+#pragma unroll
+        for (int w = 0; w < BD; ++w)
+          zz[w] = rotated(p.rot, keys + key_s[tk], (int)p.perm[blk * BD + w], pos_s[tk]);
+        for (int c = lane; c < p.C; c += 32) {
+          double d = 0.0;
+#pragma unroll
+          for (int w = 0; w < BD; ++w) {
+            const double e = zz[w] - (double)cb_s[c * BD + w];
+            d = fma(e, e, d);
+          }
+          if (d < bd64) {
+            bd64 = d;
+            a64 = c;
+          }
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double od = __shfl_xor_sync(0xffffffffu, bd64, o);
+          const int oc = __shfl_xor_sync(0xffffffffu, a64, o);
+          if (od < bd64 || (od == bd64 && oc < a64)) {
+            bd64 = od;
+            a64 = oc;
+          }
+        }
+        if ((lane >> 1) == (who >> 1)) at = a64;
+      }
+      if (live && half == 0) idx_s[tok * p.blocks + j] = (uint8_t)(at < p.C ? at : 0);   // no finite distance: 0
+    }
   }
-  if (slot >= 0 && s == 0) p.idx[row * p.nb + blk] = (uint8_t)(at < p.C ? at : 0);   // no finite distance: 0
+  __syncthreads();
+  if (nblk == p.nb && p.nb % 16 == 0) {
+    const int per = p.nb / 16;
+    for (int i = tid; i < n_tok * per; i += kWarps * 32) {
+      const int tok = i / per, q = i - tok * per;
+      if (slot_s[tok] >= 0)
+        reinterpret_cast<uint4*>(p.idx + slot_s[tok] * p.nb)[q] = reinterpret_cast<const uint4*>(idx_s + tok * p.nb)[q];
+    }
+  } else {
+    for (int i = tid; i < n_tok * nblk; i += kWarps * 32) {
+      const int tok = i / nblk, q = i - tok * nblk;
+      if (slot_s[tok] >= 0) p.idx[slot_s[tok] * p.nb + b0 + q] = idx_s[tok * p.blocks + q];
+    }
+  }
+}
+
+template <typename T, int BD>
+void launch(AppendParams& p, cudaStream_t st) {
+  const int64_t tiles = (p.tokens + kTokens - 1) / kTokens;
+  // a head's blocks are shared out until every SM has two CTAs: one token a sequence leaves one tile of tokens
+  p.splits = (int)std::min<int64_t>(p.nb, std::max<int64_t>(1, 2 * sm_count() / (tiles * p.H)));
+  p.blocks = (p.nb + p.splits - 1) / p.splits;
+  p.splits = (p.nb + p.blocks - 1) / p.blocks;
+  const int smem = (kTokens * (p.blocks * BD + 8) + 256 * BD + 256) * 4 + 8192 + 3 * kTokens * 8 + kTokens * p.blocks;
+  cudaFuncSetAttribute(append_kernel<T, BD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  append_kernel<T, BD><<<dim3((unsigned)tiles, p.H, p.splits + 1), kWarps * 32, smem, st>>>(p);
 }
 
 template <typename T>
-void launch(const AppendParams& p, cudaStream_t st) {
-  const dim3 grid((unsigned)((p.tokens + kTokens - 1) / kTokens), p.H, p.nb + 1);
-  if (p.bd == 8) append_kernel<T, 8><<<grid, kTokens * kLanes, 0, st>>>(p);
-  else if (p.bd == 4) append_kernel<T, 4><<<grid, kTokens * kLanes, 0, st>>>(p);
-  else append_kernel<T, 2><<<grid, kTokens * kLanes, 0, st>>>(p);
+void launch(AppendParams& p, int bd, cudaStream_t st) {
+  if (bd == 8) launch<T, 8>(p, st);
+  else if (bd == 4) launch<T, 4>(p, st);
+  else launch<T, 2>(p, st);
+}
+
+int check_paged_codec(const sunshape_codec_t* c) {
+  if (int rc = check_codec_args(c)) return rc;
+  if (c->block_dim != 2 && c->block_dim != 4 && c->block_dim != 8)
+    return set_last_error(SUNSHAPE_E_UNSUPPORTED, "the paged cache takes block_dim 2, 4 or 8.");
+  if (c->n_centroids > 256)
+    return set_last_error(SUNSHAPE_E_UNSUPPORTED, "the paged cache takes at most 256 codewords a block.");
+  return SUNSHAPE_OK;
 }
 
 }  // namespace
 
 int check_pages(const sunshape_codec_t* c, const sunshape_pages_t* pg) {
-  if (int rc = check_codec_args(c)) return rc;
+  if (int rc = check_paged_codec(c)) return rc;
   if (!pg) return set_last_error(SUNSHAPE_E_INVALID, "page pool descriptor is NULL.");
-  if (c->block_dim != 2 && c->block_dim != 4 && c->block_dim != 8)
-    return set_last_error(SUNSHAPE_E_UNSUPPORTED, "the paged cache takes block_dim 2, 4 or 8.");
-  if (c->n_centroids > 256)
-    return set_last_error(SUNSHAPE_E_UNSUPPORTED, "the paged cache takes at most 256 codewords a block.");
   if (pg->dtype != SUNSHAPE_BF16 && pg->dtype != SUNSHAPE_F16)
     return set_last_error(SUNSHAPE_E_UNSUPPORTED, "the paged cache holds BF16 or F16 values.");
   if (pg->kv_heads < 1 || pg->kv_heads > 65535 || pg->num_pages < 0 || pg->page_size < 16 || pg->page_size % 16 ||
@@ -222,7 +492,35 @@ int check_pages(const sunshape_codec_t* c, const sunshape_pages_t* pg) {
 
 using namespace sunshape;
 
-extern "C" int sunshape_paged_append(const sunshape_codec_t* codec, const sunshape_pages_t* pages,
+extern "C" {
+
+int64_t sunshape_paged_tables_bytes(const sunshape_codec_t* codec) {
+  if (int rc = check_paged_codec(codec)) return rc;
+  return Tables(codec->n_cb, codec->head_dim / codec->block_dim, codec->head_dim).total;
+}
+
+int sunshape_paged_tables(const sunshape_codec_t* codec, void* tables, int64_t tables_bytes, void* stream) {
+  if (int rc = check_paged_codec(codec)) return rc;
+  const int nb = codec->head_dim / codec->block_dim;
+  const Tables at(codec->n_cb, nb, codec->head_dim);
+  if (!tables || (uintptr_t)tables % 256 || tables_bytes < at.total)
+    return set_last_error(SUNSHAPE_E_INVALID, "tables buffer missing, misaligned or too small.");
+  if (codec->n_cb > 65535) return set_last_error(SUNSHAPE_E_UNSUPPORTED, "at most 65535 codebooks.");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const dim3 grid(nb, codec->n_cb);
+  uint8_t* out = static_cast<uint8_t*>(tables);
+#define SUNSHAPE_TABLES_CASE(BD)                                                                                     \
+  if (codec->block_dim == BD)                                                                                        \
+    tables_kernel<BD><<<grid, 256, 0, st>>>(codec->centroids, codec->centroid_norm_max, codec->n_centroids, nb,      \
+                                            codec->head_dim, out, at);
+  SUNSHAPE_TABLES_CASE(2)
+  SUNSHAPE_TABLES_CASE(4)
+  SUNSHAPE_TABLES_CASE(8)
+#undef SUNSHAPE_TABLES_CASE
+  return launch_status("paged tables launch");
+}
+
+int sunshape_paged_append(const sunshape_codec_t* codec, const void* tables, const sunshape_pages_t* pages,
                                      const sunshape_rows_t* key, const sunshape_rows_t* value, int32_t batch,
                                      int32_t length, const int64_t* slots, int64_t slot_stride_b,
                                      int64_t slot_stride_l, const sunshape_rotation_t* rotation, void* stream) {
@@ -235,7 +533,8 @@ extern "C" int sunshape_paged_append(const sunshape_codec_t* codec, const sunsha
   if (int rc = make_rotation(rotation, codec->head_dim, batch == 0 || length == 0, &p.rot)) return rc;
   p.tokens = (int64_t)batch * length;
   if (p.tokens == 0) return SUNSHAPE_OK;
-  if (!key->data || !value->data || !slots) return set_last_error(SUNSHAPE_E_INVALID, "key / value / slots pointer is NULL.");
+  if (!key->data || !value->data || !slots || !tables)
+    return set_last_error(SUNSHAPE_E_INVALID, "key / value / slots pointer or tables are NULL.");
   if (p.tokens > (int64_t)1 << 30) return set_last_error(SUNSHAPE_E_UNSUPPORTED, "at most 2^30 rows a call.");
   p.key = key->data;
   p.val = value->data;
@@ -249,8 +548,7 @@ extern "C" int sunshape_paged_append(const sunshape_codec_t* codec, const sunsha
   p.H = pages->kv_heads;
   p.D = codec->head_dim;
   p.Dv = pages->value_dim;
-  p.bd = codec->block_dim;
-  p.nb = p.D / p.bd;
+  p.nb = p.D / codec->block_dim;
   p.C = codec->n_centroids;
   p.n_cb = codec->n_cb;
   p.ps = pages->page_size;
@@ -260,6 +558,11 @@ extern "C" int sunshape_paged_append(const sunshape_codec_t* codec, const sunsha
   p.slot_sb = slot_stride_b;
   p.slot_sl = slot_stride_l;
   p.cb = codec->centroids;
+  const Tables tab(p.n_cb, p.nb, p.D);
+  const uint8_t* base = static_cast<const uint8_t*>(tables);
+  p.frags = reinterpret_cast<const uint2*>(base + tab.frags);
+  p.norms = reinterpret_cast<const float*>(base + tab.norms);
+  p.bscale = reinterpret_cast<const float*>(base + tab.bscale);
   p.perm = codec->permutation;
   p.heavy_mask = p.n_heavy ? codec->heavy_mask : nullptr;
   p.idx = pages->indices;
@@ -268,7 +571,9 @@ extern "C" int sunshape_paged_append(const sunshape_codec_t* codec, const sunsha
   p.err = paged_error_word();
   if (!p.err) return set_last_error(SUNSHAPE_E_CUDA, "the paged error word is unavailable on this device.");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (pages->dtype == SUNSHAPE_BF16) launch<__nv_bfloat16>(p, st);
-  else launch<__half>(p, st);
+  if (pages->dtype == SUNSHAPE_BF16) launch<__nv_bfloat16>(p, codec->block_dim, st);
+  else launch<__half>(p, codec->block_dim, st);
   return launch_status("paged append launch");
 }
+
+}  // extern "C"

@@ -78,9 +78,9 @@ int64_t sunshape_paged_attention_workspace_bytes(int32_t batch, int32_t q_heads,
   return layout(sm_count(), rows, item_rows(prefix_len > 0 ? own * batch : own), value_dim, prefix_len > 0).total;
 }
 
-int sunshape_paged_attention(const sunshape_codec_t* codec, const sunshape_pages_t* pages, const void* codebook,
-                             const float* codebook_scale, const sunshape_rows_t* query, int32_t batch,
-                             int32_t query_len, const int32_t* page_table, int64_t table_stride, int32_t table_cols,
+int sunshape_paged_attention(const sunshape_codec_t* codec, const void* tables, const sunshape_pages_t* pages,
+                             const sunshape_rows_t* query, int32_t batch, int32_t query_len,
+                             const int32_t* page_table, int64_t table_stride, int32_t table_cols,
                              const int32_t* seq_lens, const int32_t* prefix_table, int32_t prefix_len, float scale,
                              int32_t causal, void* out, void* workspace, int64_t workspace_bytes, void* stream) {
   if (int rc = check_pages(codec, pages)) return rc;
@@ -99,9 +99,8 @@ int sunshape_paged_attention(const sunshape_codec_t* codec, const sunshape_pages
   if (rows == 0) return SUNSHAPE_OK;
   if (batch > 65535 || rows > (int64_t)1 << 30)
     return set_last_error(SUNSHAPE_E_UNSUPPORTED, "at most 65535 sequences and 2^30 query rows a call.");
-  if (!query->data || !out || !seq_lens || (table_cols && !page_table) || (prefix_len && !prefix_table) || !codebook ||
-      !codebook_scale)
-    return set_last_error(SUNSHAPE_E_INVALID, "query / out / seq_lens / page table / codebook pointer is NULL.");
+  if (!query->data || !out || !seq_lens || (table_cols && !page_table) || (prefix_len && !prefix_table) || !tables)
+    return set_last_error(SUNSHAPE_E_INVALID, "query / out / seq_lens / page table / tables pointer is NULL.");
   if (!workspace || (uintptr_t)workspace % 256 ||
       workspace_bytes < sunshape_paged_attention_workspace_bytes(batch, query->heads, pages->kv_heads, query_len,
                                                                  pages->value_dim, table_cols, pages->page_size,
@@ -134,8 +133,9 @@ int sunshape_paged_attention(const sunshape_codec_t* codec, const sunshape_pages
   p.heavy_mask = p.n_heavy ? codec->heavy_mask : nullptr;
   p.idx = pages->indices;
   p.heavy = pages->heavy;
-  p.image = codebook;
-  p.image_scale = codebook_scale;
+  const Tables tab(p.n_cb, p.nb, d);
+  p.image = static_cast<const uint8_t*>(tables) + tab.image;
+  p.image_scale = reinterpret_cast<const float*>(static_cast<const uint8_t*>(tables) + tab.iscale);
   p.out = out;
   const int grid = sm_count();
   const Layout at = layout(grid, rows, item_rows((prefix_len ? (int64_t)p.B : 1) * p.G * p.L), dv, prefix_len > 0);

@@ -170,7 +170,7 @@ class SunShapePagedCache:
         self.device = dev
         self._pages = _lib.PagesDesc(_lib.ptr(indices), _lib.ptr(heavy), _lib.ptr(values), indices.shape[0],
                                      indices.shape[1], indices.shape[2], values.shape[3], _lib.dtype_code(values))
-        self._image()
+        self._tables()
 
     @classmethod
     def from_pools(cls, codec, indices, values, heavy=None) -> "SunShapePagedCache":
@@ -192,24 +192,13 @@ class SunShapePagedCache:
     value_dim = property(lambda self: int(self.values.shape[3]))
     dtype = property(lambda self: self.values.dtype)
 
-    def _image(self):
-        """The codec's codewords as the attention kernel reads them (kept by the codec until ``invalidate``): fp16
-        times a power of two that puts a codebook's largest codeword norm into [0.5, 1), laid out [n_cb, D / 64,
-        256, 64] so that a block's codewords all lie in one 16-byte column of the shared-memory banks."""
-        c = self.codec
-        desc, keep, _ = c.kernel_desc()
-        kept = getattr(c, "_paged_image", None)
-        if kept is None or kept[2] is not keep[0]:
-            cents, norm = keep[0], keep[3]
-            n_cb, nb, C, bd = cents.shape
-            exponent = torch.where(norm > 0, torch.frexp(norm)[1], 0).clamp(-100, 100)
-            factor = torch.ldexp(torch.ones_like(norm), -exponent)
-            full = cents.new_zeros(n_cb, nb, 256, bd)
-            full[:, :, :C] = cents * factor[:, None, None, None]
-            if c.head_dim % 64 == 0:
-                full = full.view(n_cb, c.head_dim // 64, 64 // bd, 256, bd).transpose(2, 3)
-            kept = c._paged_image = (full.to(torch.float16).contiguous(), factor.contiguous(), cents)
-        return kept
+    def _tables(self) -> torch.Tensor:
+        """What the kernels read of the codec's codebooks, derived once and kept by the codec until ``invalidate``."""
+        desc, keep, _ = self.codec.kernel_desc()
+        kept = getattr(self.codec, "_paged_tables", None)
+        if kept is None or kept[1] is not keep[0]:
+            kept = self.codec._paged_tables = (_lib.paged_tables(desc, self.device), keep[0])
+        return kept[0]
 
     def slots(self, page_table: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
         """Slots [B, L] of the token positions [B, L] (within their sequences) under ``page_table`` [B, cols]; -1
@@ -255,8 +244,8 @@ def append_paged(cache: SunShapePagedCache, key: torch.Tensor, value: torch.Tens
     if slots.dtype != torch.int64 or slots.shape != (B, L):
         raise RuntimeError("slots must be int64 [batch, length].")
     rot = _rotation(cos, sin, positions, interleaved, B, L, D, dev)
-    _lib.paged_append(dev, codec.kernel_desc()[0], cache._pages, _rows(key, "key"), _rows(value, "value"), B, L, slots,
-                      rot)
+    _lib.paged_append(dev, codec.kernel_desc()[0], cache._tables(), cache._pages, _rows(key, "key"), _rows(value, "value"), B,
+                      L, slots, rot)
 
 
 def paged_attention(cache: SunShapePagedCache, query: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor, *,
@@ -303,8 +292,7 @@ def paged_attention(cache: SunShapePagedCache, query: torch.Tensor, page_table: 
         out = torch.empty(shape, dtype=query.dtype, device=dev)
     elif out.shape != shape or out.dtype != query.dtype or out.device != dev or not out.is_contiguous():
         raise RuntimeError("out must be contiguous [batch, q_heads, query_len, value_dim] of the query's dtype.")
-    image, factor, _ = cache._image()
-    _lib.paged_attention(dev, codec.kernel_desc()[0], cache._pages, image, factor, _rows(query, "query"), B, L, page_table,
+    _lib.paged_attention(dev, codec.kernel_desc()[0], cache._tables(), cache._pages, _rows(query, "query"), B, L, page_table,
                          seq_lens, prefix_table if prefix_len else None, prefix_len,
                          1.0 / math.sqrt(D) if scale is None else float(scale), causal, out)
     return out

@@ -37,21 +37,21 @@ def test_append_refusals():
     f = _lib.load_library().sunshape_paged_append
     cd = _lib.CodecDesc(16, 16, None, 1, 64, 8, 256, 0, None)
     pg = _lib.PagesDesc(16, None, 16, 4, 2, 16, 64, _lib.BF16)
-    assert f(cd, pg, _rows(), _rows(), 0, 1, 16, 1, 1, None, None) == 0
-    _expect(f(cd, None, _rows(), _rows(), 1, 1, 16, 1, 1, None, None), -1, "page pool descriptor")
-    _expect(f(cd, pg, _rows(3), _rows(), 1, 1, 16, 1, 1, None, None), -1, "kv_heads")
-    _expect(f(cd, pg, _rows(), _rows(), 1, 1, None, 1, 1, None, None), -1, "slots pointer")
+    assert f(cd, 256, pg, _rows(), _rows(), 0, 1, 16, 1, 1, None, None) == 0
+    _expect(f(cd, 256, None, _rows(), _rows(), 1, 1, 16, 1, 1, None, None), -1, "page pool descriptor")
+    _expect(f(cd, 256, pg, _rows(3), _rows(), 1, 1, 16, 1, 1, None, None), -1, "kv_heads")
+    _expect(f(cd, 256, pg, _rows(), _rows(), 1, 1, None, 1, 1, None, None), -1, "slots pointer")
     for change, code, text in ((dict(page_size=8), -1, "page_size"), (dict(dtype=_lib.F32), -2, "BF16 or F16"),
                                (dict(value=24), -1, "16-byte aligned"), (dict(indices=None), -1, "pool pointer")):
         bad = _lib.PagesDesc(16, None, 16, 4, 2, 16, 64, _lib.BF16)
         for k, v in change.items():
             setattr(bad, k, v)
-        _expect(f(cd, bad, _rows(), _rows(), 1, 1, 16, 1, 1, None, None), code, text)
-    _expect(f(_lib.CodecDesc(16, 16, None, 1, 64, 16, 256, 0, None), pg, _rows(), _rows(), 1, 1, 16, 1, 1, None, None), -2,
+        _expect(f(cd, 256, bad, _rows(), _rows(), 1, 1, 16, 1, 1, None, None), code, text)
+    _expect(f(_lib.CodecDesc(16, 16, None, 1, 64, 16, 256, 0, None), 256, pg, _rows(), _rows(), 1, 1, 16, 1, 1, None, None), -2,
             "block_dim 2, 4 or 8")
-    _expect(f(_lib.CodecDesc(16, 16, None, 1, 64, 8, 300, 0, None), pg, _rows(), _rows(), 1, 1, 16, 1, 1, None, None), -2,
+    _expect(f(_lib.CodecDesc(16, 16, None, 1, 64, 8, 300, 0, None), 256, pg, _rows(), _rows(), 1, 1, 16, 1, 1, None, None), -2,
             "256 codewords")
-    _expect(f(_lib.CodecDesc(16, 16, 16, 1, 64, 8, 256, 2, None), pg, _rows(), _rows(), 1, 1, 16, 1, 1, None, None), -1,
+    _expect(f(_lib.CodecDesc(16, 16, 16, 1, 64, 8, 256, 2, None), 256, pg, _rows(), _rows(), 1, 1, 16, 1, 1, None, None), -1,
             "heavy pool")
 
 
@@ -63,7 +63,7 @@ def test_attention_refusals():
 
     def call(codec=cd, pages=pg, query=None, batch=1, query_len=1, table=16, cols=2, lens=16, prefix=None, prefix_len=0,
              ws=256, size=1 << 24):
-        return f(codec, pages, 16, 16, query or _rows(4), batch, query_len, table, 2, cols, lens, prefix, prefix_len, 1.0, 1, 16,
+        return f(codec, 256, pages, query or _rows(4), batch, query_len, table, 2, cols, lens, prefix, prefix_len, 1.0, 1, 16,
                  ws, size, None)
 
     assert call(batch=0) == 0 and call(query_len=0) == 0
@@ -77,6 +77,17 @@ def test_attention_refusals():
     _expect(call(codec=_lib.CodecDesc(16, 16, None, 1, 96, 8, 256, 0, None)), -2, "head_dim 64 or 128")
     _expect(call(pages=_lib.PagesDesc(16, None, 16, 4, 2, 16, 72, _lib.BF16)), -2, "value_dim 64 or 128")
     assert lib.sunshape_paged_attention_workspace_bytes(4, 8, 2, 1, 64, 100, 16, 0) > 0
+
+
+def test_tables_refusals():
+    lib = _lib.load_library()
+    cd = _lib.CodecDesc(16, 16, None, 2, 64, 8, 256, 0, None)
+    n = lib.sunshape_paged_tables_bytes(cd)
+    assert n > 0
+    _expect(lib.sunshape_paged_tables(cd, None, n, None), -1, "tables buffer")
+    _expect(lib.sunshape_paged_tables(cd, 256, n - 1, None), -1, "tables buffer")
+    _expect(lib.sunshape_paged_tables(cd, 128, n, None), -1, "tables buffer")
+    assert lib.sunshape_paged_tables_bytes(_lib.CodecDesc(16, 16, None, 2, 64, 8, 300, 0, None)) == -2
 
 
 def test_cpu_tensors_raise():
