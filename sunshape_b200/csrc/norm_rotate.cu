@@ -78,7 +78,7 @@ __device__ __forceinline__ void load_weights(const void* w, int e, int dtype, bo
 // HC heads of one token and one tensor per group of `width` threads; heads of a group are `chunks` apart, so
 // neighbouring groups touch neighbouring rows.
 template <typename T, int HC, bool INTER>
-__global__ void __launch_bounds__(128) norm_rotate_vec(const __grid_constant__ NormRotateParams p) {
+__global__ void __launch_bounds__(128, HC == 1 ? 1 : 8) norm_rotate_vec(const __grid_constant__ NormRotateParams p) {
   const int W = p.width;
   const int s = threadIdx.x & (W - 1);
   const unsigned item = (blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32) * (32 / W) + (threadIdx.x & 31) / W;
@@ -236,15 +236,15 @@ void launch(NormRotateParams& p, bool vec, cudaStream_t st) {
   // four heads a thread group once that still leaves every SM two full blocks of threads several times over;
   // below it one head, so that a decode step's few rows spread over the SMs
   const bool four = p.tokens * (p.heads[0] + p.heads[1]) * w >= (int64_t)148 * 2048 * 4;
-  const int hc = four ? 4 : 1;
+  const int hc = four ? 2 : 1;
   for (int i = 0; i < 2; ++i) p.chunks[i] = (p.heads[i] + hc - 1) / hc;
   p.items = p.tokens * (p.chunks[0] + p.chunks[1]);
   const unsigned grid = (unsigned)((p.items * w + 127) / 128);
   if (p.rot.interleaved) {
-    if (four) norm_rotate_vec<T, 4, true><<<grid, 128, 0, st>>>(p);
+    if (four) norm_rotate_vec<T, 2, true><<<grid, 128, 0, st>>>(p);
     else norm_rotate_vec<T, 1, true><<<grid, 128, 0, st>>>(p);
   } else {
-    if (four) norm_rotate_vec<T, 4, false><<<grid, 128, 0, st>>>(p);
+    if (four) norm_rotate_vec<T, 2, false><<<grid, 128, 0, st>>>(p);
     else norm_rotate_vec<T, 1, false><<<grid, 128, 0, st>>>(p);
   }
 }

@@ -22,22 +22,24 @@ int sm_count();
 int check_pages(const sunshape_codec_t* c, const sunshape_pages_t* pg);
 
 // What the paged kernels read of a codec, in one buffer (paged_append.cu fills it).
-//   image   [n_cb][ceil(D / 64)][256][64] fp16: codewords times their codebook's image scale; row (i, c) holds codeword
+//   image   at 0, [n_cb][ceil(D / 64)][256][64] fp16: codewords times their codebook's image scale; row (i, c) holds codeword
 //           c of the 64 / BD blocks from i * 64 / BD on, so that in shared memory a block's codewords lie in one
 //           column of the banks
-//   frags   [n_cb][nb][32][32][2]: the B operands of the encoder's MMAs over 8 codewords, lane by lane
-//   norms   [n_cb][nb][256]: -|c|^2 / 2 in the block's scale, far below all others where there is no codeword
-//   iscale  [n_cb], bscale [n_cb][nb]: powers of two that bring the largest codeword norm of a codebook, and of a
-//           block, into [0.5, 1)
+//   iscale  [n_cb]: the image's scale, a power of two that brings the codebook's largest codeword norm into [0.5, 1)
+//   records [n_cb][nb]: what the encoder reads of a block, one copy each --
+//     frags [32][32][2]: the B operands of the MMAs over 8 codewords, lane by lane
+//     norms [256]: -|c|^2 / 2 in the block's scale, far below all others where there is no codeword
+//     words [256][BD] fp32, far from all others where there is no codeword
+//     scale: a power of two that brings the block's largest codeword norm into [0.5, 1); three unused
+constexpr int kRecNorms = 8192, kRecWords = 9216;
+__host__ __device__ constexpr int record_bytes(int bd) { return kRecWords + 1024 * bd + 16; }
+
 struct Tables {
-  int64_t image, frags, norms, iscale, bscale, total;
+  int64_t iscale, records, total;
   __host__ __device__ Tables(int64_t n_cb, int64_t nb, int64_t D) {
-    image = 0;
-    frags = n_cb * ((D + 63) / 64) * 32768;
-    norms = frags + n_cb * nb * 8192;
-    iscale = norms + n_cb * nb * 1024;
-    bscale = iscale + (n_cb * 4 + 15) / 16 * 16;
-    total = bscale + (n_cb * nb * 4 + 255) / 256 * 256;
+    iscale = n_cb * ((D + 63) / 64) * 32768;
+    records = iscale + (n_cb * 4 + 255) / 256 * 256;
+    total = records + (n_cb * nb * record_bytes((int)(D / nb)) + 255) / 256 * 256;
   }
 };
 

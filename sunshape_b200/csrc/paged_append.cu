@@ -4,9 +4,9 @@
 // key z, decided exactly in three steps of growing precision:
 //   1. on the tensor cores, z and c as sums of two fp16 numbers and -|c|^2 / 2 as the accumulator's start, every
 //      thread keeps the maximum of each group of 16 codewords that it sees.  Where one group alone comes within
-//      twice the error bound (kFilter) of the overall maximum, the answer is in it;
-//   2. its 16 codewords are compared in fp32, keeping the smallest and the second smallest distance.  Where they
-//      differ by more than twice the bound kBound, the smallest is the answer;
+//      twice the error bound of the overall maximum, the answer is in it;
+//   2. its 16 codewords (otherwise all) are compared in fp32, keeping the smallest and the second smallest distance.
+//      Where they differ by more than twice the error bound, the smallest is the answer;
 //   3. otherwise (borders between codewords, repeated codewords, infinities and NaN) a warp scans the block in 64 bits.
 //
 // Bound by instructions: 256 distances for every block against 2 (D + Dv) bytes a key and head.  Step 1 takes per 16
@@ -29,9 +29,7 @@ struct AppendParams {
   const int64_t* slots;
   int64_t slot_sb, slot_sl;
   const float* cb;
-  const uint2* frags;
-  const float* norms;
-  const float* bscale;
+  const uint8_t* records;
   const int64_t* perm;
   const uint8_t* heavy_mask;
   uint8_t* idx;
@@ -41,15 +39,15 @@ struct AppendParams {
   int* err;
 };
 
-// Step 1's error relative to |c|max (|z| + |c|max), the block's scale bringing |c|max below 1: each factor is off by at
-// most 2^-22 of itself + 2^-25 (its remainder in fp16), the product of the remainders is left out, and 24 products and
-// the start are summed in fp32 with at most 2^-23 of the largest term each: below 2^-18 in all.
-constexpr float kFilter = 1.f / 131072.f;
-// Step 2's: z rounded to fp32 (relative u = 2^-24), bd products summed by fma, |c|^2 summed by fma, one last fma: at most
-// u (bd + 2) (|c|^2 + 2 |z| |c|) <= 10 u (...) for bd <= 8; 16 covers the terms of second order and the rounding of the
-// bound itself, kTiny what underflows.
-constexpr float kBound = 16.f / 16777216.f;
-constexpr float kTiny = 1e-37f;
+// Step 1's error is below filter(BD) (|z| + 0.5), the block's scale bringing |c| below 1: of the products' and the
+// start's sum, every addend may be cut to 2^-23 of the largest (|z| or 0.5; BD 8: 25 addends in two steps, BD 4: 13, BD
+// 2: 7, and one rounding a step), and z and c are off by at most 2^-22 of themselves, or 2^-25, and the product of their
+// remainders is left out: four times 2^-22 |z| for all of these.
+__host__ __device__ constexpr float filter(int bd) { return (bd == 8 ? 28 + 8 : bd == 4 ? 14 + 8 : 8 + 8) * 1.1f / 8388608.f; }
+// Step 2's: d = sum (c - z)^2 in fp32 is off by at most (bd + 3) u d (u = 2^-24) for its own roundings, and by
+// 2 sqrt(d) r + r^2 for z being off by r <= 2 u |z| + 4 u^2 |y| (see rotate32; |y|: the key's largest element).  kBound
+// covers bd <= 8, terms of second order and the rounding of the bound itself, kTiny what underflows.
+constexpr float kUlp = 1.f / 16777216.f, kBound = 16.f * kUlp, kTiny = 1e-37f;
 
 constexpr int kWarps = 4;
 constexpr int kTokens = 32 * kWarps;   // tokens of a CTA: two groups of 16 a warp
@@ -67,6 +65,13 @@ __device__ __forceinline__ double rotated(const Rotation& r, const T* row, int d
   return second ? y * c + o * s : y * c - o * s;
 }
 
+// the same in fp32, y c -+ o s with the rounding of the second product taken back: off by at most two roundings of
+// the result and of 2^-24 of that product
+__device__ __forceinline__ float rotate32(float y, float o, float c, float s) {
+  const float q = o * s, e = fmaf(o, s, -q);
+  return fmaf(y, c, q) + e;
+}
+
 // slot of a token, -1 where it is left out; records what is out of range
 __device__ __forceinline__ int64_t slot_of(const AppendParams& p, int64_t b, int64_t l, int64_t& pos) {
   int64_t slot = p.slots[b * p.slot_sb + l * p.slot_sl];
@@ -82,15 +87,39 @@ __device__ __forceinline__ int64_t slot_of(const AppendParams& p, int64_t b, int
   return slot;
 }
 
-__device__ __forceinline__ void mma_k16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// d = a b + (start of each column, the same in all rows) -- or + c
+__device__ __forceinline__ void mma_k16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, float2 c) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c.x), "f"(c.y));
 }
-__device__ __forceinline__ void mma_k8(float* c, uint32_t a0, uint32_t a1, uint32_t b0) {
+__device__ __forceinline__ void mma_k8(float* d, uint32_t a0, uint32_t a1, uint32_t b0, float2 c) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%8,%7,%8};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(b0), "f"(c.x), "f"(c.y));
+}
+__device__ __forceinline__ void mma_k8(float* d, uint32_t a0, uint32_t a1, uint32_t b0) {
   asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(b0));
+}
+
+// for error bounds, which have room for its own error of 2^-22
+__device__ __forceinline__ float sqrt_approx(float x) {
+  float y;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// a block's elements, aligned to 16 bytes (8 for two)
+template <int BD>
+__device__ __forceinline__ void load_block(const float* p, float* v) {
+  if constexpr (BD == 2) {
+    *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < BD / 4; ++i) reinterpret_cast<float4*>(v)[i] = reinterpret_cast<const float4*>(p)[i];
+  }
 }
 
 // two fp32 numbers as a pair of fp16 and the pair of their remainders
@@ -152,16 +181,17 @@ __global__ void __launch_bounds__(256) tables_kernel(const float* cb, const floa
   const float bs = factor(sqrtf(most(n)));
   const float is = factor(norm_max ? norm_max[k] : sqrtf(most(all)));
   constexpr int PER = 64 / BD;      // blocks of an image row
-  __half* image = reinterpret_cast<__half*>(out + at.image) +
+  __half* image = reinterpret_cast<__half*>(out) +
                   (((int64_t)k * ((D + 63) / 64) + blk / PER) * 256 + c) * 64 + blk % PER * BD;
 #pragma unroll
   for (int w = 0; w < BD; ++w) image[w] = __float2half_rn(v_s[c][w] * is);
-  reinterpret_cast<float*>(out + at.norms)[((int64_t)k * nb + blk) * 256 + c] = c < C ? -0.5f * (n * bs) * bs : -1e30f;
-  if (c == 0) {
-    reinterpret_cast<float*>(out + at.bscale)[(int64_t)k * nb + blk] = bs;
-    if (blk == 0) reinterpret_cast<float*>(out + at.iscale)[k] = is;
-  }
-  uint2* frags = reinterpret_cast<uint2*>(out + at.frags) + ((int64_t)k * nb + blk) * 1024;
+  uint8_t* rec = out + at.records + ((int64_t)k * nb + blk) * record_bytes(BD);
+  reinterpret_cast<float*>(rec + kRecNorms)[c] = c < C ? -0.5f * (n * bs) * bs : -1e30f;
+#pragma unroll
+  for (int w = 0; w < BD; ++w) reinterpret_cast<float*>(rec + kRecWords)[c * BD + w] = c < C ? v_s[c][w] : 1e18f;
+  if (c < 4) reinterpret_cast<float*>(rec + kRecWords + 1024 * BD)[c] = c == 0 ? bs : 0.f;
+  if (c == 0 && blk == 0) reinterpret_cast<float*>(out + at.iscale)[k] = is;
+  uint2* frags = reinterpret_cast<uint2*>(rec);
   for (int i = c; i < 1024; i += 256) {
     const int word = i >> 5, g = (i & 31) >> 2, t = i & 3;
     const float* v = v_s[word * 8 + g];
@@ -184,17 +214,17 @@ __global__ void __launch_bounds__(256) tables_kernel(const float* cb, const floa
 // grid (token tiles, heads, splits + 1): the last z copies the values
 template <typename T, int BD>
 __global__ void __launch_bounds__(kWarps * 32) append_kernel(const __grid_constant__ AppendParams p) {
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ __align__(128) uint8_t smem[];
+  constexpr int REC = record_bytes(BD);
   const int width = p.blocks * BD, ld = width + 8;                 // permuted elements of this CTA, row stride
-  float* const z_s = reinterpret_cast<float*>(smem);               // [kTokens][ld]
-  float* const cb_s = z_s + kTokens * ld;                          // [256][BD]
-  uint2* const frag_s = reinterpret_cast<uint2*>(cb_s + 256 * BD); // [32][32]
-  float* const norm_s = reinterpret_cast<float*>(frag_s + 1024);   // [256]
-  int64_t* const slot_s = reinterpret_cast<int64_t*>(norm_s + 256);   // [kTokens] page row of this head, -1: left out
+  uint8_t* const rec_s = smem;                                     // [2][REC]
+  float* const z_s = reinterpret_cast<float*>(rec_s + 2 * REC);    // [kTokens][ld]
+  int64_t* const slot_s = reinterpret_cast<int64_t*>(z_s + kTokens * ld);   // [kTokens] page row of this head, -1: left out
   int64_t* const pos_s = slot_s + kTokens;
   int64_t* const key_s = pos_s + kTokens;                          // offset of the key row
-  uint8_t* const idx_s = reinterpret_cast<uint8_t*>(key_s + kTokens);   // [kTokens][blocks]
-  __shared__ int most_s;
+  int* const most_s = reinterpret_cast<int*>(key_s + kTokens);     // [kTokens] largest element of the key, as an integer
+  uint8_t* const idx_s = reinterpret_cast<uint8_t*>(most_s + kTokens);   // [kTokens][blocks]
+  __shared__ uint64_t bar_s[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y;
   const int64_t t0 = (int64_t)blockIdx.x * kTokens;
   const int n_tok = (int)min((int64_t)kTokens, p.tokens - t0);
@@ -208,8 +238,9 @@ __global__ void __launch_bounds__(kWarps * 32) append_kernel(const __grid_consta
       at = values ? b * p.vs[0] + h * p.vs[1] + l * p.vs[2] : b * p.ks[0] + h * p.ks[1] + l * p.ks[2];
     }
     slot_s[tid] = slot;
-    pos_s[tid] = pos;
+    pos_s[tid] = slot < 0 ? 0 : pos;            // rows that are left out are read, not used
     key_s[tid] = at;
+    most_s[tid] = 0;
   }
   __syncthreads();
   if (values) {
@@ -230,207 +261,276 @@ __global__ void __launch_bounds__(kWarps * 32) append_kernel(const __grid_consta
     return;
   }
   const int b0 = blockIdx.z * p.blocks, nblk = min(p.blocks, p.nb - b0);
-  const T* const keys = reinterpret_cast<const T*>(p.key);
-  // rotated keys, rounded once to fp32
-  for (int i = tid; i < n_tok * width; i += kWarps * 32) {
-    const int tok = i / width, e = i - tok * width;
-    if (e >= nblk * BD) continue;
-    z_s[tok * ld + e] = slot_s[tok] < 0 ? 0.f : (float)rotated(p.rot, keys + key_s[tok], (int)p.perm[b0 * BD + e], pos_s[tok]);
+  const uint8_t* const records = p.records + ((int64_t)(p.n_cb == 1 ? 0 : h % p.n_cb) * p.nb + b0) * REC;
+  if (tid == 0) {                               // the first two blocks' records
+    for (int i = 0; i < 2; ++i) mbar_init(&bar_s[i], 1);
+    fence_mbar_init();
+    for (int i = 0; i < min(2, nblk); ++i) {
+      mbar_arrive_expect_tx(&bar_s[i], REC);
+      bulk_g2s(rec_s + i * REC, records + (int64_t)i * REC, REC, &bar_s[i]);
+    }
   }
-  const int64_t kb = (int64_t)(p.n_cb == 1 ? 0 : h % p.n_cb) * p.nb;
+  const T* const keys = reinterpret_cast<const T*>(p.key);
+  {
+    // rotated keys: a thread keeps its column of the permuted rows and takes every `step`th token
+    const int step = kWarps * 32 / width;       // blocks are chosen so that width is at most the threads
+    const int e = tid % width;
+    if (tid < step * width && e < nblk * BD) {
+      const int d = (int)p.perm[b0 * BD + e];
+      int other = d, i = 0;
+      bool second = false;
+      const bool turned = d < p.rot.rot;
+      if (turned) pair_of(p.rot, d, other, i, second);
+      const int half = p.rot.rot / 2;
+      constexpr int N = 8;                      // tokens in flight
+      for (int first = tid / width; first < n_tok; first += N * step) {
+        float y[N], o[N], c[N], sn[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          const int tok = min(first + k * step, n_tok - 1);
+          const T* row = keys + key_s[tok];
+          y[k] = Elem<T>::to_float(row[d]);
+          o[k] = 0.f;
+          if (turned) {
+            o[k] = Elem<T>::to_float(row[other]);
+            c[k] = p.rot.cos[pos_s[tok] * half + i];
+            sn[k] = p.rot.sin[pos_s[tok] * half + i];
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          const int tok = first + k * step;
+          if (tok >= n_tok) break;
+          // not negative: ordered as integers, NaN above all
+          const int size = max(__float_as_int(fabsf(y[k])), __float_as_int(fabsf(o[k])));
+          if (size > most_s[tok]) atomicMax(&most_s[tok], size);
+          z_s[tok * ld + e] = turned ? rotate32(y[k], o[k], c[k], second ? sn[k] : -sn[k]) : y[k];
+        }
+      }
+    }
+  }
   const int g = lane >> 2, t = lane & 3;
   const float INF = __int_as_float(0x7f800000);
   const int w0 = warp * 32;                     // the warp's first token
+  __syncthreads();
 
   for (int j = 0; j < nblk; ++j) {
     const int blk = b0 + j;
-    __syncthreads();                            // keys are staged, the last block's codebook is read
+    uint8_t* const rec = rec_s + (j & 1) * REC;
+    mbar_wait(&bar_s[j & 1], (j >> 1) & 1, p.err, kErrWait);
     if (p.heavy_mask && p.heavy_mask[blk]) {
       int at = 0;
       for (int i = 0; i < blk; ++i) at += p.heavy_mask[i] != 0;
       for (int i = tid; i < n_tok * BD; i += kWarps * 32) {
         const int tok = i / BD, w = i % BD;
         if (slot_s[tok] >= 0)
-          reinterpret_cast<T*>(p.heavy)[(slot_s[tok] * p.n_heavy + at) * BD + w] = Elem<T>::from_float(z_s[tok * ld + j * BD + w]);
+          reinterpret_cast<T*>(p.heavy)[(slot_s[tok] * p.n_heavy + at) * BD + w] =
+              Elem<T>::from_float((float)rotated(p.rot, keys + key_s[tok], (int)p.perm[blk * BD + w], pos_s[tok]));
       }
       if (tid < n_tok) idx_s[tid * p.blocks + j] = 0;
-      continue;
-    }
-    const float* cb = p.cb + (kb + blk) * p.C * BD;
-    const float4* fr = reinterpret_cast<const float4*>(p.frags + (kb + blk) * 1024);
-    if (tid == 0) most_s = 0;
-    for (int i = tid; i < 512; i += kWarps * 32) reinterpret_cast<float4*>(frag_s)[i] = fr[i];
-    for (int i = tid; i < p.C * BD; i += kWarps * 32) cb_s[i] = cb[i];
-    for (int i = tid; i < 256; i += kWarps * 32) norm_s[i] = p.norms[(kb + blk) * 256 + i];
-    const float scale = p.bscale[kb + blk];
-    __syncthreads();
-    for (int c = tid; c < p.C; c += kWarps * 32) {                 // largest |c|^2, as step 2 sums it
-      float n = 0.f;
+    } else if (w0 < n_tok) {
+      const uint2* const frag_s = reinterpret_cast<const uint2*>(rec);
+      const float* const norm_s = reinterpret_cast<const float*>(rec + kRecNorms);
+      const float* const cb_s = reinterpret_cast<const float*>(rec + kRecWords);
+      const float scale = cb_s[256 * BD];
+      // ---- step 1
+      uint32_t a[2][4], a8[2][2];
+      float bound[2][2];                                             // twice the error of rows g and g + 8
+      const bool some[2] = {w0 < n_tok, w0 + 16 < n_tok};
 #pragma unroll
-      for (int w = 0; w < BD; ++w) n = fmaf(cb_s[c * BD + w], cb_s[c * BD + w], n);
-      atomicMax(&most_s, __float_as_int(n));                       // not negative: ordered as integers, NaN above all
-    }
-    // ---- step 1
-    uint32_t a[2][4], a8[2][2];
-    float bound[2][2];                                             // twice the error of rows g and g + 8
-    const bool some[2] = {w0 < n_tok, w0 + 16 < n_tok};
+      for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
+        for (int y = 0; y < 2; ++y) {
+          const float* z = z_s + min(w0 + mt * 16 + y * 8 + g, n_tok - 1) * ld + j * BD;
+          alignas(16) float x[BD];
+          load_block<BD>(z, x);
+          float q = 0.f;
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        const float* z = z_s + min(w0 + mt * 16 + y * 8 + g, n_tok - 1) * ld + j * BD;
-        float q = 0.f;
-#pragma unroll
-        for (int w = 0; w < BD; ++w) q = fmaf(z[w] * scale, z[w] * scale, q);
-        bound[mt][y] = 2.f * kFilter * (sqrtf(q) + 1.f);
-        uint32_t hi, lo;
-        const int e = BD == 8 ? 2 * t : (BD == 4 ? 2 * (t & 1) : 0);
-        split2(z[e] * scale, z[e + 1] * scale, hi, lo);
-        if constexpr (BD == 8) {
-          a[mt][y] = hi;
-          a[mt][2 + y] = lo;
-          a8[mt][y] = hi;
-        } else if constexpr (BD == 4) {
-          a[mt][y] = t < 2 ? hi : lo;
-          a[mt][2 + y] = t < 2 ? hi : 0u;
-        } else {
-          a8[mt][y] = t == 1 ? lo : (t == 3 ? 0u : hi);
-        }
-      }
-    }
-    float top[2][2][4];                                            // maxima of groups of eight n-tiles
-#pragma unroll
-    for (int grp = 0; grp < 4; ++grp) {
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt) top[mt][0][grp] = top[mt][1][grp] = -INF;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int nt = grp * 8 + i;
-        const uint2 f = frag_s[nt * 32 + lane];
-        const float2 nn = *reinterpret_cast<const float2*>(norm_s + nt * 8 + 2 * t);
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-          float s[4] = {nn.x, nn.y, nn.x, nn.y};
+          for (int w = 0; w < BD; ++w) q = fmaf(x[w] * scale, x[w] * scale, q);
+          bound[mt][y] = 2.f * filter(BD) * (sqrt_approx(q) + 0.5f);
+          uint32_t hi, lo;
+          const int e = BD == 8 ? 2 * t : (BD == 4 ? 2 * (t & 1) : 0);
+          split2(z[e] * scale, z[e + 1] * scale, hi, lo);
           if constexpr (BD == 8) {
-            mma_k16(s, a[mt], f.x, f.x);
-            mma_k8(s, a8[mt][0], a8[mt][1], f.y);
+            a[mt][y] = hi;
+            a[mt][2 + y] = lo;
+            a8[mt][y] = hi;
           } else if constexpr (BD == 4) {
-            mma_k16(s, a[mt], f.x, f.y);
+            a[mt][y] = t < 2 ? hi : lo;
+            a[mt][2 + y] = t < 2 ? hi : 0u;
           } else {
-            mma_k8(s, a8[mt][0], a8[mt][1], f.x);
+            a8[mt][y] = t == 1 ? lo : (t == 3 ? 0u : hi);
           }
-          top[mt][0][grp] = fmaxf(top[mt][0][grp], fmaxf(s[0], s[1]));
-          top[mt][1][grp] = fmaxf(top[mt][1][grp], fmaxf(s[2], s[3]));
         }
       }
-    }
-    __syncthreads();                                               // most_s
-    const float cm2 = __int_as_float(most_s);
+      float top[2][2][4];                                            // maxima of groups of eight n-tiles
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-      if (!some[mt]) continue;
-      // the group of 16 codewords (lane of the quad, n-tile group) that alone is near the maximum; -1: not one
-      int where[2];
+      for (int grp = 0; grp < 4; ++grp) {
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        float m = fmaxf(fmaxf(top[mt][y][0], top[mt][y][1]), fmaxf(top[mt][y][2], top[mt][y][3]));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        int v = 0;                                                 // number of groups, and the sum of what names them
-#pragma unroll
-        for (int grp = 0; grp < 4; ++grp)
-          if (top[mt][y][grp] >= m - bound[mt][y]) v += 256 + (grp * 4 + t);
-        v += __shfl_xor_sync(0xffffffffu, v, 1);
-        v += __shfl_xor_sync(0xffffffffu, v, 2);
-        // a bound that is no number, or a key beyond fp16 in the block's scale, decides nothing
-        where[y] = (v >> 8) == 1 && bound[mt][y] < 2.f * kFilter * 30000.f ? v & 255 : -1;
-      }
-      // ---- step 2: two lanes a token
-      const int r = lane >> 1, half = lane & 1, tok = w0 + mt * 16 + r;
-      const int from_lo = __shfl_sync(0xffffffffu, where[0], (r & 7) * 4);
-      const int from_hi = __shfl_sync(0xffffffffu, where[1], (r & 7) * 4);
-      const int found = r < 8 ? from_lo : from_hi;
-      const bool live = tok < n_tok && slot_s[min(tok, n_tok - 1)] >= 0;
-      const float* z = z_s + min(tok, n_tok - 1) * ld + j * BD;
-      float x[BD], zn = 0.f, best = INF, next = INF;
-      int at = p.C;
-#pragma unroll
-      for (int w = 0; w < BD; ++w) {
-        x[w] = z[w];
-        zn = fmaf(x[w], x[w], zn);
-      }
-      if (found >= 0) {
+        for (int mt = 0; mt < 2; ++mt) top[mt][0][grp] = top[mt][1][grp] = -INF;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int c = ((found >> 2) * 8 + half * 4 + (i >> 1)) * 8 + 2 * (found & 3) + (i & 1);
-          if (c >= p.C) continue;
-          const float* v = cb_s + c * BD;
-          float dot = 0.f, n = 0.f;
+          const int nt = grp * 8 + i;
+          const uint2 f = frag_s[nt * 32 + lane];
+          const float2 nn = *reinterpret_cast<const float2*>(norm_s + nt * 8 + 2 * t);
 #pragma unroll
-          for (int w = 0; w < BD; ++w) {
-            dot = fmaf(x[w], v[w], dot);
-            n = fmaf(v[w], v[w], n);
-          }
-          const float d = fmaf(-2.f, dot, n);
-          if (d < best) {
-            next = best;
-            best = d;
-            at = c;
-          } else {
-            next = fminf(next, d);
+          for (int mt = 0; mt < 2; ++mt) {
+            float s[4];
+            if constexpr (BD == 8) {
+              mma_k16(s, a[mt], f.x, f.x, nn);
+              mma_k8(s, a8[mt][0], a8[mt][1], f.y);
+            } else if constexpr (BD == 4) {
+              mma_k16(s, a[mt], f.x, f.y, nn);
+            } else {
+              mma_k8(s, a8[mt][0], a8[mt][1], f.x, nn);
+            }
+            top[mt][0][grp] = fmaxf(top[mt][0][grp], fmaxf(s[0], s[1]));
+            top[mt][1][grp] = fmaxf(top[mt][1][grp], fmaxf(s[2], s[3]));
           }
         }
       }
-      const float ob = __shfl_xor_sync(0xffffffffu, best, 1), on = __shfl_xor_sync(0xffffffffu, next, 1);
-      const int oa = __shfl_xor_sync(0xffffffffu, at, 1);
-      next = fminf(fminf(next, on), fmaxf(best, ob));
-      if (ob < best) {
-        best = ob;
-        at = oa;
-      }
-      const float E = kBound * (cm2 + 2.f * sqrtf(zn) * sqrtf(cm2)) + kTiny;
-      // ---- step 3
-      unsigned unsure = __ballot_sync(0xffffffffu, live && !(found >= 0 && next - best > 2.f * E));
-      for (; unsure; unsure &= unsure - 1, unsure &= unsure - 1) {   // both lanes of a token
-        const int who = __ffs(unsure) - 1, tk = w0 + mt * 16 + (who >> 1);
-        double zz[BD], bd64 = __longlong_as_double(0x7ff0000000000000ll);
-        int a64 = p.C;
 #pragma unroll
-        for (int w = 0; w < BD; ++w)
-          zz[w] = rotated(p.rot, keys + key_s[tk], (int)p.perm[blk * BD + w], pos_s[tk]);
-        for (int c = lane; c < p.C; c += 32) {
-          double d = 0.0;
+      for (int mt = 0; mt < 2; ++mt) {
+        if (!some[mt]) continue;
+        // the group of 16 codewords (lane of the quad, n-tile group) that alone is near the maximum; -1: there are several
+        int where[2];
 #pragma unroll
-          for (int w = 0; w < BD; ++w) {
-            const double e = zz[w] - (double)cb_s[c * BD + w];
-            d = fma(e, e, d);
-          }
-          if (d < bd64) {
-            bd64 = d;
-            a64 = c;
+        for (int y = 0; y < 2; ++y) {
+          float m = fmaxf(fmaxf(top[mt][y][0], top[mt][y][1]), fmaxf(top[mt][y][2], top[mt][y][3]));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+          int v = 0;                                                 // number of groups, and the sum of what names them
+#pragma unroll
+          for (int grp = 0; grp < 4; ++grp)
+            if (top[mt][y][grp] >= m - bound[mt][y]) v += 256 + (grp * 4 + t);
+          v += __shfl_xor_sync(0xffffffffu, v, 1);
+          v += __shfl_xor_sync(0xffffffffu, v, 2);
+          // -2: a bound that is no number, or a key beyond fp16 in the block's scale
+          where[y] = !(bound[mt][y] < 2.f * filter(BD) * 30000.f) ? -2 : ((v >> 8) == 1 ? v & 255 : -1);
+        }
+        // ---- step 2: two lanes a token
+        const int r = lane >> 1, half = lane & 1, tok = w0 + mt * 16 + r;
+        const int from_lo = __shfl_sync(0xffffffffu, where[0], (r & 7) * 4);
+        const int from_hi = __shfl_sync(0xffffffffu, where[1], (r & 7) * 4);
+        const int found = r < 8 ? from_lo : from_hi;
+        const bool live = tok < n_tok && slot_s[min(tok, n_tok - 1)] >= 0;
+        const float* z = z_s + min(tok, n_tok - 1) * ld + j * BD;
+        alignas(16) float x[BD];
+        float zn = 0.f, best = INF, next = INF;
+        int at = p.C;
+        load_block<BD>(z, x);
+#pragma unroll
+        for (int w = 0; w < BD; ++w) zn = fmaf(x[w], x[w], zn);
+        if (found >= 0) {
+          const int c0 = ((found >> 2) * 8 + half * 4) * 8 + 2 * (found & 3);
+          const float* v = cb_s + c0 * BD;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int c = (i >> 1) * 8 + (i & 1);
+            alignas(16) float u[BD];
+            float d = 0.f;
+            load_block<BD>(v + c * BD, u);
+#pragma unroll
+            for (int w = 0; w < BD; ++w) d = fmaf(u[w] - x[w], u[w] - x[w], d);
+            next = fminf(next, fmaxf(best, d));
+            if (d < best) {
+              best = d;
+              at = c0 + c;
+            }
           }
         }
+        const float ob = __shfl_xor_sync(0xffffffffu, best, 1), on = __shfl_xor_sync(0xffffffffu, next, 1);
+        const int oa = __shfl_xor_sync(0xffffffffu, at, 1);
+        next = fminf(fminf(next, on), fmaxf(best, ob));
+        if (ob < best) {
+          best = ob;
+          at = oa;
+        }
+        // several groups near the maximum: the warp compares all of the block's codewords
+        unsigned wide = __ballot_sync(0xffffffffu, live && found == -1);
+        for (; wide; wide &= wide - 1, wide &= wide - 1) {           // both lanes of a token
+          const int who = (__ffs(wide) - 1) >> 1;
+          float near1 = INF, near2 = INF;
+          int c1 = p.C;
+          load_block<BD>(z_s + (w0 + mt * 16 + who) * ld + j * BD, x);
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const double od = __shfl_xor_sync(0xffffffffu, bd64, o);
-          const int oc = __shfl_xor_sync(0xffffffffu, a64, o);
-          if (od < bd64 || (od == bd64 && oc < a64)) {
-            bd64 = od;
-            a64 = oc;
+          for (int i = 0; i < 8; ++i) {
+            alignas(16) float u[BD];
+            float d = 0.f;
+            load_block<BD>(cb_s + (i * 32 + lane) * BD, u);
+#pragma unroll
+            for (int w = 0; w < BD; ++w) d = fmaf(u[w] - x[w], u[w] - x[w], d);
+            near2 = fminf(near2, fmaxf(near1, d));
+            if (d < near1) {
+              near1 = d;
+              c1 = i * 32 + lane;
+            }
+          }
+          const float mine = near1;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const float n1 = __shfl_xor_sync(0xffffffffu, near1, o), n2 = __shfl_xor_sync(0xffffffffu, near2, o);
+            near2 = fminf(fminf(near2, n2), fmaxf(near1, n1));
+            near1 = fminf(near1, n1);
+          }
+          const unsigned at1 = __ballot_sync(0xffffffffu, mine == near1);   // one lane, unless step 3 decides
+          c1 = __shfl_sync(0xffffffffu, c1, at1 ? __ffs(at1) - 1 : 0);
+          if ((lane >> 1) == who) {
+            best = near1;
+            next = near2;
+            at = c1;
           }
         }
-        if ((lane >> 1) == (who >> 1)) at = a64;
+        const float rz = 4.f * kUlp * sqrt_approx(zn) + 16.f * kUlp * kUlp * __int_as_float(most_s[min(tok, n_tok - 1)]);
+        const float E = kBound * next + 4.f * rz * (sqrt_approx(next) + rz) + kTiny;
+        // ---- step 3
+        unsigned unsure = __ballot_sync(0xffffffffu, live && !(found > -2 && next - best > 2.f * E));
+        for (; unsure; unsure &= unsure - 1, unsure &= unsure - 1) {   // both lanes of a token
+          const int who = __ffs(unsure) - 1, tk = w0 + mt * 16 + (who >> 1);
+          double zz[BD], bd64 = __longlong_as_double(0x7ff0000000000000ll);
+          int a64 = p.C;
+#pragma unroll
+          for (int w = 0; w < BD; ++w)
+            zz[w] = rotated(p.rot, keys + key_s[tk], (int)p.perm[blk * BD + w], pos_s[tk]);
+          for (int c = lane; c < p.C; c += 32) {
+            double d = 0.0;
+#pragma unroll
+            for (int w = 0; w < BD; ++w) {
+              const double e = zz[w] - (double)cb_s[c * BD + w];
+              d = fma(e, e, d);
+            }
+            if (d < bd64) {
+              bd64 = d;
+              a64 = c;
+            }
+          }
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const double od = __shfl_xor_sync(0xffffffffu, bd64, o);
+            const int oc = __shfl_xor_sync(0xffffffffu, a64, o);
+            if (od < bd64 || (od == bd64 && oc < a64)) {
+              bd64 = od;
+              a64 = oc;
+            }
+          }
+          if ((lane >> 1) == (who >> 1)) at = a64;
+        }
+        if (live && half == 0) idx_s[tok * p.blocks + j] = (uint8_t)(at < p.C ? at : 0);   // no finite distance: 0
       }
-      if (live && half == 0) idx_s[tok * p.blocks + j] = (uint8_t)(at < p.C ? at : 0);   // no finite distance: 0
+    }
+    __syncthreads();                            // the record is read
+    if (tid == 0 && j + 2 < nblk) {
+      mbar_arrive_expect_tx(&bar_s[j & 1], REC);
+      bulk_g2s(rec, records + (int64_t)(j + 2) * REC, REC, &bar_s[j & 1]);
     }
   }
-  __syncthreads();
-  if (nblk == p.nb && p.nb % 16 == 0) {
-    const int per = p.nb / 16;
+  if (p.blocks % 4 == 0 && p.nb % 4 == 0) {
+    const int per = nblk / 4;
     for (int i = tid; i < n_tok * per; i += kWarps * 32) {
       const int tok = i / per, q = i - tok * per;
       if (slot_s[tok] >= 0)
-        reinterpret_cast<uint4*>(p.idx + slot_s[tok] * p.nb)[q] = reinterpret_cast<const uint4*>(idx_s + tok * p.nb)[q];
+        reinterpret_cast<uint32_t*>(p.idx + slot_s[tok] * p.nb + b0)[q] =
+            reinterpret_cast<const uint32_t*>(idx_s + tok * p.blocks)[q];
     }
   } else {
     for (int i = tid; i < n_tok * nblk; i += kWarps * 32) {
@@ -443,11 +543,12 @@ __global__ void __launch_bounds__(kWarps * 32) append_kernel(const __grid_consta
 template <typename T, int BD>
 void launch(AppendParams& p, cudaStream_t st) {
   const int64_t tiles = (p.tokens + kTokens - 1) / kTokens;
-  // a head's blocks are shared out until every SM has two CTAs: one token a sequence leaves one tile of tokens
-  p.splits = (int)std::min<int64_t>(p.nb, std::max<int64_t>(1, 2 * sm_count() / (tiles * p.H)));
-  p.blocks = (p.nb + p.splits - 1) / p.splits;
+  // A head's blocks are shared out until every SM has two CTAs (one token a sequence leaves one tile of tokens), and in
+  // any case to 32 elements a CTA, with whose keys in shared memory an SM holds five
+  const int64_t fill = 2 * sm_count() / (tiles * p.H);
+  p.blocks = (int)std::min<int64_t>((p.nb + std::max<int64_t>(fill, 1) - 1) / std::max<int64_t>(fill, 1), 32 / BD);
   p.splits = (p.nb + p.blocks - 1) / p.blocks;
-  const int smem = (kTokens * (p.blocks * BD + 8) + 256 * BD + 256) * 4 + 8192 + 3 * kTokens * 8 + kTokens * p.blocks;
+  const int smem = 2 * record_bytes(BD) + kTokens * ((p.blocks * BD + 8) * 4 + 3 * 8 + 4 + p.blocks);
   cudaFuncSetAttribute(append_kernel<T, BD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   append_kernel<T, BD><<<dim3((unsigned)tiles, p.H, p.splits + 1), kWarps * 32, smem, st>>>(p);
 }
@@ -559,10 +660,7 @@ int sunshape_paged_append(const sunshape_codec_t* codec, const void* tables, con
   p.slot_sl = slot_stride_l;
   p.cb = codec->centroids;
   const Tables tab(p.n_cb, p.nb, p.D);
-  const uint8_t* base = static_cast<const uint8_t*>(tables);
-  p.frags = reinterpret_cast<const uint2*>(base + tab.frags);
-  p.norms = reinterpret_cast<const float*>(base + tab.norms);
-  p.bscale = reinterpret_cast<const float*>(base + tab.bscale);
+  p.records = static_cast<const uint8_t*>(tables) + tab.records;
   p.perm = codec->permutation;
   p.heavy_mask = p.n_heavy ? codec->heavy_mask : nullptr;
   p.idx = pages->indices;

@@ -134,7 +134,7 @@ int sunshape_paged_attention(const sunshape_codec_t* codec, const void* tables, 
   p.idx = pages->indices;
   p.heavy = pages->heavy;
   const Tables tab(p.n_cb, p.nb, d);
-  p.image = static_cast<const uint8_t*>(tables) + tab.image;
+  p.image = tables;
   p.image_scale = reinterpret_cast<const float*>(static_cast<const uint8_t*>(tables) + tab.iscale);
   p.out = out;
   const int grid = sm_count();
