@@ -7,6 +7,9 @@
 // hold whole pairs (elements 8s .. 8s+7 of each half, or 16s .. 16s+15 when neighbours pair up): the rotation
 // then needs no exchange between threads, only the norm's sum does (three shuffles at dim 128).  Cosines and
 // sines belong to the token, not to the head, so a thread keeps them in registers over the heads that it takes.
+#include <algorithm>
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace sunshape {
@@ -21,7 +24,7 @@ struct NormRotateParams {
   int w_dtype, w_vec;           // w_vec: weights are 16-byte aligned
   float eps;
   int L, dim, width;            // width: threads of a row (vector kernel)
-  int chunks[2];                // head chunks of q and k per token
+  int parts;                    // groups of threads that share a token's heads
   int64_t tokens, items;
   Rotation rot;
   int* err;
@@ -45,14 +48,24 @@ __device__ __forceinline__ void unpack8(const Vec8<T>& r, float* f) {
   for (int i = 0; i < 8; ++i) f[i] = Elem<T>::to_float(e[i]);
 }
 
+// two fp32 numbers as a pair of 16-bit ones, in one instruction
+template <typename T>
+__device__ __forceinline__ uint32_t pair_of_floats(float lo, float hi) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __half>::value) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float* f) {
-  Vec8<T> r;
-  T* e = reinterpret_cast<T*>(&r);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) e[i] = Elem<T>::from_float(f[i]);
-#pragma unroll
-  for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = r.v[i];
+  if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+  } else {
+    *reinterpret_cast<uint4*>(p) = make_uint4(pair_of_floats<T>(f[0], f[1]), pair_of_floats<T>(f[2], f[3]),
+                                              pair_of_floats<T>(f[4], f[5]), pair_of_floats<T>(f[6], f[7]));
+  }
 }
 
 // eight weights from element e on (a multiple of eight)
@@ -75,100 +88,122 @@ __device__ __forceinline__ void load_weights(const void* w, int e, int dtype, bo
   }
 }
 
-// HC heads of one token and one tensor per group of `width` threads; heads of a group are `chunks` apart, so
-// neighbouring groups touch neighbouring rows.
-template <typename T, int HC, bool INTER>
-__global__ void __launch_bounds__(128, HC == 1 ? 1 : 8) norm_rotate_vec(const __grid_constant__ NormRotateParams p) {
+// A group of `width` threads takes every `parts`th head of a token -- so that neighbouring groups touch neighbouring
+// rows -- with the next four rows always in flight.
+template <typename T, bool INTER>
+__global__ void __launch_bounds__(128) norm_rotate_vec(const __grid_constant__ NormRotateParams p) {
+  constexpr int N = 4;
   const int W = p.width;
   const int s = threadIdx.x & (W - 1);
   const unsigned item = (blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32) * (32 / W) + (threadIdx.x & 31) / W;
-  if (item >= (unsigned)p.items) return;            // whole groups leave: the shuffles below stay within a group
+  if (item >= (unsigned)p.items) return;  // whole groups leave: the shuffles below stay within a group
   const unsigned mask = W == 32 ? 0xffffffffu : ((1u << W) - 1) << ((threadIdx.x & 31) & ~(W - 1));
-  const unsigned per = p.chunks[0] + p.chunks[1];
-  const unsigned token = item / per;
-  int chunk = (int)(item - token * per);
-  const int which = chunk >= p.chunks[0];
-  if (which) chunk -= p.chunks[0];
+  const unsigned token = item / (unsigned)p.parts;
   const int64_t b = token / (unsigned)p.L, l = token - (unsigned)b * (unsigned)p.L;
-  const int heads = p.heads[which], step = p.chunks[which];
   const bool have = s * 16 < p.dim;       // the last threads of a group are idle when dim / 16 is no power of two
   const int R = p.rot.rot;
   const bool turned = s * 16 < R;
   // first elements of this thread's two runs of eight
   const int e0 = !INTER && turned ? 8 * s : 16 * s;
   const int e1 = !INTER && turned ? 8 * s + R / 2 : 16 * s + 8;
+  int h = (int)(item - token * (unsigned)p.parts);
 
-  const T* x = reinterpret_cast<const T*>(p.x[which]) + b * p.xs[which][0] + l * p.xs[which][2];
-  T* y = reinterpret_cast<T*>(p.y[which]) + b * p.ys[which][0] + l * p.ys[which][2];
-  Vec8<T> in[HC][2];
-#pragma unroll
-  for (int i = 0; i < HC; ++i) {
-    const int h = chunk + i * step;
-    if (have && h < heads) {
-      load8(x + h * p.xs[which][1] + e0, in[i][0]);
-      load8(x + h * p.xs[which][1] + e1, in[i][1]);
+  for (int which = 0; which < 2; ++which) {
+    const int heads = p.heads[which];
+    if (h >= heads) {
+      h -= heads;
+      continue;
     }
-  }
-  float c[8], sn[8];
-  bool bad = false;
-  if (R) {
-    const int64_t pos = position_of(p.rot, b, l);
-    bad = pos < 0 || pos >= p.rot.table_len;
-    if (bad && s == 0) record_error(p.err, kErrPosition);
-    if (turned) {
-      const int64_t at = (bad ? 0 : pos) * (R / 2) + 8 * s;
+    const T* x = reinterpret_cast<const T*>(p.x[which]) + b * p.xs[which][0] + l * p.xs[which][2];
+    T* y = reinterpret_cast<T*>(p.y[which]) + b * p.ys[which][0] + l * p.ys[which][2];
+    const int64_t x_step = p.xs[which][1], y_step = p.ys[which][1];
+    Vec8<T> in[N][2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        reinterpret_cast<float4*>(c)[i] = reinterpret_cast<const float4*>(p.rot.cos + at)[i];
-        reinterpret_cast<float4*>(sn)[i] = reinterpret_cast<const float4*>(p.rot.sin + at)[i];
+    for (int i = 0; i < N; ++i) {
+      if (have && h + i * p.parts < heads) {
+        load8(x + (h + i * p.parts) * x_step + e0, in[i][0]);
+        load8(x + (h + i * p.parts) * x_step + e1, in[i][1]);
       }
     }
-  }
-  float w0[8], w1[8];
-  const void* w = p.w[which];
-  if (w && have) {
-    load_weights(w, e0, p.w_dtype, p.w_vec, w0);
-    load_weights(w, e1, p.w_dtype, p.w_vec, w1);
-  }
+    // Of the pairs' elements (u, v) come u A - v B and v C + u S: the rotation with the weights multiplied in, once for
+    // all of the thread's heads.  A thread's pairs are (e0 + e, e1 + e), or neighbours in its sixteen elements.
+    float A[8], B[8], C[8], S[8];
 #pragma unroll
-  for (int i = 0; i < HC; ++i) {
-    const int h = chunk + i * step;
-    if (h >= heads) break;                // the same for the whole group
-    float a0[8], a1[8];
-    unpack8(in[i][0], a0);
-    unpack8(in[i][1], a1);
-    if (w) {
-      float q = 0.f;
-      if (have) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) q = fmaf(a0[e], a0[e], fmaf(a1[e], a1[e], q));
-      }
-      for (int o = W >> 1; o; o >>= 1) q += __shfl_xor_sync(mask, q, o);
-      const float r = rsqrtf(q / (float)p.dim + p.eps);
+    for (int e = 0; e < 8; ++e) A[e] = C[e] = 1.f, B[e] = S[e] = 0.f;
+    const void* w = p.w[which];
+    if (w && have) {
+      float w0[8], w1[8];
+      load_weights(w, e0, p.w_dtype, p.w_vec, w0);
+      load_weights(w, e1, p.w_dtype, p.w_vec, w1);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        a0[e] = a0[e] * r * w0[e];
-        a1[e] = a1[e] * r * w1[e];
+        A[e] = INTER ? (e < 4 ? w0[2 * e & 7] : w1[2 * e & 7]) : w0[e];
+        C[e] = INTER ? (e < 4 ? w0[(2 * e + 1) & 7] : w1[(2 * e + 1) & 7]) : w1[e];
       }
     }
-    if (turned) {
+    bool bad = false;
+    if (R) {
+      const int64_t pos = position_of(p.rot, b, l);
+      bad = pos < 0 || pos >= p.rot.table_len;
+      if (bad && s == 0) record_error(p.err, kErrPosition);
+      if (turned) {
+        const int64_t at = (bad ? 0 : pos) * (R / 2) + 8 * s;
+        float c[8], sn[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float& u = INTER ? (e < 4 ? a0[2 * e] : a1[2 * e - 8]) : a0[e];
-        float& v = INTER ? (e < 4 ? a0[2 * e + 1] : a1[2 * e - 7]) : a1[e];
-        const float zu = u * c[e] - v * sn[e], zv = v * c[e] + u * sn[e];
-        u = zu;
-        v = zv;
+        for (int i = 0; i < 2; ++i) {
+          reinterpret_cast<float4*>(c)[i] = reinterpret_cast<const float4*>(p.rot.cos + at)[i];
+          reinterpret_cast<float4*>(sn)[i] = reinterpret_cast<const float4*>(p.rot.sin + at)[i];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          S[e] = A[e] * sn[e];
+          B[e] = C[e] * sn[e];
+          A[e] *= c[e];
+          C[e] *= c[e];
+        }
       }
     }
-    if (bad) {
+    while (h < heads) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) a0[e] = a1[e] = __int_as_float(0x7fffffff);
+      for (int i = 0; i < N; ++i, h += p.parts) {
+        if (h >= heads) break;                // the same for the whole group
+        float a0[8], a1[8];
+        unpack8(in[i][0], a0);
+        unpack8(in[i][1], a1);
+        if (have && h + N * p.parts < heads) {
+          load8(x + (h + N * p.parts) * x_step + e0, in[i][0]);
+          load8(x + (h + N * p.parts) * x_step + e1, in[i][1]);
+        }
+        float r = 1.f;
+        if (w) {
+          float q = 0.f;
+          if (have) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) q = fmaf(a0[e], a0[e], fmaf(a1[e], a1[e], q));
+          }
+          for (int o = W >> 1; o; o >>= 1) q += __shfl_xor_sync(mask, q, o);
+          r = rsqrtf(q / (float)p.dim + p.eps);
+        }
+        if (bad) r = __int_as_float(0x7fffffff);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float& u = INTER ? (e < 4 ? a0[2 * e & 7] : a1[2 * e & 7]) : a0[e];
+          float& v = INTER ? (e < 4 ? a0[(2 * e + 1) & 7] : a1[(2 * e + 1) & 7]) : a1[e];
+          float zu = u * A[e], zv = v * C[e];
+          if (turned) {                       // not as products with zero: elements beyond R keep to themselves
+            zu = fmaf(-v, B[e], zu);
+            zv = fmaf(u, S[e], zv);
+          }
+          u = zu * r;
+          v = zv * r;
+        }
+        if (have) {
+          store8(y + h * y_step + e0, a0);
+          store8(y + h * y_step + e1, a1);
+        }
+      }
     }
-    if (have) {
-      store8(y + h * p.ys[which][1] + e0, a0);
-      store8(y + h * p.ys[which][1] + e1, a1);
-    }
+    h -= heads;
   }
 }
 
@@ -233,20 +268,14 @@ void launch(NormRotateParams& p, bool vec, cudaStream_t st) {
   int w = 1;
   while (w * 16 < p.dim) w *= 2;
   p.width = w;
-  // four heads a thread group once that still leaves every SM two full blocks of threads several times over;
-  // below it one head, so that a decode step's few rows spread over the SMs
-  const bool four = p.tokens * (p.heads[0] + p.heads[1]) * w >= (int64_t)148 * 2048 * 4;
-  const int hc = four ? 2 : 1;
-  for (int i = 0; i < 2; ++i) p.chunks[i] = (p.heads[i] + hc - 1) / hc;
-  p.items = p.tokens * (p.chunks[0] + p.chunks[1]);
+  // Groups that share a token: one where there are tokens enough to give every SM 512 threads, which a thread's cosines,
+  // weights and rows in flight allow; up to one for each head below that, so that a decode step's few rows spread out.
+  const int heads = p.heads[0] + p.heads[1];
+  p.parts = (int)std::min<int64_t>(heads, std::max<int64_t>(1, (int64_t)sm_count() * 512 / w / p.tokens));
+  p.items = p.tokens * p.parts;
   const unsigned grid = (unsigned)((p.items * w + 127) / 128);
-  if (p.rot.interleaved) {
-    if (four) norm_rotate_vec<T, 2, true><<<grid, 128, 0, st>>>(p);
-    else norm_rotate_vec<T, 1, true><<<grid, 128, 0, st>>>(p);
-  } else {
-    if (four) norm_rotate_vec<T, 2, false><<<grid, 128, 0, st>>>(p);
-    else norm_rotate_vec<T, 1, false><<<grid, 128, 0, st>>>(p);
-  }
+  if (p.rot.interleaved) norm_rotate_vec<T, true><<<grid, 128, 0, st>>>(p);
+  else norm_rotate_vec<T, false><<<grid, 128, 0, st>>>(p);
 }
 
 bool float_type(int d) { return d == SUNSHAPE_F32 || d == SUNSHAPE_BF16 || d == SUNSHAPE_F16; }
