@@ -22,9 +22,10 @@ LIB_PATH = os.path.join(HERE, LIB_NAME)
 SOURCES = ["capi.cu", "decode_f32.cu", "decode_bf16.cu", "decode_f16.cu", "decode_scores.cu", "decode_mma_bf16.cu",
            "decode_mma_f16.cu", "noalloc.cu", "peer.cu", "encode_tc.cu", "exchange.cu", "packed.cu", "norm_rotate.cu",
            "paged_append.cu", "paged_attention.cu", "paged_attention_bf16_d64.cu", "paged_attention_bf16_d128.cu",
-           "paged_attention_f16_d64.cu", "paged_attention_f16_d128.cu"]
+           "paged_attention_f16_d64.cu", "paged_attention_f16_d128.cu", "paged_prefix_bf16_d64.cu",
+           "paged_prefix_bf16_d128.cu", "paged_prefix_f16_d64.cu", "paged_prefix_f16_d128.cu"]
 DEPS = SOURCES + ["common.cuh", "decode.cuh", "decode_mma.cuh", "encode.cuh", "encode_params.cuh", "paged.cuh", "paged_attention.cuh",
-                  "paged_attention_kernel.cuh"]
+                  "paged_attention_kernel.cuh", "paged_prefix.cuh"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

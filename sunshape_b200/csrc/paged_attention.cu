@@ -11,17 +11,24 @@ constexpr int kSmemMax = 232448;    // 227 KB
 int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
 
 struct Layout {
-  int64_t slots, desc, pieces, prefix, total;
+  int64_t slots, desc, pieces, prefix, prefix_desc, prefix_slots, total;
 };
 
-Layout layout(int grid, int64_t rows, int64_t item_rows, int dv, bool prefix) {
+// Query rows of a KV head from which on the prefix goes to the tensor-core kernel: it rebuilds a key once for 256 rows
+// where the memory-bound kernel reads it again for every 16.
+constexpr int64_t kPrefixRows = 17;
+
+// item_rows: of the memory-bound kernel's calls; tensor: the prefix goes to the tensor-core kernel
+Layout layout(int grid, int64_t rows, int64_t item_rows, int dv, bool prefix, bool tensor) {
   const int64_t row = row_floats(dv) * 4;
   Layout l;
   l.slots = 0;
   l.desc = round256(2 * grid * kItemRows * row);
   l.pieces = l.desc + round256((int64_t)grid * 16);
   l.prefix = l.pieces + round256((int64_t)grid * kPairs * 2 * item_rows * row);
-  l.total = l.prefix + (prefix ? round256(rows * row) : 0);
+  l.prefix_desc = l.prefix + (prefix ? round256(rows * row) : 0);
+  l.prefix_slots = l.prefix_desc + (tensor ? round256((int64_t)grid * 16) : 0);
+  l.total = l.prefix_slots + (tensor ? round256(2 * (int64_t)grid * 256 * row) : 0);
   return l;
 }
 
@@ -47,11 +54,12 @@ bool plan(AttnParams& p, int d, int dv, int bd) {
   return p.pairs >= 1;
 }
 
-template <typename T>
+template <typename T, bool PREFIX>
 int launch(const AttnParams& p, const CUtensorMap& vmap, int d, int dv, int bd, int grid, cudaStream_t st) {
 #define SUNSHAPE_PAGED_CASE(D, DV, BD)                       \
   if (d == D && dv == DV && bd == BD) {                      \
-    return launch_paged_attention<D, DV, BD, T>(p, vmap, grid, st); \
+    if constexpr (PREFIX) return launch_paged_prefix<D, DV, BD, T>(p, vmap, grid, st); \
+    else return launch_paged_attention<D, DV, BD, T>(p, vmap, grid, st); \
   }
   SUNSHAPE_PAGED_CASE(64, 64, 2) SUNSHAPE_PAGED_CASE(64, 64, 4) SUNSHAPE_PAGED_CASE(64, 64, 8)
   SUNSHAPE_PAGED_CASE(64, 128, 2) SUNSHAPE_PAGED_CASE(64, 128, 4) SUNSHAPE_PAGED_CASE(64, 128, 8)
@@ -75,7 +83,8 @@ int64_t sunshape_paged_attention_workspace_bytes(int32_t batch, int32_t q_heads,
   (void)page_size;
   const int64_t rows = (int64_t)batch * q_heads * query_len;
   const int64_t own = kv_heads > 0 ? (int64_t)q_heads / kv_heads * query_len : 0;
-  return layout(sm_count(), rows, item_rows(prefix_len > 0 ? own * batch : own), value_dim, prefix_len > 0).total;
+  const bool tensor = prefix_len > 0 && own * batch >= kPrefixRows;
+  return layout(sm_count(), rows, item_rows(prefix_len > 0 && !tensor ? own * batch : own), value_dim, prefix_len > 0, tensor).total;
 }
 
 int sunshape_paged_attention(const sunshape_codec_t* codec, const void* tables, const sunshape_pages_t* pages,
@@ -138,12 +147,16 @@ int sunshape_paged_attention(const sunshape_codec_t* codec, const void* tables, 
   p.image_scale = reinterpret_cast<const float*>(static_cast<const uint8_t*>(tables) + tab.iscale);
   p.out = out;
   const int grid = sm_count();
-  const Layout at = layout(grid, rows, item_rows((prefix_len ? (int64_t)p.B : 1) * p.G * p.L), dv, prefix_len > 0);
+  const int64_t own = (int64_t)p.G * p.L;
+  const bool tensor = prefix_len > 0 && own * batch >= kPrefixRows;
+  const Layout at = layout(grid, rows, item_rows(prefix_len && !tensor ? own * batch : own), dv, prefix_len > 0, tensor);
   uint8_t* const ws = static_cast<uint8_t*>(workspace);
   p.slots = reinterpret_cast<float*>(ws + at.slots);
   p.desc = reinterpret_cast<int4*>(ws + at.desc);
   p.pieces = reinterpret_cast<float*>(ws + at.pieces);
   p.prefix_part = reinterpret_cast<float*>(ws + at.prefix);
+  p.prefix_desc = reinterpret_cast<int4*>(ws + at.prefix_desc);
+  p.prefix_slots = reinterpret_cast<float*>(ws + at.prefix_slots);
   const int64_t pool_rows = p.num_pages * p.H * p.ps;
   if (pool_rows > 0x7fffffff) return set_last_error(SUNSHAPE_E_UNSUPPORTED, "at most 2^31 - 1 page rows in a pool.");
   // the kernels count tiles, and the gaps between heads, in 31 bits
@@ -167,11 +180,14 @@ int sunshape_paged_attention(const sunshape_codec_t* codec, const void* tables, 
   if (prefix_len) {
     f.table = prefix_table;
     f.table_stride = 0;
-    if (int rc = bf16 ? launch<__nv_bfloat16>(f, vmap, d, dv, bd, grid, st) : launch<__half>(f, vmap, d, dv, bd, grid, st))
-      return rc;
+    int rc;
+    if (tensor) rc = bf16 ? launch<__nv_bfloat16, true>(f, vmap, d, dv, bd, grid, st) : launch<__half, true>(f, vmap, d, dv, bd, grid, st);
+    else rc = bf16 ? launch<__nv_bfloat16, false>(f, vmap, d, dv, bd, grid, st) : launch<__half, false>(f, vmap, d, dv, bd, grid, st);
+    if (rc) return rc;
     p.prefix_parts = 1;
   }
-  if (int rc = bf16 ? launch<__nv_bfloat16>(p, vmap, d, dv, bd, grid, st) : launch<__half>(p, vmap, d, dv, bd, grid, st))
+  if (int rc = bf16 ? launch<__nv_bfloat16, false>(p, vmap, d, dv, bd, grid, st)
+                    : launch<__half, false>(p, vmap, d, dv, bd, grid, st))
     return rc;
   return launch_status("paged attention launch");
 }

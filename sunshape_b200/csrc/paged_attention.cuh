@@ -54,6 +54,8 @@ struct AttnParams {
   int4* desc;                      // [grid] (head piece: 0 none, 1 cut again, 2 last; tail item's h (-1: none), b, row group)
   float* pieces;                   // [grid][kPairs][2][item_rows] rows: pieces of items cut between a CTA's pairs
   float* prefix_part;              // [prefix_parts][B * Hq * L] rows
+  float* prefix_slots;             // [2 * grid][256] rows: pieces of the prefix's items cut between CTAs
+  int4* prefix_desc;               // [grid] as desc, tail item's h (-1: none) and first row
   int* err;
   int item_rows;                   // 8 or 16: which kernel
   int smem;
@@ -156,5 +158,7 @@ __device__ __forceinline__ void join4(float& m, float& l, float4& a, float mk, f
 
 template <int D, int DV, int BD, typename T>
 int launch_paged_attention(const AttnParams& p, const CUtensorMap& vmap, int grid, cudaStream_t st);
+template <int D, int DV, int BD, typename T>
+int launch_paged_prefix(const AttnParams& p, const CUtensorMap& vmap, int grid, cudaStream_t st);
 
 }  // namespace sunshape

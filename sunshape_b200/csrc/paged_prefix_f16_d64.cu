@@ -1,0 +1,6 @@
+// Attention over a shared prefix, head_dim 64, f16 values.
+#include "paged_prefix.cuh"
+
+namespace sunshape {
+SUNSHAPE_PREFIX_INSTANCES(64, __half)
+}  // namespace sunshape

@@ -274,7 +274,12 @@ def _check_attention(got, cache, q, table, lens, pt, prefix, **kw):
     (64, 64, 8, 256, 0, 2, 7, 3, 16, [0, 2, 33], 129, torch.float16),
     (128, 128, 4, 256, 0, 1, 8, 1, 32, [1, 2, 3] * 7, 1, torch.bfloat16),
     (128, 64, 8, 256, 2, 1, 24, 2, 64, [70, 10], 700, torch.float16),
-    (64, 128, 2, 64, 0, 2, 4, 1, 48, [50, 51], 257, torch.bfloat16)])
+    (64, 128, 2, 64, 0, 2, 4, 1, 48, [50, 51], 257, torch.bfloat16),
+    (128, 128, 8, 256, 3, 2, 8, 1, 16, [1, 0, 5, 17] * 10, 2000, torch.bfloat16),
+    (64, 64, 4, 256, 0, 3, 8, 1, 32, [3] * 50, 383, torch.float16),
+    (128, 64, 4, 256, 2, 1, 4, 2, 48, [9] * 17, 128, torch.bfloat16),
+    (64, 64, 2, 256, 5, 2, 16, 1, 64, [2, 70], 1025, torch.bfloat16),
+    (128, 128, 2, 256, 0, 1, 8, 1, 128, [1] * 33, 1500, torch.float16)])
 def test_paged_attention(D, Dv, bd, C, heavy, H, G, L, page, lens, prefix, dtype):
     codec, _ = make_paged_codec(D, bd, H, heavy=heavy, C=C, seed=D + bd + G, shared=(G == 7))
     cache, q, table, n, pt = _attention_case(codec, H, G, len(lens), L, lens, prefix, page, dtype, Dv, seed=G)
