@@ -24,7 +24,7 @@ namespace sunshape {
 
 constexpr int kPfTokens = 128, kPfRows = 256;
 constexpr int kPfThreads = 512;    // warps 0: values, 1: MMA, 2-3: none, 4-7: keys, 8-11 and 12-15: softmax of the row groups
-constexpr int kPfRegs0 = 64, kPfRegsKeys = 104, kPfRegsSoftmax = 168;
+constexpr int kPfRegs0 = 48, kPfRegsKeys = 80, kPfRegsSoftmax = 192;
 static_assert(kPfRegs0 + kPfRegsKeys + 2 * kPfRegsSoftmax <= 4 * 128, "the split waits forever where it exceeds the launch");
 
 struct PrefixSmem {
@@ -96,7 +96,65 @@ __device__ __forceinline__ void tm_store32(uint32_t addr, const U* v) {
       "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31]), "r"(addr)
       : "memory");
 }
+// pairs of fp32 numbers in one instruction
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(r)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(r)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return r;
+}
+
 __device__ __forceinline__ void tm_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// One row's 128 scores to weights 2^((s - mb) f), as 16-bit pairs, with their sum and the largest score.  Scores from
+// `valid` on are left out.
+template <typename T, bool TAIL>
+__device__ __forceinline__ void tile_weights(uint32_t s_t, int valid, float mb, float f, uint32_t* pk, float& top, float& sum) {
+  const float INF = __int_as_float(0x7f800000);
+  float t0 = -INF, t1 = -INF;
+  float2 acc = make_float2(0.f, 0.f);
+  const float2 nb = make_float2(-mb, -mb), ff = make_float2(f, f);
+  float x[2][32];
+  tm_load32(x[0], s_t);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    tm_wait_load(x[c & 1]);
+    if (c < 3) tm_load32(x[(c + 1) & 1], s_t + (c + 1) * 32);
+    float* v = x[c & 1];
+    if constexpr (TAIL) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e)
+        if (c * 32 + e >= valid) v[e] = -INF;
+    }
+#pragma unroll
+    for (int e = 0; e < 32; e += 4) {
+      t0 = fmaxf(t0, fmaxf(v[e], v[e + 1]));
+      t1 = fmaxf(t1, fmaxf(v[e + 2], v[e + 3]));
+    }
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) {
+      const float2 y = mul2(add2(make_float2(v[e], v[e + 1]), nb), ff);
+      float2 w = make_float2(fast_exp2(y.x), fast_exp2(y.y));
+      if constexpr (TAIL) {             // -inf times a factor of zero
+        w.x = c * 32 + e < valid ? w.x : 0.f;
+        w.y = c * 32 + e + 1 < valid ? w.y : 0.f;
+      }
+      acc = add2(acc, w);
+      pk[c * 16 + e / 2] = pack2<T>(w.x, w.y);
+    }
+  }
+  top = fmaxf(t0, t1);
+  sum = acc.x + acc.y;
+}
+template <typename T>
+__device__ __forceinline__ void tile_weights(uint32_t s_t, int valid, float mb, float f, uint32_t* pk, float& top, float& sum) {
+  if (valid < kPfTokens) tile_weights<T, true>(s_t, valid, mb, f, pk, top, sum);
+  else tile_weights<T, false>(s_t, valid, mb, f, pk, top, sum);
+}
 
 template <int D, int DV, int BD, typename T>
 __global__ void __launch_bounds__(kPfThreads, 1)
@@ -230,7 +288,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           const uint32_t id_qk = f16_idesc(false, kPfTokens, false), id_pv = f16_idesc(BF16, DV, true);
           const uint64_t qd = smem_desc(smem_u32(q_s), 16), kd = smem_desc(smem_u32(k_s), 16);
           auto qk = [&](int g) {
-#pragma unroll 1
+#pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
               const uint64_t off = (ks >> 2) * (HALF >> 4) + (ks & 3) * 2;
               tc_mma_ss(tmem + g * 128, qd + g * ((128 * D * 2) >> 4) + off, kd + off, id_qk, ks > 0);
@@ -239,7 +297,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           };
           auto pv = [&](int g, int i) {
             const uint64_t vd = smem_desc(smem_u32(v_s + ((it + i) & 1) * PrefixSmem::v(DV)), HALF);
-#pragma unroll 1
+#pragma unroll
             for (int ks = 0; ks < kPfTokens / 16; ++ks)
               tc_mma_ts(tmem + 256 + g * DV, tmem + g * 128 + ks * 8, vd + ks * (2048 >> 4), id_pv, i > 0 || ks > 0);
             pf_commit(&pv_done[g]);
@@ -316,10 +374,11 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         constexpr int PER = 8 / BD, WORDS = BD / 2;
 #pragma unroll
         for (int half = 0; half < D / 64; ++half) {
+          uint32_t chunk[8][4];                  // all loads before the stores, which the compiler can not tell apart
 #pragma unroll
           for (int s = 0; s < 8; ++s) {
             const int j = s ^ mul;               // chunk of the half; its blocks are half * 8 * PER + j * PER + x
-            uint32_t w[4];
+            uint32_t* const w = chunk[s];
             if constexpr (PER == 1) {
               const uint32_t c = __byte_perm(ib[half * 2], ib[half * 2 + 1], j) & 0xffu;
               lds_words<16, 0>(w, image_a + half * 32768 + (c << 7) + j * 16);
@@ -338,8 +397,12 @@ __global__ void __launch_bounds__(kPfThreads, 1)
               for (int x = 0; x < 4; ++x)
                 lds_words<4, 0>(w + x, image_a + half * 32768 + (((word >> (8 * x)) & 0xffu) << 7) + j * 16 + 4 * x);
             }
+          }
+#pragma unroll
+          for (int s = 0; s < 8; ++s) {
+            const int j = s ^ mul;
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(smem_u32(dst) + half * HALF + ((j ^ (tok_l & 7)) << 4)),
-                         "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                         "r"(chunk[s][0]), "r"(chunk[s][1]), "r"(chunk[s][2]), "r"(chunk[s][3])
                          : "memory");
           }
         }
@@ -434,34 +497,8 @@ __global__ void __launch_bounds__(kPfThreads, 1)
 #pragma unroll 1
           while (true) {
             const float mb = m == -INF ? 0.f : m;
-            float top = -INF;
-            sum = 0.f;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              float x[32];
-              tm_load32(x, s_t + c * 32);
-              tm_wait_load(x);
-              if (valid < kPfTokens) {
-#pragma unroll
-                for (int e = 0; e < 32; ++e)
-                  if (c * 32 + e >= valid) x[e] = -INF;
-              }
-#pragma unroll
-              for (int e = 0; e < 32; e += 2) top = fmaxf(top, fmaxf(x[e], x[e + 1]));
-              float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-              for (int e = 0; e < 32; e += 2) {
-                float w0 = fast_exp2((x[e] - mb) * f), w1 = fast_exp2((x[e + 1] - mb) * f);
-                if (valid < kPfTokens) {             // -inf times a factor of zero
-                  w0 = c * 32 + e < valid ? w0 : 0.f;
-                  w1 = c * 32 + e + 1 < valid ? w1 : 0.f;
-                }
-                s0 += w0;
-                s1 += w1;
-                pk[c * 16 + e / 2] = pack2<T>(w0, w1);
-              }
-              sum += s0 + s1;
-            }
+            float top;
+            tile_weights<T>(s_t, valid, mb, f, pk, top, sum);
             const bool grows = m == -INF ? top != -INF : (top - m) * f > kSlack;
             if (!__any_sync(0xffffffffu, grows)) break;
             const float nm = fmaxf(m, top);
