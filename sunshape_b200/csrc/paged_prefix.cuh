@@ -9,8 +9,9 @@
 //     of eight lanes are all different: neither side has bank conflicts;
 //   * one thread issues the tcgen05.mma of both groups of 128 rows in turn -- PV of one group and QK of its next tile
 //     while the other group's softmax runs -- with accumulators in tensor memory, S and O of both groups: 512 columns;
-//   * four warps a row group, one thread a row: scores from tensor memory, weights in powers of two against a maximum
-//     that may fall behind by 2^kSlack (then, and only then, O is rescaled in place), P as 16-bit pairs over S.
+//   * eight warps a row group, two threads a row with 64 columns each: scores from tensor memory, weights in powers of
+//     two against a maximum that may fall behind by 2^kSlack (then, and only then, O is rescaled in place), P as 16-bit
+//     pairs over S.  One thread a row takes about 2150 cycles a tile, during which its group's next products wait.
 // Bound: 2 (D + DV) 256 multiply-adds a token and head against one exponential for each row: at D = DV = 128 the tensor
 // cores and the special function units both need 2048 cycles a tile of 256 rows, so the two groups' phases must overlap.
 //
@@ -23,9 +24,10 @@
 namespace sunshape {
 
 constexpr int kPfTokens = 128, kPfRows = 256;
-constexpr int kPfThreads = 512;    // warps 0: values, 1: MMA, 2-3: none, 4-7: keys, 8-11 and 12-15: softmax of the row groups
-constexpr int kPfRegs0 = 48, kPfRegsKeys = 80, kPfRegsSoftmax = 192;
-static_assert(kPfRegs0 + kPfRegsKeys + 2 * kPfRegsSoftmax <= 4 * 128, "the split waits forever where it exceeds the launch");
+constexpr int kPfThreads = 768;    // warps 0: values, 1: MMA, 2-3: none, 4-7: keys, 8-15 and 16-23: softmax of the row groups
+constexpr int kPfLaunchRegs = 80, kPfRegs0 = 40, kPfRegsKeys = 88, kPfRegsSoftmax = 88;
+static_assert(kPfRegs0 <= kPfLaunchRegs && kPfRegsKeys >= kPfLaunchRegs && kPfRegsSoftmax >= kPfLaunchRegs, "dec and inc");
+static_assert(kPfRegs0 + kPfRegsKeys + 4 * kPfRegsSoftmax <= 6 * kPfLaunchRegs, "the split waits forever where it exceeds the launch");
 
 struct PrefixSmem {
   // all operands 1024-byte aligned
@@ -33,7 +35,7 @@ struct PrefixSmem {
   static __host__ __device__ constexpr int k(int d) { return kPfTokens * d * 2; }
   static __host__ __device__ constexpr int v(int dv) { return kPfTokens * dv * 2; }
   static __host__ __device__ constexpr int total(int d, int dv) {
-    return 1024 + q(d) + k(d) + 2 * v(dv) + d * 512 + kPfRows * 4 + 256 + 128;
+    return q(d) + k(d) + 2 * v(dv) + d * 512 + 2 * kPfRows * 4 + 128 + 64;
   }
 };
 
@@ -110,7 +112,7 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
 
 __device__ __forceinline__ void tm_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// One row's 128 scores to weights 2^((s - mb) f), as 16-bit pairs, with their sum and the largest score.  Scores from
+// 64 scores of a row to weights 2^((s - mb) f), as 16-bit pairs, with their sum and the largest score.  Scores from
 // `valid` on are left out.
 template <typename T, bool TAIL>
 __device__ __forceinline__ void tile_weights(uint32_t s_t, int valid, float mb, float f, uint32_t* pk, float& top, float& sum) {
@@ -118,13 +120,11 @@ __device__ __forceinline__ void tile_weights(uint32_t s_t, int valid, float mb, 
   float t0 = -INF, t1 = -INF;
   float2 acc = make_float2(0.f, 0.f);
   const float2 nb = make_float2(-mb, -mb), ff = make_float2(f, f);
-  float x[2][32];
-  tm_load32(x[0], s_t);
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    tm_wait_load(x[c & 1]);
-    if (c < 3) tm_load32(x[(c + 1) & 1], s_t + (c + 1) * 32);
-    float* v = x[c & 1];
+  for (int c = 0; c < 2; ++c) {
+    float v[32];
+    tm_load32(v, s_t + c * 32);
+    tm_wait_load(v);
     if constexpr (TAIL) {
 #pragma unroll
       for (int e = 0; e < 32; ++e)
@@ -152,7 +152,7 @@ __device__ __forceinline__ void tile_weights(uint32_t s_t, int valid, float mb, 
 }
 template <typename T>
 __device__ __forceinline__ void tile_weights(uint32_t s_t, int valid, float mb, float f, uint32_t* pk, float& top, float& sum) {
-  if (valid < kPfTokens) tile_weights<T, true>(s_t, valid, mb, f, pk, top, sum);
+  if (valid < kPfTokens / 2) tile_weights<T, true>(s_t, valid, mb, f, pk, top, sum);
   else tile_weights<T, false>(s_t, valid, mb, f, pk, top, sum);
 }
 
@@ -162,13 +162,13 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   constexpr int NB = D / BD, KS = D / 16, IMAGE = D * 512, RF = row_floats(DV);
   constexpr int HALF = kPfTokens * 128;          // an operand's 64 columns of 128 rows
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* const q_s = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t q_s[];   // the operands' swizzle counts on the base's alignment
   uint8_t* const k_s = q_s + PrefixSmem::q(D);   // q: [2 groups][D / 64][128 rows][128 bytes], swizzled
   uint8_t* const v_s = k_s + PrefixSmem::k(D);   // [2][DV / 64][128 tokens][128 bytes]
   uint8_t* const image = v_s + 2 * PrefixSmem::v(DV);
-  float* const f_s = reinterpret_cast<float*>(image + IMAGE);              // [kPfRows] factor of a row's scores
-  uint64_t* const bars = reinterpret_cast<uint64_t*>(f_s + kPfRows);
+  // [2 groups][2 halves][128]: what the two threads of a row tell each other; first, in half 0, the rows' score factors
+  float* const row_s = reinterpret_cast<float*>(image + IMAGE);
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(row_s + 2 * kPfRows);
   uint64_t *const v_full = bars, *const v_free = bars + 2, *const k_ready = bars + 4, *const k_free = bars + 5,
                   *const s_full = bars + 6, *const p_ready = bars + 8, *const pv_done = bars + 10, *const cb_bar = bars + 12;
   uint32_t* const tmem_s = reinterpret_cast<uint32_t*>(bars + 13);
@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       mbar_init(&v_full[i], 1);
       mbar_init(&v_free[i], 1);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_ready[i], 128);
+      mbar_init(&p_ready[i], 256);
       mbar_init(&pv_done[i], 1);
     }
     mbar_init(k_ready, 128);
@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
   } else if (warp < 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPfRegsKeys));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPfRegsKeys));
     while (next_piece()) {
       named_barrier(1, kPfThreads);
       // -------------------------------------------------------------------- keys
@@ -449,7 +449,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         for (int i = 0; i < 8; ++i) src_d[i] = (int)p.perm[c * 8 + i];
         const float k_scale = p.image_scale[cb];
 #pragma unroll 2
-        for (int r = (warp - 8) * RPW + lane / CH; r < groups * 128; r += 8 * RPW) {
+        for (int r = (warp - 8) * RPW + lane / CH; r < groups * 128; r += 16 * RPW) {
           float x[8], mx = 0.f;
 #pragma unroll
           for (int i = 0; i < 8; ++i) x[i] = 0.f;
@@ -473,34 +473,39 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           w.w = pack2<__half>(x[6] * sc, x[7] * sc);
           const int row = r & 127;
           *reinterpret_cast<uint4*>(q_s + (r >> 7) * (128 * D * 2) + (c >> 3) * HALF + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = w;
-          if (c == 0) f_s[r] = fabsf(p.scale_log2) * __int_as_float((127 + ec) << 23) / k_scale;
+          if (c == 0) row_s[(r >> 7) * 256 + (r & 127)] = fabsf(p.scale_log2) * __int_as_float((127 + ec) << 23) / k_scale;
         }
         fence_proxy_async_smem();
       }
       named_barrier(1, kPfThreads);
-      if ((warp - 8) / 4 < groups) {
+      const int g = (warp - 8) / 8;
+      if (g < groups) {
         // ----------------------------------------------------------------- softmax
-        const int g = (warp - 8) / 4, r = g * 128 + (warp & 3) * 32 + lane;
+        const int half = ((warp - 8) >> 2) & 1, rl = (warp & 3) * 32 + lane, r = g * 128 + rl;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t s_t = tmem + g * 128 + lanes, o_t = tmem + 256 + g * DV + lanes;
+        const uint32_t s_t = tmem + g * 128 + lanes + half * 64, p_t = tmem + g * 128 + lanes + half * 32;
+        const uint32_t o_t = tmem + 256 + g * DV + lanes + half * (DV / 2);
+        float* const mine = row_s + g * 256 + half * 128 + rl;
+        const float* const other = row_s + g * 256 + (half ^ 1) * 128 + rl;
         const int base = g ? it1 : it;
-        const float f = f_s[r];
-        float m = -INF, l = 0.f;                   // maximum before its factor, sum
+        const int pair_bar = 2 + g * 4 + (warp & 3);   // the two warps of these rows
+        const float f = row_s[g * 256 + rl];
+        named_barrier(pair_bar, 64);
+        float m = -INF, l = 0.f;                 // maximum before its factor, sum of this half
         for (int i = 0; i < n; ++i) {
           mbar_wait(&s_full[g], (base + i) & 1, p.err, kErrWait);
           pf_fence_after();
-          const int valid = p.prefix_len - (t0 + i) * kPfTokens;
-          uint32_t pk[kPfTokens / 2];
-          float sum;
-          // weights against the last maximum; again where the tile's largest score exceeds it by too much (always for the
-          // first tile): the scores are in tensor memory until P is written over them
-#pragma unroll 1
-          while (true) {
-            const float mb = m == -INF ? 0.f : m;
-            float top;
-            tile_weights<T>(s_t, valid, mb, f, pk, top, sum);
-            const bool grows = m == -INF ? top != -INF : (top - m) * f > kSlack;
-            if (!__any_sync(0xffffffffu, grows)) break;
+          const int valid = p.prefix_len - (t0 + i) * kPfTokens - half * 64;
+          uint32_t pk[32];
+          float sum, top;
+          // weights against the last maximum; again where the row's largest score of the tile exceeds it by too much
+          // (always for the first tile): the scores are in tensor memory until P is written over them
+          tile_weights<T>(s_t, valid, m == -INF ? 0.f : m, f, pk, top, sum);
+          *mine = top;
+          named_barrier(pair_bar, 64);             // both have read their scores, too
+          top = fmaxf(top, *other);
+          const bool grows = m == -INF ? top != -INF : (top - m) * f > kSlack;
+          if (__any_sync(0xffffffffu, grows)) {  // alike in both warps of these rows
             const float nm = fmaxf(m, top);
             if (i) {
               mbar_wait(&pv_done[g], (base + i - 1) & 1, p.err, kErrWait);
@@ -508,7 +513,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
               const float e = m == -INF ? 0.f : fast_exp2((m - nm) * f);
               l *= e;
 #pragma unroll 1
-              for (int c = 0; c < DV / 32; ++c) {
+              for (int c = 0; c < DV / 64; ++c) {
                 float v[32];
                 tm_load32(v, o_t + c * 32);
                 tm_wait_load(v);
@@ -518,16 +523,20 @@ __global__ void __launch_bounds__(kPfThreads, 1)
               }
             }
             m = nm;
+            tile_weights<T>(s_t, valid, m == -INF ? 0.f : m, f, pk, top, sum);
+            named_barrier(pair_bar, 64);           // P of one half lies over scores of the other
           }
           l += sum;
-          tm_store32(s_t, pk);
-          tm_store32(s_t + 32, pk + 32);
+          tm_store32(p_t, pk);
           tm_wait_store();
           pf_fence_before();
           mbar_arrive(&p_ready[g]);
         }
         mbar_wait(&pv_done[g], (base + n - 1) & 1, p.err, kErrWait);
         pf_fence_after();
+        *mine = l;
+        named_barrier(pair_bar, 64);
+        l += *other;
         if (*bad_s) l = __int_as_float(0x7fffffff);
         float* dst = nullptr;
         if (r0 + r < rows_total) {
@@ -535,16 +544,17 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           else dst = p.prefix_slots + ((int64_t)(2 * cta + (begins ? 1 : 0)) * kPfRows + r) * RF;
         }
 #pragma unroll 1
-        for (int c = 0; c < DV / 32; ++c) {
+        for (int c = 0; c < DV / 64; ++c) {
           float v[32];
           tm_load32(v, o_t + c * 32);
           tm_wait_load(v);
           if (dst) {
 #pragma unroll
-            for (int x = 0; x < 32; x += 4) *reinterpret_cast<float4*>(dst + c * 32 + x) = make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]);
+            for (int x = 0; x < 32; x += 4)
+              *reinterpret_cast<float4*>(dst + half * (DV / 2) + c * 32 + x) = make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]);
           }
         }
-        if (dst) *reinterpret_cast<float2*>(dst + DV) = make_float2(m == -INF ? -INF : m * f, l);
+        if (dst && half == 0) *reinterpret_cast<float2*>(dst + DV) = make_float2(m == -INF ? -INF : m * f, l);
         pf_fence_before();
       }
       end_piece();
@@ -588,7 +598,7 @@ int launch_paged_prefix(const AttnParams& p, const CUtensorMap& vmap, int grid, 
   const int smem = PrefixSmem::total(D, DV);
   // the split of registers waits forever where the block has fewer than it was planned for
   cudaFuncAttributes fa;
-  if (cudaFuncGetAttributes(&fa, k) != cudaSuccess || fa.numRegs != 128)
+  if (cudaFuncGetAttributes(&fa, k) != cudaSuccess || fa.numRegs != kPfLaunchRegs)
     return set_last_error(SUNSHAPE_E_CUDA, "paged prefix kernel was built for another register count.");
   cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   k<<<grid, kPfThreads, smem, st>>>(p, vmap);
