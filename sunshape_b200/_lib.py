@@ -8,9 +8,11 @@ with the reason, in the style of the reference's fast-path gate
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 import os
+import struct as _struct
 import threading
 
 import torch
@@ -95,6 +97,8 @@ _lock = threading.Lock()
 def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
     """Load (once) and type the C ABI.  Raises if the library was not built."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib
@@ -369,11 +373,59 @@ def attention_scores_packed(cd: CodecDesc, indices: torch.Tensor, index_bits: in
             kv_heads, rows, ptr(out), stream_ptr(dev)))
 
 
-def norm_rotate(dev, q: RowsDesc, q_out: RowsDesc, q_weight, k, k_out, k_weight, dtype: int, weight_dtype: int, batch: int,
-                length: int, dim: int, eps: float, rotation) -> None:
-    with torch.cuda.device(dev):
-        _check(load_library().sunshape_norm_rotate(q, q_out, ptr(q_weight), k, k_out, ptr(k_weight), dtype, weight_dtype,
-                                                   batch, length, dim, eps, rotation, stream_ptr(dev)))
+# ---- paged serving.  These calls are made several times a layer and decode step, so their descriptors are packed in one
+# go instead of field by field, and the device is switched only where it is not the current one.
+_ROWS = _struct.Struct("PqqqiP")          # sunshape_rows_t, padded
+_ROTATION = _struct.Struct("PPPqqqiiii")  # sunshape_rotation_t, padded
+_paged_calls = None
+
+
+def _paged():
+    """The paged entry points with descriptors as bytes."""
+    global _paged_calls
+    if _paged_calls is None:
+        lib = load_library()
+        vp, i32, i64, f32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
+        calls = {}
+        for name, types in (
+                ("sunshape_norm_rotate", [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, f32, vp, vp]),
+                ("sunshape_paged_append", [vp, vp, vp, vp, vp, i32, i32, vp, i64, i64, vp, vp]),
+                ("sunshape_paged_attention", [vp, vp, vp, vp, i32, i32, vp, i64, i32, vp, vp, i32, f32, i32, vp, vp, i64,
+                                              vp])):
+            f = lib[name]
+            f.argtypes, f.restype = types, ctypes.c_int
+            calls[name] = f
+        _paged_calls = calls
+    return _paged_calls
+
+
+def rows(t: torch.Tensor) -> bytes:
+    """sunshape_rows_t of [B, heads, L, dim] rows."""
+    sb, sh, sl, _ = t.stride()
+    return _ROWS.pack(t.data_ptr(), sb, sh, sl, t.shape[1], 0)
+
+
+def rotation(cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor, sb: int, sl: int, interleaved: bool) -> bytes:
+    n, half = cos.shape
+    return _ROTATION.pack(cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), sb, sl, n,
+                          I32 if positions.dtype is torch.int32 else I64, 2 * half, 1 if interleaved else 0, 0)
+
+
+def _on_device(index: int, call, *args) -> None:
+    """One call of the C ABI on device ``index`` and its current stream (the last argument)."""
+    if torch._C._cuda_getDevice() == index:
+        rc = call(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = call(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _check(rc)
+
+
+def norm_rotate(index: int, q: bytes, q_out: bytes, q_weight, k, k_out, k_weight, dtype: int, weight_dtype: int, batch: int,
+                length: int, dim: int, eps: float, rot) -> None:
+    _on_device(index, _paged()["sunshape_norm_rotate"], q, q_out, ptr(q_weight), k, k_out, ptr(k_weight), dtype,
+               weight_dtype, batch, length, dim, eps, rot)
 
 
 def paged_tables(cd: CodecDesc, dev) -> torch.Tensor:
@@ -388,24 +440,29 @@ def paged_tables(cd: CodecDesc, dev) -> torch.Tensor:
     return tables
 
 
-def paged_append(dev, cd: CodecDesc, tables: torch.Tensor, pages: PagesDesc, key: RowsDesc, value: RowsDesc, batch: int,
-                 length: int, slots: torch.Tensor, rotation) -> None:
-    with torch.cuda.device(dev):
-        _check(load_library().sunshape_paged_append(cd, ptr(tables), pages, key, value, batch, length, ptr(slots),
-                                                    slots.stride(0), slots.stride(1), rotation, stream_ptr(dev)))
+def paged_append(index: int, cd: CodecDesc, tables: torch.Tensor, pages: PagesDesc, key: bytes, value: bytes, batch: int,
+                 length: int, slots: torch.Tensor, rot) -> None:
+    sb, sl = slots.stride()
+    _on_device(index, _paged()["sunshape_paged_append"], ctypes.addressof(cd), tables.data_ptr(), ctypes.addressof(pages),
+               key, value, batch, length, slots.data_ptr(), sb, sl, rot)
 
 
-def paged_attention(dev, cd: CodecDesc, tables: torch.Tensor, pages: PagesDesc, query: RowsDesc, batch: int, query_len: int,
-                    page_table: torch.Tensor, seq_lens: torch.Tensor, prefix_table, prefix_len: int, scale: float,
-                    causal: bool, out: torch.Tensor) -> None:
-    lib = load_library()
+def paged_attention(index: int, cd: CodecDesc, tables: torch.Tensor, pages: PagesDesc, query: torch.Tensor, batch: int,
+                    q_heads: int, query_len: int, page_table: torch.Tensor, seq_lens: torch.Tensor, prefix_table,
+                    prefix_len: int, scale: float, causal: bool, out: torch.Tensor) -> None:
     cols = page_table.shape[1]
-    with torch.cuda.device(dev):
-        need = lib.sunshape_paged_attention_workspace_bytes(batch, query.heads, pages.kv_heads, query_len,
-                                                            pages.value_dim, cols, pages.page_size, prefix_len)
-        # a block of the allocator of the current stream (of the graph's own pool under capture): two streams or
-        # two captured graphs never share one
-        ws = torch.empty(max(need, 256), dtype=torch.uint8, device=dev)
-        _check(lib.sunshape_paged_attention(cd, ptr(tables), pages, query, batch, query_len, ptr(page_table),
-                                            page_table.stride(0), cols, ptr(seq_lens), ptr(prefix_table), prefix_len,
-                                            scale, 1 if causal else 0, ptr(out), ptr(ws), ws.numel(), stream_ptr(dev)))
+    # on another device than the current one, the library sizes the workspace for the device it runs on
+    here = torch._C._cuda_getDevice() == index
+    with (_NULL if here else torch.cuda.device(index)):
+        need = load_library().sunshape_paged_attention_workspace_bytes(
+            batch, q_heads, pages.kv_heads, query_len, pages.value_dim, cols, pages.page_size, prefix_len)
+    # a block of the allocator of the current stream (of the graph's own pool under capture): two streams or two
+    # captured graphs never share one
+    ws = torch.empty(need if need > 256 else 256, dtype=torch.uint8, device=query.device)
+    _on_device(index, _paged()["sunshape_paged_attention"], ctypes.addressof(cd), tables.data_ptr(),
+               ctypes.addressof(pages), rows(query), batch, query_len, page_table.data_ptr(), page_table.stride(0), cols,
+               seq_lens.data_ptr(), ptr(prefix_table), prefix_len, scale, 1 if causal else 0, out.data_ptr(), ws.data_ptr(),
+               ws.numel())
+
+
+_NULL = contextlib.nullcontext()

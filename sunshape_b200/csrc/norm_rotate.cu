@@ -8,6 +8,7 @@
 // then needs no exchange between threads, only the norm's sum does (three shuffles at dim 128).  Cosines and
 // sines belong to the token, not to the head, so a thread keeps them in registers over the heads that it takes.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "paged.cuh"
@@ -271,7 +272,7 @@ void launch(NormRotateParams& p, bool vec, cudaStream_t st) {
   // Groups that share a token: one where there are tokens enough to give every SM 512 threads, which a thread's cosines,
   // weights and rows in flight allow; up to one for each head below that, so that a decode step's few rows spread out.
   const int heads = p.heads[0] + p.heads[1];
-  p.parts = (int)std::min<int64_t>(heads, std::max<int64_t>(1, (int64_t)sm_count() * 512 / w / p.tokens));
+  p.parts = (int)std::min<int64_t>(heads, std::max<int64_t>(1, (int64_t)paged_sm_count() * 512 / w / p.tokens));
   p.items = p.tokens * p.parts;
   const unsigned grid = (unsigned)((p.items * w + 127) / 128);
   if (p.rot.interleaved) norm_rotate_vec<T, true><<<grid, 128, 0, st>>>(p);
@@ -285,8 +286,37 @@ bool float_type(int d) { return d == SUNSHAPE_F32 || d == SUNSHAPE_BF16 || d == 
 __device__ int g_paged_error;
 
 int* paged_error_word() {
+  static std::atomic<int*> known[64];            // the address of a device's word never changes
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return nullptr;
+  int* w = dev < 64 ? known[dev].load(std::memory_order_relaxed) : nullptr;
+  if (w) return w;
   void* a = nullptr;
-  return cudaGetSymbolAddress(&a, g_paged_error) == cudaSuccess ? static_cast<int*>(a) : nullptr;
+  if (cudaGetSymbolAddress(&a, g_paged_error) != cudaSuccess) return nullptr;
+  if (dev < 64) known[dev].store(static_cast<int*>(a), std::memory_order_relaxed);
+  return static_cast<int*>(a);
+}
+
+int paged_sm_count() {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return sm_count();
+  int n = known[dev].load(std::memory_order_relaxed);
+  if (!n) known[dev].store(n = sm_count(), std::memory_order_relaxed);
+  return n;
+}
+
+bool ready_kernel(const void* kernel, int smem, int regs, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  if (dev < 64 && done.load(std::memory_order_acquire) >> dev & 1) return true;
+  if (regs) {
+    cudaFuncAttributes a;
+    if (cudaFuncGetAttributes(&a, kernel) != cudaSuccess || a.numRegs != regs) return false;
+  }
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return false;
+  if (dev < 64) done.fetch_or(uint64_t(1) << dev, std::memory_order_release);
+  return true;
 }
 
 int make_rotation(const sunshape_rotation_t* r, int dim, bool empty, Rotation* out) {

@@ -2,6 +2,8 @@
 // paged_attention.cu).
 #pragma once
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace sunshape {
@@ -16,8 +18,12 @@ int set_last_error(int code, const char* msg);
 int launch_status(const char* what);
 // argument checks shared with the contiguous entry points, capi.cu
 int check_codec_args(const sunshape_codec_t* c);
-// SMs of the current device, capi.cu
+// SMs of the current device, capi.cu; and the same, asked once a device
 int sm_count();
+int paged_sm_count();
+// Lets a kernel use `smem` bytes of dynamic shared memory -- the most that any call of it asks for -- and checks that it
+// was built for `regs` registers (0: any number), once a device.
+bool ready_kernel(const void* kernel, int smem, int regs, std::atomic<uint64_t>& done);
 // checks a page pool against its codec, paged_append.cu
 int check_pages(const sunshape_codec_t* c, const sunshape_pages_t* pg);
 

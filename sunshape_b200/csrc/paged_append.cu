@@ -545,11 +545,12 @@ void launch(AppendParams& p, cudaStream_t st) {
   const int64_t tiles = (p.tokens + kTokens - 1) / kTokens;
   // A head's blocks are shared out until every SM has two CTAs (one token a sequence leaves one tile of tokens), and in
   // any case to 32 elements a CTA, with whose keys in shared memory an SM holds five
-  const int64_t fill = 2 * sm_count() / (tiles * p.H);
+  const int64_t fill = 2 * paged_sm_count() / (tiles * p.H);
   p.blocks = (int)std::min<int64_t>((p.nb + std::max<int64_t>(fill, 1) - 1) / std::max<int64_t>(fill, 1), 32 / BD);
   p.splits = (p.nb + p.blocks - 1) / p.blocks;
   const int smem = 2 * record_bytes(BD) + kTokens * ((p.blocks * BD + 8) * 4 + 3 * 8 + 4 + p.blocks);
-  cudaFuncSetAttribute(append_kernel<T, BD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<uint64_t> done;
+  ready_kernel((const void*)append_kernel<T, BD>, 2 * record_bytes(BD) + kTokens * (40 * 4 + 28 + 32 / BD), 0, done);
   append_kernel<T, BD><<<dim3((unsigned)tiles, p.H, p.splits + 1), kWarps * 32, smem, st>>>(p);
 }
 

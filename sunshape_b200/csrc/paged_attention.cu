@@ -6,7 +6,6 @@
 namespace sunshape {
 namespace {
 
-constexpr int kSmemMax = 232448;    // 227 KB
 
 int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
 
@@ -40,17 +39,17 @@ bool plan(AttnParams& p, int d, int dv, int bd) {
   p.item_rows = item_rows((p.prefix_mode ? (int64_t)p.B : 1) * p.G * p.L);
   p.off_idx = kTile * dv * 2;
   p.off_heavy = p.off_idx + kTile * p.nb;
-  p.stage_bytes = (p.off_heavy + kTile * p.n_heavy * bd * 2 + 4 + 1023) / 1024 * 1024;
+  p.stage_bytes = (p.off_heavy + kTile * p.n_heavy * bd * 2 + 1023) / 1024 * 1024;
   // alignment, codebook, permutation, plan, codebook barrier, pieces' descriptions, dense slots
   const int fixed = 1024 + d * 512 + d * 4 + (2 * kPlanChunks + 2) * 4 + 8 + 16 + kPairs * 32 + p.nb;
   const int left = kSmemMax - fixed;
-  p.stages = std::min(6, left / (kPairs * (p.stage_bytes + 16)));
+  p.stages = std::min(6, left / (kPairs * (p.stage_bytes + 20)));
   p.pairs = kPairs;
   if (p.stages < 2) {
     p.stages = 2;
-    p.pairs = (left - kPairs * 2 * 16) / (2 * p.stage_bytes);
+    p.pairs = (left - kPairs * 2 * 20) / (2 * p.stage_bytes);
   }
-  p.smem = fixed + p.pairs * p.stages * p.stage_bytes + kPairs * p.stages * 16;
+  p.smem = fixed + p.pairs * p.stages * p.stage_bytes + kPairs * p.stages * 20;
   return p.pairs >= 1;
 }
 
@@ -84,7 +83,7 @@ int64_t sunshape_paged_attention_workspace_bytes(int32_t batch, int32_t q_heads,
   const int64_t rows = (int64_t)batch * q_heads * query_len;
   const int64_t own = kv_heads > 0 ? (int64_t)q_heads / kv_heads * query_len : 0;
   const bool tensor = prefix_len > 0 && own * batch >= kPrefixRows;
-  return layout(sm_count(), rows, item_rows(prefix_len > 0 && !tensor ? own * batch : own), value_dim, prefix_len > 0, tensor).total;
+  return layout(paged_sm_count(), rows, item_rows(prefix_len > 0 && !tensor ? own * batch : own), value_dim, prefix_len > 0, tensor).total;
 }
 
 int sunshape_paged_attention(const sunshape_codec_t* codec, const void* tables, const sunshape_pages_t* pages,
@@ -146,7 +145,7 @@ int sunshape_paged_attention(const sunshape_codec_t* codec, const void* tables, 
   p.image = tables;
   p.image_scale = reinterpret_cast<const float*>(static_cast<const uint8_t*>(tables) + tab.iscale);
   p.out = out;
-  const int grid = sm_count();
+  const int grid = paged_sm_count();
   const int64_t own = (int64_t)p.G * p.L;
   const bool tensor = prefix_len > 0 && own * batch >= kPrefixRows;
   const Layout at = layout(grid, rows, item_rows(prefix_len && !tensor ? own * batch : own), dv, prefix_len > 0, tensor);

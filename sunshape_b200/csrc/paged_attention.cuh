@@ -17,6 +17,7 @@
 
 namespace sunshape {
 
+constexpr int kSmemMax = 232448;   // 227 KB
 constexpr int kTile = 32;          // tokens of a tile
 constexpr int kItemRows = 16;      // most query rows of an item
 constexpr int kPairs = 8;          // pairs of a consumer (warps 0-7) and a producer warp (8-15)

@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   constexpr int ROT = 16 / BD;                                 // tokens that share a load phase and a column set
   constexpr int KS = D / 16, ROWS = 8 * NT, RF = row_floats(DV);
   constexpr int IMAGE = D * 512;
-  constexpr int MT = 2;                                        // groups of 16 tokens of a step
+  constexpr int MT = kTile / 16;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int ring_bytes = p.stages * p.stage_bytes;             // of a pair
@@ -140,7 +140,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   // of a pair: head piece (-1: no tiles, 0: none, 1: cut again, 2: last), its item; tail piece (0, 1), its item
   int4* const head_s = reinterpret_cast<int4*>((reinterpret_cast<uintptr_t>(cb_bar + 1) + 15) & ~uintptr_t(15));
   int4* const tail_s = head_s + kPairs;
-  int8_t* const hslot_s = reinterpret_cast<int8_t*>(tail_s + kPairs);        // [NB] dense slot, -1: codeword
+  volatile int* const bad_s = reinterpret_cast<volatile int*>(tail_s + kPairs);    // [kPairs][stages] the tile's pages are invalid
+  int8_t* const hslot_s = reinterpret_cast<int8_t*>(tail_s + kPairs) + 4 * kPairs * p.stages;   // [NB] dense slot, -1: codeword
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const float INF = __int_as_float(0x7f800000);
 
@@ -294,8 +295,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             if (lane == 0) {
               mbar_wait(&empty[stage], phase ^ 1, p.err, kErrWait);
               uint8_t* const st = my_ring + stage * p.stage_bytes;
-              // the stage's last word: whether the tile is invalid
-              *reinterpret_cast<volatile int*>(st + p.stage_bytes - 4) = w.len < 0 || ra == -2 || rb == -2;
+              bad_s[pair * p.stages + stage] = w.len < 0 || ra == -2 || rb == -2;
               mbar_arrive_expect_tx(&full[stage], ((ra >= 0) + (rb >= 0)) * (vbytes + ibytes + hbytes));
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         mbar_wait(&full[stage], phase, p.err, kErrWait);
         uint8_t* const st = my_ring + stage * p.stage_bytes;
         const uint32_t st_a = smem_u32(st);
-        bad |= *reinterpret_cast<volatile int*>(st + p.stage_bytes - 4) != 0;
+        bad |= bad_s[pair * p.stages + stage] != 0;
         if (first + kTile > w.len) {               // rows behind the end hold anything: zero times it is not zero
           for (int x = max(0, w.len - first) * (DV / 8) + lane; x < kTile * (DV / 8); x += 32) {
             const int tok = x / (DV / 8), c = x % (DV / 8);
@@ -429,134 +429,129 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           fence_proxy_async_smem();
           __syncwarp();
         }
-#pragma unroll 1
-        for (int half = 0; half < 2; half += MT) {
-          float s[MT][NT][4];
+        float s[MT][NT][4];
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            uint32_t kw[2][D / 8];
+        for (int mt = 0; mt < MT; ++mt) {
+          uint32_t kw[2][D / 8];
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              const int tok = (half + mt) * 16 + y * 8 + g;
-              uint32_t ib[UNITS];
-              const uint32_t idx_a = st_a + p.off_idx + tok * NB;
-              unrolled<(UNITS + 3) / 4>([&](auto i) {
-                lds_words<UNITS >= 4 ? 16 : 8, 16 * decltype(i)::v>(ib + 4 * decltype(i)::v, idx_a);
-              });
-              // slot u loads unit (u + rot) mod ROT of its group of ROT units
-              unrolled<UNITS>([&](auto i) {
-                constexpr int u = decltype(i)::v;
-                uint32_t word = ib[u];
+          for (int y = 0; y < 2; ++y) {
+            const int tok = mt * 16 + y * 8 + g;
+            uint32_t ib[UNITS];
+            const uint32_t idx_a = st_a + p.off_idx + tok * NB;
+            unrolled<(UNITS + 3) / 4>([&](auto i) {
+              lds_words<UNITS >= 4 ? 16 : 8, 16 * decltype(i)::v>(ib + 4 * decltype(i)::v, idx_a);
+            });
+            // slot u loads unit (u + rot) mod ROT of its group of ROT units
+            unrolled<UNITS>([&](auto i) {
+              constexpr int u = decltype(i)::v;
+              uint32_t word = ib[u];
 #pragma unroll
-                for (int x = 1; x < ROT; ++x)
-                  if (rot == x) word = ib[(u & ~(ROT - 1)) | ((u + x) & (ROT - 1))];
-                lds_words<2 * BD, (u / ROT) * 32768>(kw[y] + u * WORDS, col_a[u % ROT] + (__byte_perm(word, 0, byte_sel) << 7));
-              });
-              // put the units back in order: rotate each group by rot
+              for (int x = 1; x < ROT; ++x)
+                if (rot == x) word = ib[(u & ~(ROT - 1)) | ((u + x) & (ROT - 1))];
+              lds_words<2 * BD, (u / ROT) * 32768>(kw[y] + u * WORDS, col_a[u % ROT] + (__byte_perm(word, 0, byte_sel) << 7));
+            });
+            // put the units back in order: rotate each group by rot
 #pragma unroll
-              for (int u0 = 0; u0 < UNITS; u0 += ROT)
+            for (int u0 = 0; u0 < UNITS; u0 += ROT)
 #pragma unroll
-                for (int bit = 1; bit < ROT; bit <<= 1) {
-                  uint32_t tmp[ROT * WORDS];
+              for (int bit = 1; bit < ROT; bit <<= 1) {
+                uint32_t tmp[ROT * WORDS];
 #pragma unroll
-                  for (int x = 0; x < ROT; ++x)
+                for (int x = 0; x < ROT; ++x)
 #pragma unroll
-                    for (int z = 0; z < WORDS; ++z)
-                      tmp[x * WORDS + z] =
-                          (rot & bit) ? kw[y][(u0 + ((x - bit) & (ROT - 1))) * WORDS + z] : kw[y][(u0 + x) * WORDS + z];
+                  for (int z = 0; z < WORDS; ++z)
+                    tmp[x * WORDS + z] =
+                        (rot & bit) ? kw[y][(u0 + ((x - bit) & (ROT - 1))) * WORDS + z] : kw[y][(u0 + x) * WORDS + z];
 #pragma unroll
-                  for (int x = 0; x < ROT * WORDS; ++x) kw[y][u0 * WORDS + x] = tmp[x];
+                for (int x = 0; x < ROT * WORDS; ++x) kw[y][u0 * WORDS + x] = tmp[x];
+              }
+            if (p.n_heavy) {                       // dense blocks take the place of their codeword 0
+#pragma unroll
+              for (int u = 0; u < UNITS; ++u)
+                if ((hmask >> u) & 1) {
+                  uint32_t* dst = kw[y] + u * WORDS;
+                  lds_words<2 * BD, 0>(dst, st_a + p.off_heavy + (tok * p.n_heavy + hslot_s[4 * u + t]) * (2 * BD));
+#pragma unroll
+                  for (int x = 0; x < WORDS; ++x) dst[x] = dense_word<T>(dst[x], k_scale);
                 }
-              if (p.n_heavy) {                       // dense blocks take the place of their codeword 0
-#pragma unroll
-                for (int u = 0; u < UNITS; ++u)
-                  if ((hmask >> u) & 1) {
-                    uint32_t* dst = kw[y] + u * WORDS;
-                    lds_words<2 * BD, 0>(dst, st_a + p.off_heavy + (tok * p.n_heavy + hslot_s[4 * u + t]) * (2 * BD));
-#pragma unroll
-                    for (int x = 0; x < WORDS; ++x) dst[x] = dense_word<T>(dst[x], k_scale);
-                  }
-              }
-            }
-#pragma unroll
-            for (int c = 0; c < NT; ++c) {
-              s[mt][c][0] = s[mt][c][1] = s[mt][c][2] = s[mt][c][3] = 0.f;
-#pragma unroll
-              for (int ks = 0; ks < KS; ++ks)
-                mma_f16(s[mt][c], kw[0][2 * ks], kw[1][2 * ks], kw[0][2 * ks + 1], kw[1][2 * ks + 1], qb[c][ks][0],
-                        qb[c][ks][1]);
             }
           }
-          // online softmax, in powers of two
-          const int from_tok = first + half * 16;               // the step's first token
-          const bool edge = from_tok + MT * 16 > seen_all;
-          if (edge) {
 #pragma unroll
-            for (int c = 0; c < NT; ++c)
+          for (int c = 0; c < NT; ++c) {
+            s[mt][c][0] = s[mt][c][1] = s[mt][c][2] = s[mt][c][3] = 0.f;
 #pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                // tokens that row 8c + 2t + j sees
-                const int seen = limited ? max(0, w.len - (p.L - 1 - (r0 + 8 * c + 2 * t + j) % p.L)) : w.len;
-#pragma unroll
-                for (int e = 0; e < 2 * MT; ++e)
-                  if (from_tok + e * 8 + g >= seen) s[e >> 1][c][(e & 1) * 2 + j] = -INF;
-              }
+            for (int ks = 0; ks < KS; ++ks)
+              mma_f16(s[mt][c], kw[0][2 * ks], kw[1][2 * ks], kw[0][2 * ks + 1], kw[1][2 * ks + 1], qb[c][ks][0],
+                      qb[c][ks][1]);
           }
-          bool grows = false;
-          float top[NT][2];
+        }
+        // online softmax, in powers of two
+        const bool edge = first + kTile > seen_all;
+        if (edge) {
 #pragma unroll
           for (int c = 0; c < NT; ++c)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              top[c][j] = fmaxf(s[0][c][j], s[0][c][j + 2]);
-              if constexpr (MT == 2) top[c][j] = fmaxf(top[c][j], fmaxf(s[MT - 1][c][j], s[MT - 1][c][j + 2]));
-              grows |= m[c][j] == -INF ? top[c][j] != -INF : (top[c][j] - m[c][j]) * f[c][j] > kSlack;
+              // tokens that row 8c + 2t + j sees
+              const int seen = limited ? max(0, w.len - (p.L - 1 - (r0 + 8 * c + 2 * t + j) % p.L)) : w.len;
+#pragma unroll
+              for (int e = 0; e < 2 * MT; ++e)
+                if (first + e * 8 + g >= seen) s[e >> 1][c][(e & 1) * 2 + j] = -INF;
             }
-          if (__any_sync(0xffffffffu, grows)) {
-#pragma unroll
-            for (int c = 0; c < NT; ++c)
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                float x = top[c][j];
-#pragma unroll
-                for (int of = 4; of < 32; of <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, of));
-                const float nm = fmaxf(m[c][j], x);
-                const float e = m[c][j] == -INF ? 0.f : fast_exp2((m[c][j] - nm) * f[c][j]);
-                m[c][j] = nm;
-                l[c][j] *= e;
-#pragma unroll
-                for (int d = 0; d < DV / 16; ++d) {
-                  o[c][d][j] *= e;
-                  o[c][d][j + 2] *= e;
-                }
-              }
-          }
-          uint32_t pb[MT][NT][2];
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int c = 0; c < NT; ++c) {
-              float e[4];
-              const float mb[2] = {m[c][0] == -INF ? 0.f : m[c][0], m[c][1] == -INF ? 0.f : m[c][1]};
-#pragma unroll
-              for (int x = 0; x < 4; ++x) e[x] = fast_exp2((s[mt][c][x] - mb[x & 1]) * f[c][x & 1]);
-              if (edge) {                            // -inf times a factor of zero
-#pragma unroll
-                for (int x = 0; x < 4; ++x) e[x] = s[mt][c][x] == -INF ? 0.f : e[x];
-              }
-              l[c][0] += e[0] + e[2];
-              l[c][1] += e[1] + e[3];
-              pb[mt][c][0] = movmatrix(pack2<T>(e[0], e[1]));
-              pb[mt][c][1] = movmatrix(pack2<T>(e[2], e[3]));
-            }
-          unrolled<MT * DV / 16>([&](auto i) {
-            constexpr int mt = decltype(i)::v / (DV / 16), d = decltype(i)::v % (DV / 16);
-            uint32_t v[4];
-            ldmatrix_x4_trans<(d >> 2) * (kTile * 128) + mt * 2048>(v, st_a + v_off[d & 3] + half * 2048);
-#pragma unroll
-            for (int c = 0; c < NT; ++c) mma_pv<T>(o[c][d], v[0], v[1], v[2], v[3], pb[mt][c][0], pb[mt][c][1]);
-          });
         }
+        bool grows = false;
+        float top[NT][2];
+#pragma unroll
+        for (int c = 0; c < NT; ++c)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            top[c][j] = fmaxf(fmaxf(s[0][c][j], s[0][c][j + 2]), fmaxf(s[1][c][j], s[1][c][j + 2]));
+            grows |= m[c][j] == -INF ? top[c][j] != -INF : (top[c][j] - m[c][j]) * f[c][j] > kSlack;
+          }
+        if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+          for (int c = 0; c < NT; ++c)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float x = top[c][j];
+#pragma unroll
+              for (int of = 4; of < 32; of <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, of));
+              const float nm = fmaxf(m[c][j], x);
+              const float e = m[c][j] == -INF ? 0.f : fast_exp2((m[c][j] - nm) * f[c][j]);
+              m[c][j] = nm;
+              l[c][j] *= e;
+#pragma unroll
+              for (int d = 0; d < DV / 16; ++d) {
+                o[c][d][j] *= e;
+                o[c][d][j + 2] *= e;
+              }
+            }
+        }
+        uint32_t pb[MT][NT][2];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int c = 0; c < NT; ++c) {
+            float e[4];
+            const float mb[2] = {m[c][0] == -INF ? 0.f : m[c][0], m[c][1] == -INF ? 0.f : m[c][1]};
+#pragma unroll
+            for (int x = 0; x < 4; ++x) e[x] = fast_exp2((s[mt][c][x] - mb[x & 1]) * f[c][x & 1]);
+            if (edge) {                            // -inf times a factor of zero
+#pragma unroll
+              for (int x = 0; x < 4; ++x) e[x] = s[mt][c][x] == -INF ? 0.f : e[x];
+            }
+            l[c][0] += e[0] + e[2];
+            l[c][1] += e[1] + e[3];
+            pb[mt][c][0] = movmatrix(pack2<T>(e[0], e[1]));
+            pb[mt][c][1] = movmatrix(pack2<T>(e[2], e[3]));
+          }
+        unrolled<MT * DV / 16>([&](auto i) {
+          constexpr int mt = decltype(i)::v / (DV / 16), d = decltype(i)::v % (DV / 16);
+          uint32_t v[4];
+          ldmatrix_x4_trans<(d >> 2) * (kTile * 128) + mt * 2048>(v, st_a + v_off[d & 3]);
+#pragma unroll
+          for (int c = 0; c < NT; ++c) mma_pv<T>(o[c][d], v[0], v[1], v[2], v[3], pb[mt][c][0], pb[mt][c][1]);
+        });
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[stage]);
         if (++stage == p.stages) {
@@ -740,10 +735,9 @@ template <int D, int DV, int BD, typename T>
 int launch_paged_attention(const AttnParams& p, const CUtensorMap& vmap, int grid, cudaStream_t st) {
   // the split of registers waits forever where the block has fewer than it was planned for
   auto* k = p.item_rows == 8 ? paged_attention_kernel<D, DV, BD, T, 1> : paged_attention_kernel<D, DV, BD, T, 2>;
-  cudaFuncAttributes fa;
-  if (cudaFuncGetAttributes(&fa, k) != cudaSuccess || fa.numRegs != kLaunchRegs)
-    return set_last_error(SUNSHAPE_E_CUDA, "paged attention kernel was built for another register count.");
-  cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem);
+  static std::atomic<uint64_t> done[2];
+  if (!ready_kernel((const void*)k, kSmemMax, kLaunchRegs, done[p.item_rows == 8]))
+    return set_last_error(SUNSHAPE_E_CUDA, "the paged attention kernel is not available as it was built.");
   k<<<grid, kAttnThreads, p.smem, st>>>(p, vmap);
   // the join may be scheduled while the main grid drains; it waits for its end before it reads
   cudaLaunchConfig_t cfg{};

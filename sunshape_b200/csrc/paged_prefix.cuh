@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
 #pragma unroll
         for (int i = 0; i < 8; ++i) src_d[i] = (int)p.perm[c * 8 + i];
         const float k_scale = p.image_scale[cb];
-#pragma unroll 2
+#pragma unroll 4
         for (int r = (warp - 8) * RPW + lane / CH; r < groups * 128; r += 16 * RPW) {
           float x[8], mx = 0.f;
 #pragma unroll
@@ -597,10 +597,9 @@ int launch_paged_prefix(const AttnParams& p, const CUtensorMap& vmap, int grid, 
   auto* k = paged_prefix_kernel<D, DV, BD, T>;
   const int smem = PrefixSmem::total(D, DV);
   // the split of registers waits forever where the block has fewer than it was planned for
-  cudaFuncAttributes fa;
-  if (cudaFuncGetAttributes(&fa, k) != cudaSuccess || fa.numRegs != kPfLaunchRegs)
-    return set_last_error(SUNSHAPE_E_CUDA, "paged prefix kernel was built for another register count.");
-  cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<uint64_t> done;
+  if (!ready_kernel((const void*)k, smem, kPfLaunchRegs, done))
+    return set_last_error(SUNSHAPE_E_CUDA, "the paged prefix kernel is not available as it was built.");
   k<<<grid, kPfThreads, smem, st>>>(p, vmap);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid, kPfRows / kPfJoinRows);

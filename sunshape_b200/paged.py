@@ -51,32 +51,44 @@ def rotary_table(n_positions: int, rot_dim: int, *, base: float = 10000.0,
 
 
 # ------------------------------------------------------------------------------------------- argument checks
-def _rows(t: torch.Tensor, what: str) -> _lib.RowsDesc:
-    """Descriptor of [B, heads, L, dim] rows; any strides but a unit last one."""
-    if t.stride(3) != 1 and t.shape[3] != 1:
+_CODES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+def _device(first: torch.Tensor, *others: torch.Tensor | None) -> int:
+    """Index of the CUDA device that all of the tensors are on."""
+    dev = first.get_device()
+    same = dev >= 0
+    for t in others:
+        same = same and (t is None or t.get_device() == dev)
+    if not same:
+        _lib.require_cuda(first, *others)     # says what is wrong
+    return dev
+
+
+def _unit(t: torch.Tensor, what: str) -> torch.Tensor:
+    if t.stride(-1) != 1 and t.shape[-1] != 1:
         raise RuntimeError(f"{what}: the last axis must have unit stride.")
-    return _lib.RowsDesc(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2), t.shape[1])
+    return t
 
 
-def _rotation(cos, sin, positions, interleaved, B: int, L: int, dim: int, dev) -> _lib.RotationDesc | None:
+def _rotation(cos, sin, positions, interleaved, B: int, L: int, dim: int, dev: int) -> bytes | None:
     if cos is None and sin is None and positions is None:
         return None
     if cos is None or sin is None or positions is None:
         raise RuntimeError("a rotation needs cos, sin and positions.")
-    if cos.ndim != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+    shape = cos.shape
+    if len(shape) != 2 or shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
         raise RuntimeError("cos and sin must be fp32 tables of one shape [n_positions, rot_dim / 2].")
-    rot = 2 * cos.shape[1]
-    if rot > dim:
-        raise RuntimeError(f"cos and sin rotate {rot} elements of a head of {dim}.")
+    if 2 * shape[1] > dim:
+        raise RuntimeError(f"cos and sin rotate {2 * shape[1]} elements of a head of {dim}.")
     if positions.dtype not in (torch.int32, torch.int64):
         raise RuntimeError("positions must be int32 or int64.")
-    if cos.device != dev or sin.device != dev or positions.device != dev:
+    if not cos.get_device() == sin.get_device() == positions.get_device() == dev:
         raise RuntimeError("all sunshape_b200 inputs must live on the same CUDA device.")
     if not (cos.is_contiguous() and sin.is_contiguous()):
         raise RuntimeError("cos and sin must be contiguous.")
     sb, sl = _token_strides(positions, B, L, "positions")
-    return _lib.RotationDesc(cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), sb, sl, cos.shape[0],
-                             _lib.I32 if positions.dtype == torch.int32 else _lib.I64, rot, 1 if interleaved else 0)
+    return _lib.rotation(cos, sin, positions, sb, sl, interleaved)
 
 
 def _token_strides(t: torch.Tensor, B: int, L: int, what: str) -> tuple[int, int]:
@@ -100,19 +112,23 @@ def norm_rotate(query: torch.Tensor, key: torch.Tensor | None = None, *, q_weigh
     ``x * w / sqrt(mean(x^2) + eps)``.  ``cos``/``sin`` [n_positions, R / 2] fp32 and ``positions`` [B, L] (int32 or
     int64; [L] broadcasts) rotate the first R <= D elements: pairs (i, i + R/2), or (2i, 2i + 1) if
     ``interleaved``.  fp32 arithmetic, one rounding to the inputs' dtype.  ``out`` may be the inputs themselves."""
-    dev = _lib.require_cuda(query, key, q_weight, k_weight)
-    for t, what in ((query, "query"), (key, "key")):
-        if t is not None and t.ndim != 4:
-            raise RuntimeError(f"norm_rotate expects {what} with shape [batch, heads, seq, dim].")
-    if query.dtype not in _FLOATS:
+    dev = _device(query, key, q_weight, k_weight)
+    code = _CODES.get(query.dtype)
+    if query.ndim != 4 or (key is not None and key.ndim != 4):
+        raise RuntimeError("norm_rotate expects query and key with shape [batch, heads, seq, dim].")
+    if code is None:
         raise RuntimeError(f"norm_rotate takes fp32, bf16 or f16 rows, got {query.dtype}.")
-    B, _, L, D = query.shape
-    if key is not None and (key.dtype != query.dtype or (key.shape[0], key.shape[2], key.shape[3]) != (B, L, D)):
-        raise RuntimeError("query and key must agree in dtype, batch, length and head dimension.")
-    if k_weight is not None and key is None:
+    B, Hq, L, D = query.shape
+    if key is not None:
+        Bk, _, Lk, Dk = key.shape
+        if key.dtype != query.dtype or (Bk, Lk, Dk) != (B, L, D):
+            raise RuntimeError("query and key must agree in dtype, batch, length and head dimension.")
+        _unit(key, "key")
+    elif k_weight is not None:
         raise RuntimeError("k_weight without a key.")
+    _unit(query, "query")
     for w in (q_weight, k_weight):
-        if w is not None and (w.shape != (D,) or w.dtype not in _FLOATS or not w.is_contiguous()):
+        if w is not None and (w.ndim != 1 or w.shape[0] != D or w.dtype not in _CODES or not w.is_contiguous()):
             raise RuntimeError(f"norm weights must be contiguous fp32, bf16 or f16 tensors of shape [{D}].")
     if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
         raise RuntimeError("both norm weights must have one dtype.")
@@ -123,14 +139,16 @@ def norm_rotate(query: torch.Tensor, key: torch.Tensor | None = None, *, q_weigh
         q_out, k_out = out
         for t, o in ((query, q_out), (key, k_out)):
             if (t is None) != (o is None) or (t is not None and (
-                    o.shape != t.shape or o.dtype != t.dtype or o.device != dev)):
+                    o.shape != t.shape or o.dtype != t.dtype or o.get_device() != dev)):
                 raise RuntimeError("out must hold tensors of the inputs' shapes, dtype and device.")
             if t is not None and o.data_ptr() == t.data_ptr() and o.stride() != t.stride():
                 raise RuntimeError("out over its own input needs the input's strides.")
+            if t is not None:
+                _unit(o, "out")
     w = q_weight if q_weight is not None else k_weight
-    _lib.norm_rotate(dev, _rows(query, "query"), _rows(q_out, "out"), q_weight,
-                     None if key is None else _rows(key, "key"), None if key is None else _rows(k_out, "out"), k_weight,
-                     _lib.dtype_code(query), _lib.F32 if w is None else _lib.dtype_code(w), B, L, D, eps, rot)
+    _lib.norm_rotate(dev, _lib.rows(query), _lib.rows(q_out), q_weight, None if key is None else _lib.rows(key),
+                     None if key is None else _lib.rows(k_out), k_weight, code, _lib.F32 if w is None else _CODES[w.dtype],
+                     B, L, D, eps, rot)
     return q_out, k_out
 
 
@@ -167,7 +185,7 @@ class SunShapePagedCache:
             if t is not None and (not t.is_contiguous() or t.data_ptr() % 16):
                 raise RuntimeError("page pools must be contiguous and 16-byte aligned.")
         self.codec, self.indices, self.values, self.heavy = codec, indices, values, heavy
-        self.device = dev
+        self.device, self._index = dev, indices.get_device()
         self._pages = _lib.PagesDesc(_lib.ptr(indices), _lib.ptr(heavy), _lib.ptr(values), indices.shape[0],
                                      indices.shape[1], indices.shape[2], values.shape[3], _lib.dtype_code(values))
         self._tables()
@@ -192,13 +210,14 @@ class SunShapePagedCache:
     value_dim = property(lambda self: int(self.values.shape[3]))
     dtype = property(lambda self: self.values.dtype)
 
-    def _tables(self) -> torch.Tensor:
-        """What the kernels read of the codec's codebooks, derived once and kept by the codec until ``invalidate``."""
+    def _tables(self) -> tuple[_lib.CodecDesc, torch.Tensor]:
+        """The codec's descriptor, and what the kernels read of its codebooks, derived once and kept by the codec until
+        ``invalidate``."""
         desc, keep, _ = self.codec.kernel_desc()
         kept = getattr(self.codec, "_paged_tables", None)
         if kept is None or kept[1] is not keep[0]:
             kept = self.codec._paged_tables = (_lib.paged_tables(desc, self.device), keep[0])
-        return kept[0]
+        return desc, kept[0]
 
     def slots(self, page_table: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
         """Slots [B, L] of the token positions [B, L] (within their sequences) under ``page_table`` [B, cols]; -1
@@ -226,8 +245,8 @@ def append_paged(cache: SunShapePagedCache, key: torch.Tensor, value: torch.Tens
     must be distinct.  The codeword is the nearest to the rotated key in real arithmetic (decided in 64 bits
     where fp32 cannot tell; lowest index on ties), without rounding the rotated key in between."""
     codec = cache.codec
-    dev = _lib.require_cuda(key, value, slots)
-    if dev != cache.device:
+    dev = _device(key, value, slots)
+    if dev != cache._index:
         raise RuntimeError("all sunshape_b200 inputs must live on the same CUDA device.")
     if codec.is_metric:
         raise RuntimeError("append_paged does not encode under a SunShape-Pro metric; encode with "
@@ -235,17 +254,20 @@ def append_paged(cache: SunShapePagedCache, key: torch.Tensor, value: torch.Tens
     if key.ndim != 4 or value.ndim != 4:
         raise RuntimeError("append_paged expects key and value with shape [batch, kv_heads, seq, dim].")
     B, H, L, D = key.shape
+    pages = cache._pages
     if D != codec.head_dim:
         raise RuntimeError("Key head_dim does not match codec head_dim.")
-    if H != cache.kv_heads or value.shape != (B, H, L, cache.value_dim):
+    if H != pages.kv_heads or tuple(value.shape) != (B, H, L, pages.value_dim):
         raise RuntimeError("key and value must agree with each other and with the cache's kv_heads and value_dim.")
-    if key.dtype != cache.dtype or value.dtype != cache.dtype:
-        raise RuntimeError(f"key and value must have the cache's dtype {cache.dtype}.")
-    if slots.dtype != torch.int64 or slots.shape != (B, L):
+    dtype = cache.values.dtype
+    if key.dtype != dtype or value.dtype != dtype:
+        raise RuntimeError(f"key and value must have the cache's dtype {dtype}.")
+    if slots.dtype != torch.int64 or tuple(slots.shape) != (B, L):
         raise RuntimeError("slots must be int64 [batch, length].")
     rot = _rotation(cos, sin, positions, interleaved, B, L, D, dev)
-    _lib.paged_append(dev, codec.kernel_desc()[0], cache._tables(), cache._pages, _rows(key, "key"), _rows(value, "value"), B,
-                      L, slots, rot)
+    desc, tables = cache._tables()
+    _lib.paged_append(dev, desc, tables, pages, _lib.rows(_unit(key, "key")), _lib.rows(_unit(value, "value")), B, L, slots,
+                      rot)
 
 
 def paged_attention(cache: SunShapePagedCache, query: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor, *,
@@ -262,39 +284,42 @@ def paged_attention(cache: SunShapePagedCache, query: torch.Tensor, page_table: 
     Softmax statistics and sums are fp32.  Codewords are read as fp16 and softmax weights rounded to the cache's
     dtype before they multiply values; queries are scaled by powers of two into fp16's range.  Dense key blocks
     must stay below 65504 times the largest codeword's norm."""
-    codec = cache.codec
-    dev = _lib.require_cuda(query, page_table, seq_lens, prefix_table)
-    if dev != cache.device:
+    codec, pages = cache.codec, cache._pages
+    dev = _device(query, page_table, seq_lens, prefix_table)
+    if dev != cache._index:
         raise RuntimeError("all sunshape_b200 inputs must live on the same CUDA device.")
     if query.ndim != 4:
         raise RuntimeError("paged_attention expects query with shape [batch, heads, seq, dim].")
     B, Hq, L, D = query.shape
     if D != codec.head_dim:
         raise RuntimeError("Query head_dim does not match codec head_dim.")
-    if Hq % cache.kv_heads:
+    if Hq % pages.kv_heads:
         raise RuntimeError("Query head count must be divisible by kv-head count.")
-    if query.dtype != cache.dtype:
+    dtype = query.dtype
+    if dtype != cache.values.dtype:
         raise RuntimeError(f"query must have the cache's dtype {cache.dtype}.")
+    _unit(query, "query")
     if page_table.ndim != 2 or page_table.shape[0] != B or page_table.dtype != torch.int32:
         raise RuntimeError("page_table must be int32 [batch, pages].")
     if page_table.shape[1] > 1 and page_table.stride(1) != 1:
         raise RuntimeError("page_table: the last axis must have unit stride.")
-    if seq_lens.shape != (B,) or seq_lens.dtype != torch.int32 or not seq_lens.is_contiguous():
+    if seq_lens.ndim != 1 or seq_lens.shape[0] != B or seq_lens.dtype != torch.int32 or not seq_lens.is_contiguous():
         raise RuntimeError("seq_lens must be contiguous int32 [batch].")
     prefix_len = int(prefix_len)
     if prefix_len < 0 or (prefix_len and prefix_table is None):
         raise RuntimeError("prefix_len needs a prefix_table and must not be negative.")
     if prefix_len and (prefix_table.ndim != 1 or prefix_table.dtype != torch.int32 or not prefix_table.is_contiguous()
-                       or prefix_table.shape[0] * cache.page_size < prefix_len):
+                       or prefix_table.shape[0] * pages.page_size < prefix_len):
         raise RuntimeError("prefix_table must be contiguous int32 [pages] and hold prefix_len tokens.")
-    shape = (B, Hq, L, cache.value_dim)
+    shape = (B, Hq, L, pages.value_dim)
     if out is None:
-        out = torch.empty(shape, dtype=query.dtype, device=dev)
-    elif out.shape != shape or out.dtype != query.dtype or out.device != dev or not out.is_contiguous():
+        out = torch.empty(shape, dtype=dtype, device=query.device)
+    elif tuple(out.shape) != shape or out.dtype != dtype or out.get_device() != dev or not out.is_contiguous():
         raise RuntimeError("out must be contiguous [batch, q_heads, query_len, value_dim] of the query's dtype.")
-    _lib.paged_attention(dev, codec.kernel_desc()[0], cache._tables(), cache._pages, _rows(query, "query"), B, L, page_table,
-                         seq_lens, prefix_table if prefix_len else None, prefix_len,
-                         1.0 / math.sqrt(D) if scale is None else float(scale), causal, out)
+    desc, tables = cache._tables()
+    _lib.paged_attention(dev, desc, tables, pages, query, B, Hq, L, page_table, seq_lens,
+                         prefix_table if prefix_len else None, prefix_len, 1.0 / math.sqrt(D) if scale is None else float(scale),
+                         causal, out)
     return out
 
 
