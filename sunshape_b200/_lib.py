@@ -8,7 +8,6 @@ with the reason, in the style of the reference's fast-path gate
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 import os
@@ -451,11 +450,13 @@ def paged_attention(index: int, cd: CodecDesc, tables: torch.Tensor, pages: Page
                     q_heads: int, query_len: int, page_table: torch.Tensor, seq_lens: torch.Tensor, prefix_table,
                     prefix_len: int, scale: float, causal: bool, out: torch.Tensor) -> None:
     cols = page_table.shape[1]
-    # on another device than the current one, the library sizes the workspace for the device it runs on
-    here = torch._C._cuda_getDevice() == index
-    with (_NULL if here else torch.cuda.device(index)):
-        need = load_library().sunshape_paged_attention_workspace_bytes(
-            batch, q_heads, pages.kv_heads, query_len, pages.value_dim, cols, pages.page_size, prefix_len)
+    size, args = load_library().sunshape_paged_attention_workspace_bytes, (
+        batch, q_heads, pages.kv_heads, query_len, pages.value_dim, cols, pages.page_size, prefix_len)
+    if torch._C._cuda_getDevice() == index:
+        need = size(*args)
+    else:
+        with torch.cuda.device(index):       # sized for the device that it runs on
+            need = size(*args)
     # a block of the allocator of the current stream (of the graph's own pool under capture): two streams or two
     # captured graphs never share one
     ws = torch.empty(need if need > 256 else 256, dtype=torch.uint8, device=query.device)
@@ -464,5 +465,3 @@ def paged_attention(index: int, cd: CodecDesc, tables: torch.Tensor, pages: Page
                seq_lens.data_ptr(), ptr(prefix_table), prefix_len, scale, 1 if causal else 0, out.data_ptr(), ws.data_ptr(),
                ws.numel())
 
-
-_NULL = contextlib.nullcontext()

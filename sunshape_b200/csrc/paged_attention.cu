@@ -10,7 +10,7 @@ namespace {
 int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
 
 struct Layout {
-  int64_t slots, desc, pieces, prefix, prefix_desc, prefix_slots, total;
+  int64_t slots, desc, pieces, prefix, prefix_slots, total;
 };
 
 // Query rows of a KV head from which on the prefix goes to the tensor-core kernel: it rebuilds a key once for 256 rows
@@ -25,8 +25,7 @@ Layout layout(int grid, int64_t rows, int64_t item_rows, int dv, bool prefix, bo
   l.desc = round256(2 * grid * kItemRows * row);
   l.pieces = l.desc + round256((int64_t)grid * 16);
   l.prefix = l.pieces + round256((int64_t)grid * kPairs * 2 * item_rows * row);
-  l.prefix_desc = l.prefix + (prefix ? round256(rows * row) : 0);
-  l.prefix_slots = l.prefix_desc + (tensor ? round256((int64_t)grid * 16) : 0);
+  l.prefix_slots = l.prefix + (prefix ? round256(rows * row) : 0);
   l.total = l.prefix_slots + (tensor ? round256(2 * (int64_t)grid * 256 * row) : 0);
   return l;
 }
@@ -154,7 +153,6 @@ int sunshape_paged_attention(const sunshape_codec_t* codec, const void* tables, 
   p.desc = reinterpret_cast<int4*>(ws + at.desc);
   p.pieces = reinterpret_cast<float*>(ws + at.pieces);
   p.prefix_part = reinterpret_cast<float*>(ws + at.prefix);
-  p.prefix_desc = reinterpret_cast<int4*>(ws + at.prefix_desc);
   p.prefix_slots = reinterpret_cast<float*>(ws + at.prefix_slots);
   const int64_t pool_rows = p.num_pages * p.H * p.ps;
   if (pool_rows > 0x7fffffff) return set_last_error(SUNSHAPE_E_UNSUPPORTED, "at most 2^31 - 1 page rows in a pool.");

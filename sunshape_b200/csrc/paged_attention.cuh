@@ -56,7 +56,6 @@ struct AttnParams {
   float* pieces;                   // [grid][kPairs][2][item_rows] rows: pieces of items cut between a CTA's pairs
   float* prefix_part;              // [prefix_parts][B * Hq * L] rows
   float* prefix_slots;             // [2 * grid][256] rows: pieces of the prefix's items cut between CTAs
-  int4* prefix_desc;               // [grid] as desc, tail item's h (-1: none) and first row
   int* err;
   int item_rows;                   // 8 or 16: which kernel
   int smem;

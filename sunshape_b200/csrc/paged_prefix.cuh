@@ -35,7 +35,7 @@ struct PrefixSmem {
   static __host__ __device__ constexpr int k(int d) { return kPfTokens * d * 2; }
   static __host__ __device__ constexpr int v(int dv) { return kPfTokens * dv * 2; }
   static __host__ __device__ constexpr int total(int d, int dv) {
-    return q(d) + k(d) + 2 * v(dv) + d * 512 + 2 * kPfRows * 4 + 128 + 64;
+    return q(d) + k(d) + 2 * v(dv) + d * 512 + 2 * kPfRows * 4 + 128 + 128;
   }
 };
 
@@ -170,10 +170,12 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   float* const row_s = reinterpret_cast<float*>(image + IMAGE);
   uint64_t* const bars = reinterpret_cast<uint64_t*>(row_s + 2 * kPfRows);
   uint64_t *const v_full = bars, *const v_free = bars + 2, *const k_ready = bars + 4, *const k_free = bars + 5,
-                  *const s_full = bars + 6, *const p_ready = bars + 8, *const pv_done = bars + 10, *const cb_bar = bars + 12;
+                  *const s_full = bars + 6, *const p_ready = bars + 8, *const pv_done = bars + 10, *const cb_bar = bars + 12,
+                  *const q_ready = bars + 14;
   uint32_t* const tmem_s = reinterpret_cast<uint32_t*>(bars + 13);
   volatile int* const bad_s = reinterpret_cast<volatile int*>(tmem_s + 1);
   int8_t* const hslot_s = reinterpret_cast<int8_t*>(bars + 16);            // [NB] dense slot, -1: codeword
+  int8_t* const hblock_s = hslot_s + NB;                                   // [NB] block of a dense slot
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const float INF = __int_as_float(0x7f800000);
 
@@ -188,10 +190,15 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     mbar_init(k_ready, 128);
     mbar_init(k_free, 1);
     mbar_init(cb_bar, 1);
+    mbar_init(q_ready, 512);
     fence_mbar_init();
     *bad_s = 0;
     int n = 0;
-    for (int b = 0; b < NB; ++b) hslot_s[b] = p.heavy_mask && p.heavy_mask[b] ? (int8_t)n++ : (int8_t)-1;
+    for (int b = 0; b < NB; ++b) {
+      const bool dense = p.heavy_mask && p.heavy_mask[b];
+      if (dense) hblock_s[n] = (int8_t)b;
+      hslot_s[b] = dense ? (int8_t)n++ : (int8_t)-1;
+    }
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_s)), "r"(512) : "memory");
@@ -211,10 +218,10 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   int at = cta < grid ? part(total, cta, grid) : 0;
   const int end = cta < grid ? part(total, cta + 1, grid) : 0;
 
-  // Every role walks the same pieces (a range's part of one item) and meets the others before and after each: in between
-  // queries and codebook stand still.  it: tiles so far, it1: those of row group 1, which a head's last rows may not
+  // Every role walks the same pieces (a range's part of one item) and meets the others after each: only then are queries
+  // and codebook replaced.  it: tiles so far, it1: those of row group 1, which a head's last rows may not
   // fill -- the parities of the barriers.
-  int it = 0, it1 = 0, cb_loads = 0, head = -1;
+  int it = 0, it1 = 0, pieces = 0, cb_loads = 0, head = -1;
   int h, t0, n, r0, groups, cb;
   bool load_cb, begins, ends;
   auto next_piece = [&]() {
@@ -237,20 +244,19 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     at += n;
     it += n;
     if (groups == 2) it1 += n;
+    ++pieces;
     named_barrier(1, kPfThreads);
     pf_fence_after();
   };
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPfRegs0));
-    int4 desc = make_int4(0, -1, 0, 0);
     while (next_piece()) {
       if (load_cb && tid == 0) {
         fence_proxy_async_smem();
         mbar_arrive_expect_tx(cb_bar, IMAGE);
         bulk_g2s(image, reinterpret_cast<const uint8_t*>(p.image) + (int64_t)cb * IMAGE, IMAGE, cb_bar);
       }
-      named_barrier(1, kPfThreads);
       if (warp == 0) {
         // ------------------------------------------------------------------ values
         const unsigned ps = (unsigned)p.ps;
@@ -302,6 +308,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
               tc_mma_ts(tmem + 256 + g * DV, tmem + g * 128 + ks * 8, vd + ks * (2048 >> 4), id_pv, i > 0 || ks > 0);
             pf_commit(&pv_done[g]);
           };
+          mbar_wait(q_ready, pieces & 1, p.err, kErrWait);
           mbar_wait(k_ready, it & 1, p.err, kErrWait);
           pf_fence_after();
           for (int g = 0; g < groups; ++g) qk(g);
@@ -325,11 +332,8 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         }
         __syncwarp();
       }
-      if (!begins) desc.x = ends ? 2 : 1;
-      else if (!ends) desc = make_int4(desc.x, h, r0, 0);
       end_piece();
     }
-    if (tid == 0) p.prefix_desc[cta] = desc;
     if (warp == 1) {
       __syncwarp();
       asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
@@ -337,7 +341,6 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   } else if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPfRegsKeys));
     while (next_piece()) {
-      named_barrier(1, kPfThreads);
       // -------------------------------------------------------------------- keys
       const int tok_l = tid - 128;               // this thread's token of a tile
       const unsigned ps = (unsigned)p.ps;
@@ -346,6 +349,9 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       const float k_scale = p.image_scale[cb];
       const uint32_t image_a = smem_u32(image);
       uint32_t ib[NB / 4];
+      // block_dim 8: a dense block is one 16-byte chunk; a token's first four are read ahead, too
+      constexpr int AHEAD = BD == 8 ? 4 : 0;
+      uint4 dense_ahead[AHEAD + 1];
       int64_t row = -1;
       auto fetch = [&](int i) {                  // pool row and index row of tile i's token; zeros where there is none
         const int tok = (t0 + i) * kPfTokens + tok_l;
@@ -364,6 +370,9 @@ __global__ void __launch_bounds__(kPfThreads, 1)
 #pragma unroll
             for (int x = 0; x < NB / 16; ++x) reinterpret_cast<uint4*>(ib)[x] = reinterpret_cast<const uint4*>(src)[x];
           }
+#pragma unroll
+          for (int x = 0; x < AHEAD; ++x)
+            if (x < p.n_heavy) dense_ahead[x] = reinterpret_cast<const uint4*>(p.heavy)[row * p.n_heavy + x];
         }
       };
       fetch(0);
@@ -408,8 +417,19 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         }
         if (p.n_heavy && row >= 0) {             // dense blocks take the place of their codeword 0
           const T* dense = reinterpret_cast<const T*>(p.heavy) + row * p.n_heavy * BD;
+          if constexpr (BD == 8) {
+#pragma unroll
+            for (int x = 0; x < NB; ++x) {
+              if (x >= p.n_heavy) break;
+              uint4 w = x < AHEAD ? dense_ahead[x < AHEAD ? x : 0] : reinterpret_cast<const uint4*>(dense)[x];
+              w = make_uint4(dense_word<T>(w.x, k_scale), dense_word<T>(w.y, k_scale), dense_word<T>(w.z, k_scale),
+                             dense_word<T>(w.w, k_scale));
+              const int b = hblock_s[x];
+              *reinterpret_cast<uint4*>(dst + (b >> 3) * HALF + (((b & 7) ^ (tok_l & 7)) << 4)) = w;
+            }
+          }
 #pragma unroll 4
-          for (int b = 0; b < NB; ++b) {
+          for (int b = 0; b < (BD == 8 ? 0 : NB); ++b) {
             const int at_b = hslot_s[b];
             if (at_b < 0) continue;
             uint32_t w[WORDS];
@@ -477,7 +497,8 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         }
         fence_proxy_async_smem();
       }
-      named_barrier(1, kPfThreads);
+      mbar_arrive(q_ready);
+      named_barrier(10, 512);                    // the rows' factors
       const int g = (warp - 8) / 8;
       if (g < groups) {
         // ----------------------------------------------------------------- softmax
@@ -564,32 +585,31 @@ __global__ void __launch_bounds__(kPfThreads, 1)
 
 constexpr int kPfJoinRows = 8;
 
-// Adds up the pieces of cut items: a warp a row of the item that begins in CTA c's range and does not end there.
+// Adds up the pieces of cut items: block (k, .) takes rows of item k, a warp a row.
 template <int DV>
-__global__ void __launch_bounds__(kPfJoinRows * 32) paged_prefix_join(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(kPfJoinRows * 32) paged_prefix_join(const __grid_constant__ AttnParams p, int ctas) {
   constexpr int RF = row_floats(DV);
+  const int rows_total = p.B * p.G * p.L, items = (rows_total + kPfRows - 1) / kPfRows;
+  const int tiles = (p.prefix_len + kPfTokens - 1) / kPfTokens, total = tiles * items * p.H, grid = min(ctas, total);
+  const int h = blockIdx.x / items, r0 = (blockIdx.x - h * items) * kPfRows;
+  const int r = blockIdx.y * kPfJoinRows + threadIdx.x / 32, d = (threadIdx.x & 31) * 4;
+  // by every block: what follows this grid counts on the grid before it, too
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int c = blockIdx.x, r = blockIdx.y * kPfJoinRows + threadIdx.x / 32, lane = threadIdx.x & 31, d = lane * 4;
-  const int4 tail = p.prefix_desc[c];
-  if (tail.y < 0 || tail.z + r >= p.B * p.G * p.L) return;
-  int last = c + 1;                              // the first range behind that does not go on
-  for (; last < gridDim.x; last += 32) {
-    const unsigned stop = __ballot_sync(0xffffffffu, last + lane >= gridDim.x || p.prefix_desc[last + lane].x != 1);
-    if (stop) {
-      last += __ffs(stop) - 1;
-      break;
-    }
-  }
-  const int n = min(last, (int)gridDim.x - 1) - c + 1;
+  if (r0 + r >= rows_total) return;
+  // the range that holds a tile of the list: the first total % grid ranges are one longer
+  const int q = total / grid, longer = total % grid;
+  auto owner = [&](int at) { return at < (q + 1) * longer ? at / (q + 1) : longer + (at - (q + 1) * longer) / q; };
+  const int c = owner((int)blockIdx.x * tiles), n = owner(((int)blockIdx.x + 1) * tiles - 1) - c + 1;
+  if (n == 1) return;                            // written whole
   float m = -__int_as_float(0x7f800000), l = 0.f;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+#pragma unroll 8
   for (int k = 0; k < n; ++k) {
     const float* src = p.prefix_slots + ((int64_t)(2 * (c + k) + (k == 0)) * kPfRows + r) * RF;
     const float4 v = d < DV ? *reinterpret_cast<const float4*>(src + d) : make_float4(0.f, 0.f, 0.f, 0.f);
     join4(m, l, a, src[DV], src[DV + 1], v);
   }
-  if (d < DV) finish4<float, DV>(p, row_of(p, tail.y, 0, tail.z + r), d, m, l, a);
+  if (d < DV) finish4<float, DV>(p, row_of(p, h, 0, r0 + r), d, m, l, a);
 }
 
 template <int D, int DV, int BD, typename T>
@@ -602,7 +622,8 @@ int launch_paged_prefix(const AttnParams& p, const CUtensorMap& vmap, int grid, 
     return set_last_error(SUNSHAPE_E_CUDA, "the paged prefix kernel is not available as it was built.");
   k<<<grid, kPfThreads, smem, st>>>(p, vmap);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid, kPfRows / kPfJoinRows);
+  const int64_t rows = (int64_t)p.B * p.G * p.L;
+  cfg.gridDim = dim3((unsigned)((rows + kPfRows - 1) / kPfRows * p.H), kPfRows / kPfJoinRows);
   cfg.blockDim = dim3(kPfJoinRows * 32);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -610,7 +631,7 @@ int launch_paged_prefix(const AttnParams& p, const CUtensorMap& vmap, int grid, 
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, paged_prefix_join<DV>, p);
+  cudaLaunchKernelEx(&cfg, paged_prefix_join<DV>, p, grid);
   return SUNSHAPE_OK;
 }
 
