@@ -157,9 +157,9 @@ int sunshape_paged_attention(const sunshape_codec_t* codec, const void* tables, 
   const int64_t pool_rows = p.num_pages * p.H * p.ps;
   if (pool_rows > 0x7fffffff) return set_last_error(SUNSHAPE_E_UNSUPPORTED, "at most 2^31 - 1 page rows in a pool.");
   // the kernels count tiles, and the gaps between heads, in 31 bits
-  const int64_t most = (int64_t)std::max(batch, 1) * (((int64_t)table_cols * p.ps + kTile - 1) / kTile + 1) *
+  const int64_t most = (int64_t)std::max(batch, 1) * (((int64_t)table_cols * p.ps + kTile - 1) / kTile + 1 + kItemTiles) *
                        ((p.G * (int64_t)p.L + 7) / 8);
-  const int64_t most_prefix = (prefix_len / kTile + 1) * ((rows / p.H + 7) / 8);
+  const int64_t most_prefix = (prefix_len / kTile + 1 + kItemTiles) * ((rows / p.H + 7) / 8);
   if ((std::max(most, most_prefix) + kHeadTiles) * p.H > 0x7fffffff)
     return set_last_error(SUNSHAPE_E_UNSUPPORTED, "paged attention: more than 2^31 tiles of 32 tokens in a call.");
   CUtensorMap vmap{};

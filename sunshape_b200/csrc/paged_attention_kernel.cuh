@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     int n = 0;
     for (int i = tid * per; i < min(seqs, (tid + 1) * per); ++i) {
       const int len = own_length(p, i);
-      n += tiles_of(len);
+      n += tiles_of(len) + kItemTiles;
       if (per == 1) len_s[i] = len;
     }
     for (int o = 1; o < 32; o <<= 1) {
@@ -183,7 +183,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 
   // ---- this CTA's range.  With a codebook per head, a head's tiles are followed by kHeadTiles that stand for the
   // change and a range falls into one portion per head; with one codebook for all it is one portion.
-  // the entry refuses calls whose tiles may not fit into 31 bits
+  // An item's tiles are followed by kItemTiles that stand for its queries and result.  The entry refuses calls whose
+  // tiles may not fit into 31 bits.
   const int per_head = cum_s[kPlanChunks] * mtiles;
   const int gap = p.n_cb > 1 ? kHeadTiles : 0;
   const int stride = per_head + gap, total = stride * p.H - gap;
@@ -203,6 +204,23 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 
   const int pair = warp & (kPairs - 1);
   Walk w;
+  // n more tiles of the item are walked: where they end it, on to the next one's first
+  auto next_item = [&](int n) {
+    w.at += n;
+    if (w.t + n < w.tiles) return;               // cut: the range ends here
+    w.at += w.tiles + kItemTiles - (w.t + n);
+    w.t = 0;
+    if (++w.mt < mtiles) return;
+    w.mt = 0;
+    if (++w.b == seqs) {
+      w.b = 0;
+      ++w.h;
+    }
+    if (w.at < w.end) {
+      w.len = length_of(w.b);
+      w.tiles = tiles_of(w.len);
+    }
+  };
   // the pair's part of portion k, in tiles without gaps
   auto enter = [&](int k) {
     int a = from, b = to;
@@ -227,28 +245,15 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     w.b = lo * per;
     w.len = length_of(w.b);
     w.tiles = tiles_of(w.len);
-    while (o >= w.tiles * mtiles) {
-      o -= w.tiles * mtiles;
+    while (o >= (w.tiles + kItemTiles) * mtiles) {
+      o -= (w.tiles + kItemTiles) * mtiles;
       ++w.b;
       w.len = length_of(w.b);
       w.tiles = tiles_of(w.len);
     }
-    w.mt = o / w.tiles;
-    w.t = o - w.mt * w.tiles;
-  };
-  auto next_item = [&](int n) {                // n: tiles of the item just walked
-    w.at += n;
-    w.t = 0;
-    if (++w.mt < mtiles) return;
-    w.mt = 0;
-    if (++w.b == seqs) {
-      w.b = 0;
-      ++w.h;
-    }
-    if (w.at < w.end) {
-      w.len = length_of(w.b);
-      w.tiles = tiles_of(w.len);
-    }
+    w.mt = o / (w.tiles + kItemTiles);
+    w.t = o - w.mt * (w.tiles + kItemTiles);
+    if (w.t >= w.tiles) next_item(0);
   };
   uint8_t* const my_ring = ring + (size_t)pair * ring_bytes;
   uint64_t* const full = full_s + pair * p.stages;

@@ -24,6 +24,7 @@
 namespace sunshape {
 
 constexpr int kPfTokens = 128, kPfRows = 256;
+constexpr int kPfItemTiles = 14;   // tiles that an item's queries, codebook and result are charged in the split
 constexpr int kPfThreads = 768;    // warps 0: values, 1: MMA, 2-3: none, 4-7: keys, 8-15 and 16-23: softmax of the row groups
 constexpr int kPfLaunchRegs = 80, kPfRegs0 = 40, kPfRegsKeys = 88, kPfRegsSoftmax = 88;
 static_assert(kPfRegs0 <= kPfLaunchRegs && kPfRegsKeys >= kPfLaunchRegs && kPfRegsSoftmax >= kPfLaunchRegs, "dec and inc");
@@ -213,7 +214,9 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   // this CTA's range of the list (head, group of 256 rows, tile)
   const int rows_total = p.B * p.G * p.L, items = (rows_total + kPfRows - 1) / kPfRows;
   const int tiles = (p.prefix_len + kPfTokens - 1) / kPfTokens;
-  const int total = tiles * items * p.H, grid = min((int)gridDim.x, total), cta = blockIdx.x;
+  // an item's tiles are followed by kPfItemTiles that stand for the rest of its work
+  const int stride = tiles + kPfItemTiles, total = stride * items * p.H - kPfItemTiles;
+  const int grid = min((int)gridDim.x, total), cta = blockIdx.x;
   auto part = [](int size, int i, int n) { return size / n * i + min(i, size % n); };
   int at = cta < grid ? part(total, cta, grid) : 0;
   const int end = cta < grid ? part(total, cta + 1, grid) : 0;
@@ -225,9 +228,13 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   int h, t0, n, r0, groups, cb;
   bool load_cb, begins, ends;
   auto next_piece = [&]() {
+    int item = at / stride;
+    t0 = at - item * stride;
+    if (t0 >= tiles) {
+      at = ++item * stride;
+      t0 = 0;
+    }
     if (at >= end) return false;
-    const int item = at / tiles;
-    t0 = at - item * tiles;
     n = min(end - at, tiles - t0);
     h = item / items;
     r0 = (item - h * items) * kPfRows;
@@ -241,7 +248,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     return true;
   };
   auto end_piece = [&]() {
-    at += n;
+    at += ends ? n + kPfItemTiles : n;
     it += n;
     if (groups == 2) it1 += n;
     ++pieces;
@@ -590,7 +597,8 @@ template <int DV>
 __global__ void __launch_bounds__(kPfJoinRows * 32) paged_prefix_join(const __grid_constant__ AttnParams p, int ctas) {
   constexpr int RF = row_floats(DV);
   const int rows_total = p.B * p.G * p.L, items = (rows_total + kPfRows - 1) / kPfRows;
-  const int tiles = (p.prefix_len + kPfTokens - 1) / kPfTokens, total = tiles * items * p.H, grid = min(ctas, total);
+  const int tiles = (p.prefix_len + kPfTokens - 1) / kPfTokens, stride = tiles + kPfItemTiles;
+  const int total = stride * items * p.H - kPfItemTiles, grid = min(ctas, total);
   const int h = blockIdx.x / items, r0 = (blockIdx.x - h * items) * kPfRows;
   const int r = blockIdx.y * kPfJoinRows + threadIdx.x / 32, d = (threadIdx.x & 31) * 4;
   // by every block: what follows this grid counts on the grid before it, too
@@ -599,7 +607,7 @@ __global__ void __launch_bounds__(kPfJoinRows * 32) paged_prefix_join(const __gr
   // the range that holds a tile of the list: the first total % grid ranges are one longer
   const int q = total / grid, longer = total % grid;
   auto owner = [&](int at) { return at < (q + 1) * longer ? at / (q + 1) : longer + (at - (q + 1) * longer) / q; };
-  const int c = owner((int)blockIdx.x * tiles), n = owner(((int)blockIdx.x + 1) * tiles - 1) - c + 1;
+  const int c = owner((int)blockIdx.x * stride), n = owner((int)blockIdx.x * stride + tiles - 1) - c + 1;
   if (n == 1) return;                            // written whole
   float m = -__int_as_float(0x7f800000), l = 0.f;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
