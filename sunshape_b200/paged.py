@@ -213,11 +213,11 @@ class SunShapePagedCache:
     def _tables(self) -> tuple[_lib.CodecDesc, torch.Tensor]:
         """The codec's descriptor, and what the kernels read of its codebooks, derived once and kept by the codec until
         ``invalidate``."""
-        desc, keep, _ = self.codec.kernel_desc()
+        made = self.codec.kernel_desc()          # another object after each ``invalidate``, over the same buffers
         kept = getattr(self.codec, "_paged_tables", None)
-        if kept is None or kept[1] is not keep[0]:
-            kept = self.codec._paged_tables = (_lib.paged_tables(desc, self.device), keep[0])
-        return desc, kept[0]
+        if kept is None or kept[1] is not made:
+            kept = self.codec._paged_tables = (_lib.paged_tables(made[0], self.device), made)
+        return made[0], kept[0]
 
     def slots(self, page_table: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
         """Slots [B, L] of the token positions [B, L] (within their sequences) under ``page_table`` [B, cols]; -1

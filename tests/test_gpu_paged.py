@@ -353,6 +353,89 @@ def test_paged_attention_empty_calls():
     assert paged.paged_attention(cache, q[:, :, :0], table, n).shape == (3, 4, 0, 64)
 
 
+@pytest.mark.parametrize("B,H,G,L,prefix,shared", [(300, 2, 2, 1, 0, False), (700, 1, 1, 2, 0, True), (300, 1, 2, 1, 70, True)])
+def test_paged_attention_many_sequences(B, H, G, L, prefix, shared):
+    """More sequences than the plan's chunks, many of them empty, and one codebook for all heads."""
+    codec, _ = make_paged_codec(64, 8, H, seed=B, shared=shared)
+    lens = [(i * 37) % 41 if i % 3 else 0 for i in range(B)]
+    cache, q, table, n, pt = _attention_case(codec, H, G, B, L, lens, prefix, 16, torch.bfloat16, seed=1)
+    got = paged.paged_attention(cache, q, table, n, prefix_table=pt, prefix_len=prefix)
+    _check_attention(got, cache, q, table, n, pt, prefix)
+
+
+@pytest.mark.parametrize("H,G,L,n,prefix,shared", [(1, 8, 1, 30000, 0, False), (3, 2, 1, 5000, 0, True), (1, 4, 1, 1, 20000, False),
+                                                   (2, 16, 2, 7, 20000, False)])
+def test_paged_attention_one_sequence_over_all_blocks(H, G, L, n, prefix, shared):
+    """One sequence whose runs are spread over the whole device and joined in order."""
+    codec, _ = make_paged_codec(128, 8, H, seed=n, shared=shared)
+    cache, q, table, lens, pt = _attention_case(codec, H, G, 1, L, [n], prefix, 128, torch.bfloat16, seed=3)
+    got = paged.paged_attention(cache, q, table, lens, prefix_table=pt, prefix_len=prefix)
+    _check_attention(got, cache, q, table, lens, pt, prefix)
+    assert torch.equal(got, paged.paged_attention(cache, q, table, lens, prefix_table=pt, prefix_len=prefix))
+
+
+def test_paged_attention_views_and_out():
+    """Queries as a view of a fused projection's output, a sliced page table, a given output, and pages that two
+    sequences share."""
+    codec, _ = make_paged_codec(64, 4, 2, seed=4)
+    cache, q, table, n, _ = _attention_case(codec, 2, 3, 4, 1, [40, 33, 5, 64], 0, 16, torch.float16, seed=6)
+    wide = torch.zeros(4, table.shape[1] + 5, dtype=torch.int32, device=DEV)
+    wide[:, 2:2 + table.shape[1]] = table
+    wide[3] = wide[0]
+    t = wide[:, 2:2 + table.shape[1]]
+    n = torch.tensor([40, 33, 5, 40], dtype=torch.int32, device=DEV)
+    fused = _randn(4, 1, 10, 64, seed=5, dtype=torch.float16)
+    q = fused[:, :, 2:8].transpose(1, 2)
+    out = torch.full((4, 6, 1, 64), 7.0, dtype=torch.float16, device=DEV)
+    got = paged.paged_attention(cache, q, t, n, out=out)
+    assert got is out
+    _check_attention(got, cache, q, t, n, None, 0)
+
+
+def test_codebook_edited_in_place():
+    """``invalidate`` renews what the paged kernels derived from the codebooks."""
+    codec, scale = make_paged_codec(64, 8, 2, seed=8)
+    cache, k, v, slots, rot = _append_case(codec, 2, 1, 30, page=16, dtype=torch.bfloat16, R=64, scale=scale)
+    for _ in range(2):
+        before = _state(cache)
+        cache.append(k, v, slots, **rot)
+        _check_append(cache, k, v, slots, rot, before)
+        codec.centroids.mul_(0.5).add_(0.1)
+        codec.invalidate()
+    q = _randn(1, 4, 1, 64, seed=3, dtype=torch.bfloat16)
+    table, n = torch.arange(2, dtype=torch.int32, device=DEV)[None], torch.tensor([20], dtype=torch.int32, device=DEV)
+    _check_attention(cache.attention(q, table, n), cache, q, table, n, None, 0)
+
+
+def test_append_strided_and_misaligned_rows():
+    """Values and keys that begin off a 16-byte boundary, a flat ragged batch, positions that broadcast."""
+    codec, scale = make_paged_codec(64, 8, 2, seed=9)
+    cache = SunShapePagedCache.allocate(codec, 6, 2, page_size=16)
+    fused = _randn(37, 2 * 2 * 64 + 3, seed=2, dtype=torch.bfloat16)
+    kv = fused[:, 1:1 + 256].unflatten(1, (4, 64)).transpose(0, 1).unsqueeze(0)      # [1, 4, 37, 64]
+    k, v = kv[:, :2], kv[:, 2:]
+    cos, sin = paged.rotary_table(64, 32, device=DEV)
+    rot = dict(cos=cos, sin=sin, positions=torch.arange(37, device=DEV, dtype=torch.int32))
+    slots = torch.randperm(96, generator=torch.Generator().manual_seed(1))[:37][None].to(DEV)
+    before = _state(cache)
+    cache.append(k, v, slots, **rot)
+    _check_append(cache, k, v, slots, dict(rot, positions=rot["positions"][None]), before)
+
+
+def test_calls_on_a_stream_of_their_own():
+    """A chain of calls on a side stream, without any synchronisation in between."""
+    codec, scale = make_paged_codec(128, 8, 2, seed=10)
+    cache, q, table, n, pt = _attention_case(codec, 2, 8, 3, 1, [300, 64, 7], 130, 64, torch.bfloat16, seed=5)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            q2, _ = paged.norm_rotate(q, q_weight=torch.ones(128, device=DEV))
+            got = paged.paged_attention(cache, q2, table, n, prefix_table=pt, prefix_len=130)
+    side.synchronize()
+    _check_attention(got, cache, q2, table, n, pt, 130)
+
+
 # ---------------------------------------------------------------------------------------------- used together
 def test_decode_steps_together_match_contiguous_cache():
     """A prompt and three decode steps as an engine runs them -- norms and rotation, append, attention behind a shared
