@@ -26,6 +26,9 @@ def __getattr__(name):
     if name in ("SunShapeVLLMHandle", "SunShapeVLLMRuntimeState", "load_runtime_state", "runtime_state_from_bundle"):
         from .integration import vllm
         return getattr(vllm, name)
+    if name in ("SunShapePagedCache", "append_paged", "norm_rotate", "paged_attention", "paged_error", "rotary_table"):
+        from . import paged
+        return getattr(paged, name)
     if name in ("SunShapeAttentionImpl", "SunShapeQuantizedKeys", "quantize_key_states"):
         from . import vllm_attn_backend
         return getattr(vllm_attn_backend, name)
@@ -36,4 +39,5 @@ __all__ = [
     "SunShapeBlockCodec", "SunShapeQuantized", "sunshape_attention_scores", "sunshape_attention_scores_strict",
     "_torch_attention_scores", "SunShapeCache", "SunShapeBundle", "SunShapeConfig", "SunShapeForCausalLM",
     "SunShapeAttentionImpl", "SunShapeQuantizedKeys", "quantize_key_states",
+    "SunShapePagedCache", "norm_rotate", "append_paged", "paged_attention",
 ]
