@@ -13,6 +13,7 @@
 // tokens x 8 codewords one or two MMAs and four maxima -- comparing all in fp32 (the kernel before this) takes 8
 // multiply-adds and 3 comparisons a distance.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.cuh"
 
@@ -102,6 +103,16 @@ __device__ __forceinline__ void mma_k8(float* d, uint32_t a0, uint32_t a1, uint3
   asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(b0));
+}
+
+// Whether a result of rotate32, off by two units of its last place, may round to T otherwise than the exact one: it
+// lies near the middle of two neighbours, is below f16's normal range, or so much smaller than the key's largest element
+// that the second product's error counts.
+template <typename T>
+__device__ __forceinline__ bool near_tie(float z, float most) {
+  constexpr int LOW = std::is_same<T, __half>::value ? 13 : 16;
+  const int off = (__float_as_int(z) & ((1 << LOW) - 1)) - (1 << (LOW - 1));
+  return abs(off) <= 8 || !(fabsf(z) > most * (1.f / 1048576.f)) || (LOW == 13 && fabsf(z) < 6.2e-5f);
 }
 
 // for error bounds, which have room for its own error of 2^-22
@@ -323,9 +334,11 @@ __global__ void __launch_bounds__(kWarps * 32) append_kernel(const __grid_consta
       for (int i = 0; i < blk; ++i) at += p.heavy_mask[i] != 0;
       for (int i = tid; i < n_tok * BD; i += kWarps * 32) {
         const int tok = i / BD, w = i % BD;
-        if (slot_s[tok] >= 0)
-          reinterpret_cast<T*>(p.heavy)[(slot_s[tok] * p.n_heavy + at) * BD + w] =
-              Elem<T>::from_float((float)rotated(p.rot, keys + key_s[tok], (int)p.perm[blk * BD + w], pos_s[tok]));
+        if (slot_s[tok] < 0) continue;
+        float z = z_s[tok * ld + j * BD + w];
+        if (near_tie<T>(z, __int_as_float(most_s[tok])))
+          z = (float)rotated(p.rot, keys + key_s[tok], (int)p.perm[blk * BD + w], pos_s[tok]);
+        reinterpret_cast<T*>(p.heavy)[(slot_s[tok] * p.n_heavy + at) * BD + w] = Elem<T>::from_float(z);
       }
       if (tid < n_tok) idx_s[tid * p.blocks + j] = 0;
     } else if (w0 < n_tok) {
@@ -336,7 +349,6 @@ __global__ void __launch_bounds__(kWarps * 32) append_kernel(const __grid_consta
       // ---- step 1
       uint32_t a[2][4], a8[2][2];
       float bound[2][2];                                             // twice the error of rows g and g + 8
-      const bool some[2] = {w0 < n_tok, w0 + 16 < n_tok};
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
@@ -389,134 +401,127 @@ __global__ void __launch_bounds__(kWarps * 32) append_kernel(const __grid_consta
           }
         }
       }
+      // the group of 16 codewords (lane of the quad, n-tile group) that alone is near the maximum; -1: there are several
+      int where[2][2];
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        if (!some[mt]) continue;
-        // the group of 16 codewords (lane of the quad, n-tile group) that alone is near the maximum; -1: there are several
-        int where[2];
+      for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
           float m = fmaxf(fmaxf(top[mt][y][0], top[mt][y][1]), fmaxf(top[mt][y][2], top[mt][y][3]));
           m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
           m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-          int v = 0;                                                 // number of groups, and the sum of what names them
+          int v = 0;                                               // number of groups, and the sum of what names them
 #pragma unroll
           for (int grp = 0; grp < 4; ++grp)
             if (top[mt][y][grp] >= m - bound[mt][y]) v += 256 + (grp * 4 + t);
           v += __shfl_xor_sync(0xffffffffu, v, 1);
           v += __shfl_xor_sync(0xffffffffu, v, 2);
           // -2: a bound that is no number, or a key beyond fp16 in the block's scale
-          where[y] = !(bound[mt][y] < 2.f * filter(BD) * 30000.f) ? -2 : ((v >> 8) == 1 ? v & 255 : -1);
+          where[mt][y] = !(bound[mt][y] < 2.f * filter(BD) * 30000.f) ? -2 : ((v >> 8) == 1 ? v & 255 : -1);
         }
-        // ---- step 2: two lanes a token
-        const int r = lane >> 1, half = lane & 1, tok = w0 + mt * 16 + r;
-        const int from_lo = __shfl_sync(0xffffffffu, where[0], (r & 7) * 4);
-        const int from_hi = __shfl_sync(0xffffffffu, where[1], (r & 7) * 4);
-        const int found = r < 8 ? from_lo : from_hi;
-        const bool live = tok < n_tok && slot_s[min(tok, n_tok - 1)] >= 0;
-        const float* z = z_s + min(tok, n_tok - 1) * ld + j * BD;
-        alignas(16) float x[BD];
-        float zn = 0.f, best = INF, next = INF;
-        int at = p.C;
-        load_block<BD>(z, x);
+      // ---- step 2: a lane a token
+      const int tok = w0 + lane, from = (lane & 7) * 4;
+      int found = __shfl_sync(0xffffffffu, where[0][0], from);
+      const int f01 = __shfl_sync(0xffffffffu, where[0][1], from), f10 = __shfl_sync(0xffffffffu, where[1][0], from);
+      const int f11 = __shfl_sync(0xffffffffu, where[1][1], from);
+      if (lane & 16) found = lane & 8 ? f11 : f10;
+      else if (lane & 8) found = f01;
+      const bool live = tok < n_tok && slot_s[min(tok, n_tok - 1)] >= 0;
+      alignas(16) float x[BD];
+      float zn = 0.f, best = INF, next = INF;
+      int at = p.C;
+      load_block<BD>(z_s + min(tok, n_tok - 1) * ld + j * BD, x);
 #pragma unroll
-        for (int w = 0; w < BD; ++w) zn = fmaf(x[w], x[w], zn);
-        if (found >= 0) {
-          const int c0 = ((found >> 2) * 8 + half * 4) * 8 + 2 * (found & 3);
-          const float* v = cb_s + c0 * BD;
+      for (int w = 0; w < BD; ++w) zn = fmaf(x[w], x[w], zn);
+      if (found >= 0) {
+        const int c0 = (found >> 2) * 64 + 2 * (found & 3);
+        const float* v = cb_s + c0 * BD;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int c = (i >> 1) * 8 + (i & 1);
-            alignas(16) float u[BD];
-            float d = 0.f;
-            load_block<BD>(v + c * BD, u);
+        for (int i = 0; i < 16; ++i) {
+          const int c = (i >> 1) * 8 + (i & 1);
+          alignas(16) float u[BD];
+          float d = 0.f;
+          load_block<BD>(v + c * BD, u);
 #pragma unroll
-            for (int w = 0; w < BD; ++w) d = fmaf(u[w] - x[w], u[w] - x[w], d);
-            next = fminf(next, fmaxf(best, d));
-            if (d < best) {
-              best = d;
-              at = c0 + c;
-            }
-          }
-        }
-        const float ob = __shfl_xor_sync(0xffffffffu, best, 1), on = __shfl_xor_sync(0xffffffffu, next, 1);
-        const int oa = __shfl_xor_sync(0xffffffffu, at, 1);
-        next = fminf(fminf(next, on), fmaxf(best, ob));
-        if (ob < best) {
-          best = ob;
-          at = oa;
-        }
-        // several groups near the maximum: the warp compares all of the block's codewords
-        unsigned wide = __ballot_sync(0xffffffffu, live && found == -1);
-        for (; wide; wide &= wide - 1, wide &= wide - 1) {           // both lanes of a token
-          const int who = (__ffs(wide) - 1) >> 1;
-          float near1 = INF, near2 = INF;
-          int c1 = p.C;
-          load_block<BD>(z_s + (w0 + mt * 16 + who) * ld + j * BD, x);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            alignas(16) float u[BD];
-            float d = 0.f;
-            load_block<BD>(cb_s + (i * 32 + lane) * BD, u);
-#pragma unroll
-            for (int w = 0; w < BD; ++w) d = fmaf(u[w] - x[w], u[w] - x[w], d);
-            near2 = fminf(near2, fmaxf(near1, d));
-            if (d < near1) {
-              near1 = d;
-              c1 = i * 32 + lane;
-            }
-          }
-          const float mine = near1;
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const float n1 = __shfl_xor_sync(0xffffffffu, near1, o), n2 = __shfl_xor_sync(0xffffffffu, near2, o);
-            near2 = fminf(fminf(near2, n2), fmaxf(near1, n1));
-            near1 = fminf(near1, n1);
-          }
-          const unsigned at1 = __ballot_sync(0xffffffffu, mine == near1);   // one lane, unless step 3 decides
-          c1 = __shfl_sync(0xffffffffu, c1, at1 ? __ffs(at1) - 1 : 0);
-          if ((lane >> 1) == who) {
-            best = near1;
-            next = near2;
-            at = c1;
+          for (int w = 0; w < BD; ++w) d = fmaf(u[w] - x[w], u[w] - x[w], d);
+          next = fminf(next, fmaxf(best, d));
+          if (d < best) {
+            best = d;
+            at = c0 + c;
           }
         }
-        const float rz = 4.f * kUlp * sqrt_approx(zn) + 16.f * kUlp * kUlp * __int_as_float(most_s[min(tok, n_tok - 1)]);
-        const float E = kBound * next + 4.f * rz * (sqrt_approx(next) + rz) + kTiny;
-        // ---- step 3
-        unsigned unsure = __ballot_sync(0xffffffffu, live && !(found > -2 && next - best > 2.f * E));
-        for (; unsure; unsure &= unsure - 1, unsure &= unsure - 1) {   // both lanes of a token
-          const int who = __ffs(unsure) - 1, tk = w0 + mt * 16 + (who >> 1);
-          double zz[BD], bd64 = __longlong_as_double(0x7ff0000000000000ll);
-          int a64 = p.C;
-#pragma unroll
-          for (int w = 0; w < BD; ++w)
-            zz[w] = rotated(p.rot, keys + key_s[tk], (int)p.perm[blk * BD + w], pos_s[tk]);
-          for (int c = lane; c < p.C; c += 32) {
-            double d = 0.0;
-#pragma unroll
-            for (int w = 0; w < BD; ++w) {
-              const double e = zz[w] - (double)cb_s[c * BD + w];
-              d = fma(e, e, d);
-            }
-            if (d < bd64) {
-              bd64 = d;
-              a64 = c;
-            }
-          }
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const double od = __shfl_xor_sync(0xffffffffu, bd64, o);
-            const int oc = __shfl_xor_sync(0xffffffffu, a64, o);
-            if (od < bd64 || (od == bd64 && oc < a64)) {
-              bd64 = od;
-              a64 = oc;
-            }
-          }
-          if ((lane >> 1) == (who >> 1)) at = a64;
-        }
-        if (live && half == 0) idx_s[tok * p.blocks + j] = (uint8_t)(at < p.C ? at : 0);   // no finite distance: 0
       }
+      // several groups near the maximum: the warp compares all of the block's codewords
+      unsigned wide = __ballot_sync(0xffffffffu, live && found == -1);
+      for (; wide; wide &= wide - 1) {
+        const int who = __ffs(wide) - 1;
+        alignas(16) float xw[BD];
+        float near1 = INF, near2 = INF;
+        int c1 = p.C;
+        load_block<BD>(z_s + (w0 + who) * ld + j * BD, xw);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          alignas(16) float u[BD];
+          float d = 0.f;
+          load_block<BD>(cb_s + (i * 32 + lane) * BD, u);
+#pragma unroll
+          for (int w = 0; w < BD; ++w) d = fmaf(u[w] - xw[w], u[w] - xw[w], d);
+          near2 = fminf(near2, fmaxf(near1, d));
+          if (d < near1) {
+            near1 = d;
+            c1 = i * 32 + lane;
+          }
+        }
+        const float mine = near1;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const float n1 = __shfl_xor_sync(0xffffffffu, near1, o), n2 = __shfl_xor_sync(0xffffffffu, near2, o);
+          near2 = fminf(fminf(near2, n2), fmaxf(near1, n1));
+          near1 = fminf(near1, n1);
+        }
+        const unsigned at1 = __ballot_sync(0xffffffffu, mine == near1);   // one lane, unless step 3 decides
+        c1 = __shfl_sync(0xffffffffu, c1, at1 ? __ffs(at1) - 1 : 0);
+        if (lane == who) {
+          best = near1;
+          next = near2;
+          at = c1;
+        }
+      }
+      const float rz = 4.f * kUlp * sqrt_approx(zn) + 16.f * kUlp * kUlp * __int_as_float(most_s[min(tok, n_tok - 1)]);
+      const float E = kBound * next + 4.f * rz * (sqrt_approx(next) + rz) + kTiny;
+      // ---- step 3
+      unsigned unsure = __ballot_sync(0xffffffffu, live && !(found > -2 && next - best > 2.f * E));
+      for (; unsure; unsure &= unsure - 1) {
+        const int who = __ffs(unsure) - 1, tk = w0 + who;
+        double zz[BD], bd64 = __longlong_as_double(0x7ff0000000000000ll);
+        int a64 = p.C;
+#pragma unroll
+        for (int w = 0; w < BD; ++w)
+          zz[w] = rotated(p.rot, keys + key_s[tk], (int)p.perm[blk * BD + w], pos_s[tk]);
+        for (int c = lane; c < p.C; c += 32) {
+          double d = 0.0;
+#pragma unroll
+          for (int w = 0; w < BD; ++w) {
+            const double e = zz[w] - (double)cb_s[c * BD + w];
+            d = fma(e, e, d);
+          }
+          if (d < bd64) {
+            bd64 = d;
+            a64 = c;
+          }
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double od = __shfl_xor_sync(0xffffffffu, bd64, o);
+          const int oc = __shfl_xor_sync(0xffffffffu, a64, o);
+          if (od < bd64 || (od == bd64 && oc < a64)) {
+            bd64 = od;
+            a64 = oc;
+          }
+        }
+        if (lane == who) at = a64;
+      }
+      if (live) idx_s[tok * p.blocks + j] = (uint8_t)(at < p.C ? at : 0);   // no finite distance: 0
     }
     __syncthreads();                            // the record is read
     if (tid == 0 && j + 2 < nblk) {
