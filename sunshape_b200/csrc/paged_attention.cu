@@ -182,6 +182,7 @@ int sunshape_paged_attention(const sunshape_codec_t* codec, const void* tables, 
     else rc = bf16 ? launch<__nv_bfloat16, false>(f, vmap, d, dv, bd, grid, st) : launch<__half, false>(f, vmap, d, dv, bd, grid, st);
     if (rc) return rc;
     p.prefix_parts = 1;
+    p.overlap = tensor;                // else both use the same slots of the workspace
   }
   if (int rc = bf16 ? launch<__nv_bfloat16, false>(p, vmap, d, dv, bd, grid, st)
                     : launch<__half, false>(p, vmap, d, dv, bd, grid, st))

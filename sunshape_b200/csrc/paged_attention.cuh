@@ -41,6 +41,7 @@ struct AttnParams {
   int prefix_mode;                 // 1: the one sequence is the prefix, rows are those of all sequences
   int prefix_len;
   int prefix_parts;                // partial sets of the prefix that a finished row joins (0: none)
+  int overlap;                     // 1: may start before the prefix's sets are written (griddepcontrol.wait comes before them)
   int64_t num_pages, table_stride;
   float scale_log2;                // scale * log2(e)
   const int32_t* table;

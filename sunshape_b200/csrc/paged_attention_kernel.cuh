@@ -191,8 +191,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   const int cta = blockIdx.x;
   const int grid = min((int)gridDim.x, (total + kMinTiles - 1) / kMinTiles);
   asm volatile("griddepcontrol.launch_dependents;");           // the join waits for this grid's end by itself
+  // What comes before this grid is done: before the prefix's sets are read, and in every CTA, since what follows this grid
+  // counts on that, too.
+  auto prefix_written = [&]() {
+    if (p.overlap) asm volatile("griddepcontrol.wait;" ::: "memory");
+  };
   if (cta >= grid) {
     if (tid == 0) p.desc[cta] = make_int4(0, -1, 0, 0);
+    prefix_written();
     return;
   }
   // part i of n of a range of `size`: the first size % n parts are one longer
@@ -567,6 +573,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       // the item's or piece's result
       bad = __any_sync(0xffffffffu, bad);
       const bool begins = w.t == 0, ends = w.t + n == w.tiles;
+      if (begins && ends) prefix_written();
 #pragma unroll
       for (int c = 0; c < NT; ++c)
 #pragma unroll
@@ -626,6 +633,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       head_s[pair] = head;
       tail_s[pair] = tail;
     }
+    prefix_written();
     named_barrier(1, kPairs * 32);
 
     // Items cut between pairs, in the list's order: each starts with a pair's tail piece (or, begun by an earlier
@@ -743,16 +751,21 @@ int launch_paged_attention(const AttnParams& p, const CUtensorMap& vmap, int gri
   static std::atomic<uint64_t> done[2];
   if (!ready_kernel((const void*)k, kSmemMax, kLaunchRegs, done[p.item_rows == 8]))
     return set_last_error(SUNSHAPE_E_CUDA, "the paged attention kernel is not available as it was built.");
-  k<<<grid, kAttnThreads, p.smem, st>>>(p, vmap);
-  // the join may be scheduled while the main grid drains; it waits for its end before it reads
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid, p.item_rows);
-  cfg.blockDim = dim3(kJoinParts * DV / 4);
-  cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
+  cfg.numAttrs = p.overlap;
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kAttnThreads);
+  cfg.dynamicSmemBytes = p.smem;
+  cfg.stream = st;
+  cudaLaunchKernelEx(&cfg, k, p, vmap);
+  // the join may be scheduled while the main grid drains; it waits for its end before it reads
+  cfg.gridDim = dim3(grid, p.item_rows);
+  cfg.blockDim = dim3(kJoinParts * DV / 4);
+  cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;
   cudaLaunchKernelEx(&cfg, paged_attention_join<DV, T>, p);
   return SUNSHAPE_OK;

@@ -601,6 +601,7 @@ __global__ void __launch_bounds__(kPfJoinRows * 32) paged_prefix_join(const __gr
   const int total = stride * items * p.H - kPfItemTiles, grid = min(ctas, total);
   const int h = blockIdx.x / items, r0 = (blockIdx.x - h * items) * kPfRows;
   const int r = blockIdx.y * kPfJoinRows + threadIdx.x / 32, d = (threadIdx.x & 31) * 4;
+  asm volatile("griddepcontrol.launch_dependents;");   // the sequences' own tokens need the prefix only where rows are finished
   // by every block: what follows this grid counts on the grid before it, too
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (r0 + r >= rows_total) return;
