@@ -24,7 +24,7 @@ constexpr int kPairs = 8;          // pairs of a consumer (warps 0-7) and a prod
 constexpr int kAttnThreads = 2 * kPairs * 32;
 constexpr int kMinTiles = kPairs;  // tiles of a CTA's range, unless there are fewer: one for each pair
 constexpr int kHeadTiles = 48;     // tiles that the change to another head's codebook is charged in the split
-constexpr int kItemTiles = 2;      // tiles that an item's queries and result are charged
+constexpr int kItemTiles = 5;      // tiles that the queries and result of an item of 16 rows are charged; of 8 rows, 2
 constexpr int kPlanChunks = 256;   // sequence chunks of the in-kernel plan
 // Registers of a thread: what the block is launched with, and its split between the roles (setmaxnreg).
 constexpr int kLaunchRegs = 128, kConsumerRegs = 216, kProducerRegs = 40;

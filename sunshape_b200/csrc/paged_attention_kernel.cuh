@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   constexpr int NB = D / BD, UNITS = NB / 4, WORDS = BD / 2;   // units: gathers of a lane per token
   constexpr int ROT = 16 / BD;                                 // tokens that share a load phase and a column set
   constexpr int KS = D / 16, ROWS = 8 * NT, RF = row_floats(DV);
-  constexpr int IMAGE = D * 512;
+  constexpr int IMAGE = D * 512, ITEM = NT == 1 ? 2 : kItemTiles;
   constexpr int MT = kTile / 16;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     int n = 0;
     for (int i = tid * per; i < min(seqs, (tid + 1) * per); ++i) {
       const int len = own_length(p, i);
-      n += tiles_of(len) + kItemTiles;
+      n += tiles_of(len) + ITEM;
       if (per == 1) len_s[i] = len;
     }
     for (int o = 1; o < 32; o <<= 1) {
@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 
   // ---- this CTA's range.  With a codebook per head, a head's tiles are followed by kHeadTiles that stand for the
   // change and a range falls into one portion per head; with one codebook for all it is one portion.
-  // An item's tiles are followed by kItemTiles that stand for its queries and result.  The entry refuses calls whose
+  // An item's tiles are followed by ITEM ones that stand for its queries and result.  The entry refuses calls whose
   // tiles may not fit into 31 bits.
   const int per_head = cum_s[kPlanChunks] * mtiles;
   const int gap = p.n_cb > 1 ? kHeadTiles : 0;
@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   auto next_item = [&](int n) {
     w.at += n;
     if (w.t + n < w.tiles) return;               // cut: the range ends here
-    w.at += w.tiles + kItemTiles - (w.t + n);
+    w.at += w.tiles + ITEM - (w.t + n);
     w.t = 0;
     if (++w.mt < mtiles) return;
     w.mt = 0;
@@ -251,14 +251,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     w.b = lo * per;
     w.len = length_of(w.b);
     w.tiles = tiles_of(w.len);
-    while (o >= (w.tiles + kItemTiles) * mtiles) {
-      o -= (w.tiles + kItemTiles) * mtiles;
+    while (o >= (w.tiles + ITEM) * mtiles) {
+      o -= (w.tiles + ITEM) * mtiles;
       ++w.b;
       w.len = length_of(w.b);
       w.tiles = tiles_of(w.len);
     }
-    w.mt = o / (w.tiles + kItemTiles);
-    w.t = o - w.mt * (w.tiles + kItemTiles);
+    w.mt = o / (w.tiles + ITEM);
+    w.t = o - w.mt * (w.tiles + ITEM);
     if (w.t >= w.tiles) next_item(0);
   };
   uint8_t* const my_ring = ring + (size_t)pair * ring_bytes;
