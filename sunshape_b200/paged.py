@@ -15,6 +15,7 @@ only (bf16, f16); ``norm_rotate`` also takes fp32.  Every call runs on the curre
 takes no workspace that outlives it and can be captured into a CUDA graph; tensors used on another stream than
 the one they were made on need the usual ``record_stream``.  What only the device can see is checked there: a
 position, slot, page or length out of range is skipped (or makes the row NaN) and recorded, see ``paged_error``.
+Nothing here is differentiable.
 """
 from __future__ import annotations
 
@@ -186,6 +187,7 @@ class SunShapePagedCache:
                 raise RuntimeError("page pools must be contiguous and 16-byte aligned.")
         self.codec, self.indices, self.values, self.heavy = codec, indices, values, heavy
         self.device, self._index = dev, indices.get_device()
+        self._n_heavy, self._made = n_heavy, None
         self._pages = _lib.PagesDesc(_lib.ptr(indices), _lib.ptr(heavy), _lib.ptr(values), indices.shape[0],
                                      indices.shape[1], indices.shape[2], values.shape[3], _lib.dtype_code(values))
         self._tables()
@@ -214,6 +216,10 @@ class SunShapePagedCache:
         """The codec's descriptor, and what the kernels read of its codebooks, derived once and kept by the codec until
         ``invalidate``."""
         made = self.codec.kernel_desc()          # another object after each ``invalidate``, over the same buffers
+        if made is not self._made:
+            if made[2] != self._n_heavy or made[1][0].get_device() != self._index:
+                raise RuntimeError("the codec's dense blocks or device are not those that the page pools were made for.")
+            self._made = made
         kept = getattr(self.codec, "_paged_tables", None)
         if kept is None or kept[1] is not made:
             kept = self.codec._paged_tables = (_lib.paged_tables(made[0], self.device), made)
@@ -221,10 +227,14 @@ class SunShapePagedCache:
 
     def slots(self, page_table: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
         """Slots [B, L] of the token positions [B, L] (within their sequences) under ``page_table`` [B, cols]; -1
-        where a position is negative."""
-        p = positions.long().clamp(min=0)
-        s = page_table.long().gather(1, p // self.page_size) * self.page_size + p % self.page_size
-        return torch.where(positions >= 0, s, s.new_full((), -1))
+        where a position is negative, a slot outside the pool (which ``append_paged`` records) beyond the table."""
+        cols, outside = page_table.shape[1], self.num_pages * self.page_size
+        p = positions.long()
+        s = p.new_full(p.shape, outside)
+        if cols:
+            page = page_table.long().gather(1, (p // self.page_size).clamp(0, cols - 1))
+            s = torch.where(p < cols * self.page_size, page * self.page_size + p % self.page_size, s)
+        return torch.where(p >= 0, s, -1)
 
     def append(self, key, value, slots, **rotation) -> None:
         append_paged(self, key, value, slots, **rotation)

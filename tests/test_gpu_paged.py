@@ -407,6 +407,29 @@ def test_codebook_edited_in_place():
     _check_attention(cache.attention(q, table, n), cache, q, table, n, None, 0)
 
 
+def test_positions_beyond_the_table_are_recorded():
+    codec, scale = make_paged_codec(64, 8, 2, seed=9)
+    cache, k, v, _, _ = _append_case(codec, 2, 1, 4, page=16, dtype=torch.bfloat16, R=0, scale=scale)
+    table = torch.tensor([[2, 0]], dtype=torch.int32, device=DEV)
+    slots = cache.slots(table, torch.tensor([[31, 32, 1000000, -5]], device=DEV))
+    before = _state(cache)
+    cache.append(k, v, slots)
+    assert "slot" in paged.paged_error(DEV)
+    _check_append(cache, k, v, torch.tensor([[15, -1, -1, -1]]), {}, before)
+
+
+def test_codec_that_no_longer_fits_its_pools():
+    codec, _ = make_paged_codec(64, 8, 2, heavy=2, seed=9)
+    cache = SunShapePagedCache.allocate(codec, 6, 2, page_size=16)
+    k = _randn(1, 2, 3, 64, seed=1, dtype=torch.bfloat16)
+    codec.mixed_high_precision_blocks.fill_(True)
+    codec.invalidate()
+    with pytest.raises(RuntimeError, match="dense blocks or device"):
+        cache.append(k, k, torch.arange(3, device=DEV)[None])
+    with pytest.raises(RuntimeError, match="dense blocks or device"):
+        cache.attention(k, torch.zeros(1, 1, dtype=torch.int32, device=DEV), torch.ones(1, dtype=torch.int32, device=DEV))
+
+
 def test_append_strided_and_misaligned_rows():
     """Values and keys that begin off a 16-byte boundary, a flat ragged batch, positions that broadcast."""
     codec, scale = make_paged_codec(64, 8, 2, seed=9)

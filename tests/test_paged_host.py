@@ -113,3 +113,7 @@ def test_slots_of_positions():
     table = torch.tensor([[5, 2], [7, 0]], dtype=torch.int32)
     got = paged.SunShapePagedCache.slots(cache, table, torch.tensor([[0, 17, -1], [15, 16, 31]]))
     assert got.tolist() == [[80, 33, -1], [127, 0, 15]]
+    # beyond the table: a slot outside the pool of one page, for the append to record
+    got = paged.SunShapePagedCache.slots(cache, table, torch.tensor([[32, 5], [10 ** 9, -1]]))
+    assert got.tolist() == [[16, 85], [16, -1]]
+    assert paged.SunShapePagedCache.slots(cache, table[:, :0], torch.tensor([[0, -1], [3, 4]])).tolist() == [[16, -1], [16, 16]]
