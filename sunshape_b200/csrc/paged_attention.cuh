@@ -23,8 +23,13 @@ constexpr int kItemRows = 16;      // most query rows of an item
 constexpr int kPairs = 8;          // pairs of a consumer (warps 0-7) and a producer warp (8-15)
 constexpr int kAttnThreads = 2 * kPairs * 32;
 constexpr int kMinTiles = kPairs;  // tiles of a CTA's range, unless there are fewer: one for each pair
-constexpr int kHeadTiles = 48;     // tiles that the change to another head's codebook is charged in the split
-constexpr int kItemTiles = 5;      // tiles that the queries and result of an item of 16 rows are charged; of 8 rows, 2
+// Tiles that other work is charged in the split.  The change to another head's codebook (the pairs drain, 64 KB are copied,
+// queries and first tiles follow) takes a CTA about as long as 50 tiles at HBM's pace: 64 sequences of 1k to 8k take 118 us
+// with 16 charged, 114 with 48.
+constexpr int kHeadTiles = 48;
+// The queries and the result of an item of 16 rows (16 sequences of 3 to 6k, 4 queries: 64 us with 2, 54 with 5, 53 with
+// 14); of 8 rows, 2 (0: 161 us, 2: 149 for 64 short sequences behind a prefix).
+constexpr int kItemTiles = 5;
 constexpr int kPlanChunks = 256;   // sequence chunks of the in-kernel plan
 // Registers of a thread: what the block is launched with, and its split between the roles (setmaxnreg).
 constexpr int kLaunchRegs = 128, kConsumerRegs = 216, kProducerRegs = 40;
