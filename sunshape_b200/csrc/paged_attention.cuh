@@ -28,7 +28,7 @@ constexpr int kMinTiles = kPairs;  // tiles of a CTA's range, unless there are f
 // with 16 charged, 114 with 48.
 constexpr int kHeadTiles = 48;
 // The queries and the result of an item of 16 rows (16 sequences of 3 to 6k, 4 queries: 64 us with 2, 54 with 5, 53 with
-// 14); of 8 rows, 2 (0: 161 us, 2: 149 for 64 short sequences behind a prefix).
+// 14); of 8 rows, 2 (64 sequences of up to 700 tokens, 64/8 heads: 28.9 us with 0, 25.7 with 2).
 constexpr int kItemTiles = 5;
 constexpr int kPlanChunks = 256;   // sequence chunks of the in-kernel plan
 // Registers of a thread: what the block is launched with, and its split between the roles (setmaxnreg).
