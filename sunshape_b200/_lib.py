@@ -427,16 +427,18 @@ def norm_rotate(index: int, q: bytes, q_out: bytes, q_weight, k, k_out, k_weight
                weight_dtype, batch, length, dim, eps, rot)
 
 
-def paged_tables(cd: CodecDesc, dev) -> torch.Tensor:
-    """What the paged kernels read of a codec, in one buffer."""
-    lib = load_library()
-    n = lib.sunshape_paged_tables_bytes(cd)
+def paged_tables_bytes(cd: CodecDesc) -> int:
+    n = load_library().sunshape_paged_tables_bytes(cd)
     if n < 0:
         _check(int(n))
-    tables = torch.empty(n, dtype=torch.uint8, device=dev)
+    return n
+
+
+def paged_tables(cd: CodecDesc, tables: torch.Tensor) -> None:
+    """Writes what the paged kernels read of a codec's codebooks into ``tables``."""
+    dev = tables.device
     with torch.cuda.device(dev):
-        _check(lib.sunshape_paged_tables(cd, ptr(tables), n, stream_ptr(dev)))
-    return tables
+        _check(load_library().sunshape_paged_tables(cd, ptr(tables), tables.numel(), stream_ptr(dev)))
 
 
 def paged_append(index: int, cd: CodecDesc, tables: torch.Tensor, pages: PagesDesc, key: bytes, value: bytes, batch: int,

@@ -92,6 +92,8 @@ class SunShapeBlockCodec(torch.nn.Module):
         self.register_buffer("rotation", torch.eye(head_dim, device=dev))
         self._desc_cache = None
         self._metric_cache = None
+        self._paged_tables = None       # what the paged kernels read (paged.py), and those of other shapes before
+        self._paged_retired = ()
 
     # ------------------------------------------------------------------ state
     def _load_from_state_dict(self, state_dict, prefix, *args, **kwargs):
@@ -99,8 +101,7 @@ class SunShapeBlockCodec(torch.nn.Module):
         if key in state_dict and state_dict[key].shape != self.centroids.shape:
             self.centroids = torch.empty_like(state_dict[key], device=self.centroids.device)
         super()._load_from_state_dict(state_dict, prefix, *args, **kwargs)
-        self._desc_cache = None
-        self._metric_cache = None
+        self.invalidate()
 
     def _apply(self, fn, *args, **kwargs):
         out = super()._apply(fn, *args, **kwargs)
@@ -110,9 +111,16 @@ class SunShapeBlockCodec(torch.nn.Module):
         return out
 
     def invalidate(self) -> None:
-        """Call after editing buffers in place (centroids, permutation, heavy mask, metric)."""
+        """Call after editing buffers in place (centroids, permutation, heavy mask, metric).
+
+        Where a paged cache uses the codec, what its kernels read is renewed at once, for graphs that are replayed without
+        another call in between; this waits for the device."""
         self._desc_cache = None
         self._metric_cache = None
+        if self._paged_tables is not None:
+            from .paged import renew_after_edit
+
+            renew_after_edit(self)
 
     @property
     def n_codebooks(self) -> int:

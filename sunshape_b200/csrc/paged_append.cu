@@ -30,7 +30,6 @@ struct AppendParams {
   int64_t tokens, slots_total;
   const int64_t* slots;
   int64_t slot_sb, slot_sl;
-  const float* cb;
   const uint8_t* records;
   const int64_t* perm;
   const uint8_t* heavy_mask;
@@ -665,7 +664,6 @@ int sunshape_paged_append(const sunshape_codec_t* codec, const void* tables, con
   p.slots = slots;
   p.slot_sb = slot_stride_b;
   p.slot_sl = slot_stride_l;
-  p.cb = codec->centroids;
   const Tables tab(p.n_cb, p.nb, p.D);
   p.records = static_cast<const uint8_t*>(tables) + tab.records;
   p.perm = codec->permutation;

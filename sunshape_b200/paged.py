@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import threading
 
 import torch
 
@@ -153,6 +154,76 @@ def norm_rotate(query: torch.Tensor, key: torch.Tensor | None = None, *, q_weigh
     return q_out, k_out
 
 
+# ----------------------------------------------------------------------------------------- what a codec amounts to
+class _CodecTables:
+    """What the paged kernels read of a codec: tables derived from its codebooks, its permutation and its dense blocks'
+    mask, in one buffer per tensor that the codec keeps.  They are renewed in place, so that captured graphs, which hold
+    their addresses, see what the codec holds."""
+
+    def __init__(self, key: tuple, desc: _lib.CodecDesc):
+        self.key, self.desc, self.made, self.streams = key, None, None, set()
+        device, _, n_heavy = key
+        self.device, self.index, self.n_heavy = device, device.index, n_heavy
+        self.buffer = torch.empty(_lib.paged_tables_bytes(desc), dtype=torch.uint8, device=device)
+        self.perm = torch.empty(desc.head_dim, dtype=torch.int64, device=device)
+        self.mask = torch.empty(desc.head_dim // desc.block_dim, dtype=torch.uint8, device=device) if n_heavy else None
+
+    def fill(self, made: tuple) -> None:
+        desc, (cents, perm, mask, _), _ = made
+        self.perm.copy_(perm)
+        if mask is not None:
+            self.mask.copy_(mask)
+        _lib.paged_tables(desc, self.buffer)
+        # the kernels read no centroids of the descriptor, only the tables
+        self.desc = _lib.codec_desc(cents, self.perm, self.mask, self.n_heavy, desc.head_dim, desc.block_dim)
+
+    def used_on(self, stream: int) -> None:
+        """Keeps the buffers from the allocator until what runs on this stream is done, once they are given up."""
+        for t in (self.buffer, self.perm, self.mask):
+            if t is not None:
+                t.record_stream(torch.cuda.current_stream(self.device))
+        self.streams.add(stream)
+
+
+_renewing = threading.Lock()
+
+
+def renew_tables(codec: SunShapeBlockCodec) -> _CodecTables:
+    """Derives a codec's tables again.  Waits for the device on both sides: edits of the codec's buffers and readers of the
+    tables, on whatever stream, come before; every later reader finds them written."""
+    device = _lib.require_cuda(codec.centroids)
+    # the buffers outlive an inference mode that they happen to be made in, and are written again outside it
+    with _renewing, torch.cuda.device(device), torch.inference_mode(False), torch.no_grad():
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a codec's tables can not be derived while a CUDA graph is captured: make the cache, and call "
+                               "codec.invalidate() after edits of the codec, before the capture.")
+        torch.cuda.synchronize()
+        made = codec.kernel_desc()
+        desc, (cents, *_), n_heavy = made
+        key = (device, tuple(cents.shape), n_heavy)
+        tables = codec._paged_tables
+        if tables is None or tables.key != key:
+            if tables is not None:              # graphs captured with them may still be replayed
+                codec._paged_retired = (*codec._paged_retired, tables)
+            tables = _CodecTables(key, desc)
+        tables.fill(made)
+        torch.cuda.synchronize()
+        tables.made = made
+        codec._paged_tables = tables
+    return tables
+
+
+def renew_after_edit(codec: SunShapeBlockCodec) -> None:
+    """Renews the tables of a codec that still has the shape they were made for; else the next call does, or says why not."""
+    device, shape, _ = codec._paged_tables.key
+    cents = codec.centroids
+    if cents.device == device and tuple(cents.shape)[-3:] == shape[-3:] and codec.n_codebooks == shape[0]:
+        with torch.cuda.device(device):
+            capturing = torch.cuda.is_current_stream_capturing()
+        if not capturing and codec.mode not in ("rotated", "legacy_strict"):
+            renew_tables(codec)
+
+
 # ---------------------------------------------------------------------------------------------------- the cache
 class SunShapePagedCache:
     """One layer's page pool and the codec of its keys.  ``allocate`` makes the pool, ``from_pools`` takes one."""
@@ -187,7 +258,7 @@ class SunShapePagedCache:
                 raise RuntimeError("page pools must be contiguous and 16-byte aligned.")
         self.codec, self.indices, self.values, self.heavy = codec, indices, values, heavy
         self.device, self._index = dev, indices.get_device()
-        self._n_heavy, self._made = n_heavy, None
+        self._n_heavy, self._held = n_heavy, None
         self._pages = _lib.PagesDesc(_lib.ptr(indices), _lib.ptr(heavy), _lib.ptr(values), indices.shape[0],
                                      indices.shape[1], indices.shape[2], values.shape[3], _lib.dtype_code(values))
         self._tables()
@@ -212,18 +283,22 @@ class SunShapePagedCache:
     value_dim = property(lambda self: int(self.values.shape[3]))
     dtype = property(lambda self: self.values.dtype)
 
-    def _tables(self) -> tuple[_lib.CodecDesc, torch.Tensor]:
-        """The codec's descriptor, and what the kernels read of its codebooks, derived once and kept by the codec until
-        ``invalidate``."""
-        made = self.codec.kernel_desc()          # another object after each ``invalidate``, over the same buffers
-        if made is not self._made:
-            if made[2] != self._n_heavy or made[1][0].get_device() != self._index:
-                raise RuntimeError("the codec's dense blocks or device are not those that the page pools were made for.")
-            self._made = made
-        kept = getattr(self.codec, "_paged_tables", None)
-        if kept is None or kept[1] is not made:
-            kept = self.codec._paged_tables = (_lib.paged_tables(made[0], self.device), made)
-        return made[0], kept[0]
+    def _tables(self) -> _CodecTables:
+        """The codec's tables, derived once and renewed after ``invalidate``, for calls on the current stream."""
+        codec = self.codec
+        tables = codec._paged_tables
+        if tables is None or tables.made is not codec._desc_cache:   # a descriptor of its own after each ``invalidate``
+            tables = renew_tables(codec)
+        if tables is not self._held:
+            if (tables.n_heavy != self._n_heavy or tables.index != self._index
+                    or tables.desc.n_cb not in (1, self.indices.shape[1])):
+                raise RuntimeError("the codec's codebooks, dense blocks or device are not those that the page pools were made "
+                                   "for.")
+            self._held = tables
+        stream = torch._C._cuda_getCurrentRawStream(self._index)
+        if stream not in tables.streams:
+            tables.used_on(stream)
+        return tables
 
     def slots(self, page_table: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
         """Slots [B, L] of the token positions [B, L] (within their sequences) under ``page_table`` [B, cols]; -1
@@ -275,9 +350,9 @@ def append_paged(cache: SunShapePagedCache, key: torch.Tensor, value: torch.Tens
     if slots.dtype != torch.int64 or tuple(slots.shape) != (B, L):
         raise RuntimeError("slots must be int64 [batch, length].")
     rot = _rotation(cos, sin, positions, interleaved, B, L, D, dev)
-    desc, tables = cache._tables()
-    _lib.paged_append(dev, desc, tables, pages, _lib.rows(_unit(key, "key")), _lib.rows(_unit(value, "value")), B, L, slots,
-                      rot)
+    tables = cache._tables()
+    _lib.paged_append(dev, tables.desc, tables.buffer, pages, _lib.rows(_unit(key, "key")), _lib.rows(_unit(value, "value")),
+                      B, L, slots, rot)
 
 
 def paged_attention(cache: SunShapePagedCache, query: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor, *,
@@ -326,8 +401,8 @@ def paged_attention(cache: SunShapePagedCache, query: torch.Tensor, page_table: 
         out = torch.empty(shape, dtype=dtype, device=query.device)
     elif tuple(out.shape) != shape or out.dtype != dtype or out.get_device() != dev or not out.is_contiguous():
         raise RuntimeError("out must be contiguous [batch, q_heads, query_len, value_dim] of the query's dtype.")
-    desc, tables = cache._tables()
-    _lib.paged_attention(dev, desc, tables, pages, query, B, Hq, L, page_table, seq_lens,
+    tables = cache._tables()
+    _lib.paged_attention(dev, tables.desc, tables.buffer, pages, query, B, Hq, L, page_table, seq_lens,
                          prefix_table if prefix_len else None, prefix_len, 1.0 / math.sqrt(D) if scale is None else float(scale),
                          causal, out)
     return out
