@@ -286,7 +286,7 @@ int sunshape_paged_append(const sunshape_codec_t* codec, const void* tables, con
  * the prefix_len tokens of the pages prefix_table (prefix_len 0: no prefix), whose attention is computed
  * once for the whole batch.
  * query [batch, q_heads, query_len, head_dim] (unit last stride; BF16 or F16, the pages' dtype), out
- * [batch, q_heads, query_len, value_dim] contiguous, of the same dtype.
+ * [batch, q_heads, query_len, value_dim] contiguous, of the same dtype, 8-byte aligned.
  * The last query_len tokens of a sequence are the queries' own: query l sees all but the last
  * query_len - 1 - l of the sequence's own tokens (and all of the prefix); causal = 0: all of them.  A row
  * that sees no token is zero.  Softmax of scale * <q, k_hat>, statistics and sums in fp32.

@@ -109,6 +109,7 @@ int sunshape_paged_attention(const sunshape_codec_t* codec, const void* tables, 
     return set_last_error(SUNSHAPE_E_UNSUPPORTED, "at most 65535 sequences and 2^30 query rows a call.");
   if (!query->data || !out || !seq_lens || (table_cols && !page_table) || (prefix_len && !prefix_table) || !tables)
     return set_last_error(SUNSHAPE_E_INVALID, "query / out / seq_lens / page table / tables pointer is NULL.");
+  if ((uintptr_t)out % 8) return set_last_error(SUNSHAPE_E_INVALID, "paged attention: out must be 8-byte aligned.");
   if (!workspace || (uintptr_t)workspace % 256 ||
       workspace_bytes < sunshape_paged_attention_workspace_bytes(batch, query->heads, pages->kv_heads, query_len,
                                                                  pages->value_dim, table_cols, pages->page_size,

@@ -364,7 +364,8 @@ def paged_attention(cache: SunShapePagedCache, query: torch.Tensor, page_table: 
     on the device: lengths never visit the host).  With ``prefix_table`` [n] int32 and ``prefix_len``, the first
     ``prefix_len`` tokens of those pages come before every sequence's own, and are read and attended to once for
     the whole batch.  The last L tokens of a sequence are the queries' own: query l sees all but the last L - 1 -
-    l of them, unless ``causal`` is false.  A row that sees nothing is zero.  ``scale`` defaults to 1 / sqrt(D).
+    l of them, unless ``causal`` is false.  A row that sees nothing is zero.  ``scale`` defaults to 1 / sqrt(D).  ``out``
+    must be contiguous and begin at a multiple of 8 bytes.
 
     Softmax statistics and sums are fp32.  Codewords are read as fp16 and softmax weights rounded to the cache's
     dtype before they multiply values; queries are scaled by powers of two into fp16's range.  Dense key blocks
