@@ -328,6 +328,8 @@ int make_rotation(const sunshape_rotation_t* r, int dim, bool empty, Rotation* o
     return set_last_error(SUNSHAPE_E_INVALID, "rot_dim must be even and between 0 and the head dimension.");
   if (!empty && (!r->cos || !r->sin || !r->positions)) return set_last_error(SUNSHAPE_E_INVALID, "rotation pointer is NULL.");
   if (r->table_len < 0) return set_last_error(SUNSHAPE_E_INVALID, "rotation table length must be >= 0.");
+  // the kernels read row 0 where a position is outside the table
+  if (!empty && r->table_len == 0) return set_last_error(SUNSHAPE_E_INVALID, "the rotation table has no rows.");
   if (r->position_dtype != SUNSHAPE_I32 && r->position_dtype != SUNSHAPE_I64)
     return set_last_error(SUNSHAPE_E_INVALID, "positions must be I32 or I64.");
   *out = Rotation{r->cos, r->sin, r->positions, r->position_stride_b, r->position_stride_l, r->table_len,

@@ -18,3 +18,16 @@ def test_attention_output_alignment():
     pg = _lib.PagesDesc(16, None, 16, 4, 2, 16, 64, _lib.BF16)
     for out in (16 + 2, 16 + 4, 16 + 6):
         _expect(f(cd, 256, pg, _rows(4), 1, 1, 16, 2, 2, 16, None, 0, 1.0, 1, out, 256, 1 << 24, None), -1, "8-byte aligned")
+
+
+def test_rotation_table_without_rows():
+    """A position outside the table reads row 0 in its place: a table has one."""
+    lib = _lib.load_library()
+    rot = _lib.RotationDesc(16, 16, 16, 1, 1, 0, _lib.I64, 64, 0)
+    _expect(lib.sunshape_norm_rotate(_rows(), _rows(), None, None, None, None, _lib.BF16, _lib.BF16, 1, 1, 64, 1e-6, rot, None),
+            -1, "table has no rows")
+    cd = _lib.CodecDesc(16, 16, None, 1, 64, 8, 256, 0, None)
+    pg = _lib.PagesDesc(16, None, 16, 4, 2, 16, 64, _lib.BF16)
+    _expect(lib.sunshape_paged_append(cd, 256, pg, _rows(), _rows(), 1, 1, 16, 1, 1, rot, None), -1, "table has no rows")
+    # nothing to rotate: nothing is read
+    assert lib.sunshape_norm_rotate(_rows(), _rows(), None, None, None, None, _lib.BF16, _lib.BF16, 0, 1, 64, 1e-6, rot, None) == 0
