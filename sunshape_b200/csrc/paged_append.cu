@@ -546,7 +546,7 @@ __global__ void __launch_bounds__(kWarps * 32) append_kernel(const __grid_consta
 }
 
 template <typename T, int BD>
-void launch(AppendParams& p, cudaStream_t st) {
+int launch(AppendParams& p, cudaStream_t st) {
   const int64_t tiles = (p.tokens + kTokens - 1) / kTokens;
   // A head's blocks are shared out until every SM has two CTAs (one token a sequence leaves one tile of tokens), and in
   // any case to 32 elements a CTA, with whose keys in shared memory an SM holds five
@@ -555,15 +555,16 @@ void launch(AppendParams& p, cudaStream_t st) {
   p.splits = (p.nb + p.blocks - 1) / p.blocks;
   const int smem = 2 * record_bytes(BD) + kTokens * ((p.blocks * BD + 8) * 4 + 3 * 8 + 4 + p.blocks);
   static std::atomic<uint64_t> done;
-  ready_kernel((const void*)append_kernel<T, BD>, 2 * record_bytes(BD) + kTokens * (40 * 4 + 28 + 32 / BD), 0, done);
+  if (!ready_kernel((const void*)append_kernel<T, BD>, 2 * record_bytes(BD) + kTokens * (40 * 4 + 28 + 32 / BD), 0, done))
+    return set_last_error(SUNSHAPE_E_CUDA, "the paged append kernel is not available as it was built.");
   append_kernel<T, BD><<<dim3((unsigned)tiles, p.H, p.splits + 1), kWarps * 32, smem, st>>>(p);
+  return launch_status("paged append launch");
 }
 
 template <typename T>
-void launch(AppendParams& p, int bd, cudaStream_t st) {
-  if (bd == 8) launch<T, 8>(p, st);
-  else if (bd == 4) launch<T, 4>(p, st);
-  else launch<T, 2>(p, st);
+int launch(AppendParams& p, int bd, cudaStream_t st) {
+  if (bd == 8) return launch<T, 8>(p, st);
+  return bd == 4 ? launch<T, 4>(p, st) : launch<T, 2>(p, st);
 }
 
 int check_paged_codec(const sunshape_codec_t* c) {
@@ -674,9 +675,7 @@ int sunshape_paged_append(const sunshape_codec_t* codec, const void* tables, con
   p.err = paged_error_word();
   if (!p.err) return set_last_error(SUNSHAPE_E_CUDA, "the paged error word is unavailable on this device.");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (pages->dtype == SUNSHAPE_BF16) launch<__nv_bfloat16>(p, codec->block_dim, st);
-  else launch<__half>(p, codec->block_dim, st);
-  return launch_status("paged append launch");
+  return pages->dtype == SUNSHAPE_BF16 ? launch<__nv_bfloat16>(p, codec->block_dim, st) : launch<__half>(p, codec->block_dim, st);
 }
 
 }  // extern "C"

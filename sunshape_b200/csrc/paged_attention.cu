@@ -186,10 +186,8 @@ int sunshape_paged_attention(const sunshape_codec_t* codec, const void* tables, 
     p.prefix_parts = 1;
     p.overlap = tensor;                // else both use the same slots of the workspace
   }
-  if (int rc = bf16 ? launch<__nv_bfloat16, false>(p, vmap, d, dv, bd, grid, st)
-                    : launch<__half, false>(p, vmap, d, dv, bd, grid, st))
-    return rc;
-  return launch_status("paged attention launch");
+  return bf16 ? launch<__nv_bfloat16, false>(p, vmap, d, dv, bd, grid, st)
+              : launch<__half, false>(p, vmap, d, dv, bd, grid, st);
 }
 
 }  // extern "C"

@@ -764,13 +764,14 @@ int launch_paged_attention(const AttnParams& p, const CUtensorMap& vmap, int gri
   cfg.blockDim = dim3(kAttnThreads);
   cfg.dynamicSmemBytes = p.smem;
   cfg.stream = st;
-  cudaLaunchKernelEx(&cfg, k, p, vmap);
+  // a kernel of this call reads what the one before it wrote: none follows one that was refused
+  if (cudaLaunchKernelEx(&cfg, k, p, vmap) != cudaSuccess) return launch_status("paged attention launch");
   // the join may be scheduled while the main grid drains; it waits for its end before it reads
   cfg.gridDim = dim3(grid, p.item_rows);
   cfg.blockDim = dim3(kJoinParts * DV / 4);
   cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, paged_attention_join<DV, T>, p);
+  if (cudaLaunchKernelEx(&cfg, paged_attention_join<DV, T>, p) != cudaSuccess) return launch_status("paged attention join launch");
   return SUNSHAPE_OK;
 }
 

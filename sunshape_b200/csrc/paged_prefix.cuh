@@ -634,6 +634,7 @@ int launch_paged_prefix(const AttnParams& p, const CUtensorMap& vmap, int grid, 
   if (!ready_kernel((const void*)k, smem, kPfLaunchRegs, done))
     return set_last_error(SUNSHAPE_E_CUDA, "the paged prefix kernel is not available as it was built.");
   k<<<grid, kPfThreads, smem, st>>>(p, vmap);
+  if (int rc = launch_status("paged prefix launch")) return rc;
   cudaLaunchConfig_t cfg{};
   const int64_t rows = (int64_t)p.B * p.G * p.L;
   cfg.gridDim = dim3((unsigned)((rows + kPfRows - 1) / kPfRows * p.H), kPfRows / kPfJoinRows);
@@ -644,7 +645,7 @@ int launch_paged_prefix(const AttnParams& p, const CUtensorMap& vmap, int grid, 
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, paged_prefix_join<DV>, p, grid);
+  if (cudaLaunchKernelEx(&cfg, paged_prefix_join<DV>, p, grid) != cudaSuccess) return launch_status("paged prefix join launch");
   return SUNSHAPE_OK;
 }
 

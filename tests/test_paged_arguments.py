@@ -1,4 +1,7 @@
 """Arguments of the paged-serving entry points that would fault on the device, refused before any launch (no GPU)."""
+import os
+import re
+
 from sunshape_b200 import _lib
 
 
@@ -31,3 +34,15 @@ def test_rotation_table_without_rows():
     _expect(lib.sunshape_paged_append(cd, 256, pg, _rows(), _rows(), 1, 1, 16, 1, 1, rot, None), -1, "table has no rows")
     # nothing to rotate: nothing is read
     assert lib.sunshape_norm_rotate(_rows(), _rows(), None, None, None, None, _lib.BF16, _lib.BF16, 0, 1, 64, 1e-6, rot, None) == 0
+
+
+def test_no_launch_status_is_dropped():
+    """A kernel that reads what another one wrote must not be launched where that one was refused: each launch of the paged
+    entry points is checked before the next."""
+    csrc = os.path.join(os.path.dirname(_lib.LIB_PATH), "csrc")
+    for name in ("paged_append.cu", "paged_attention.cu", "paged_attention_kernel.cuh", "paged_prefix.cuh"):
+        with open(os.path.join(csrc, name)) as f:
+            text = f.read()
+        assert not re.findall(r"^\s*(?:cudaLaunchKernelEx|ready_kernel|launch<.*>)\(.*", text, re.M), name
+        after = re.findall(r"<<<[^;]*;\s*(.*)", text)
+        assert all("launch_status" in line or line.startswith("SUNSHAPE_TABLES_CASE") for line in after), (name, after)
