@@ -305,7 +305,8 @@ int sunshape_paged_attention(const sunshape_codec_t* codec, const void* tables, 
 
 /* First code recorded on the current device by the kernels above since the last clear: 0 none, 131 position
  * out of the table, 132 slot out of the pool, 133 page out of the pool, 134 sequence longer than its page
- * table, 135 a bounded pipeline wait gave up.  Waits for the device's queued work. */
+ * table, 135 a bounded pipeline wait gave up.  Waits for the work that is queued on any of the
+ * device's streams. */
 int sunshape_paged_error(int32_t* code, int32_t clear);
 
 /* Size of the scratch array built into the library for sunshape_decode_attention_noalloc. */

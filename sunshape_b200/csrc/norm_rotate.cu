@@ -346,9 +346,12 @@ extern "C" {
 int sunshape_paged_error(int32_t* code, int32_t clear) {
   if (!code) return set_last_error(SUNSHAPE_E_INVALID, "code pointer is NULL.");
   int* w = paged_error_word();
-  if (!w || cudaMemcpy(code, w, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess)
+  // the copy alone would not wait for streams that do not block the default one
+  if (!w || cudaDeviceSynchronize() != cudaSuccess || cudaMemcpy(code, w, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess)
     return set_last_error(SUNSHAPE_E_CUDA, "reading the paged error word failed.");
-  if (clear && cudaMemset(w, 0, sizeof(int)) != cudaSuccess)
+  // A word that holds a code takes no other one, so a clear loses none; one that holds none is not cleared, and a
+  // clear is done before the call returns.
+  if (clear && *code && (cudaMemset(w, 0, sizeof(int)) != cudaSuccess || cudaStreamSynchronize(nullptr) != cudaSuccess))
     return set_last_error(SUNSHAPE_E_CUDA, "clearing the paged error word failed.");
   return SUNSHAPE_OK;
 }

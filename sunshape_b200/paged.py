@@ -35,7 +35,8 @@ _ERRORS = {131: "a position is outside the cosine/sine table", 132: "a slot is o
 
 
 def paged_error(device: torch.device | str | None = None, clear: bool = True) -> str | None:
-    """What the paged kernels recorded on ``device`` since the last clear (None: nothing).  Waits for the device."""
+    """What the paged kernels recorded on ``device`` since the last clear (None: nothing).  Waits for all of the
+    device's streams; not to be called while one is captured."""
     code = ctypes.c_int32(0)
     dev = torch.device("cuda" if device is None else device)
     with torch.cuda.device(dev):
