@@ -303,13 +303,14 @@ class SunShapePagedCache:
 
     def slots(self, page_table: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
         """Slots [B, L] of the token positions [B, L] (within their sequences) under ``page_table`` [B, cols]; -1
-        where a position is negative, a slot outside the pool (which ``append_paged`` records) beyond the table."""
+        where a position is negative, a slot outside the pool (which ``append_paged`` records) beyond the table and where
+        the table names no page."""
         cols, outside = page_table.shape[1], self.num_pages * self.page_size
         p = positions.long()
         s = p.new_full(p.shape, outside)
         if cols:
             page = page_table.long().gather(1, (p // self.page_size).clamp(0, cols - 1))
-            s = torch.where(p < cols * self.page_size, page * self.page_size + p % self.page_size, s)
+            s = torch.where((p < cols * self.page_size) & (page >= 0), page * self.page_size + p % self.page_size, s)
         return torch.where(p >= 0, s, -1)
 
     def append(self, key, value, slots, **rotation) -> None:

@@ -90,3 +90,12 @@ def test_another_shape_waits_for_the_next_call(codec):
     codec.centroids = torch.zeros(2, 8, 300, 8)
     codec.invalidate()
     assert codec.log == []
+
+
+def test_slots_of_table_entries_that_name_no_page():
+    """An entry of -1 (no page yet) is no padding, not even in a page's last row, where it would come out as -1."""
+    cache = object.__new__(paged.SunShapePagedCache)
+    cache.indices = torch.zeros(4, 1, 16, 8)
+    table = torch.tensor([[2, -1], [-3, 3]], dtype=torch.int32)
+    got = cache.slots(table, torch.tensor([[15, 16, 31, -1], [0, 15, 31, 47]]))
+    assert got.tolist() == [[47, 64, 64, -1], [64, 64, 63, 64]]
