@@ -15,7 +15,7 @@ only (bf16, f16); ``norm_rotate`` also takes fp32.  Every call runs on the curre
 takes no workspace that outlives it and can be captured into a CUDA graph; tensors used on another stream than
 the one they were made on need the usual ``record_stream``.  What only the device can see is checked there: a
 position, slot, page or length out of range is skipped (or makes the row NaN) and recorded, see ``paged_error``.
-Nothing here is differentiable.
+Nothing here is differentiable: inputs that require gradients are refused where gradients are recorded.
 """
 from __future__ import annotations
 
@@ -68,6 +68,14 @@ def _device(first: torch.Tensor, *others: torch.Tensor | None) -> int:
     return dev
 
 
+def _forward_only(*tensors: torch.Tensor | None) -> None:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("the paged calls have no backward pass: call them under torch.no_grad() or "
+                                   "torch.inference_mode(), or detach their inputs.")
+
+
 def _unit(t: torch.Tensor, what: str) -> torch.Tensor:
     if t.stride(-1) != 1 and t.shape[-1] != 1:
         raise RuntimeError(f"{what}: the last axis must have unit stride.")
@@ -115,6 +123,7 @@ def norm_rotate(query: torch.Tensor, key: torch.Tensor | None = None, *, q_weigh
     ``x * w / sqrt(mean(x^2) + eps)``.  ``cos``/``sin`` [n_positions, R / 2] fp32 and ``positions`` [B, L] (int32 or
     int64; [L] broadcasts) rotate the first R <= D elements: pairs (i, i + R/2), or (2i, 2i + 1) if
     ``interleaved``.  fp32 arithmetic, one rounding to the inputs' dtype.  ``out`` may be the inputs themselves."""
+    _forward_only(query, key, q_weight, k_weight)
     dev = _device(query, key, q_weight, k_weight)
     code = _CODES.get(query.dtype)
     if query.ndim != 4 or (key is not None and key.ndim != 4):
@@ -331,6 +340,7 @@ def append_paged(cache: SunShapePagedCache, key: torch.Tensor, value: torch.Tens
     ragged batch [N, kv_heads, D] is ``key.transpose(0, 1).unsqueeze(0)`` with slots [1, N].  Slots of one call
     must be distinct.  The codeword is the nearest to the rotated key in real arithmetic (decided in 64 bits
     where fp32 cannot tell; lowest index on ties), without rounding the rotated key in between."""
+    _forward_only(key, value)
     codec = cache.codec
     dev = _device(key, value, slots)
     if dev != cache._index:
@@ -372,6 +382,7 @@ def paged_attention(cache: SunShapePagedCache, query: torch.Tensor, page_table: 
     Softmax statistics and sums are fp32.  Codewords are read as fp16 and softmax weights rounded to the cache's
     dtype before they multiply values; queries are scaled by powers of two into fp16's range.  Dense key blocks
     must stay below 65504 times the largest codeword's norm."""
+    _forward_only(query)
     codec, pages = cache.codec, cache._pages
     dev = _device(query, page_table, seq_lens, prefix_table)
     if dev != cache._index:

@@ -2,7 +2,10 @@
 import os
 import re
 
-from sunshape_b200 import _lib
+import pytest
+import torch
+
+from sunshape_b200 import _lib, paged
 
 
 def _expect(rc, code, text):
@@ -46,3 +49,17 @@ def test_no_launch_status_is_dropped():
         assert not re.findall(r"^\s*(?:cudaLaunchKernelEx|ready_kernel|launch<.*>)\(.*", text, re.M), name
         after = re.findall(r"<<<[^;]*;\s*(.*)", text)
         assert all("launch_status" in line or line.startswith("SUNSHAPE_TABLES_CASE") for line in after), (name, after)
+
+
+def test_gradients_are_not_dropped_silently():
+    """No paged call has a backward pass: an input that wants gradients is refused where they are recorded."""
+    x, w = torch.zeros(1, 2, 1, 64), torch.ones(64)
+    cases = [lambda g: paged.norm_rotate(g(x)), lambda g: paged.norm_rotate(x, g(x)), lambda g: paged.norm_rotate(x, q_weight=g(w)),
+             lambda g: paged.norm_rotate(x, x, k_weight=g(w)), lambda g: paged.append_paged(None, g(x), x, None),
+             lambda g: paged.append_paged(None, x, g(x), None), lambda g: paged.paged_attention(None, g(x), None, None)]
+    for call in cases:
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            call(lambda t: t.clone().requires_grad_())
+        with torch.no_grad(), pytest.raises(Exception) as other:      # CPU tensors, or no cache
+            call(lambda t: t.clone().requires_grad_())
+        assert "no backward pass" not in str(other.value)
