@@ -12,7 +12,7 @@
 //   * eight warps a row group, two threads a row with 64 columns each: scores from tensor memory, weights in powers of
 //     two against a maximum that may fall behind by 2^kSlack (then, and only then, O is rescaled in place), P as 16-bit
 //     pairs over S.  One thread a row takes about 2150 cycles a tile, during which its group's next products wait.
-// Bound: 2 (D + DV) 256 multiply-adds a token and head against one exponential for each row: at D = DV = 128 the tensor
+// Bound: (D + DV) 256 multiply-adds a token and head against one exponential for each row: at D = DV = 128 the tensor
 // cores and the special function units both need 2048 cycles a tile of 256 rows, so the two groups' phases must overlap.
 // Measured on B200: 512 rows of 8 heads over 32768 tokens (69 GFLOP): 2.5 us a tile of 256 rows, 88 us the kernel with 12 us
 // of start and 5 us of results; the whole call, with the sequences' own 180k tokens, 139 us (memory-bound kernel alone: 477).

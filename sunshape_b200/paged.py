@@ -380,8 +380,9 @@ def paged_attention(cache: SunShapePagedCache, query: torch.Tensor, page_table: 
     must be contiguous and begin at a multiple of 8 bytes.
 
     Softmax statistics and sums are fp32.  Codewords are read as fp16 and softmax weights rounded to the cache's
-    dtype before they multiply values; queries are scaled by powers of two into fp16's range.  Dense key blocks
-    must stay below 65504 times the largest codeword's norm."""
+    dtype before they multiply values; a codebook and a query row are each scaled by a power of two into fp16's range, and
+    what is below 2^-25 of their largest is read as zero.  Dense key blocks must stay below 65504 times the largest
+    codeword's norm."""
     _forward_only(query)
     codec, pages = cache.codec, cache._pages
     dev = _device(query, page_table, seq_lens, prefix_table)

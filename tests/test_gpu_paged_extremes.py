@@ -1,0 +1,149 @@
+"""Paged attention where numbers are large, small, unequal or none at all; both attention kernels."""
+import pytest
+import torch
+
+from sunshape_b200 import paged
+from sunshape_b200.codec import SunShapeBlockCodec
+from sunshape_b200.paged import SunShapePagedCache
+from tests.paged_bounds import attention_bounds
+from tests.paged_reference import make_paged_codec
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16, F16 = torch.bfloat16, torch.float16
+
+
+@pytest.fixture(autouse=True)
+def no_error_left():
+    paged.paged_error(DEV)
+    yield
+    assert paged.paged_error(DEV) is None
+
+
+def _randn(*shape, seed, dtype=torch.float32):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(DEV, dtype)
+
+
+def _cache(codec, H, lens, prefix, page, dtype, seed=0):
+    """A cache with a page table for ``lens``, a prefix, and a page more than both."""
+    cols, first = max(1, -(-max(lens) // page)), -(-prefix // page)
+    pages = len(lens) * cols + first + 1
+    cache = SunShapePagedCache.allocate(codec, pages, H, page_size=page, dtype=dtype)
+    g = torch.Generator().manual_seed(seed)
+    cache.indices.copy_(torch.randint(0, codec.n_centroids, cache.indices.shape, generator=g))
+    cache.values.copy_(_randn(*cache.values.shape, seed=seed + 1))
+    if cache.heavy is not None:
+        cache.heavy.copy_(_randn(*cache.heavy.shape, seed=seed + 2))
+    order = torch.randperm(pages, generator=g).to(DEV, torch.int32)
+    table = order[first:first + len(lens) * cols].view(len(lens), cols).contiguous()
+    return cache, table, torch.tensor(lens, dtype=torch.int32, device=DEV), order[:first].contiguous()
+
+
+def _near(got, cache, q, table, n, pt=None, prefix=0, rows=None, **kw):
+    ref, bound, worst = attention_bounds(cache, q, table, n, pt, prefix, **kw)
+    bad = ~((got.double().cpu() - ref).abs() <= bound)
+    if rows is not None:
+        bad = bad & rows[:, :, None, None]
+    assert not bool(bad.any())
+    return worst
+
+
+# rows of a KV head: 8 go to the memory-bound kernel, 24 and more to the tensor-core one (one and two groups of 128 rows,
+# the second one not full; more than 256)
+ROWS = [(1, 8), (3, 8), (20, 8), (33, 8)]
+
+
+@pytest.mark.parametrize("B,G", ROWS)
+@pytest.mark.parametrize("value", ["pool", -1, 2 ** 31 - 1])
+def test_bad_prefix_page(B, G, value):
+    codec, _ = make_paged_codec(64, 8, 2, seed=1)
+    cache, table, n, pt = _cache(codec, 2, [5] * B, 600, 16, BF16)
+    q = _randn(B, 2 * G, 1, 64, seed=3, dtype=BF16)
+    bad = pt.clone()
+    bad[20] = cache.num_pages if value == "pool" else value
+    got = cache.attention(q, table, n, prefix_table=bad, prefix_len=600)
+    assert "page number" in paged.paged_error(DEV) and bool(got.isnan().all())
+    _near(cache.attention(q, table, n, prefix_table=pt, prefix_len=600), cache, q, table, n, pt, 600)
+    # entries behind the prefix's end are not read
+    bad = torch.cat((pt, torch.full((3,), -7, dtype=torch.int32, device=DEV)))
+    _near(cache.attention(q, table, n, prefix_table=bad, prefix_len=600), cache, q, table, n, pt, 600)
+
+
+@pytest.mark.parametrize("B,G", ROWS)
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_queries_of_every_kind_behind_a_prefix(B, G, dtype):
+    """Zero, tiny, huge, infinite and NaN queries: each row is its own affair."""
+    codec, _ = make_paged_codec(64, 8, 2, heavy=2, seed=2)
+    cache, table, n, pt = _cache(codec, 2, [5, 0, 17] * (B // 3) + [1] * (B % 3), 300, 16, dtype)
+    q = _randn(B, 2 * G, 1, 64, seed=3, dtype=dtype)
+    q[0, 0] = 0
+    q[0, 1] *= 1e-4 if dtype == F16 else 1e-30
+    q[-1, 2] *= 1e3 if dtype == F16 else 1e30
+    q[-1, 3, 0, 5] = float("nan")
+    q[0, 4, 0, 7] = float("inf")
+    got = cache.attention(q, table, n, prefix_table=pt, prefix_len=300)
+    rows = torch.ones(B, 2 * G, dtype=torch.bool)
+    rows[-1, 2] = rows[-1, 3] = rows[0, 4] = False
+    _near(got, cache, q.nan_to_num(0, 0, 0), table, n, pt, 300, rows=rows)
+    assert bool(got[-1, 3].isnan().all()) and bool(got[-1, 2].isfinite().all())
+
+
+@pytest.mark.parametrize("B,G", ROWS)
+@pytest.mark.parametrize("scale", [0.0, -0.7, 3.0])
+def test_scales_behind_a_prefix(B, G, scale):
+    codec, _ = make_paged_codec(64, 8, 2, seed=4)
+    cache, table, n, pt = _cache(codec, 2, [5] * B, 300, 16, BF16)
+    q = (0.1 * _randn(B, 2 * G, 1, 64, seed=3)).to(BF16)
+    got = cache.attention(q, table, n, prefix_table=pt, prefix_len=300, scale=scale)
+    _near(got, cache, q, table, n, pt, 300, scale=scale)
+
+
+def _ramp(H, dtype, pages, page):
+    """A codec whose key is one number, its codeword's index / 4, and a cache of them."""
+    codec = SunShapeBlockCodec(64, 8, 256, device=torch.device(DEV), kv_heads=H)
+    codec.centroids.zero_()
+    codec.centroids[:, 0, :, 0] = torch.arange(256, device=DEV) / 4
+    codec.invalidate()
+    cache = SunShapePagedCache.allocate(codec, pages, H, page_size=page, dtype=dtype)
+    cache.values.copy_(_randn(*cache.values.shape, seed=1))
+    return cache
+
+
+@pytest.mark.parametrize("B,G", ROWS)
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("order", ["up", "down", "steps", "last"])
+def test_maximum_that_moves(B, G, dtype, order):
+    """Scores that grow by more than the slack from tile to tile, fall, jump, or have one large one at the very end; some
+    rows see the opposite."""
+    T, page = 1500, 32
+    cache = _ramp(1, dtype, -(-T // page) + B, page)
+    t = torch.arange(T)
+    level = {"up": t * 255 // (T - 1), "down": 255 - t * 255 // (T - 1), "steps": (t // 128 * 37) % 256, "last": t // (T - 1) * 255}[order]
+    first = -(-T // page)
+    cache.indices[:first, 0, :, 0].view(-1)[:T] = level.to(DEV, torch.uint8)
+    pt = torch.arange(first, dtype=torch.int32, device=DEV)
+    table = first + torch.arange(B, dtype=torch.int32, device=DEV)[:, None]
+    n = torch.full((B,), 3, dtype=torch.int32, device=DEV)
+    q = torch.zeros(B, G, 1, 64, dtype=dtype, device=DEV)
+    q[..., 0] = torch.tensor([1.0, -1.0, 4.0, -4.0, 0.25, 0.0, 2.0, -0.5], device=DEV)[:G, None].to(dtype)
+    got = cache.attention(q, table, n, prefix_table=pt, prefix_len=T, scale=1.0)
+    _near(got, cache, q, table, n, pt, T, scale=1.0, exact_scores=True)
+
+
+@pytest.mark.parametrize("B,G", ROWS)
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_blocks_far_smaller_than_the_largest(B, G, dtype):
+    """Blocks at 1e-5 and 1e-8 of the codebook's largest codewords, and queries that look at these blocks alone."""
+    codec, _ = make_paged_codec(64, 8, 2, seed=5)
+    codec.centroids[:, 1] *= 1e-5
+    codec.centroids[:, 2] *= 1e-8
+    codec.invalidate()
+    cache, table, n, pt = _cache(codec, 2, [40] * B, 300, 16, dtype)
+    looks = torch.zeros(4, 64, device=DEV)
+    for i, blocks in enumerate(([1], [2], [1, 2], [0, 1, 2, 3, 4, 5, 6, 7])):
+        for b in blocks:
+            looks[i, codec.permutation[8 * b:8 * b + 8]] = 4e3 if len(blocks) < 8 else 1.0
+    q = (_randn(B, 2 * G, 1, 64, seed=3) * looks[torch.arange(2 * G, device=DEV) % 4, None]).to(dtype)
+    got = cache.attention(q, table, n, prefix_table=pt, prefix_len=300)
+    worst = _near(got, cache, q, table, n, pt, 300)
+    assert worst < 0.3                                                   # the bound says something
