@@ -273,7 +273,7 @@ int sunshape_paged_tables(const sunshape_codec_t* codec, void* tables, int64_t t
  * [batch, length] (int64; -1 = leave the row out): the key is rotated (rotation NULL: taken as it is),
  * permuted and encoded to the nearest codeword of every block -- exactly: the first minimum of the distances
  * in real arithmetic as 64-bit floats give it, of the rotated key without an intermediate rounding -- or
- * kept, rounded to dtype, where the block is dense (index 0); the value is copied.  Slots must be distinct:
+ * kept, rounded to fp32 and then to dtype, where the block is dense (index 0); the value is copied.  Slots must be distinct:
  * of two rows for one slot either may stay.  A slot outside [-1, num_pages * page_size) is left out and
  * records 132. */
 int sunshape_paged_append(const sunshape_codec_t* codec, const void* tables, const sunshape_pages_t* pages,

@@ -105,7 +105,8 @@ __device__ __forceinline__ void mma_k8(float* d, uint32_t a0, uint32_t a1, uint3
       : "r"(a0), "r"(a1), "r"(b0));
 }
 
-// Whether a result of rotate32, off by two units of its last place, may round to T otherwise than the exact one: it
+// Whether a result of rotate32, off by two units of its last place, may round to T otherwise than the exact one, itself
+// rounded to fp32 first (as torch rounds 64 bits to 16): it
 // lies near the middle of two neighbours, is below f16's normal range, or so much smaller than the key's largest element
 // that the second product's error counts.
 template <typename T>
