@@ -115,9 +115,15 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   return r;
 }
 
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<uint64_t&>(r)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+  return r;
+}
+
 __device__ __forceinline__ void tm_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// 64 scores of a row to weights 2^((s - mb) f), as 16-bit pairs, with their sum and the largest score.  Scores from
+// 64 scores of a row to weights 2^((s - mb) f + kShift), as 16-bit pairs, with their sum and the largest score.  Scores from
 // `valid` on are left out.
 template <typename T, bool TAIL>
 __device__ __forceinline__ void tile_weights(uint32_t s_t, int valid, float mb, float f, uint32_t* pk, float& top, float& sum) {
@@ -142,7 +148,10 @@ __device__ __forceinline__ void tile_weights(uint32_t s_t, int valid, float mb, 
     }
 #pragma unroll
     for (int e = 0; e < 32; e += 2) {
-      const float2 y = mul2(add2(make_float2(v[e], v[e + 1]), nb), ff);
+      const float2 d = add2(make_float2(v[e], v[e + 1]), nb);
+      float2 y;
+      if constexpr (kShift<T> != 0.f) y = fma2(d, ff, make_float2(kShift<T>, kShift<T>));
+      else y = mul2(d, ff);
       float2 w = make_float2(fast_exp2(y.x), fast_exp2(y.y));
       if constexpr (TAIL) {             // -inf times a factor of zero
         w.x = c * 32 + e < valid ? w.x : 0.f;
@@ -586,7 +595,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
               *reinterpret_cast<float4*>(dst + half * (DV / 2) + c * 32 + x) = make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]);
           }
         }
-        if (dst && half == 0) *reinterpret_cast<float2*>(dst + DV) = make_float2(m == -INF ? -INF : m * f, l);
+        if (dst && half == 0) *reinterpret_cast<float2*>(dst + DV) = make_float2(m == -INF ? -INF : m * f - kShift<T>, l);
         pf_fence_before();
       }
       end_piece();

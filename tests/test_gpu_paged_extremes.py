@@ -147,3 +147,26 @@ def test_blocks_far_smaller_than_the_largest(B, G, dtype):
     got = cache.attention(q, table, n, prefix_table=pt, prefix_len=300)
     worst = _near(got, cache, q, table, n, pt, 300)
     assert worst < 0.3                                                   # the bound says something
+
+
+@pytest.mark.parametrize("B,G,prefix", [(1200, 1, False), (296, 128, True)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_many_small_weights_beside_a_large_one(B, G, prefix, dtype):
+    """20000 tokens whose weights are 2^-25.5 of the first one's and that carry the result.  All sequences read the same
+    pages, and are so many that a warp or thread block walks a whole one beside that first maximum."""
+    T, page = 20000, 128
+    first = -(-T // page)
+    cache = _ramp(1, dtype, first, page)
+    cache.values.fill_(1)
+    cache.values[0, :, 0] = 0
+    cache.indices[0, 0, 0, 0] = 68                                       # key 17, the others 0
+    pages = torch.arange(first, dtype=torch.int32, device=DEV)
+    q = torch.zeros(B, G, 1, 64, dtype=dtype, device=DEV)
+    q[..., 0] = 1
+    scale = 25.5 * 0.6931471805599453 / 17
+    own = torch.full((B,), 0 if prefix else T, dtype=torch.int32, device=DEV)
+    got = cache.attention(q, pages.expand(B, -1), own, prefix_table=pages if prefix else None, prefix_len=T if prefix else 0,
+                          scale=scale)
+    ref, bound, _ = attention_bounds(cache, q[:1, :1], pages[None], [T], scale=scale, exact_scores=True)
+    # the scores' fp32 roundings: 2^-23 of 17.7 each
+    assert bool(((got.double().cpu() - ref).abs() <= bound + 2.0 ** -18 * ref.abs()).all())
