@@ -291,7 +291,9 @@ int sunshape_paged_append(const sunshape_codec_t* codec, const void* tables, con
  * query_len - 1 - l of the sequence's own tokens (and all of the prefix); causal = 0: all of them.  A row
  * that sees no token is zero.  Softmax of scale * <q, k_hat>, statistics and sums in fp32.
  * head_dim and value_dim 64 or 128; block_dim 2, 4 or 8.  A page outside the pool records 133 and a length
- * outside [0, table_cols * page_size] 134; both make the sequence's rows NaN.
+ * outside [0, table_cols * page_size] 134; both make the sequence's rows NaN.  Dense key blocks are read as fp16 in the
+ * scale of the codebook: one of 65504 times the largest codeword's norm or more records 136 and makes the rows NaN that
+ * see it.
  * workspace: sunshape_paged_attention_workspace_bytes, 256-byte aligned, needs no initial value and keeps
  * none; calls that overlap need separate ones. */
 int64_t sunshape_paged_attention_workspace_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t query_len,
@@ -305,7 +307,7 @@ int sunshape_paged_attention(const sunshape_codec_t* codec, const void* tables, 
 
 /* First code recorded on the current device by the kernels above since the last clear: 0 none, 131 position
  * out of the table, 132 slot out of the pool, 133 page out of the pool, 134 sequence longer than its page
- * table, 135 a bounded pipeline wait gave up.  Waits for the work that is queued on any of the
+ * table, 135 a bounded pipeline wait gave up, 136 a dense key block beyond fp16.  Waits for the work that is queued on any of the
  * device's streams. */
 int sunshape_paged_error(int32_t* code, int32_t clear);
 

@@ -8,7 +8,7 @@
 
 namespace sunshape {
 
-enum PagedError { kErrPosition = 131, kErrSlot = 132, kErrPage = 133, kErrLength = 134, kErrWait = 135 };
+enum PagedError { kErrPosition = 131, kErrSlot = 132, kErrPage = 133, kErrLength = 134, kErrWait = 135, kErrDense = 136 };
 
 // device address of the paged kernels' error word on the current device (null with a CUDA error set)
 int* paged_error_word();

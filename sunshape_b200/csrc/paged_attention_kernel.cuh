@@ -95,9 +95,10 @@ __device__ __forceinline__ void unrolled(F&& f) {
   unrolled(std::make_integer_sequence<int, N>(), f);
 }
 
-// dense block words (two 16-bit elements each) into the codebook's fp16 scale
+// Dense block words (two 16-bit elements each) into the codebook's fp16 scale; `most`: the largest element so far, NaN left
+// out.  fp16 ends at 65504 where bf16 and scaled f16 numbers go on: see beyond_fp16.
 template <typename T>
-__device__ __forceinline__ uint32_t dense_word(uint32_t w, float s) {
+__device__ __forceinline__ uint32_t dense_word(uint32_t w, float s, float& most) {
   float lo, hi;
   if constexpr (std::is_same<T, __half>::value) {
     const __half2 v = *reinterpret_cast<const __half2*>(&w);
@@ -107,8 +108,15 @@ __device__ __forceinline__ uint32_t dense_word(uint32_t w, float s) {
     lo = __uint_as_float(w << 16);
     hi = __uint_as_float(w & 0xffff0000u);
   }
-  return pack2<__half>(lo * s, hi * s);
+  lo *= s;
+  hi *= s;
+  most = fmaxf(most, fmaxf(fabsf(lo), fabsf(hi)));
+  return pack2<__half>(lo, hi);
 }
+// Whether a number that is none of fp16's and rounds to infinity is the largest.  Such a token's key is made NaN: infinities
+// would turn into a plausible result where their products have one sign.  An infinite key is taken as it is.
+__device__ __forceinline__ bool beyond_fp16(float most) { return most >= 65520.f && most < __int_as_float(0x7f800000); }
+constexpr uint32_t kNanWord = 0x7fff7fffu;     // two fp16 NaN
 
 // A running maximum may fall behind by a factor of 2^kSlack before sums and accumulators are rescaled to a new one;
 // weights stay below 2^kSlack, in reach of every type.
@@ -485,14 +493,19 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                 for (int x = 0; x < ROT * WORDS; ++x) kw[y][u0 * WORDS + x] = tmp[x];
               }
             if (p.n_heavy) {                       // dense blocks take the place of their codeword 0
+              float most = 0.f;
 #pragma unroll
               for (int u = 0; u < UNITS; ++u)
                 if ((hmask >> u) & 1) {
                   uint32_t* dst = kw[y] + u * WORDS;
                   lds_words<2 * BD, 0>(dst, st_a + p.off_heavy + (tok * p.n_heavy + hslot_s[4 * u + t]) * (2 * BD));
 #pragma unroll
-                  for (int x = 0; x < WORDS; ++x) dst[x] = dense_word<T>(dst[x], k_scale);
+                  for (int x = 0; x < WORDS; ++x) dst[x] = dense_word<T>(dst[x], k_scale, most);
                 }
+              if (beyond_fp16(most)) {
+                kw[y][0] = kNanWord;
+                if (first + tok < w.len) record_error(p.err, kErrDense);
+              }
             }
           }
 #pragma unroll

@@ -437,13 +437,14 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         }
         if (p.n_heavy && row >= 0) {             // dense blocks take the place of their codeword 0
           const T* dense = reinterpret_cast<const T*>(p.heavy) + row * p.n_heavy * BD;
+          float most = 0.f;
           if constexpr (BD == 8) {
 #pragma unroll
             for (int x = 0; x < NB; ++x) {
               if (x >= p.n_heavy) break;
               uint4 w = x < AHEAD ? dense_ahead[x < AHEAD ? x : 0] : reinterpret_cast<const uint4*>(dense)[x];
-              w = make_uint4(dense_word<T>(w.x, k_scale), dense_word<T>(w.y, k_scale), dense_word<T>(w.z, k_scale),
-                             dense_word<T>(w.w, k_scale));
+              w = make_uint4(dense_word<T>(w.x, k_scale, most), dense_word<T>(w.y, k_scale, most),
+                             dense_word<T>(w.z, k_scale, most), dense_word<T>(w.w, k_scale, most));
               const int b = hblock_s[x];
               *reinterpret_cast<uint4*>(dst + (b >> 3) * HALF + (((b & 7) ^ (tok_l & 7)) << 4)) = w;
             }
@@ -454,11 +455,15 @@ __global__ void __launch_bounds__(kPfThreads, 1)
             if (at_b < 0) continue;
             uint32_t w[WORDS];
 #pragma unroll
-            for (int x = 0; x < WORDS; ++x) w[x] = dense_word<T>(reinterpret_cast<const uint32_t*>(dense + at_b * BD)[x], k_scale);
+            for (int x = 0; x < WORDS; ++x) w[x] = dense_word<T>(reinterpret_cast<const uint32_t*>(dense + at_b * BD)[x], k_scale, most);
             const int byte = b * BD * 2, j = (byte >> 4) & 7;
             uint8_t* to = dst + (byte >> 7) * HALF + ((j ^ (tok_l & 7)) << 4) + (byte & 15);
 #pragma unroll
             for (int x = 0; x < WORDS; ++x) reinterpret_cast<uint32_t*>(to)[x] = w[x];
+          }
+          if (beyond_fp16(most)) {
+            *reinterpret_cast<uint32_t*>(dst + ((tok_l & 7) << 4)) = kNanWord;      // elements 0 and 1
+            record_error(p.err, kErrDense);
           }
         }
         const int first = (t0 + i) * kPfTokens;

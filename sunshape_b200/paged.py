@@ -14,7 +14,8 @@ Counterpart for contiguous caches: ``codec.quantize_packed`` and ``vllm_attn_bac
 only (bf16, f16); ``norm_rotate`` also takes fp32.  Every call runs on the current stream of its tensors' device,
 takes no workspace that outlives it and can be captured into a CUDA graph; tensors used on another stream than
 the one they were made on need the usual ``record_stream``.  What only the device can see is checked there: a
-position, slot, page or length out of range is skipped (or makes the row NaN) and recorded, see ``paged_error``.
+position, slot, page, length or dense key out of range is skipped (or makes the row NaN) and recorded, see
+``paged_error``.
 Nothing here is differentiable: inputs that require gradients are refused where gradients are recorded.
 """
 from __future__ import annotations
@@ -31,7 +32,7 @@ from .codec import SunShapeBlockCodec
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 _ERRORS = {131: "a position is outside the cosine/sine table", 132: "a slot is outside the page pool",
            133: "a page number is outside the page pool", 134: "a sequence is longer than its page table",
-           135: "a pipeline wait gave up"}
+           135: "a pipeline wait gave up", 136: "a dense key block is too large for its codebook's scale in fp16"}
 
 
 def paged_error(device: torch.device | str | None = None, clear: bool = True) -> str | None:
@@ -382,7 +383,7 @@ def paged_attention(cache: SunShapePagedCache, query: torch.Tensor, page_table: 
     Softmax statistics and sums are fp32.  Codewords are read as fp16 and softmax weights rounded to the cache's
     dtype before they multiply values; a codebook and a query row are each scaled by a power of two into fp16's range, and
     what is below 2^-25 of their largest is read as zero.  Dense key blocks must stay below 65504 times the largest
-    codeword's norm."""
+    codeword's norm: a larger one is recorded and makes the rows NaN that see it."""
     _forward_only(query)
     codec, pages = cache.codec, cache._pages
     dev = _device(query, page_table, seq_lens, prefix_table)
