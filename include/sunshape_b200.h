@@ -291,9 +291,9 @@ int sunshape_paged_append(const sunshape_codec_t* codec, const void* tables, con
  * query_len - 1 - l of the sequence's own tokens (and all of the prefix); causal = 0: all of them.  A row
  * that sees no token is zero.  Softmax of scale * <q, k_hat>, statistics and sums in fp32.
  * head_dim and value_dim 64 or 128; block_dim 2, 4 or 8.  A page outside the pool records 133 and a length
- * outside [0, table_cols * page_size] 134; both make the sequence's rows NaN.  Dense key blocks are read as fp16 in the
- * scale of the codebook: one of 65504 times the largest codeword's norm or more records 136 and makes the rows NaN that
- * see it.
+ * outside [0, table_cols * page_size] 134; both make the sequence's rows NaN.  Dense key blocks are read as fp16: a bf16
+ * element of 65504 or more (times the largest codeword's norm, where that is above 1) records 136 and makes the rows NaN
+ * that see it.
  * workspace: sunshape_paged_attention_workspace_bytes, 256-byte aligned, needs no initial value and keeps
  * none; calls that overlap need separate ones. */
 int64_t sunshape_paged_attention_workspace_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t query_len,

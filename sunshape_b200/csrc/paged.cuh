@@ -31,7 +31,8 @@ int check_pages(const sunshape_codec_t* c, const sunshape_pages_t* pg);
 //   image   at 0, [n_cb][ceil(D / 64)][256][64] fp16: codewords times their codebook's image scale; row (i, c) holds codeword
 //           c of the 64 / BD blocks from i * 64 / BD on, so that in shared memory a block's codewords lie in one
 //           column of the banks
-//   iscale  [n_cb]: the image's scale, a power of two that brings the codebook's largest codeword norm into [0.5, 1)
+//   iscale  [n_cb]: the image's scale, a power of two that brings the codebook's largest codeword norm into [0.5, 1), at most 1
+//           where the codec has dense blocks
 //   records [n_cb][nb]: what the encoder reads of a block, one copy each --
 //     frags [32][32][2]: the B operands of the MMAs over 8 codewords, lane by lane
 //     norms [256]: -|c|^2 / 2 in the block's scale, far below all others where there is no codeword

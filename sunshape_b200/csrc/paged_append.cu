@@ -150,8 +150,8 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
 
 // Codebooks into the attention image and the encoder's fragments: a CTA a block, a thread a codeword.
 template <int BD>
-__global__ void __launch_bounds__(256) tables_kernel(const float* cb, const float* norm_max, int C, int nb, int D,
-                                                     uint8_t* out, Tables at) {
+__global__ void __launch_bounds__(256) tables_kernel(const float* cb, const float* norm_max, bool dense, int C, int nb,
+                                                     int D, uint8_t* out, Tables at) {
   __shared__ float red[256];
   __shared__ float v_s[256][BD];
   const int blk = blockIdx.x, k = blockIdx.y, c = threadIdx.x;
@@ -191,7 +191,8 @@ __global__ void __launch_bounds__(256) tables_kernel(const float* cb, const floa
     return ldexpf(1.f, -max(-100, min(100, e)));
   };
   const float bs = factor(sqrtf(most(n)));
-  const float is = factor(norm_max ? norm_max[k] : sqrtf(most(all)));
+  // at most 1 beside dense blocks, which are read in the same scale: all of fp16 stays in reach
+  const float is = fminf(factor(norm_max ? norm_max[k] : sqrtf(most(all))), dense ? 1.f : 2e30f);
   constexpr int PER = 64 / BD;      // blocks of an image row
   __half* image = reinterpret_cast<__half*>(out) +
                   (((int64_t)k * ((D + 63) / 64) + blk / PER) * 256 + c) * 64 + blk % PER * BD;
@@ -620,7 +621,8 @@ int sunshape_paged_tables(const sunshape_codec_t* codec, void* tables, int64_t t
   uint8_t* out = static_cast<uint8_t*>(tables);
 #define SUNSHAPE_TABLES_CASE(BD)                                                                                     \
   if (codec->block_dim == BD)                                                                                        \
-    tables_kernel<BD><<<grid, 256, 0, st>>>(codec->centroids, codec->centroid_norm_max, codec->n_centroids, nb,      \
+    tables_kernel<BD><<<grid, 256, 0, st>>>(codec->centroids, codec->centroid_norm_max,                              \
+                                            codec->heavy_mask && codec->n_heavy > 0, codec->n_centroids, nb,         \
                                             codec->head_dim, out, at);
   SUNSHAPE_TABLES_CASE(2)
   SUNSHAPE_TABLES_CASE(4)

@@ -129,6 +129,16 @@ __device__ __forceinline__ Finish finish_of(const AttnParams& p, int64_t row, fl
   return e;
 }
 
+// Of a row of a codec with dense blocks whose sum is no number: records it, unless that is the query's doing.
+template <int D, typename T>
+__device__ __forceinline__ void report_dense(const AttnParams& p, const RowMap& at) {
+  const T* q = reinterpret_cast<const T*>(p.q) + at.b * p.qs[0] + at.hq * p.qs[1] + at.l * p.qs[2];
+#pragma unroll 1
+  for (int d = 0; d < D; ++d)
+    if (!(fabsf(Elem<T>::to_float(q[d])) < __int_as_float(0x7f800000))) return;
+  record_error(p.err, kErrDense);
+}
+
 // Four columns of a row.
 template <typename T, int DV>
 __device__ __forceinline__ void finish4(const AttnParams& p, const RowMap& at, int d, float m, float l, float4 a) {

@@ -95,28 +95,38 @@ __device__ __forceinline__ void unrolled(F&& f) {
   unrolled(std::make_integer_sequence<int, N>(), f);
 }
 
-// Dense block words (two 16-bit elements each) into the codebook's fp16 scale; `most`: the largest element so far, NaN left
-// out.  fp16 ends at 65504 where bf16 and scaled f16 numbers go on: see beyond_fp16.
+// Dense block words (two 16-bit elements each) into the codebook's fp16 scale, a power of two of at most 1: no number of
+// fp16 grows.  What bf16 has beyond fp16's 65504 becomes NaN, since an infinity would turn into a plausible result where its
+// products have one sign.
 template <typename T>
-__device__ __forceinline__ uint32_t dense_word(uint32_t w, float s, float& most) {
-  float lo, hi;
-  if constexpr (std::is_same<T, __half>::value) {
-    const __half2 v = *reinterpret_cast<const __half2*>(&w);
-    lo = __low2float(v);
-    hi = __high2float(v);
-  } else {
-    lo = __uint_as_float(w << 16);
-    hi = __uint_as_float(w & 0xffff0000u);
+struct DenseScale {
+  uint64_t s;
+  __device__ __forceinline__ explicit DenseScale(float v) {
+    const float2 two = make_float2(v, v);
+    s = reinterpret_cast<const uint64_t&>(two);
   }
-  lo *= s;
-  hi *= s;
-  most = fmaxf(most, fmaxf(fabsf(lo), fabsf(hi)));
-  return pack2<__half>(lo, hi);
-}
-// Whether a number that is none of fp16's and rounds to infinity is the largest.  Such a token's key is made NaN: infinities
-// would turn into a plausible result where their products have one sign.  An infinite key is taken as it is.
-__device__ __forceinline__ bool beyond_fp16(float most) { return most >= 65520.f && most < __int_as_float(0x7f800000); }
-constexpr uint32_t kNanWord = 0x7fff7fffu;     // two fp16 NaN
+  __device__ __forceinline__ uint32_t operator()(uint32_t w) const {
+    float2 v = make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(reinterpret_cast<uint64_t&>(v)) : "l"(s));
+    uint32_t r = pack2<__half>(v.x, v.y);
+    asm("fma.rn.f16x2 %0, %0, %1, %0;" : "+r"(r) : "r"(0u));      // x + 0 x
+    return r;
+  }
+};
+template <>
+struct DenseScale<__half> {
+  uint32_t a, b;                               // in two steps, since a scale may be below fp16's numbers
+  __device__ __forceinline__ explicit DenseScale(float v) {
+    const float first = fmaxf(v, 6.103515625e-5f);
+    a = pack2<__half>(first, first);
+    b = pack2<__half>(v / first, v / first);
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t w) const {
+    asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(w) : "r"(a));
+    asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(w) : "r"(b));
+    return w;
+  }
+};
 
 // A running maximum may fall behind by a factor of 2^kSlack before sums and accumulators are rescaled to a new one;
 // weights stay below 2^kSlack, in reach of every type.
@@ -379,6 +389,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       bulk_g2s(image, reinterpret_cast<const uint8_t*>(p.image) + (int64_t)cb * IMAGE, IMAGE, cb_bar);
     }
     const float k_scale = p.image_scale[p.n_cb == 1 ? 0 : (h0 + k) % p.n_cb];
+    const DenseScale<T> dense_scale(k_scale);
     enter(k);
     int4 head = make_int4(w.at < w.end ? 0 : -1, 0, 0, 0), tail = make_int4(0, 0, 0, 0);
     bool waited = false;
@@ -493,19 +504,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                 for (int x = 0; x < ROT * WORDS; ++x) kw[y][u0 * WORDS + x] = tmp[x];
               }
             if (p.n_heavy) {                       // dense blocks take the place of their codeword 0
-              float most = 0.f;
 #pragma unroll
               for (int u = 0; u < UNITS; ++u)
                 if ((hmask >> u) & 1) {
                   uint32_t* dst = kw[y] + u * WORDS;
                   lds_words<2 * BD, 0>(dst, st_a + p.off_heavy + (tok * p.n_heavy + hslot_s[4 * u + t]) * (2 * BD));
 #pragma unroll
-                  for (int x = 0; x < WORDS; ++x) dst[x] = dense_word<T>(dst[x], k_scale, most);
+                  for (int x = 0; x < WORDS; ++x) dst[x] = dense_scale(dst[x]);
                 }
-              if (beyond_fp16(most)) {
-                kw[y][0] = kNanWord;
-                if (first + tok < w.len) record_error(p.err, kErrDense);
-              }
             }
           }
 #pragma unroll
@@ -598,6 +604,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       bad = __any_sync(0xffffffffu, bad);
       const bool begins = w.t == 0, ends = w.t + n == w.tiles;
       if (begins && ends) prefix_written();
+      uint32_t odd = 0;                            // this lane's rows whose sums are no numbers
 #pragma unroll
       for (int c = 0; c < NT; ++c)
 #pragma unroll
@@ -605,8 +612,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 #pragma unroll
           for (int of = 4; of < 32; of <<= 1) l[c][j] += __shfl_xor_sync(0xffffffffu, l[c][j], of);
           if (bad) l[c][j] = __int_as_float(0x7fffffff);
+          else if (l[c][j] != l[c][j]) odd |= 1u << (2 * c + j);
           m[c][j] = m[c][j] == -INF ? -INF : m[c][j] * f[c][j] - kShift<T>;
         }
+      for (odd = p.n_heavy ? odd : 0; odd; odd &= odd - 1) {
+        const int x = __ffs(odd) - 1, r = 8 * (x >> 1) + 2 * t + (x & 1);
+        if (r < nr) report_dense<D, T>(p, row_of(p, w.h, w.b, r0 + r));
+      }
 #pragma unroll
       for (int c = 0; c < NT; ++c)
 #pragma unroll

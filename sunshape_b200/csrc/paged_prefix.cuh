@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       const unsigned ps = (unsigned)p.ps;
       const int l8 = lane & 7, mul = ((l8 << 1) ^ (l8 & 4 ? 0xb : 0)) & 7;   // 2 l in GF(8) modulo x^3 + x + 1
       if (load_cb) mbar_wait(cb_bar, (cb_loads - 1) & 1, p.err, kErrWait);
-      const float k_scale = p.image_scale[cb];
+      const DenseScale<T> dense_scale(p.image_scale[cb]);
       const uint32_t image_a = smem_u32(image);
       uint32_t ib[NB / 4];
       // block_dim 8: a dense block is one 16-byte chunk; a token's first four are read ahead, too
@@ -437,14 +437,12 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         }
         if (p.n_heavy && row >= 0) {             // dense blocks take the place of their codeword 0
           const T* dense = reinterpret_cast<const T*>(p.heavy) + row * p.n_heavy * BD;
-          float most = 0.f;
           if constexpr (BD == 8) {
 #pragma unroll
             for (int x = 0; x < NB; ++x) {
               if (x >= p.n_heavy) break;
               uint4 w = x < AHEAD ? dense_ahead[x < AHEAD ? x : 0] : reinterpret_cast<const uint4*>(dense)[x];
-              w = make_uint4(dense_word<T>(w.x, k_scale, most), dense_word<T>(w.y, k_scale, most),
-                             dense_word<T>(w.z, k_scale, most), dense_word<T>(w.w, k_scale, most));
+              w = make_uint4(dense_scale(w.x), dense_scale(w.y), dense_scale(w.z), dense_scale(w.w));
               const int b = hblock_s[x];
               *reinterpret_cast<uint4*>(dst + (b >> 3) * HALF + (((b & 7) ^ (tok_l & 7)) << 4)) = w;
             }
@@ -455,15 +453,11 @@ __global__ void __launch_bounds__(kPfThreads, 1)
             if (at_b < 0) continue;
             uint32_t w[WORDS];
 #pragma unroll
-            for (int x = 0; x < WORDS; ++x) w[x] = dense_word<T>(reinterpret_cast<const uint32_t*>(dense + at_b * BD)[x], k_scale, most);
+            for (int x = 0; x < WORDS; ++x) w[x] = dense_scale(reinterpret_cast<const uint32_t*>(dense + at_b * BD)[x]);
             const int byte = b * BD * 2, j = (byte >> 4) & 7;
             uint8_t* to = dst + (byte >> 7) * HALF + ((j ^ (tok_l & 7)) << 4) + (byte & 15);
 #pragma unroll
             for (int x = 0; x < WORDS; ++x) reinterpret_cast<uint32_t*>(to)[x] = w[x];
-          }
-          if (beyond_fp16(most)) {
-            *reinterpret_cast<uint32_t*>(dst + ((tok_l & 7) << 4)) = kNanWord;      // elements 0 and 1
-            record_error(p.err, kErrDense);
           }
         }
         const int first = (t0 + i) * kPfTokens;
@@ -584,6 +578,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         named_barrier(pair_bar, 64);
         l += *other;
         if (*bad_s) l = __int_as_float(0x7fffffff);
+        else if (p.n_heavy && l != l && half == 0 && r0 + r < rows_total) report_dense<D, T>(p, row_of(p, h, 0, r0 + r));
         float* dst = nullptr;
         if (r0 + r < rows_total) {
           if (begins && ends) dst = p.prefix_part + flat_row(p, row_of(p, h, 0, r0 + r)) * RF;

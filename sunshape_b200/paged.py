@@ -32,7 +32,7 @@ from .codec import SunShapeBlockCodec
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 _ERRORS = {131: "a position is outside the cosine/sine table", 132: "a slot is outside the page pool",
            133: "a page number is outside the page pool", 134: "a sequence is longer than its page table",
-           135: "a pipeline wait gave up", 136: "a dense key block is too large for its codebook's scale in fp16"}
+           135: "a pipeline wait gave up", 136: "a dense key block does not fit into fp16"}
 
 
 def paged_error(device: torch.device | str | None = None, clear: bool = True) -> str | None:
@@ -382,8 +382,9 @@ def paged_attention(cache: SunShapePagedCache, query: torch.Tensor, page_table: 
 
     Softmax statistics and sums are fp32.  Codewords are read as fp16 and softmax weights rounded to the cache's
     dtype before they multiply values; a codebook and a query row are each scaled by a power of two into fp16's range, and
-    what is below 2^-25 of their largest is read as zero.  Dense key blocks must stay below 65504 times the largest
-    codeword's norm: a larger one is recorded and makes the rows NaN that see it."""
+    what is below 2^-25 of their largest is read as zero.  Dense key elements of bf16 must stay below 65504, or
+    that many times the largest codeword's norm where that is above 1: a larger one is recorded and makes the rows NaN that
+    see it."""
     _forward_only(query)
     codec, pages = cache.codec, cache._pages
     dev = _device(query, page_table, seq_lens, prefix_table)

@@ -10,7 +10,8 @@ def attention_bounds(cache, q, table, lens, prefix_table=None, prefix_len=0, sca
     """(output, bound, largest error of a score) in 64 bits.
 
     A key element is off by half a step of fp16, 2^-11 of itself or, below 2^-14 of the scaled codebook's largest norm,
-    2^-25 of the scale's unit, which is at most twice the largest codeword norm C: 2^-24 C.  A query element (fp16 and bf16
+    2^-25 of the scale's unit, which is at most twice the largest codeword norm C: 2^-24 C (C is 1/2 at least where the codec
+    has dense blocks, whose scale is at most 1).  A query element (fp16 and bf16
     have no more bits than fp16) is off by 2^-25 of the row's unit where it is below 2^-14 of it: 2^-25 max |q|.  So
         |ds| <= scale * sum_d (2^-11 |q_d k_d| + 2^-24 C |q_d| + 2^-25 max|q| |k_d|) =: e
     (and 2^-10 of that for terms of second order and fp32 sums).  A weight is then off by a factor within exp(2 e), by
@@ -26,7 +27,7 @@ def attention_bounds(cache, q, table, lens, prefix_table=None, prefix_len=0, sca
     cents = cache.codec.centroids.double().cpu()
     cents = cents if cents.ndim == 4 else cents[None]
     for h in range(H):
-        C = float(cents[h % cents.shape[0]].norm(dim=-1).max())
+        C = max(float(cents[h % cents.shape[0]].norm(dim=-1).max()), 0.0 if cache.heavy is None else 0.5)
         shared = dense_tokens(cache, prefix_table, prefix_len, h) if prefix_len else None
         for b in range(B):
             n = int(lens[b])

@@ -173,40 +173,41 @@ def test_many_small_weights_beside_a_large_one(B, G, prefix, dtype):
 
 
 @pytest.mark.parametrize("B,G,L,bd", [(1, 8, 1, 8), (2, 2, 2, 4), (1, 2, 3, 2), (20, 8, 1, 8), (9, 2, 2, 4), (20, 1, 1, 2)])
-@pytest.mark.parametrize("dtype", [BF16, F16])
-def test_dense_blocks_beyond_fp16(B, G, L, bd, dtype):
-    """A dense key that fp16 can not hold in the codebook's scale is recorded and makes the rows NaN that see it; one at
-    the limit is exact, and neither infinite keys nor what lies behind a sequence's end count."""
+@pytest.mark.parametrize("dtype,unit", [(BF16, 1.0), (BF16, 1024.0), (F16, 1.0)])
+def test_dense_blocks_beyond_fp16(B, G, L, bd, dtype, unit):
+    """A dense key that fp16 can not hold is recorded and makes the rows NaN that see it; one at the limit is exact, and
+    neither NaN queries nor what lies behind a sequence's end count.  Codewords far smaller than dense keys do not narrow
+    the range, larger ones widen it."""
     codec, _ = make_paged_codec(64, bd, 1, heavy=3, seed=6)
-    codec.centroids.mul_(0.75 * 2.0 ** -8 / codec.centroids.norm(dim=-1).max())    # scaled by 2^8
+    codec.centroids.mul_((0.75 * 2.0 ** -8 if unit == 1 else 0.75 * unit) / codec.centroids.norm(dim=-1).max())
     codec.invalidate()
-    lens = [33] * B
-    cache, table, n, pt = _cache(codec, 1, lens, 300, 16, dtype)
-    cache.heavy.mul_(2.0 ** -4)
-    q = (0.25 * _randn(B, G, L, 64, seed=3)).to(dtype)
+    cache, table, n, pt = _cache(codec, 1, [33] * B, 300, 16, dtype)
+    q = (0.25 / unit * _randn(B, G, L, 64, seed=3)).to(dtype)
     dense = codec.permutation.view(-1, bd)[codec.mixed_high_precision_blocks].flatten()
-    q[..., dense[0]] = 0.0009765625                                         # of the element that grows
+    q[..., dense[0]] = 2.0 ** -10 / unit                                    # of the element that grows
     run = lambda: cache.attention(q, table, n, prefix_table=pt, prefix_len=300)
     at_prefix, own_last = (int(pt[7]), 0, 3, 0, 0), (int(table[0, 2]), 0, 0, 0, 0)
     behind = (int(table[0, 2]), 0, 1, 0, 0)
-    limit = 255.875 if dtype == F16 else 255.0                              # times 2^8: 65504 or less
+    limit, beyond = (65504.0, None) if dtype == F16 else (65280.0 * unit, 65536.0 * unit)
     for place in (at_prefix, own_last):
         was = cache.heavy[place].item()
-        cache.heavy[place] = limit
-        _near(run(), cache, q, table, n, pt, 300)
-        assert paged.paged_error(DEV) is None
-        cache.heavy[place] = 256.0
-        got = run()
-        assert "dense key block" in paged.paged_error(DEV)
-        if place is at_prefix:
-            assert bool(got.isnan().all())
-        else:                                                               # the last token: of the last query alone
-            assert bool(got[0, :, -1].isnan().all()) and not bool(got[1:].isnan().any())
-            assert not bool(got[0, :, :-1].isnan().any())
+        for sign in (1, -1):
+            cache.heavy[place] = sign * limit
+            _near(run(), cache, q, table, n, pt, 300)
+            assert paged.paged_error(DEV) is None
+            if beyond is None:
+                continue
+            cache.heavy[place] = sign * beyond
+            got = run()
+            assert "dense key block" in paged.paged_error(DEV)
+            if place is at_prefix:
+                assert bool(got.isnan().all())
+            else:                                                           # the last token: of the last query alone
+                assert bool(got[0, :, -1].isnan().all()) and not bool(got[1:].isnan().any())
+                assert not bool(got[0, :, :-1].isnan().any())
         cache.heavy[place] = was
-    cache.heavy[behind] = 256.0
-    _near(run(), cache, q, table, n, pt, 300)
-    q[..., dense[0]] = -1
-    cache.heavy[at_prefix] = float("inf")                                   # its score is -inf: no weight, as in the formula
-    got = run()
-    assert bool(got.isfinite().all())
+    for value in (limit if beyond is None else beyond, float("inf"), float("nan")):
+        cache.heavy[behind] = value
+        _near(run(), cache, q, table, n, pt, 300)
+    q[0, 0, 0, 0] = float("nan")                                            # the query's doing: not recorded
+    assert bool(run()[0, 0, 0].isnan().all())
