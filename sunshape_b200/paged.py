@@ -123,7 +123,8 @@ def norm_rotate(query: torch.Tensor, key: torch.Tensor | None = None, *, q_weigh
     last one (views of a fused projection's output are read in place).  A weight [D] turns that tensor's norm on:
     ``x * w / sqrt(mean(x^2) + eps)``.  ``cos``/``sin`` [n_positions, R / 2] fp32 and ``positions`` [B, L] (int32 or
     int64; [L] broadcasts) rotate the first R <= D elements: pairs (i, i + R/2), or (2i, 2i + 1) if
-    ``interleaved``.  fp32 arithmetic, one rounding to the inputs' dtype.  ``out`` may be the inputs themselves."""
+    ``interleaved``.  fp32 arithmetic, one rounding to the inputs' dtype.  ``out`` may be the inputs themselves, each
+    over its own; any other overlap of the tensors gives wrong results."""
     _forward_only(query, key, q_weight, k_weight)
     dev = _device(query, key, q_weight, k_weight)
     code = _CODES.get(query.dtype)
@@ -158,6 +159,12 @@ def norm_rotate(query: torch.Tensor, key: torch.Tensor | None = None, *, q_weigh
                 raise RuntimeError("out over its own input needs the input's strides.")
             if t is not None:
                 _unit(o, "out")
+                if 0 in o.stride() and any(n > 1 and st == 0 for n, st in zip(o.shape, o.stride())):
+                    raise RuntimeError("out must not hold an element twice.")
+        if key is not None:
+            at, k_at = q_out.data_ptr(), k_out.data_ptr()
+            if at and (at == key.data_ptr() or at == k_at) or k_at and k_at == query.data_ptr():
+                raise RuntimeError("out must not be another tensor's input or output.")
     w = q_weight if q_weight is not None else k_weight
     _lib.norm_rotate(dev, _lib.rows(query), _lib.rows(q_out), q_weight, None if key is None else _lib.rows(key),
                      None if key is None else _lib.rows(k_out), k_weight, code, _lib.F32 if w is None else _CODES[w.dtype],

@@ -211,3 +211,17 @@ def test_dense_blocks_beyond_fp16(B, G, L, bd, dtype, unit):
         _near(run(), cache, q, table, n, pt, 300)
     q[0, 0, 0, 0] = float("nan")                                            # the query's doing: not recorded
     assert bool(run()[0, 0, 0].isnan().all())
+
+
+def test_norm_rotate_outputs_over_other_inputs():
+    """An output over another tensor's input, over the other output or over itself would be written while it is read."""
+    q = torch.randn(2, 4, 3, 64, device=DEV).to(BF16)
+    k, other = q.clone(), q.clone()
+    for out in ((k, other), (other, q), (other, other), (k, q), (other[:, :1].expand(-1, 4, -1, -1), k)):
+        before = [t.clone() for t in (q, k)]
+        with pytest.raises(RuntimeError, match="out must not"):
+            paged.norm_rotate(q, k, out=out)
+        assert torch.equal(q, before[0]) and torch.equal(k, before[1])
+    paged.norm_rotate(q, k, q_weight=torch.ones(64, device=DEV), out=(q, k))
+    e = q[:0]
+    paged.norm_rotate(e, e, out=(e, e))
