@@ -494,8 +494,8 @@ __global__ void __launch_bounds__(kWarps * 32) append_kernel(const __grid_consta
       }
       const float rz = 4.f * kUlp * sqrt_approx(zn) + 16.f * kUlp * kUlp * __int_as_float(most_s[min(tok, n_tok - 1)]);
       const float E = kBound * next + 4.f * rz * (sqrt_approx(next) + rz) + kTiny;
-      // ---- step 3
-      unsigned unsure = __ballot_sync(0xffffffffu, live && !(found > -2 && next - best > 2.f * E));
+      // ---- step 3; also where a codeword that is none was the nearest (keys that lie where those are kept)
+      unsigned unsure = __ballot_sync(0xffffffffu, live && !(found > -2 && at < p.C && next - best > 2.f * E));
       for (; unsure; unsure &= unsure - 1) {
         const int who = __ffs(unsure) - 1, tk = w0 + who;
         double zz[BD], bd64 = __longlong_as_double(0x7ff0000000000000ll);

@@ -48,3 +48,20 @@ def test_two_nearest_codewords(bd, dtype, size):
     first = where[..., 0].reshape(H, nb, L, 2)[..., 0].transpose(1, 2)
     share = (got.long() == first).float().mean()
     assert 0.3 < float(share) < 0.7 and paged.paged_error(DEV) is None
+
+
+@pytest.mark.parametrize("bd", [2, 4, 8])
+@pytest.mark.parametrize("C", [1, 70, 255])
+def test_keys_where_missing_codewords_are_kept(bd, C):
+    """Codebooks of fewer than 256 codewords, keys and codewords around 1e18, where the search keeps the missing ones."""
+    H, D, L = 2, 64, 48
+    g = torch.Generator().manual_seed(C)
+    codec = SunShapeBlockCodec(D, bd, C, device=torch.device(DEV), kv_heads=H)
+    codec.centroids.copy_(1e18 * (1 + 0.5 * torch.randn(codec.centroids.shape, generator=g)))
+    codec.invalidate()
+    cache = SunShapePagedCache.allocate(codec, L // 16, H, page_size=16)
+    k = (1e18 * (1 + 0.1 * torch.randn(1, H, L, D, generator=g))).to(torch.bfloat16).to(DEV)
+    k[:, :, :4] = 1e18
+    cache.append(k, k, torch.arange(L, device=DEV)[None])
+    want, _ = encode64(codec, k.double().cpu())
+    assert torch.equal(cache.indices.cpu().transpose(0, 1).flatten(1, 2), want[0].to(torch.uint8))

@@ -165,3 +165,35 @@ def test_codec_loaded_again_and_inference_mode():
     codec.invalidate()
     _check_attention(cache.attention(q, table, n), cache, q, table, n)
     assert paged.paged_error(DEV) is None
+
+
+def test_shared_prefix_in_two_graphs():
+    """The tensor-core prefix kernel, its join and the sequences' own tokens beside it, captured twice and replayed on two
+    streams at once, over and over."""
+    codec, _ = make_paged_codec(D, 8, H, heavy=2, seed=11)
+    B, n, prefix = 20, 50, 700
+    sides = []
+    for side in range(2):
+        cache = SunShapePagedCache.allocate(codec, 44 + 4 * B, H, page_size=PAGE)
+        cache.indices.copy_(torch.randint(0, 256, cache.indices.shape, generator=torch.Generator().manual_seed(side)))
+        cache.values.copy_(_randn(*cache.values.shape, seed=side))
+        cache.heavy.copy_(_randn(*cache.heavy.shape, seed=side + 1))
+        pt = torch.arange(44, dtype=torch.int32, device=DEV)
+        table = 44 + torch.arange(4 * B, dtype=torch.int32, device=DEV).view(B, 4)
+        lens = torch.full((B,), n, dtype=torch.int32, device=DEV)
+        q = _randn(B, 2 * H, 1, D, seed=side + 2)
+        want = cache.attention(q, table, lens, prefix_table=pt, prefix_len=prefix)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = [cache.attention(q, table, lens, prefix_table=pt, prefix_len=prefix) for _ in range(3)]
+        sides.append((graph, outs, want, torch.cuda.Stream(), (cache, pt, table, lens, q)))
+        ref, bound = attention64(cache, q, table, lens, pt, prefix)
+        assert bool(((want.double().cpu() - ref).abs() <= bound).all())
+    for _ in range(20):
+        for graph, *_, stream, _ in sides:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, outs, want, _, _ in sides:
+        assert all(torch.equal(out, want) for out in outs)
