@@ -69,12 +69,11 @@ def _device(first: torch.Tensor, *others: torch.Tensor | None) -> int:
     return dev
 
 
-def _forward_only(*tensors: torch.Tensor | None) -> None:
+def _forward_only() -> None:
+    """For a call with an input that requires gradients."""
     if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise RuntimeError("the paged calls have no backward pass: call them under torch.no_grad() or "
-                                   "torch.inference_mode(), or detach their inputs.")
+        raise RuntimeError("the paged calls have no backward pass: call them under torch.no_grad() or "
+                           "torch.inference_mode(), or detach their inputs.")
 
 
 def _unit(t: torch.Tensor, what: str) -> torch.Tensor:
@@ -125,7 +124,9 @@ def norm_rotate(query: torch.Tensor, key: torch.Tensor | None = None, *, q_weigh
     int64; [L] broadcasts) rotate the first R <= D elements: pairs (i, i + R/2), or (2i, 2i + 1) if
     ``interleaved``.  fp32 arithmetic, one rounding to the inputs' dtype.  ``out`` may be the inputs themselves, each
     over its own; any other overlap of the tensors gives wrong results."""
-    _forward_only(query, key, q_weight, k_weight)
+    if (query.requires_grad or (key is not None and key.requires_grad) or (q_weight is not None and q_weight.requires_grad)
+            or (k_weight is not None and k_weight.requires_grad)):
+        _forward_only()
     dev = _device(query, key, q_weight, k_weight)
     code = _CODES.get(query.dtype)
     if query.ndim != 4 or (key is not None and key.ndim != 4):
@@ -348,7 +349,8 @@ def append_paged(cache: SunShapePagedCache, key: torch.Tensor, value: torch.Tens
     ragged batch [N, kv_heads, D] is ``key.transpose(0, 1).unsqueeze(0)`` with slots [1, N].  Slots of one call
     must be distinct.  The codeword is the nearest to the rotated key in real arithmetic (decided in 64 bits
     where fp32 cannot tell; lowest index on ties), without rounding the rotated key in between."""
-    _forward_only(key, value)
+    if key.requires_grad or value.requires_grad:
+        _forward_only()
     codec = cache.codec
     dev = _device(key, value, slots)
     if dev != cache._index:
@@ -392,7 +394,8 @@ def paged_attention(cache: SunShapePagedCache, query: torch.Tensor, page_table: 
     what is below 2^-25 of their largest is read as zero.  Dense key elements of bf16 must stay below 65504, or
     that many times the largest codeword's norm where that is above 1: a larger one is recorded and makes the rows NaN that
     see it."""
-    _forward_only(query)
+    if query.requires_grad:
+        _forward_only()
     codec, pages = cache.codec, cache._pages
     dev = _device(query, page_table, seq_lens, prefix_table)
     if dev != cache._index:
