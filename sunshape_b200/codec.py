@@ -58,6 +58,9 @@ class SunShapeBlockCodec(torch.nn.Module):
     the encode's distance) and ``identity_baseline``; ``rotated`` / ``legacy_strict`` raise.
     """
 
+    _paged_tables = None                # what the paged kernels read (paged.py), and those of other shapes before
+    _paged_retired = ()
+
     def __init__(self, head_dim: int, block_dim: int = 8, n_centroids: int = 256, c: float = 5.0,
                  n_refine_dsq: int = 3, mode: str = "profileperm_baseline", use_rotation: bool = False,
                  rotation_seed: int = 0, device: torch.device | None = None, kv_heads: int | None = None):
@@ -92,8 +95,6 @@ class SunShapeBlockCodec(torch.nn.Module):
         self.register_buffer("rotation", torch.eye(head_dim, device=dev))
         self._desc_cache = None
         self._metric_cache = None
-        self._paged_tables = None       # what the paged kernels read (paged.py), and those of other shapes before
-        self._paged_retired = ()
 
     # ------------------------------------------------------------------ state
     def _load_from_state_dict(self, state_dict, prefix, *args, **kwargs):

@@ -14,8 +14,15 @@ struct Layout {
 };
 
 // Query rows of a KV head from which on the prefix goes to the tensor-core kernel: it rebuilds a key once for 256 rows
-// where the memory-bound kernel reads it again for every 16.  512 rows over 32768 tokens of 8 heads: 477 us there, 139 here;
-// 128 rows over 10007: 144 and 75.
+// where the memory-bound kernel reads it again for every 16.  The whole call in us, 8 heads, 100 to 500 own tokens a sequence,
+// prefixes of 100, 1000, 10000 and 40000 tokens:
+//   rows   tensor cores        memory-bound
+//    16    23  27  38  71      35  36  41   71
+//    20    27  30  41  71      34  36  44   79
+//    64    31  34  46  80      36  38  54  113
+//   128    36  40  52  88      39  43  72  175
+// With one head, whose tiles spread over all blocks, the memory-bound kernel is ahead from about 8000 tokens on (40 rows, 10000
+// tokens: 53 against 41).
 constexpr int64_t kPrefixRows = 17;
 
 // item_rows: of the memory-bound kernel's calls; tensor: the prefix goes to the tensor-core kernel

@@ -31,7 +31,9 @@ constexpr int kHeadTiles = 48;
 // 14); of 8 rows, 2 (64 sequences of up to 700 tokens, 64/8 heads: 28.9 us with 0, 25.7 with 2).
 constexpr int kItemTiles = 5;
 constexpr int kPlanChunks = 256;   // sequence chunks of the in-kernel plan
-// Registers of a thread: what the block is launched with, and its split between the roles (setmaxnreg).
+// Registers of a thread: what the block is launched with, and its split between the roles (setmaxnreg).  Not enough for either:
+// at D = DV = 128 the compiler spills 148 to 200 bytes a thread with one group of eight rows and 516 to 612 with two, whose
+// consumer holds 2 x 32 accumulators, 2 x 16 words of queries and a tile's keys.
 constexpr int kLaunchRegs = 128, kConsumerRegs = 216, kProducerRegs = 40;
 static_assert(kConsumerRegs + kProducerRegs <= 2 * kLaunchRegs, "the split waits forever where it exceeds the launch");
 

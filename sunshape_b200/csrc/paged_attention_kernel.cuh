@@ -17,6 +17,11 @@
 // sequences of 1k to 8k, 32/8 heads: 114 us (5.6 TB/s); a call of one tile a head 12 us, which is plan, codebook, queries,
 // one tile and the join.
 // P^T comes from the accumulators of S^T by a register transpose (movmatrix).
+//
+// What is rounded: codewords to fp16 (a second term of them would double the codebook in shared memory and halve the ring),
+// queries to fp16 in a scale of the row's own (exact but for elements below 2^-14 of its largest), weights to the cache's type
+// (the MMA multiplies equal types).  Scores, maxima, sums and accumulators are fp32.  On 517 tokens in f16 the result is off
+// by 4e-4 where its own rounding alone is 2e-4, on 1k to 8k tokens in bf16 by 2.3e-3 against 1.7e-3.
 #pragma once
 
 #include <type_traits>

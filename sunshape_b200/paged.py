@@ -216,11 +216,13 @@ def renew_tables(codec: SunShapeBlockCodec) -> _CodecTables:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("a codec's tables can not be derived while a CUDA graph is captured: make the cache, and call "
                                "codec.invalidate() after edits of the codec, before the capture.")
+        tables = codec._paged_tables
+        if tables is not None and tables.made is codec._desc_cache:      # another thread was faster
+            return tables
         torch.cuda.synchronize()
         made = codec.kernel_desc()
         desc, (cents, *_), n_heavy = made
         key = (device, tuple(cents.shape), n_heavy)
-        tables = codec._paged_tables
         if tables is None or tables.key != key:
             if tables is not None:              # graphs captured with them may still be replayed
                 codec._paged_retired = (*codec._paged_retired, tables)
