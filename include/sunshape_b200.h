@@ -264,7 +264,7 @@ typedef struct sunshape_pages {
 } sunshape_pages_t;
 
 /* What the paged kernels read of a codec (at most 256 codewords, block_dim 2, 4 or 8), derived from its codebooks
- * once and kept as long as they stay: tables is a buffer of sunshape_paged_tables_bytes, 256-byte aligned.  The caller
+ * once and kept as long as they stay; the calls get the descriptor (dense blocks or none) that it was derived from: tables is a buffer of sunshape_paged_tables_bytes, 256-byte aligned.  The caller
  * orders calls on other streams behind the one that writes it, and a second writing behind the readers. */
 int64_t sunshape_paged_tables_bytes(const sunshape_codec_t* codec);
 int sunshape_paged_tables(const sunshape_codec_t* codec, void* tables, int64_t tables_bytes, void* stream);

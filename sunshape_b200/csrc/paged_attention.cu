@@ -25,6 +25,8 @@ struct Layout {
 // tokens: 53 against 41).
 constexpr int64_t kPrefixRows = 17;
 
+constexpr int64_t kOverlapTiles = kWaitLimitNs / 2500 / 8;
+
 // item_rows: of the memory-bound kernel's calls; tensor: the prefix goes to the tensor-core kernel
 Layout layout(int grid, int64_t rows, int64_t item_rows, int dv, bool prefix, bool tensor) {
   const int64_t row = row_floats(dv) * 4;
@@ -191,7 +193,10 @@ int sunshape_paged_attention(const sunshape_codec_t* codec, const void* tables, 
     else rc = bf16 ? launch<__nv_bfloat16, false>(f, vmap, d, dv, bd, grid, st) : launch<__half, false>(f, vmap, d, dv, bd, grid, st);
     if (rc) return rc;
     p.prefix_parts = 1;
-    p.overlap = tensor;                // else both use the same slots of the workspace
+    // else both use the same slots of the workspace.  Producers that run ahead wait for the prefix's end with their rings full,
+    // and give up after kWaitLimitNs: not beside a prefix of more than kOverlapTiles tiles of 2.5 us a thread block
+    const int64_t tiles = ((prefix_len + 127) / 128) * ((own * batch + 255) / 256) * p.H / grid;
+    p.overlap = tensor && tiles <= kOverlapTiles;
   }
   return bf16 ? launch<__nv_bfloat16, false>(p, vmap, d, dv, bd, grid, st)
               : launch<__half, false>(p, vmap, d, dv, bd, grid, st);
